@@ -985,6 +985,176 @@ int kvx_scatter_blocks(uint64_t storage_table, int64_t num_storages,
                        int64_t n, uint64_t staging, int32_t order,
                        uint64_t error, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators that fill and read the paged pool. No counterpart in the
+ * reference, which moves blocks as opaque bytes: here a storage [blocks]
+ * [block_tokens][heads][head_dim] also takes a step's new keys and values and
+ * is attended over in place.
+ *
+ * Each call enqueues kernels on `stream` and returns no future: order later
+ * work after it on that stream. Nothing is allocated, kept or synchronised, so
+ * a call can be captured into a graph, and a replay follows the contents that
+ * lengths, starts and tables then have. Those contents are not checked on the
+ * host; whatever they hold, no kernel reads or writes outside the arguments:
+ * a start is bounded to [0, tokens] and from below by the one before, a
+ * negative length is 0, and a token whose position is past the table or whose
+ * block id is outside the pool has no place (append_kv drops it, attend does
+ * not see it). Strides are in elements and not negative.
+ * ------------------------------------------------------------------------- */
+
+/* Element types. */
+#define KVX_BF16 0
+#define KVX_F16 1
+#define KVX_F32 2
+#define KVX_E4M3 3 /* OCP e4m3 with one fp32 scale a (block, head) */
+
+/*
+ * RMS norm and position rotation of query and key heads in one pass, for each
+ * row x of head_dim (1..256) elements:
+ *   y = x * weight / sqrt(mean(x^2) + eps)         (weight 0: y = x)
+ *   (u, v) -> (u cos a_i - v sin a_i, v cos a_i + u sin a_i),
+ *   a_i = position * inv_freq[i], i < rotary_dim / 2
+ * over the pairs (y_i, y_{i + rotary_dim / 2}), or (y_2i, y_2i+1) with
+ * interleaved; dimensions from rotary_dim on keep y. Computed in fp32 (the
+ * angle of any position up to 2^53 reduced exactly enough for it), rounded once. q and k are [tokens][heads]
+ * [head_dim] with the last dimension contiguous; either may have 0 heads. An
+ * output may be its input (same address and strides) and may otherwise not
+ * overlap an input or output.
+ */
+typedef struct kvx_norm_rope_args {
+  int32_t device;
+  int32_t dtype; /* KVX_BF16, KVX_F16 or KVX_F32 */
+  int64_t tokens;
+  int32_t q_heads;
+  int32_t k_heads;
+  int32_t head_dim;
+  int32_t rotary_dim; /* even, 0..head_dim */
+  uint64_t q;
+  uint64_t k;
+  uint64_t q_out;
+  uint64_t k_out;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride;
+  int64_t k_out_token_stride, k_out_head_stride;
+  uint64_t q_weight; /* [head_dim] or 0: no norm */
+  uint64_t k_weight;
+  int32_t weight_dtype; /* of both: dtype or KVX_F32 */
+  int32_t positions_64; /* positions are int64 rather than int32 */
+  uint64_t positions;   /* [tokens] */
+  uint64_t inv_freq;    /* [rotary_dim / 2] fp32 */
+  float eps;
+  int32_t interleaved;
+} kvx_norm_rope_args;
+
+int kvx_norm_rope(const kvx_norm_rope_args* args, void* stream);
+
+/* The storages of one layer. */
+typedef struct kvx_paged_cache {
+  int64_t k_layer;
+  int64_t v_layer;
+  int64_t shard;
+  int64_t k_scale_layer; /* KVX_E4M3: tables [blocks][heads] fp32 */
+  int64_t v_scale_layer;
+  int32_t dtype; /* the tensors' type or KVX_E4M3 */
+  int32_t block_tokens;
+  int32_t heads;
+  int32_t head_dim;
+} kvx_paged_cache;
+
+/*
+ * The sequences of a step (device arrays, int32). Sequence s owns the tokens
+ * [starts[s], starts[s + 1]) of the call's tensors (starts 0: token s, one
+ * each) and holds lengths[s] tokens with them; token p of it is in slot p %
+ * block_tokens of block tables[s][p / block_tokens]. Its new tokens are its
+ * last. Up to 4096 sequences; tokens from starts[sequences] on belong to none
+ * and are left alone.
+ */
+typedef struct kvx_paged_batch {
+  uint64_t tables; /* [sequences][table_width] */
+  int64_t table_stride;
+  int64_t table_width;
+  uint64_t lengths;
+  uint64_t starts; /* [sequences + 1] or 0 */
+  int64_t sequences;
+} kvx_paged_batch;
+
+/*
+ * Stores new keys and values [tokens][heads][head_dim] into their slots, the
+ * key normed (k_weight) and rotated (rotary_dim) on the way as kvx_norm_rope
+ * does, at its place in the sequence or at positions[token]. In a KVX_E4M3
+ * cache the scale of each touched (block, head) becomes
+ *   max(old, largest finite |x| of its new tokens / 448),
+ * old = 0 unless the block holds earlier tokens of the sequence; values are
+ * clamped to +-448 scales, and earlier tokens are stored again under a scale
+ * that grew. A block that takes new tokens must belong to one sequence of the
+ * call, and a token to one slot: with the same block or slot twice, which of
+ * the values remain is not defined.
+ */
+typedef struct kvx_append_kv_args {
+  kvx_paged_cache cache;
+  kvx_paged_batch batch;
+  int64_t tokens;
+  int32_t dtype; /* KVX_BF16 or KVX_F16 */
+  int32_t rotary_dim;
+  uint64_t k;
+  uint64_t v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  uint64_t k_weight;
+  int32_t weight_dtype;
+  int32_t positions_64;
+  uint64_t positions; /* [tokens] or 0 */
+  uint64_t inv_freq;
+  float eps;
+  int32_t interleaved;
+} kvx_append_kv_args;
+
+int kvx_manager_append_kv(kvx_manager* m, const kvx_append_kv_args* args, void* stream);
+
+/*
+ * Attention of q [tokens][q_heads][head_dim] over the cached tokens of each
+ * sequence; q_heads is a multiple of the cache's heads, neighbouring query
+ * heads sharing one. The query of a token at position p sees positions 0..p
+ * (non_causal: all of the sequence's). Scores, sums and partial results are
+ * fp32; exponentials are rounded to the products' 16-bit type. A query that
+ * sees nothing gets zeros and an lse of -inf. In a chunk, a value that is not
+ * finite reaches the earlier queries of its own sequence too.
+ *
+ * Groups: the sequences [group_starts[g], group_starts[g + 1]) (ascending,
+ * device int32) hold their first prefix_lengths[g] tokens in the same blocks,
+ * which the first sequence's table names. The prefix is then read once for
+ * all. The result is the same as without groups.
+ *
+ * workspace: device memory of kvx_manager_attend_workspace bytes (a function of
+ * the sizes alone, addresses may still be 0; starts only has to be set or not
+ * set as in the call), 16-byte aligned; its contents mean nothing between calls.
+ * Calls that can run at the same time need one each.
+ */
+typedef struct kvx_attend_args {
+  kvx_paged_cache cache;
+  kvx_paged_batch batch;
+  int64_t tokens;
+  int32_t dtype; /* KVX_BF16 or KVX_F16 */
+  int32_t q_heads;
+  uint64_t q;
+  uint64_t out; /* may be q itself */
+  int64_t q_token_stride, q_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  uint64_t lse; /* fp32 [tokens][q_heads] or 0: log of the sum of exponentials */
+  uint64_t group_starts;   /* [groups + 1] */
+  uint64_t prefix_lengths; /* [groups] */
+  int32_t groups;          /* 0..256 */
+  int32_t non_causal;
+  float scale; /* positive */
+  int32_t reserved;
+  uint64_t workspace;
+  int64_t workspace_bytes;
+} kvx_attend_args;
+
+int kvx_manager_attend_workspace(kvx_manager* m, const kvx_attend_args* args, int64_t* bytes);
+int kvx_manager_attend(kvx_manager* m, const kvx_attend_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

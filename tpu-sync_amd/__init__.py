@@ -10,7 +10,8 @@ from .kv_cache_manager import (KVCacheManager, LogicalBlockManager, RaidenFuture
                                probe_stream_queues, measure_link_peaks)
 from .kv_cache_store import (BlockStatus, KVCacheMetadata, KVCacheMetadataShmRegion,
                              KVCacheStore, LRUCache, RaidenBlockId, RaidenId)
-from . import copy_plan, pool_layout, tiling, transport
+from . import copy_plan, paged_attention, pool_layout, tiling, transport
+from .paged_attention import norm_rope
 from .pool_layout import PoolSpec, RegionSpec
 from .weight_synchronizer import (StridedEntry, StridedPlan, WeightSynchronizer,
                                   column_split_entries, compute_nd_shard_slices, copy_strided)
@@ -20,7 +21,7 @@ __all__ = ["KVCacheManager", "LogicalBlockManager", "RaidenFuture", "KvxError", 
            "KVCacheMetadata", "KVCacheMetadataShmRegion", "WeightSynchronizer",
            "StridedEntry", "StridedPlan", "copy_strided", "column_split_entries",
            "compute_nd_shard_slices", "pool_layout", "copy_plan", "tiling", "transport", "PoolSpec", "RegionSpec",
-           "library_path"]
+           "paged_attention", "norm_rope", "library_path"]
 
 
 def library_path() -> str:

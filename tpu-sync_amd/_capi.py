@@ -216,6 +216,65 @@ class PushItemC(ctypes.Structure):
     _fields_ = [(k, ctypes.c_int64) for k in ("layer", "shard", "k", "staging_offset", "size")]
 
 
+BF16, F16, F32, E4M3 = 0, 1, 2, 3  # KVX_BF16 ...
+
+
+class NormRopeArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("device", "dtype")]
+                + [("tokens", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("q_heads", "k_heads", "head_dim", "rotary_dim")]
+                + [(n, ctypes.c_uint64) for n in ("q", "k", "q_out", "k_out")]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                    "q_out_token_stride", "q_out_head_stride", "k_out_token_stride",
+                    "k_out_head_stride")]
+                + [(n, ctypes.c_uint64) for n in ("q_weight", "k_weight")]
+                + [(n, ctypes.c_int32) for n in ("weight_dtype", "positions_64")]
+                + [(n, ctypes.c_uint64) for n in ("positions", "inv_freq")]
+                + [("eps", ctypes.c_float), ("interleaved", ctypes.c_int32)])
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int64) for n in ("k_layer", "v_layer", "shard", "k_scale_layer",
+                                               "v_scale_layer")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "block_tokens", "heads", "head_dim")])
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [
+        ("tables", ctypes.c_uint64),
+        ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("lengths", ctypes.c_uint64),
+        ("starts", ctypes.c_uint64),
+        ("sequences", ctypes.c_int64),
+    ]
+
+
+class AppendKvArgs(ctypes.Structure):
+    _fields_ = ([("cache", PagedCache), ("batch", PagedBatch), ("tokens", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "rotary_dim")]
+                + [(n, ctypes.c_uint64) for n in ("k", "v")]
+                + [(n, ctypes.c_int64) for n in ("k_token_stride", "k_head_stride",
+                                                 "v_token_stride", "v_head_stride")]
+                + [("k_weight", ctypes.c_uint64)]
+                + [(n, ctypes.c_int32) for n in ("weight_dtype", "positions_64")]
+                + [(n, ctypes.c_uint64) for n in ("positions", "inv_freq")]
+                + [("eps", ctypes.c_float), ("interleaved", ctypes.c_int32)])
+
+
+class AttendArgs(ctypes.Structure):
+    _fields_ = ([("cache", PagedCache), ("batch", PagedBatch), ("tokens", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "q_heads")]
+                + [(n, ctypes.c_uint64) for n in ("q", "out")]
+                + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride",
+                                                 "out_token_stride", "out_head_stride")]
+                + [(n, ctypes.c_uint64) for n in ("lse", "group_starts", "prefix_lengths")]
+                + [(n, ctypes.c_int32) for n in ("groups", "non_causal")]
+                + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                   ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64)])
+
+
 # kvx_ready_fn(user, code)
 READY_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int32)
 
@@ -455,6 +514,10 @@ PROTOTYPES = {
                                            ctypes.POINTER(_vp)]),
     "kvx_manager_h2d_pool_blocks": (_int, [_vp, _i64, _i64p, _i64, _i64, _vp,
                                            ctypes.POINTER(_vp)]),
+    "kvx_norm_rope": (_int, [ctypes.POINTER(NormRopeArgs), _vp]),
+    "kvx_manager_append_kv": (_int, [_vp, ctypes.POINTER(AppendKvArgs), _vp]),
+    "kvx_manager_attend_workspace": (_int, [_vp, ctypes.POINTER(AttendArgs), _i64p]),
+    "kvx_manager_attend": (_int, [_vp, ctypes.POINTER(AttendArgs), _vp]),
 }
 
 _lib = None

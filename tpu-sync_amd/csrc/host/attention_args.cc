@@ -1,0 +1,434 @@
+#include "attention_args.h"
+
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "device_memory.h"
+
+namespace kvx {
+namespace {
+
+constexpr int64_t kMostTokens = int64_t{1} << 30;  // of a call and of a table row
+
+Status Bad(const std::string& what) { return InvalidArgumentError(what); }
+
+// Rows [tokens][heads][dim] at strides in elements.
+struct Rows {
+  uint64_t at;
+  int64_t token_stride, head_stride;
+  int64_t tokens, heads, dim, item;
+
+  bool empty() const { return tokens == 0 || heads == 0; }
+  // Bytes from the first to behind the last element; false on overflow.
+  bool Extent(uint64_t* bytes) const {
+    int64_t t = 0, h = 0, n = 0;
+    if (__builtin_mul_overflow(tokens - 1, token_stride, &t) ||
+        __builtin_mul_overflow(heads - 1, head_stride, &h) || __builtin_add_overflow(t, h, &n) ||
+        __builtin_add_overflow(n, dim, &n) || __builtin_mul_overflow(n, item, &n)) {
+      return false;
+    }
+    *bytes = static_cast<uint64_t>(n);
+    return true;
+  }
+  // Whether two rows share elements.
+  bool SelfOverlaps() const {
+    const int64_t t = tokens > 1 ? token_stride : INT64_MAX;
+    const int64_t h = heads > 1 ? head_stride : INT64_MAX;
+    if (t >= h) return h < dim || (tokens > 1 && (heads - 1) * h + dim > t);
+    return t < dim || (heads > 1 && (tokens - 1) * t + dim > h);
+  }
+  bool Same(const Rows& o) const {
+    return at == o.at && (tokens == 1 || token_stride == o.token_stride) &&
+           (heads == 1 || head_stride == o.head_stride);
+  }
+};
+
+Status CheckRows(DeviceRangeChecker* ranges, const Rows& r, const char* what) {
+  if (r.token_stride < 0 || r.head_stride < 0) return Bad(std::string(what) + ": negative stride");
+  if (r.empty()) return OkStatus();
+  uint64_t bytes = 0;
+  if (!r.Extent(&bytes)) return Bad(std::string(what) + ": size overflows");
+  if (r.at % static_cast<uint64_t>(r.item) != 0) {
+    return Bad(std::string(what) + ": address is not a multiple of the element size");
+  }
+  return ranges->Check(r.at, bytes, what);
+}
+
+bool Meet(uint64_t a, uint64_t a_bytes, uint64_t b, uint64_t b_bytes) {
+  return a_bytes > 0 && b_bytes > 0 && a < b + b_bytes && b < a + a_bytes;
+}
+
+bool Meet(const Rows& a, const Rows& b) {
+  uint64_t x = 0, y = 0;
+  if (a.empty() || b.empty() || !a.Extent(&x) || !b.Extent(&y)) return false;
+  if (!Meet(a.at, x, b.at, y)) return false;
+  // Parts of one wider row (a fused projection): apart if no row of one
+  // reaches into a row of the other.
+  if (a.token_stride == b.token_stride && a.tokens > 1 && a.item == b.item) {
+    const int64_t period = a.token_stride * a.item;
+    const int64_t la = ((a.heads - 1) * a.head_stride + a.dim) * a.item;
+    const int64_t lb = ((b.heads - 1) * b.head_stride + b.dim) * b.item;
+    const int64_t gap = a.at <= b.at ? static_cast<int64_t>(b.at - a.at)
+                                     : static_cast<int64_t>(a.at - b.at);
+    const int64_t first = a.at <= b.at ? la : lb, second = a.at <= b.at ? lb : la;
+    if (gap < period && first <= gap && gap + second <= period) return false;
+  }
+  return true;
+}
+
+// Results may take the place of what they are computed from, row for row;
+// any other overlap would be read after it is written.
+Status CheckInPlace(const Rows& in, const Rows& out, const char* in_name, const char* out_name) {
+  if (out.empty()) return OkStatus();
+  if (out.SelfOverlaps()) return Bad(std::string(out_name) + ": rows overlap");
+  if (!in.Same(out) && Meet(in, out)) {
+    return Bad(std::string(out_name) + ": overlaps " + in_name +
+               " (in place it has to have the same address and strides)");
+  }
+  return OkStatus();
+}
+
+Status CheckTokens(int64_t tokens, int64_t heads, int64_t dim) {
+  if (tokens < 0 || tokens > kMostTokens) return Bad("tokens must be 0..2^30");
+  if (heads < 0 || heads > 1024) return Bad("heads must be at most 1024");
+  if (dim < 1 || dim > kMaxHeadDim) return Bad("head_dim must be 1..256");
+  if (tokens * heads > INT32_MAX / 4) return Bad("tokens * heads must be below 2^29");
+  return OkStatus();
+}
+
+Status CheckRotation(DeviceRangeChecker* ranges, int64_t rotary, int64_t dim, uint64_t inv_freq,
+                     uint64_t positions, bool positions_64, int64_t tokens) {
+  if (rotary < 0 || rotary % 2 != 0 || rotary > dim) {
+    return Bad("rotary_dim must be even and at most head_dim");
+  }
+  if (rotary == 0 || tokens == 0) return OkStatus();
+  KVX_RETURN_IF_ERROR(ranges->Check(inv_freq, static_cast<uint64_t>(rotary / 2) * 4, "inv_freq"));
+  if (positions != 0) {
+    if (positions % (positions_64 ? 8 : 4) != 0) return Bad("positions: unaligned address");
+    KVX_RETURN_IF_ERROR(
+        ranges->Check(positions, static_cast<uint64_t>(tokens) * (positions_64 ? 8 : 4),
+                      "positions"));
+  }
+  return OkStatus();
+}
+
+Status CheckWeight(DeviceRangeChecker* ranges, uint64_t at, int32_t type, int32_t row_type,
+                   int64_t dim, float eps, const char* what) {
+  if (at == 0) return OkStatus();
+  if (type != row_type && type != kF32) {
+    return Bad(std::string(what) + ": must be of the rows' type or fp32");
+  }
+  if (!std::isfinite(eps) || eps < 0) return Bad("eps must be finite and not negative");
+  if (at % static_cast<uint64_t>(ElementBytes(type)) != 0) {
+    return Bad(std::string(what) + ": unaligned address");
+  }
+  return ranges->Check(at, static_cast<uint64_t>(dim * ElementBytes(type)), what);
+}
+
+Status CheckWords(DeviceRangeChecker* ranges, uint64_t at, int64_t n, const char* what) {
+  if (at % 4 != 0) return Bad(std::string(what) + ": unaligned address");
+  return ranges->Check(at, static_cast<uint64_t>(n) * 4, what);
+}
+
+Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t tokens,
+                  int64_t block_tokens, int64_t num_blocks, BatchView* out) {
+  if (b.sequences < 0 || b.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
+  if (b.starts == 0 && tokens != b.sequences) {
+    return Bad("without starts there is one token a sequence: tokens must equal sequences");
+  }
+  if (b.table_width < 0 || b.table_stride < 0) return Bad("negative table width or stride");
+  if (block_tokens < 1) return Bad("block_tokens must be positive");
+  if (b.table_width > kMostTokens / block_tokens) {
+    return Bad("table_width * block_tokens must be at most 2^30");
+  }
+  if (b.sequences > 0) {
+    int64_t words = 0;
+    if (__builtin_mul_overflow(b.sequences - 1, b.table_stride, &words) ||
+        __builtin_add_overflow(words, b.table_width, &words) || words > INT64_MAX / 4) {
+      return Bad("tables: size overflows");
+    }
+    KVX_RETURN_IF_ERROR(CheckWords(ranges, b.tables, words, "tables"));
+    KVX_RETURN_IF_ERROR(CheckWords(ranges, b.lengths, b.sequences, "lengths"));
+    if (b.starts != 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(ranges, b.starts, b.sequences + 1, "starts"));
+    }
+  }
+  out->tables = reinterpret_cast<const int32_t*>(b.tables);
+  out->lengths = reinterpret_cast<const int32_t*>(b.lengths);
+  out->starts = reinterpret_cast<const int32_t*>(b.starts);
+  out->table_stride = b.table_stride;
+  out->table_width = static_cast<int32_t>(b.table_width);
+  out->sequences = static_cast<int32_t>(b.sequences);
+  out->tokens = static_cast<int32_t>(tokens);
+  out->block_tokens = static_cast<int32_t>(block_tokens);
+  out->capacity = static_cast<int32_t>(b.table_width * block_tokens);
+  out->num_blocks = static_cast<int32_t>(num_blocks);
+  return OkStatus();
+}
+
+struct Cache {
+  PoolStorage k, v;
+  uint64_t k_scales = 0, v_scales = 0;
+  int64_t num_blocks = 0;
+};
+
+Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type, Cache* out) {
+  if (!pool.device_backed) {
+    return FailedPreconditionError("needs a device-backed KVCacheManagerBase");
+  }
+  if (!Is16Bit(type)) return Bad("dtype must be KVX_BF16 or KVX_F16");
+  if (c.dtype != type && c.dtype != kE4m3) {
+    return Bad("the cache must be of the tensors' type or KVX_E4M3");
+  }
+  if (c.heads < 1 || c.heads > 1024) return Bad("heads must be 1..1024");
+  if (c.head_dim < 1 || c.head_dim > kMaxHeadDim) return Bad("head_dim must be 1..256");
+  if (c.block_tokens < 1 || c.block_tokens > (1 << 20)) return Bad("block_tokens must be 1..2^20");
+  if (!pool.find(pool.context, c.k_layer, c.shard, &out->k) ||
+      !pool.find(pool.context, c.v_layer, c.shard, &out->v)) {
+    return OutOfRangeError("layer or shard index out of range");
+  }
+  const int64_t block = static_cast<int64_t>(c.block_tokens) * c.heads * c.head_dim *
+                        ElementBytes(c.dtype);
+  if (out->k.block_bytes != block || out->v.block_bytes != block) {
+    return Bad("blocks of " + std::to_string(out->k.block_bytes) + " and " +
+               std::to_string(out->v.block_bytes) + " bytes do not hold [" +
+               std::to_string(c.block_tokens) + ", " + std::to_string(c.heads) + ", " +
+               std::to_string(c.head_dim) + "] of " + std::to_string(ElementBytes(c.dtype)) +
+               " bytes");
+  }
+  int64_t blocks = std::min(out->k.bytes, out->v.bytes) / block;
+  if (c.dtype == kE4m3) {
+    PoolStorage s[2];
+    if (!pool.find(pool.context, c.k_scale_layer, c.shard, &s[0]) ||
+        !pool.find(pool.context, c.v_scale_layer, c.shard, &s[1])) {
+      return OutOfRangeError("scale layer or shard index out of range");
+    }
+    for (const PoolStorage& t : s) {
+      if (t.block_bytes != static_cast<int64_t>(c.heads) * 4) {
+        return Bad("scale tables must hold one fp32 a (block, head): " +
+                   std::to_string(c.heads * 4) + " bytes a block, not " +
+                   std::to_string(t.block_bytes));
+      }
+      if (t.base % 4 != 0) return Bad("scale tables: unaligned address");
+      blocks = std::min(blocks, t.bytes / t.block_bytes);
+    }
+    if (s[0].base == s[1].base) return Bad("keys and values need scale tables of their own");
+    out->k_scales = s[0].base;
+    out->v_scales = s[1].base;
+  } else if ((out->k.base | out->v.base) % 2 != 0) {
+    return Bad("cache storages: unaligned address");
+  }
+  if (out->k.base == out->v.base) return Bad("keys and values need storages of their own");
+  out->num_blocks = std::min<int64_t>(blocks, INT32_MAX);
+  return OkStatus();
+}
+
+}  // namespace
+
+Status CheckNormRope(const kvx_norm_rope_args& a, NormRopeLaunch* out) {
+  if (a.dtype != kBf16 && a.dtype != kF16 && a.dtype != kF32) {
+    return Bad("dtype must be KVX_BF16, KVX_F16 or KVX_F32");
+  }
+  KVX_RETURN_IF_ERROR(CheckTokens(a.tokens, static_cast<int64_t>(a.q_heads) + a.k_heads,
+                                  a.head_dim));
+  if (a.q_heads < 0 || a.k_heads < 0) return Bad("negative number of heads");
+  DeviceRangeChecker ranges(a.device);
+  const int64_t item = ElementBytes(a.dtype);
+  const Rows q = {a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.q_heads, a.head_dim, item};
+  const Rows k = {a.k, a.k_token_stride, a.k_head_stride, a.tokens, a.k_heads, a.head_dim, item};
+  const Rows qo = {a.q_out, a.q_out_token_stride, a.q_out_head_stride, a.tokens, a.q_heads,
+                   a.head_dim, item};
+  const Rows ko = {a.k_out, a.k_out_token_stride, a.k_out_head_stride, a.tokens, a.k_heads,
+                   a.head_dim, item};
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, q, "q"));
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, k, "k"));
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, qo, "q_out"));
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, ko, "k_out"));
+  KVX_RETURN_IF_ERROR(CheckInPlace(q, qo, "q", "q_out"));
+  KVX_RETURN_IF_ERROR(CheckInPlace(k, ko, "k", "k_out"));
+  if (Meet(k, qo) || Meet(qo, ko)) return Bad("q_out: overlaps k or k_out");
+  if (Meet(q, ko)) return Bad("k_out: overlaps q");
+  if (a.rotary_dim > 0 && a.tokens > 0 && a.positions == 0) return Bad("positions: null");
+  KVX_RETURN_IF_ERROR(CheckRotation(&ranges, a.rotary_dim, a.head_dim, a.inv_freq, a.positions,
+                                    a.positions_64 != 0, a.tokens));
+  KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.q_weight, a.weight_dtype, a.dtype, a.head_dim, a.eps,
+                                  "q_weight"));
+  KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.k_weight, a.weight_dtype, a.dtype, a.head_dim, a.eps,
+                                  "k_weight"));
+  const auto rows = [](const Rows& in, const Rows& o, uint64_t weight) {
+    HeadRows r;
+    r.in = reinterpret_cast<const void*>(in.at);
+    r.out = reinterpret_cast<void*>(o.at);
+    r.weight = reinterpret_cast<const void*>(weight);
+    r.in_token = in.token_stride;
+    r.in_head = in.head_stride;
+    r.out_token = o.token_stride;
+    r.out_head = o.head_stride;
+    r.heads = static_cast<int32_t>(in.heads);
+    return r;
+  };
+  *out = NormRopeLaunch{};
+  out->q = rows(q, qo, a.q_weight);
+  out->k = rows(k, ko, a.k_weight);
+  out->positions = reinterpret_cast<const void*>(a.positions);
+  out->inv_freq = reinterpret_cast<const float*>(a.inv_freq);
+  out->tokens = a.q_heads + a.k_heads > 0 ? static_cast<int32_t>(a.tokens) : 0;
+  out->head_dim = a.head_dim;
+  out->rotary_dim = a.rotary_dim;
+  out->type = a.dtype;
+  out->weight_f32 = a.weight_dtype == kF32;
+  out->positions_64 = a.positions_64 != 0;
+  out->interleaved = a.interleaved != 0;
+  out->eps = a.eps;
+  return OkStatus();
+}
+
+Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, AppendLaunch* out) {
+  Cache cache;
+  KVX_RETURN_IF_ERROR(FindCache(pool, a.cache, a.dtype, &cache));
+  const kvx_paged_cache& c = a.cache;
+  KVX_RETURN_IF_ERROR(CheckTokens(a.tokens, c.heads, c.head_dim));
+  DeviceRangeChecker ranges(pool.device);
+  const Rows k = {a.k, a.k_token_stride, a.k_head_stride, a.tokens, c.heads, c.head_dim, 2};
+  const Rows v = {a.v, a.v_token_stride, a.v_head_stride, a.tokens, c.heads, c.head_dim, 2};
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, k, "k"));
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, v, "v"));
+  for (const Rows* r : {&k, &v}) {
+    uint64_t bytes = 0;
+    if (r->empty() || !r->Extent(&bytes)) continue;
+    for (const PoolStorage* s : {&cache.k, &cache.v}) {
+      if (Meet(r->at, bytes, s->base, static_cast<uint64_t>(s->bytes))) {
+        return Bad(std::string(r == &k ? "k" : "v") + ": overlaps the cache");
+      }
+    }
+  }
+  *out = AppendLaunch{};
+  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
+                                 &out->batch));
+  KVX_RETURN_IF_ERROR(CheckRotation(&ranges, a.rotary_dim, c.head_dim, a.inv_freq, a.positions,
+                                    a.positions_64 != 0, a.tokens));
+  KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.k_weight, a.weight_dtype, a.dtype, c.head_dim, a.eps,
+                                  "k_weight"));
+  if (a.batch.sequences == 0 || cache.num_blocks == 0) out->batch.tokens = 0;
+  out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
+  out->k = reinterpret_cast<const void*>(a.k);
+  out->v = reinterpret_cast<const void*>(a.v);
+  out->k_token = a.k_token_stride;
+  out->k_head = a.k_head_stride;
+  out->v_token = a.v_token_stride;
+  out->v_head = a.v_head_stride;
+  out->k_pool = reinterpret_cast<void*>(cache.k.base);
+  out->v_pool = reinterpret_cast<void*>(cache.v.base);
+  out->k_scales = reinterpret_cast<float*>(cache.k_scales);
+  out->v_scales = reinterpret_cast<float*>(cache.v_scales);
+  out->k_weight = reinterpret_cast<const void*>(a.k_weight);
+  out->positions = reinterpret_cast<const void*>(a.positions);
+  out->inv_freq = reinterpret_cast<const float*>(a.inv_freq);
+  out->heads = c.heads;
+  out->head_dim = c.head_dim;
+  out->rotary_dim = a.rotary_dim;
+  out->type = a.dtype;
+  out->e4m3 = c.dtype == kE4m3;
+  out->weight_f32 = a.weight_dtype == kF32;
+  out->positions_64 = a.positions_64 != 0;
+  out->interleaved = a.interleaved != 0;
+  out->eps = a.eps;
+  return OkStatus();
+}
+
+Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunch* out,
+                   int64_t* workspace_bytes) {
+  Cache cache;
+  KVX_RETURN_IF_ERROR(FindCache(pool, a.cache, a.dtype, &cache));
+  const kvx_paged_cache& c = a.cache;
+  KVX_RETURN_IF_ERROR(CheckTokens(a.tokens, a.q_heads, c.head_dim));
+  if (c.head_dim % 8 != 0) return Bad("head_dim must be a multiple of 8");
+  if (a.q_heads < 1 || a.q_heads % c.heads != 0) {
+    return Bad("q_heads must be a multiple of the cache's heads");
+  }
+  if (!std::isfinite(a.scale) || a.scale <= 0) return Bad("scale must be finite and positive");
+  if (a.groups < 0 || a.groups > kMaxGroups) return Bad("groups must be 0..256");
+  DeviceRangeChecker ranges(pool.device);
+  const Rows q = {a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.q_heads, c.head_dim, 2};
+  const Rows o = {a.out, a.out_token_stride, a.out_head_stride, a.tokens, a.q_heads, c.head_dim,
+                  2};
+  *out = AttendLaunch{};
+  if (workspace_bytes == nullptr) {
+    KVX_RETURN_IF_ERROR(CheckRows(&ranges, q, "q"));
+    KVX_RETURN_IF_ERROR(CheckRows(&ranges, o, "out"));
+    KVX_RETURN_IF_ERROR(CheckInPlace(q, o, "q", "out"));
+    KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
+                                   &out->batch));
+    if (a.groups > 0 && a.batch.sequences > 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.group_starts, a.groups + 1, "group_starts"));
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.prefix_lengths, a.groups, "prefix_lengths"));
+    }
+    if (a.lse != 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
+      uint64_t bytes = 0;
+      if (!o.empty() && o.Extent(&bytes) &&
+          Meet(a.lse, static_cast<uint64_t>(a.tokens * a.q_heads) * 4, a.out, bytes)) {
+        return Bad("lse: overlaps out");
+      }
+    }
+  } else {
+    // Sizes only: the address arguments may still be unset.
+    if (a.batch.sequences < 0 || a.batch.sequences > kMaxSequences) {
+      return Bad("sequences must be 0..4096");
+    }
+    if (a.batch.table_width < 0 || a.batch.table_width > kMostTokens / c.block_tokens) {
+      return Bad("table_width * block_tokens must be at most 2^30");
+    }
+    out->batch.starts = reinterpret_cast<const int32_t*>(a.batch.starts);
+    out->batch.sequences = static_cast<int32_t>(a.batch.sequences);
+    out->batch.tokens = static_cast<int32_t>(a.tokens);
+    out->batch.capacity = static_cast<int32_t>(a.batch.table_width * c.block_tokens);
+  }
+  const int64_t G = a.q_heads / c.heads;
+  const int64_t tiles = a.tokens * G / kManyRows + a.batch.sequences + a.groups;
+  const int64_t steps = out->batch.capacity / kManyStep + 1;
+  if (tiles > INT32_MAX / c.heads / steps) {
+    return Bad("tokens * table_width is too large for one call");
+  }
+  if (a.batch.sequences == 0) out->batch.tokens = 0;
+  out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
+  out->group_div = MakeFastDivU32(static_cast<uint32_t>(G));
+  out->q = reinterpret_cast<const void*>(a.q);
+  out->out = reinterpret_cast<void*>(a.out);
+  out->lse = reinterpret_cast<float*>(a.lse);
+  out->q_token = a.q_token_stride;
+  out->q_head = a.q_head_stride;
+  out->out_token = a.out_token_stride;
+  out->out_head = a.out_head_stride;
+  out->k_pool = reinterpret_cast<const void*>(cache.k.base);
+  out->v_pool = reinterpret_cast<const void*>(cache.v.base);
+  out->k_scales = reinterpret_cast<const float*>(cache.k_scales);
+  out->v_scales = reinterpret_cast<const float*>(cache.v_scales);
+  out->group_starts = reinterpret_cast<const int32_t*>(a.group_starts);
+  out->prefix_lengths = reinterpret_cast<const int32_t*>(a.prefix_lengths);
+  out->groups = a.groups;
+  out->q_heads = a.q_heads;
+  out->k_heads = c.heads;
+  out->head_dim = c.head_dim;
+  out->type = a.dtype;
+  out->e4m3 = c.dtype == kE4m3;
+  out->causal = a.non_causal == 0;
+  out->scale = a.scale;
+  const int64_t need = out->batch.tokens == 0 ? 0 : PlanAttend(out);
+  if (workspace_bytes != nullptr) {
+    *workspace_bytes = need;
+    return OkStatus();
+  }
+  if (need > 0) {
+    if (a.workspace_bytes < need) {
+      return Bad("workspace: " + std::to_string(need) + " bytes are needed");
+    }
+    if (a.workspace % 16 != 0) return Bad("workspace: must be aligned to 16 bytes");
+    KVX_RETURN_IF_ERROR(ranges.Check(a.workspace, static_cast<uint64_t>(need), "workspace"));
+    out->parts = reinterpret_cast<float*>(a.workspace);
+  }
+  return OkStatus();
+}
+
+}  // namespace kvx

@@ -1,0 +1,394 @@
+// New keys and values into the paged pool.
+//
+// Token i of sequence s sits at position p = lengths[s] - count[s] + i, slot
+// p % B of block tables[s][p / B]. A key is normed and rotated on the way
+// (head_row.h); a value is copied. A token whose position or block id has no
+// place is dropped.
+//
+// Pool of the inputs' type (append_kv_kernel): a workgroup takes a few tokens,
+// finds their sequences (all lengths at once, one a lane), puts places and
+// (cos, sin) into LDS and walks the tokens' key rows and value rows.
+//
+// e4m3 pool (append_e4m3_kernel): one fp32 scale per (block, head), so all
+// rows of a block and head have to be seen before the first is written. A
+// workgroup takes the new rows of one block, K or V, a wave the heads in turn:
+//   amax = max |x| over the finite new values
+//   new  = max(old, amax / 448),  old = 0 where no earlier token is in the block
+//   q    = e4m3(clamp(x / new, -448, 448)),
+// first reading the rows for amax, then again (from the cache) to store them.
+// Earlier tokens of the block are stored again at old / new where new is
+// larger, so they keep their values within e4m3's rounding. Nothing is
+// accumulated over blocks or waves: the same call gives the same bytes.
+#include <hip/hip_runtime.h>
+
+#include "append_kv.h"
+#include "head_row.h"
+
+namespace kvx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxTokens = 16;  // of one workgroup, or of a pass over a block
+
+__device__ __forceinline__ int FastDiv(const FastDivU32& f, int n) {
+  const uint32_t u = static_cast<uint32_t>(n);
+  return static_cast<int>((__umulhi(u, f.m) + u) >> f.s);
+}
+
+__device__ __forceinline__ int64_t RotationPosition(const AppendLaunch& a, int64_t token,
+                                                    int place) {
+  if (a.positions == nullptr) return place;
+  return a.positions_64 ? static_cast<const int64_t*>(a.positions)[token]
+                        : static_cast<const int32_t*>(a.positions)[token];
+}
+
+template <class E, int VEC, int LPR>
+__global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch a,
+                                                             const int tokens_each) {
+  extern __shared__ f32x2 cs[];  // [tokens_each][rotary_dim / 2]
+  __shared__ int sequence[kMaxTokens], place[kMaxTokens];
+  __shared__ int64_t row_at[kMaxTokens];  // first element of the token's rows, or -1
+  using Scalar = typename E::Scalar;
+  constexpr int kRows = kThreads / LPR;
+  const int pairs = a.rotary_dim / 2;
+  const int t0 = blockIdx.x * tokens_each;
+  const int nt = min(tokens_each, a.batch.tokens - t0);
+  // Rows of the workgroup: the tokens' keys, then their values, shared out
+  // over gridDim.y workgroups.
+  const int rows = nt * a.heads, step = kRows * gridDim.y;
+  int r = blockIdx.y * kRows + threadIdx.x / LPR;
+  const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
+  Row<E, VEC, LPR> row;
+  int t = 0, h = 0;
+  const auto load = [&]() {
+    const int i = r < rows ? r : r - rows;
+    t = i / a.heads;
+    h = i - t * a.heads;
+    const int64_t token = t0 + t;
+    row.Load(lane, r < rows ? static_cast<const Scalar*>(a.k) + token * a.k_token + h * a.k_head
+                            : static_cast<const Scalar*>(a.v) + token * a.v_token + h * a.v_head);
+  };
+  if (r < 2 * rows) load();  // in flight while the places are found
+  float w[lane.kChunks][VEC], wo[lane.kChunks][VEC];
+  LoadWeights(lane, a.k_weight, a.weight_f32, w, wo);
+
+  if (threadIdx.x < kMaxTokens) sequence[threadIdx.x] = -1;
+  __syncthreads();
+  if (a.batch.starts == nullptr) {
+    if (threadIdx.x < nt) {
+      const int s = t0 + threadIdx.x;
+      const SequenceSpan q = LoadSequence(a.batch, s);
+      sequence[threadIdx.x] = s;
+      place[threadIdx.x] = q.length - 1;
+    }
+  } else {
+    for (int s = threadIdx.x; s < a.batch.sequences; s += kThreads) {
+      const SequenceSpan q = LoadSequence(a.batch, s);
+      const int end = min(q.first + q.count, t0 + nt);
+      for (int i = max(q.first, t0); i < end; ++i) {
+        sequence[i - t0] = s;
+        place[i - t0] = q.length - q.count + (i - q.first);
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < nt) {
+    const int s = sequence[threadIdx.x], p = place[threadIdx.x];
+    int64_t at = -1;
+    if (s >= 0 && p >= 0 && p < a.batch.capacity) {
+      const int b = FastDiv(a.block_div, p);
+      const int id = a.batch.tables[s * a.batch.table_stride + b];
+      if (id >= 0 && id < a.batch.num_blocks) {
+        at = (static_cast<int64_t>(id) * a.batch.block_tokens + (p - b * a.batch.block_tokens)) *
+             a.heads * a.head_dim;
+      }
+    }
+    row_at[threadIdx.x] = at;
+  }
+  for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
+    const int ti = i / pairs;
+    if (sequence[ti] >= 0) {
+      cs[i] = Turn(RotationPosition(a, t0 + ti, place[ti]), a.inv_freq[i - ti * pairs]);
+    }
+  }
+  __syncthreads();
+  while (r < 2 * rows) {
+    const int64_t at = row_at[t];
+    const bool key = r < rows;
+    if (key) {
+      if (a.k_weight != nullptr) row.Norm(lane, w, wo, a.eps);
+      row.Rotate(lane, cs + t * pairs);
+    }
+    if (at >= 0) {
+      row.Store(lane, static_cast<Scalar*>(key ? a.k_pool : a.v_pool) + at + h * a.head_dim);
+    }
+    r += step;
+    if (r < 2 * rows) load();
+  }
+}
+
+// The new rows of one block.
+struct BlockRows {
+  int id;      // the block
+  int token;   // first new token in it
+  int count;   // new tokens in it
+  int place;   // position of the first
+  int slot;    // its slot: the block holds as many earlier tokens
+};
+
+template <class E, int VEC, int LPR>
+struct E4m3Row {
+  using Lane = RowLane<E, VEC, LPR>;
+  static __device__ __forceinline__ float Quantised(float x, float inverse) {
+    const float y = x * inverse;
+    return y > kE4m3Max ? kE4m3Max : y < -kE4m3Max ? -kE4m3Max : y;  // a NaN stays one
+  }
+  static __device__ __forceinline__ void Store(uint8_t* p, const float* y) {
+    if constexpr (VEC == 8) {
+      u32x2 w = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        int q = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j], y[4 * j + 1], 0, false);
+        q = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * j + 2], y[4 * j + 3], q, true);
+        w[j] = static_cast<uint32_t>(q);
+      }
+      *reinterpret_cast<u32x2*>(p) = w;
+    } else {
+      *p = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[0], 0, false));
+    }
+  }
+  static __device__ __forceinline__ void Load(const uint8_t* p, float* y) {
+    if constexpr (VEC == 8) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), true);
+        y[4 * j] = lo[0];
+        y[4 * j + 1] = lo[1];
+        y[4 * j + 2] = hi[0];
+        y[4 * j + 3] = hi[1];
+      }
+    } else {
+      y[0] = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(*p), false)[0];
+    }
+  }
+};
+
+template <class E, int VEC, int LPR>
+__global__ __launch_bounds__(kThreads) void append_e4m3_kernel(const AppendLaunch a) {
+  extern __shared__ f32x2 cs[];  // [kMaxTokens][rotary_dim / 2], then amax [heads]
+  __shared__ int counted[kThreads / 64];
+  __shared__ BlockRows found;
+  using Scalar = typename E::Scalar;
+  using Q = E4m3Row<E, VEC, LPR>;
+  constexpr int kWaveRows = 64 / LPR;
+  const int pairs = a.rotary_dim / 2;
+  float* amax = reinterpret_cast<float*>(cs + kMaxTokens * pairs);
+  const BatchView& b = a.batch;
+  const int wave = threadIdx.x / 64, in_wave = threadIdx.x % 64;
+
+  // The block: the blockIdx.x-th of those that the sequences touch, in order.
+  if (threadIdx.x == 0) found.id = -1;
+  const auto touched = [&](const SequenceSpan& q, int& lo, int& hi) {
+    lo = max(q.length - q.count, 0);
+    hi = min(q.length, b.capacity);
+    if (q.count == 0 || hi <= lo) return 0;
+    return FastDiv(a.block_div, hi - 1) - FastDiv(a.block_div, lo) + 1;
+  };
+  int before = 0;  // blocks of the sequences before this thread's
+  const int each = (b.sequences + kThreads - 1) / kThreads;
+  const int s0 = threadIdx.x * each, s1 = min(s0 + each, b.sequences);
+  if (b.starts != nullptr) {
+    int mine = 0, lo, hi;
+    for (int s = s0; s < s1; ++s) mine += touched(LoadSequence(b, s), lo, hi);
+    int sum = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const int o = __shfl_up(sum, m);
+      if (in_wave >= m) sum += o;
+    }
+    if (in_wave == 63) counted[wave] = sum;
+    __syncthreads();
+    before = sum - mine;
+    for (int w = 0; w < wave; ++w) before += counted[w];
+  } else {
+    before = s0;  // one token, so one block, a sequence
+    __syncthreads();
+  }
+  for (int s = s0; s < s1; ++s) {
+    if (b.starts == nullptr && s != static_cast<int>(blockIdx.x)) continue;
+    int lo, hi;
+    const SequenceSpan q = LoadSequence(b, s);
+    const int n = touched(q, lo, hi), j = static_cast<int>(blockIdx.x) - (b.starts ? before : s);
+    if (j >= 0 && j < n) {
+      const int at = FastDiv(a.block_div, lo) + j, from = at * b.block_tokens;
+      found.place = max(lo, from);
+      found.slot = found.place - from;
+      found.count = min(hi, from + b.block_tokens) - found.place;
+      found.token = q.first + found.place - (q.length - q.count);
+      const int id = b.tables[s * b.table_stride + at];
+      found.id = id < b.num_blocks ? id : -1;
+    }
+    before += n;
+  }
+  for (int h = threadIdx.x; h < a.heads; h += kThreads) amax[h] = 0.0f;
+  __syncthreads();
+  const BlockRows rows = found;
+  if (rows.id < 0) return;
+
+  const bool key = blockIdx.y == 0;
+  const Scalar* in = static_cast<const Scalar*>(key ? a.k : a.v);
+  const int64_t token_stride = key ? a.k_token : a.v_token;
+  const int64_t head_stride = key ? a.k_head : a.v_head;
+  const int64_t slot_bytes = static_cast<int64_t>(a.heads) * a.head_dim;
+  uint8_t* block = static_cast<uint8_t*>(key ? a.k_pool : a.v_pool) +
+                   rows.id * (slot_bytes * b.block_tokens);
+  float* scales = (key ? a.k_scales : a.v_scales) + static_cast<int64_t>(rows.id) * a.heads;
+  const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
+  Row<E, VEC, LPR> row;
+  float w[lane.kChunks][VEC], wo[lane.kChunks][VEC];
+  LoadWeights(lane, key ? a.k_weight : nullptr, a.weight_f32, w, wo);
+  const int heads_step = kWaves * gridDim.z;
+
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int c0 = 0; c0 < rows.count; c0 += kMaxTokens) {
+      const int nc = min(kMaxTokens, rows.count - c0);
+      if (key && (pass == 0 || rows.count > kMaxTokens)) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < nc * pairs; i += kThreads) {
+          const int ti = i / pairs;
+          cs[i] = Turn(RotationPosition(a, rows.token + c0 + ti, rows.place + c0 + ti),
+                       a.inv_freq[i - ti * pairs]);
+        }
+        __syncthreads();
+      }
+      for (int h = blockIdx.z * kWaves + wave; h < a.heads; h += heads_step) {
+        float scale = 0.0f, inverse = 0.0f;
+        if (pass == 1) {
+          float old = rows.slot > 0 ? scales[h] : 0.0f;
+          old = old > 0.0f ? old : 0.0f;
+          // After the first rows the table holds the new scale already.
+          scale = c0 == 0 ? fmaxf(old, amax[h] / kE4m3Max) : amax[h];
+          inverse = scale > 0.0f ? fminf(1.0f / scale, 3.0e38f) : 0.0f;
+          if (c0 == 0) {
+            if (scale > old && rows.slot > 0) {
+              const float ratio = old / scale;
+              for (int i = in_wave / LPR; i < rows.slot; i += kWaveRows) {
+                uint8_t* p = block + i * slot_bytes + h * a.head_dim;
+#pragma unroll
+                for (int n = 0; n < lane.kChunks; ++n) {
+                  if (!lane.Has(n)) continue;
+                  float y[VEC];
+                  Q::Load(p + lane.Dim(n), y);
+#pragma unroll
+                  for (int j = 0; j < VEC; ++j) y[j] *= ratio;
+                  Q::Store(p + lane.Dim(n), y);
+                }
+              }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (in_wave == 0) {
+              scales[h] = scale;
+              amax[h] = scale;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
+        float largest = 0.0f;
+        // Every lane takes part in the rows' sums, so all make the same steps.
+        for (int i0 = 0; i0 < nc; i0 += kWaveRows) {
+          const int i = min(i0 + in_wave / LPR, nc - 1);
+          row.Load(lane, in + (rows.token + c0 + i) * token_stride + h * head_stride);
+          if (key) {
+            if (a.k_weight != nullptr) row.Norm(lane, w, wo, a.eps);
+            row.Rotate(lane, cs + i * pairs);
+          }
+          if (pass == 0) {
+#pragma unroll
+            for (int n = 0; n < lane.kChunks; ++n) {
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) {
+                const float x = fabsf(row.x[n][j]);
+                largest = fmaxf(largest, x < __builtin_inff() ? x : 0.0f);
+              }
+            }
+          } else {
+            uint8_t* p = block + (rows.slot + c0 + i) * slot_bytes + h * a.head_dim;
+#pragma unroll
+            for (int n = 0; n < lane.kChunks; ++n) {
+              if (!lane.Has(n)) continue;
+              float y[VEC];
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) y[j] = Q::Quantised(row.x[n][j], inverse);
+              Q::Store(p + lane.Dim(n), y);
+            }
+          }
+        }
+        if (pass == 0) {
+#pragma unroll
+          for (int m = 32; m > 0; m /= 2) largest = fmaxf(largest, __shfl_xor(largest, m));
+          if (in_wave == 0) amax[h] = fmaxf(amax[h], largest);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+      }
+    }
+  }
+}
+
+template <class E, int VEC, int LPR>
+hipError_t Launch(const AppendLaunch& l, hipStream_t stream) {
+  const size_t pairs = static_cast<size_t>(l.rotary_dim / 2) * sizeof(f32x2);
+  const int tokens = l.batch.tokens;
+  if (l.e4m3) {
+    // A block for every one that the tokens can touch: whole ones, and a first
+    // and a last part of each sequence.
+    const int64_t blocks =
+        l.batch.starts == nullptr
+            ? l.batch.sequences
+            : std::min<int64_t>(tokens, tokens / l.batch.block_tokens +
+                                            2 * static_cast<int64_t>(l.batch.sequences));
+    // Few blocks: their heads spread over workgroups.
+    int split = 1;
+    while (split * kWaves < l.heads && blocks * 2 * split < 512) ++split;
+    const dim3 grid(static_cast<unsigned>(blocks), 2, split);
+    const size_t lds = kMaxTokens * pairs + static_cast<size_t>(l.heads) * sizeof(float);
+    hipLaunchKernelGGL((append_e4m3_kernel<E, VEC, LPR>), grid, dim3(kThreads), lds, stream, l);
+    return hipGetLastError();
+  }
+  constexpr int kRows = kThreads / LPR;
+  int each = 1, split = 1;
+  if (tokens > 1024) {
+    while (each < kMaxTokens && each * l.heads < 64) each *= 2;
+  } else {
+    const int groups = (2 * l.heads + kRows - 1) / kRows;
+    while (split < groups && tokens * split < 512) ++split;
+  }
+  const dim3 grid((tokens + each - 1) / each, split);
+  hipLaunchKernelGGL((append_kv_kernel<E, VEC, LPR>), grid, dim3(kThreads), each * pairs, stream,
+                     l, each);
+  return hipGetLastError();
+}
+
+template <class E>
+hipError_t Pick(const AppendLaunch& l, hipStream_t stream) {
+  const auto at = [](const void* p) { return reinterpret_cast<uint64_t>(p); };
+  if ((at(l.k) | at(l.v)) % 16 == 0 && (at(l.k_pool) | at(l.v_pool)) % 16 == 0 &&
+      (l.k_token | l.k_head | l.v_token | l.v_head) % 8 == 0 &&
+      ChunksFit(8, l.head_dim, l.rotary_dim, l.interleaved)) {
+    const int chunks = l.head_dim / 8;
+    if (chunks <= 8) return Launch<E, 8, 8>(l, stream);
+    if (chunks <= 16) return Launch<E, 8, 16>(l, stream);
+    return Launch<E, 8, 32>(l, stream);
+  }
+  return Launch<E, 1, 64>(l, stream);
+}
+
+}  // namespace
+
+hipError_t LaunchAppendKv(const AppendLaunch& l, hipStream_t stream) {
+  return l.type == kBf16 ? Pick<Bf16>(l, stream) : Pick<F16>(l, stream);
+}
+
+}  // namespace kvx

@@ -482,6 +482,72 @@ class KVCacheManager:
         return self._device_copy(_capi.load().kvx_manager_scatter, "KVCacheManager scatter",
                                  block_ids, staging, order, layer_idx, shard_idx, stream)
 
+    # -- a step's work on the pool -------------------------------------------
+    def append_kv(self, k_layer: int, v_layer: int, k, v, tables, lengths, *, starts=None,
+                  inv_freq=None, positions=None, k_weight=None, eps: float = 1e-6,
+                  interleaved: bool = False, shard_idx: int = 0, stream=None) -> None:
+        """Stores a step's keys and values into their blocks (one kernel).
+
+        The storages k_layer and v_layer must be [blocks, tokens, heads,
+        head_dim] tensors of k's type, or float8_e4m3fn with one scale table
+        [blocks, heads] a KV storage (scale_tables, in the storages' order).
+
+        Args:
+          k, v: [tokens, heads, head_dim], bf16 or fp16, last dimension
+            contiguous.
+          tables: int32 [sequences, blocks] block ids; token p of sequence s is
+            in slot p % tokens_a_block of block tables[s, p // tokens_a_block].
+          lengths: int32 [sequences], tokens of each sequence with the new
+            ones, which are its last.
+          starts: int32 [sequences + 1]: sequence s owns the tokens [starts[s],
+            starts[s + 1]); None: one token a sequence. Tokens behind the last
+            sequence are not stored.
+          inv_freq: rotate keys (see ``norm_rope``), at their place in the
+            sequence or at ``positions`` [tokens].
+          k_weight: RMS norm of each key head before that.
+        The contents of tables, lengths and starts are read on the device: a
+        token past its table or with a block id outside the pool is dropped. A
+        block that takes tokens must belong to one sequence of the call. In a
+        float8 storage the scale of a (block, head) grows with its largest
+        value, and earlier tokens of the block are stored again under it.
+        """
+        from . import paged_attention
+        paged_attention.append_kv(self, k_layer, v_layer, k, v, tables, lengths, starts=starts,
+                                  inv_freq=inv_freq, positions=positions, k_weight=k_weight,
+                                  eps=eps, interleaved=interleaved, shard_idx=shard_idx,
+                                  stream=stream)
+
+    def attend(self, k_layer: int, v_layer: int, q, tables, lengths, *, starts=None,
+               group_starts=None, prefix_lengths=None, scale: Optional[float] = None,
+               causal: bool = True, out=None, return_lse: bool = False, shard_idx: int = 0,
+               stream=None):
+        """Attention of ``q`` [tokens, q_heads, head_dim] over the cached tokens
+        of each sequence, from one query a sequence to long chunks.
+
+        tables, lengths, starts and the storages are those of ``append_kv``
+        (append a step's tokens first); q_heads is a multiple of the storages'
+        heads, head_dim a multiple of 8. A query at position p sees positions
+        0..p, or with causal=False the whole sequence. One that sees nothing
+        gets zeros and an lse of -inf; rows behind the last sequence are left
+        as they are (undefined in a new tensor).
+
+        Args:
+          group_starts, prefix_lengths: int32 [groups + 1] and [groups]:
+            sequences [group_starts[g], group_starts[g + 1]) hold their first
+            prefix_lengths[g] tokens in the same blocks (those in the first
+            one's table), which are then read once for all of them. The result
+            is the same as without.
+          scale: of the scores, positive; default head_dim ** -0.5.
+          out: result; q itself, or apart from it.
+          return_lse: also return the log of each row's sum of exponentials,
+            float32 [tokens, q_heads].
+        """
+        from . import paged_attention
+        return paged_attention.attend(self, k_layer, v_layer, q, tables, lengths, starts=starts,
+                                      group_starts=group_starts, prefix_lengths=prefix_lengths,
+                                      scale=scale, causal=causal, out=out, return_lse=return_lse,
+                                      shard_idx=shard_idx, stream=stream)
+
     # -- staging slots and host blocks --------------------------------------
     def configure_host_staging_slots(self, num_slots: int, max_major_per_slot: int) -> None:
         _capi.check(_capi.load().kvx_manager_configure_host_staging_slots(
