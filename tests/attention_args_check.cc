@@ -304,11 +304,11 @@ void AttendArgs() {
                 static_cast<long long>(bare));
     ++failures;
   }
-  a.batch.table_width = 8;
+  a.batch.table_width = 2;  // 32 tokens
   a.batch.starts = 0;
   a.tokens = 3;
   Passes(kvx::CheckAttend(Pool(), a, &l, &bytes), "attend: one step");
-  if (bytes != 0 || l.join) {
+  if (bytes != 0 || l.join_grid != 0) {
     std::printf("FAIL attend: one step needs %lld bytes\n", static_cast<long long>(bytes));
     ++failures;
   }

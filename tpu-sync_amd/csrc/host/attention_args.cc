@@ -220,6 +220,7 @@ Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type,
     return Bad("cache storages: unaligned address");
   }
   if (out->k.base == out->v.base) return Bad("keys and values need storages of their own");
+  if (blocks < 1) return Bad("the cache has no blocks");
   out->num_blocks = std::min<int64_t>(blocks, INT32_MAX);
   return OkStatus();
 }
@@ -310,7 +311,7 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
                                     a.positions_64 != 0, a.tokens));
   KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.k_weight, a.weight_dtype, a.dtype, c.head_dim, a.eps,
                                   "k_weight"));
-  if (a.batch.sequences == 0 || cache.num_blocks == 0) out->batch.tokens = 0;
+  if (a.batch.sequences == 0) out->batch.tokens = 0;
   out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
   out->k = reinterpret_cast<const void*>(a.k);
   out->v = reinterpret_cast<const void*>(a.v);
@@ -386,9 +387,11 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
     out->batch.capacity = static_cast<int32_t>(a.batch.table_width * c.block_tokens);
   }
   const int64_t G = a.q_heads / c.heads;
-  const int64_t tiles = a.tokens * G / kManyRows + a.batch.sequences + a.groups;
-  const int64_t steps = out->batch.capacity / kManyStep + 1;
-  if (tiles > INT32_MAX / c.heads / steps) {
+  // Work is counted in 32 bits: tiles by steps of 64 tokens, sequences by steps
+  // of 32, each for every key head, and squares of tiles.
+  const int64_t tiles = 2 * (a.tokens * G / kManyRows + 1) + a.batch.sequences + a.groups;
+  const int64_t steps = out->batch.capacity / kManyStep + 3 + a.tokens / kManyStep;
+  if (tiles > 65536 || tiles > INT32_MAX / 2 / c.heads / steps) {
     return Bad("tokens * table_width is too large for one call");
   }
   if (a.batch.sequences == 0) out->batch.tokens = 0;

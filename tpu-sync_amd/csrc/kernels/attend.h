@@ -5,9 +5,9 @@
 // count + i sees tokens 0..p of its sequence (causal) or all of them.
 //
 // Kernels.
-//  * attend_few: sequences of up to kFewRows rows a key head (single tokens, a
-//    few drafted ones). One wave holds all their rows; the key axis is split.
-//  * attend_many: longer runs of queries, in tiles of kManyRows rows, and the
+//  * attend_few: every sequence has up to kFewRows rows a key head (single
+//    tokens, a few drafted ones). One wave holds them; the key axis is split.
+//  * attend_mixed: longer runs of queries too, in tiles of kManyRows rows, and
 //    shared prefixes: all rows of a group's sequences against the prefix.
 //  * attend_join: merges the parts of rows that were split.
 //
@@ -27,7 +27,7 @@
 namespace kvx {
 
 constexpr int kFewRows = 32;
-constexpr int kFewStep = 128;   // tokens of one step of a workgroup
+constexpr int kFewStep = 32;    // tokens of one step of a wave
 constexpr int kManyRows = 128;  // rows of one tile
 constexpr int kManyStep = 64;   // tokens of one step
 constexpr int kMaxSequences = 4096;
@@ -56,20 +56,18 @@ struct AttendLaunch {
   bool e4m3 = false;
   bool causal = true;
   float scale = 1.0f;
-  // Parts of split rows, each row padded_dim floats relative to its maximum:
-  // two slots of few_rows rows a workgroup of attend_few, many_parts slots of
-  // kManyRows rows, and with groups a row for every (token, head), for what
-  // attend_few did not cut; then the (maximum in powers of two, sum) of each.
+  // Parts of split rows, part_rows rows of padded_dim floats relative to their
+  // maximum; then the (maximum in powers of two, sum) of each; then the plan
+  // that attend_join reads (attend_plan.h).
   float* parts = nullptr;
   // Filled by PlanAttend.
   int32_t padded_dim = 0;
-  int32_t few_grid = 0;    // workgroups of attend_few, 0: not launched
-  int32_t few_rows = 0;    // rows of its slots (16 or 32)
-  int32_t many_grid = 0;   // workgroups of attend_many, 0: not launched
-  int32_t many_target = 0; // items that attend_many is split into where rows are few
-  int32_t many_parts = 0;
+  int32_t few_grid = 0;   // workgroups for few rows
+  int32_t few_rows = 0;   // most rows of such a sequence
+  int32_t many_grid = 0;  // workgroups for many rows and groups, 0: attend_few alone
   int64_t part_rows = 0;
-  bool join = false;
+  int32_t join_grid = 0;  // workgroups of attend_join, 0: no row can be split
+  int32_t join_rows = 0;  // rows that one of them joins at once
 };
 
 // Sizes of the launches of a call (from its shapes only). Returns the bytes of
@@ -81,7 +79,7 @@ hipError_t LaunchAttend(const AttendLaunch& l, hipStream_t stream);
 
 // The parts, by translation unit.
 hipError_t LaunchAttendFew(const AttendLaunch& l, hipStream_t stream);
-hipError_t LaunchAttendMany(const AttendLaunch& l, hipStream_t stream);
+hipError_t LaunchAttendMixed(const AttendLaunch& l, hipStream_t stream);
 hipError_t LaunchAttendJoin(const AttendLaunch& l, hipStream_t stream);
 
 }  // namespace kvx

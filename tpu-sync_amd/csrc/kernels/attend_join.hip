@@ -1,11 +1,14 @@
 // Joins the parts of attention rows whose keys were split, or read with a
 // group's: with (m, l, o) of each part, o relative to its maximum m,
 //   M = max m,  out = sum o e^{m - M} / sum l e^{m - M},  lse = M + log sum l e^{m - M}.
-// A workgroup takes a row at a time, a part to every head_dim / 4 threads, so
-// a row of many parts (one long sequence) is read at once; parts are merged in
-// a fixed order. Rows that attend_few or attend_many finished are not visited.
-#include "attend_plan.h"
+// The cuts are found from the plan that the kernel before this one left: a row's
+// keys were cut where a worker's part starts inside them. A workgroup takes
+// join_rows rows of one sequence and key head at a time, a part to every head_dim
+// / 4 threads, so a row of many parts (one long sequence) is read at once; parts
+// are merged in a fixed order. Rows that were finished are not visited.
+#include <algorithm>
 
+#include "attend_plan.h"
 namespace kvx {
 namespace {
 
@@ -31,100 +34,104 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
   using Scalar = typename E::Scalar;
   const BatchView& b = a.batch;
   const int S = b.sequences, units = a.groups + S, G = a.q_heads / a.k_heads;
-  int* few = reinterpret_cast<int*>(lds);  // [sequences] steps of attend_few
-  int* many = few + S;                     // [groups + sequences] items of attend_many
-  int* todo = many + units;                // [sequences] rows to join
+  int* words = reinterpret_cast<int*>(lds);
   const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const auto unit_of = [&](int i) {
-    return i < a.groups ? LoadGroup(a, i) : LoadManySequence(LoadOwnKeys(a, i - a.groups));
-  };
-  int few_all = 0;
-  if (a.few_grid > 0) {
-    for (int s = threadIdx.x; s < S; s += kAttendThreads) few[s] = FewSteps(LoadOwnKeys(a, s));
-    BlockSums(few, S);
-    few_all = one(few[S - 1]);
-  }
-  int each = 0;
-  if (a.many_grid > 0) {
-    for (int i = threadIdx.x; i < units; i += kAttendThreads) many[i] = ManyTiles(unit_of(i));
-    BlockSums(many, units);
-    const int tiles = one(many[units - 1]) * a.k_heads;
-    if (tiles > 0 && tiles < a.many_target) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < units; i += kAttendThreads) {
-        const ManyUnit u = unit_of(i);
-        many[i] = ManyTiles(u) * ManySteps(u);
-      }
-      BlockSums(many, units);
-      each = ManyEach(a, tiles, static_cast<int64_t>(one(many[units - 1])) * a.k_heads);
-      __syncthreads();
-      for (int i = threadIdx.x; i < units; i += kAttendThreads) {
-        const ManyUnit u = unit_of(i);
-        many[i] = ManyTiles(u) * ManyParts(ManySteps(u), each);
-      }
-      BlockSums(many, units);
-    }
-  }
-  const FewAxis axis(a, max(few_all, 1));
-  for (int s = threadIdx.x; s < S; s += kAttendThreads) {
-    const OwnKeys k = LoadOwnKeys(a, s);
-    bool split = k.grouped;
-    if (k.rows > 0 && k.rows <= kFewRows && few_all > 0) {
-      const int x0 = (s > 0 ? few[s - 1] : 0) * a.k_heads, x1 = few[s] * a.k_heads;
-      split = split || axis.Owner(x0) != axis.Owner(x1 - 1);
-    } else if (k.rows > kFewRows) {
-      split = split || ManyParts(ManySteps(LoadManySequence(k)), each) > 1;
-    }
-    todo[s] = split ? k.rows * a.k_heads : 0;
-  }
-  BlockSums(todo, S);
-  const int all = one(todo[S - 1]);
+  const int* from = Plan(a);
+  for (int i = threadIdx.x; i < PlanWords(a); i += kAttendThreads) words[i] = from[i];
+  __syncthreads();
+  const PlanView plan(a, words);
+  const Axis few = FewAxis(a, one(plan.few[S - 1]));
+  const Axis many = ManyAxis(a, one(plan.many[units - 1]));
+  const auto before = [](const int* sums, int i) { return i > 0 ? sums[i - 1] : 0; };
 
-  const int lanes = a.padded_dim / 4;
-  const int at_once = kAttendThreads / lanes;  // parts
-  const int mine = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
-  for (int j = blockIdx.x; j < all; j += gridDim.x) {
-    const int s = one(FirstAbove(todo, S, j));
-    const OwnKeys k = LoadOwnKeys(a, s);
-    const int rest = j - (s > 0 ? one(todo[s - 1]) : 0);
-    const int rows = one(k.rows);
-    const int h = rest / rows, row = rest - h * rows;
+  const int lanes = a.padded_dim / 4, d = threadIdx.x % lanes * 4;
+  const int team = threadIdx.x / lanes;  // threads of one part's row
+  const int at_once = kAttendThreads / lanes / a.join_rows;  // parts
+  const int mine = team / a.join_rows, in_group = team % a.join_rows;
+
+  // Items: the row groups of what may have been cut. Few rows: every (sequence,
+  // key head), or what each worker's start is in, where that is less; then many
+  // rows: the tile that each worker's start is in, behind the groups' prefixes;
+  // then the grouped sequences, whose rows all have a part of the prefix.
+  const int few_shift = 32 - __clz(max((a.few_rows - 1) / a.join_rows, 0));
+  const int many_shift = 31 - __clz(kManyRows / a.join_rows);
+  const bool by_cut = few.workers <= S * a.k_heads;
+  const int few_items = (by_cut ? max(few.workers - 1, 0) : few.total > 0 ? S * a.k_heads : 0)
+                        << few_shift;
+  const int many_first = a.groups > 0 ? many.Owner(before(plan.many, a.groups) * a.k_heads) : 0;
+  const int many_items = max(many.workers - 1 - many_first, 0) << many_shift;
+  const int items = few_items + many_items + one(plan.todo[S - 1]) * a.k_heads;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    int s, h, row0;           // sequence, key head, first row
+    int x = 0, size = 0;      // the rows' place on their axis
+    const bool is_cut = item < few_items + many_items;
+    bool is_few = item < few_items;
+    if (is_few) {
+      const int n = item >> few_shift, cut = few.Start(n + 1);
+      s = by_cut ? one(FirstAbove(plan.few, S, cut / a.k_heads)) : n / a.k_heads;
+      const int at = one(before(plan.few, s));
+      size = one(plan.few[s]) - at;
+      if (size == 0) continue;
+      h = by_cut ? (cut - at * a.k_heads) / size : n - s * a.k_heads;
+      x = at * a.k_heads + h * size;
+      row0 = (item & ((1 << few_shift) - 1)) * a.join_rows;
+      // The first cut inside takes it.
+      if (by_cut && (cut == x || cut - few.each > x)) continue;
+    } else if (is_cut) {
+      const int n = item - few_items, cut = many.Start(many_first + (n >> many_shift) + 1);
+      const int i = one(FirstAbove(plan.many, units, cut / a.k_heads));
+      if (i < a.groups) continue;  // with its sequences, below
+      s = i - a.groups;
+      const int at = one(before(plan.many, i)), per_head = one(plan.many[i]) - at;
+      const int base = one(plan.base[i]), tiles = (one(plan.rows[s]) + kManyRows - 1) / kManyRows;
+      h = (cut - at * a.k_heads) / per_head;
+      const int unit = at * a.k_heads + h * per_head;
+      const int tile = one(TileAt(a, false, base, tiles, cut - unit));
+      x = unit + ManyCost(a, false, base, tile);
+      size = unit + ManyCost(a, false, base, tile + 1) - x;
+      row0 = tile * kManyRows + (n & ((1 << many_shift) - 1)) * a.join_rows;
+      if (cut == x || cut - many.each > x) continue;
+    } else {
+      const int n = item - few_items - many_items;
+      s = one(FirstAbove(plan.todo, S, n / a.k_heads));
+      const int rest = n - one(before(plan.todo, s)) * a.k_heads;
+      h = rest % a.k_heads;
+      row0 = rest / a.k_heads * a.join_rows;
+      is_few = one(plan.rows[s]) <= kFewRows;
+      if (is_few) {
+        const int at = one(before(plan.few, s));
+        size = one(plan.few[s]) - at;
+        x = at * a.k_heads + h * size;
+      } else {
+        const int i = a.groups + s, at = one(before(plan.many, i)), base = one(plan.base[i]);
+        const int tile = row0 / kManyRows;
+        x = at * a.k_heads + h * (one(plan.many[i]) - at) + ManyCost(a, false, base, tile);
+        size = ManyCost(a, false, base, tile + 1) - ManyCost(a, false, base, tile);
+      }
+    }
+    const int rows = one(plan.rows[s]), g = one(plan.group[s]);
+    if (row0 >= rows || (is_cut && g >= 0)) continue;
+    const int row = min(row0 + in_group, rows - 1);
+    const bool has_row = row0 + in_group < rows;
     const int t = FastDivI(a.group_div, row);
-    const int64_t token = k.q.first + t;
+    const int64_t token = one(plan.first[s]) + t;
     const int head = h * G + (row - t * G);
 
-    // The row's parts: `own` of them, then `shared` of its group's prefix.
-    int own = 0, shared = 0, w0 = 0, x0 = 0;
-    int64_t own_row = 0, own_step = 0, shared_row = 0, shared_step = 0;
-    const bool is_few = rows <= kFewRows;
-    if (is_few) {
-      const int steps = one(few[s] - (s > 0 ? few[s - 1] : 0));
-      x0 = (s > 0 ? one(few[s - 1]) : 0) * a.k_heads + h * steps;
-      w0 = axis.Owner(x0);
-      own = axis.Owner(x0 + steps - 1) - w0 + 1;
-      own_row = row;
-    } else {
-      const ManyUnit u = LoadManySequence(k);
-      const int tiles = ManyTiles(u), i = a.groups + s;
-      own = ManyParts(ManySteps(u), each);
-      own_row = ManySlotRow(a, (i > 0 ? many[i - 1] : 0) * a.k_heads +
-                                   h * own * tiles + (tiles - 1 - row / kManyRows)) +
-                row % kManyRows;
-      own_step = static_cast<int64_t>(tiles) * kManyRows;
-    }
-    if (k.grouped) {
-      const int g = GroupOf(a, s);
-      const ManyUnit u = LoadGroup(a, g);
-      if (u.rows > 0) {
-        const int tiles = ManyTiles(u), r = (static_cast<int>(token) - u.first) * G + (row - t * G);
-        shared = ManyParts(ManySteps(u), each);
-        shared_row = ManySlotRow(a, (g > 0 ? many[g - 1] : 0) * a.k_heads + h * shared * tiles +
-                                        (tiles - 1 - r / kManyRows)) +
-                     r % kManyRows;
-        shared_step = static_cast<int64_t>(tiles) * kManyRows;
+    // The row's parts: workers [w0, w0 + own) of its own keys' axis and, of a
+    // group's, [v0, v0 + shared) of the prefix's.
+    const Axis& axis = is_few ? few : many;
+    const int w0 = axis.Owner(x), own = axis.Owner(x + size - 1) - w0 + 1;
+    if (g < 0 && own == 1) continue;
+    int shared_row = 0, y = 0, v0 = 0, shared = 0;
+    if (g >= 0) {
+      const int at = before(plan.many, g), per_head = plan.many[g] - at;
+      if (per_head > 0) {
+        shared_row = (static_cast<int>(token) - plan.gfirst[g]) * G + (row - t * G);
+        const int tile = shared_row / kManyRows, base = plan.base[g];
+        y = at * a.k_heads + h * per_head + ManyCost(a, true, base, tile);
+        v0 = many.Owner(y);
+        shared = many.Owner(y + base - 1) - v0 + 1;
       }
-    } else if (own == 1) {
-      continue;  // this key head's keys were not cut
     }
     Merged sum;
     if (mine < at_once) {
@@ -132,14 +139,15 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
       for (int n = mine; n < own + shared; n += at_once) {
         int64_t from;
         if (n >= own) {
-          from = shared_row + (n - own) * shared_step;
-        } else if (is_few && own == 1) {
-          from = WholeRow(a, token, head);
-        } else if (is_few) {
-          const int w = w0 + n;
-          from = FewSlotRow(a, n == 0 && axis.Start(w) != x0 ? 2 * w + 1 : 2 * w) + own_row;
+          const int w = v0 + n - own;
+          from = shared == 1 ? WholeRow(a, true, token, head)
+                             : ManySlotRow(a, n == own ? many.Slot(w, y) : 2 * w) +
+                                   shared_row % kManyRows;
+        } else if (own == 1) {
+          from = WholeRow(a, false, token, head);
         } else {
-          from = own_row + n * own_step;
+          const int w = w0 + n, slot = n == 0 ? axis.Slot(w, x) : 2 * w;
+          from = is_few ? FewSlotRow(a, slot) + row : ManySlotRow(a, slot) + row % kManyRows;
         }
         const f32x2 st = PartStats(a)[from];
         sum.Add(st[0], st[1], *reinterpret_cast<const f32x4*>(a.parts + from * a.padded_dim + d));
@@ -149,11 +157,12 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
     }
     __syncthreads();
     if (mine == 0) {
-      for (int n = 1; n < min(at_once, own + shared); ++n) {
-        const f32x2 st = part_s[n * lanes + threadIdx.x];
-        sum.Add(st[0], st[1], part_v[n * lanes + threadIdx.x]);
+      for (int n = 1; n < at_once; ++n) {
+        const int other = n * a.join_rows * lanes + threadIdx.x;
+        const f32x2 st = part_s[other];
+        sum.Add(st[0], st[1], part_v[other]);
       }
-      if (d < a.head_dim) {
+      if (has_row && d < a.head_dim) {
         const float inverse = sum.l > 0.0f ? 1.0f / sum.l : (sum.l == 0.0f ? 0.0f : sum.l);
         using Pair = u32x2 __attribute__((aligned(2)));
         *reinterpret_cast<Pair*>(static_cast<Scalar*>(a.out) + token * a.out_token +
@@ -161,7 +170,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
             u32x2{Pack2<E>(sum.v[0] * inverse, sum.v[1] * inverse),
                   Pack2<E>(sum.v[2] * inverse, sum.v[3] * inverse)};
       }
-      if (a.lse != nullptr && d == 0) {
+      if (has_row && a.lse != nullptr && d == 0) {
         a.lse[token * a.q_heads + head] = (sum.m + log2f(sum.l)) / kLog2e;
       }
     }
@@ -174,14 +183,12 @@ int64_t CeilDiv(int64_t n, int64_t d) { return (n + d - 1) / d; }
 }  // namespace
 
 hipError_t LaunchAttendJoin(const AttendLaunch& l, hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(l.batch.tokens) * l.q_heads;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(rows, 2048));
-  const size_t lds = static_cast<size_t>(3 * l.batch.sequences + l.groups) * sizeof(int);
-  if (l.type == kBf16) {
-    hipLaunchKernelGGL(attend_join_kernel<Bf16>, dim3(grid), dim3(kAttendThreads), lds, stream, l);
-  } else {
-    hipLaunchKernelGGL(attend_join_kernel<F16>, dim3(grid), dim3(kAttendThreads), lds, stream, l);
-  }
+  const size_t lds = PlanWords(l) * sizeof(int);
+  constexpr auto bf16 = attend_join_kernel<Bf16>, f16 = attend_join_kernel<F16>;
+  const hipError_t e = l.type == kBf16 ? AllowDynamicLds<bf16>(lds) : AllowDynamicLds<f16>(lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(l.type == kBf16 ? bf16 : f16, dim3(l.join_grid), dim3(kAttendThreads), lds,
+                     stream, l);
   return hipGetLastError();
 }
 
@@ -189,45 +196,47 @@ int64_t PlanAttend(AttendLaunch* l) {
   constexpr int kCus = 256;
   const int64_t G = l->q_heads / l->k_heads;
   const int64_t T = l->batch.tokens, S = l->batch.sequences;
+  const int64_t capacity = std::max(l->batch.capacity, 1);
   const bool single = l->batch.starts == nullptr;
   l->padded_dim = l->head_dim <= 64 ? 64 : l->head_dim <= 96 ? 96 : l->head_dim <= 128 ? 128 : 256;
-  l->few_grid = l->many_grid = l->many_parts = 0;
+  l->few_grid = l->few_rows = l->many_grid = l->join_grid = l->join_rows = 0;
   l->part_rows = 0;
-  // Rows of one sequence that may meet attend_few.
-  const int64_t most = single ? G : std::min<int64_t>(T * G, kFewRows);
-  const bool full = l->head_dim == l->padded_dim;
-  l->few_rows = most <= 16 && full ? 16 : 32;
+  const int resident = (l->padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
   if (G <= kFewRows) {
-    const int per_cu = l->padded_dim > 128 ? 1 : l->few_rows == 16 ? 3 : 2;
-    const int64_t steps = S * l->k_heads * CeilDiv(std::max(l->batch.capacity, 1), kFewStep);
-    l->few_grid = static_cast<int>(std::min<int64_t>(kCus * per_cu, steps));
+    l->few_rows = static_cast<int>(single ? G : std::min<int64_t>(T * G, kFewRows));
+    const int64_t steps = S * l->k_heads * CeilDiv(capacity, kFewStep);
+    // One place is left to the plan's workgroup.
+    l->few_grid = static_cast<int>(std::min<int64_t>(resident - 1, CeilDiv(steps, kWaves)));
   }
   const bool many_sequences = single ? G > kFewRows : T * G > kFewRows;
   if (many_sequences || l->groups > 0) {
-    l->many_target = l->padded_dim > 128 ? kCus : 2 * kCus;
-    int64_t tiles = 0;
-    if (many_sequences) tiles += CeilDiv(T * G, kManyRows) + std::min(S, T * G / (kFewRows + 1));
-    if (l->groups > 0) tiles += CeilDiv(T * G, kManyRows) + l->groups;
-    tiles *= l->k_heads;
-    const int64_t split = std::min<int64_t>(2 * l->many_target, l->many_target + tiles);
-    const int64_t steps = CeilDiv(std::max(l->batch.capacity, 1), kManyStep);
-    l->many_grid = static_cast<int>(std::min(std::max(tiles, split), tiles * CeilDiv(steps, 8)));
-    l->many_parts = l->groups > 0 ? l->many_grid
-                                  : static_cast<int>(std::min<int64_t>(l->many_grid, split));
+    const int64_t tiles = CeilDiv(T * G, kManyRows) * 2 + S + l->groups;
+    const int64_t steps = tiles * l->k_heads * (CeilDiv(capacity, kManyStep) + 2);
+    l->many_grid = static_cast<int>(std::min<int64_t>(resident, std::max<int64_t>(steps / 8, 1)));
   }
-  l->join = l->groups > 0 || l->batch.capacity > kFewStep;
-  if (!l->join) return 0;
-  l->part_rows = 2ll * l->few_grid * l->few_rows +
-                 static_cast<int64_t>(l->many_parts) * kManyRows +
-                 (l->groups > 0 ? T * l->q_heads : 0);
-  return l->part_rows * (l->padded_dim + 2) * static_cast<int64_t>(sizeof(float));
+  if (l->groups == 0 && l->many_grid == 0 && capacity <= kFewStep) return 0;  // nothing to split
+  // Rows that a workgroup joins at once: as many as it has teams of a row's
+  // threads, but fewer where that leaves CUs without work.
+  const int64_t rows = T * l->q_heads;
+  const int teams = l->padded_dim == 64 ? 16 : l->padded_dim <= 128 ? 8 : 4;
+  const int64_t most = l->many_grid > 0 ? kManyRows : l->few_rows;
+  l->join_rows = 1;
+  while (l->join_rows < teams && l->join_rows < most && rows / l->join_rows >= 4 * kCus) {
+    l->join_rows *= 2;
+  }
+  const int64_t units = std::min<int64_t>(S * l->k_heads, kWaves * l->few_grid);
+  const int64_t groups = 2 * units * CeilDiv(l->few_rows, l->join_rows) +
+                         l->many_grid * CeilDiv(kManyRows, l->join_rows) +
+                         (l->groups > 0 ? CeilDiv(rows, l->join_rows) + S * l->k_heads : 0);
+  l->join_grid = static_cast<int>(std::min<int64_t>(groups, 2048));
+  l->part_rows = 2ll * kWaves * l->few_grid * l->few_rows + 2ll * l->many_grid * kManyRows +
+                 (l->groups > 0 ? 2 * rows : 0);
+  return (l->part_rows * (l->padded_dim + 2) + PlanWords(*l)) * static_cast<int64_t>(sizeof(float));
 }
 
 hipError_t LaunchAttend(const AttendLaunch& l, hipStream_t stream) {
-  hipError_t e = hipSuccess;
-  if (l.many_grid > 0) e = LaunchAttendMany(l, stream);
-  if (e == hipSuccess && l.few_grid > 0) e = LaunchAttendFew(l, stream);
-  if (e == hipSuccess && l.join) e = LaunchAttendJoin(l, stream);
+  hipError_t e = l.many_grid > 0 ? LaunchAttendMixed(l, stream) : LaunchAttendFew(l, stream);
+  if (e == hipSuccess && l.join_grid > 0) e = LaunchAttendJoin(l, stream);
   return e;
 }
 

@@ -1,0 +1,435 @@
+// Paged attention of many rows a key head: chunks of new tokens, and all rows
+// of sequences that share a prefix against that prefix.
+//
+// A workgroup takes a tile of 128 rows, 32 a wave, and steps through its keys
+// 64 at a time: the tile of K and V lies in LDS for all four waves, the next
+// one is on its way from memory in registers. Matrix instructions bound it,
+// so the layout keeps everything between the two products in place: S^T = K Q^T
+// in 32 x 32 x 16 products leaves lane l with the scores of row l % 32, so a
+// row's maximum takes one swap between the wave's halves, and the packed
+// exponentials are the operand of O^T = V^T P^T as they stand (the contraction
+// runs over tokens in the order that the scores lie in). V is transposed by
+// the LDS reads.
+//
+// Work. The tiles of all groups and sequences make one axis, weighed by the
+// keys they see, and every workgroup gets an equal part of it: no tail of late
+// tiles. What a part cuts is at its two ends and goes to slots 2w and 2w + 1 of
+// `parts`; whole tiles go straight to the output, or, where a row has a group's
+// part and one of its own, to its row of `parts`. The workgroups of one XCD take
+// neighbouring parts, so its L2 serves a key head's tokens to all of them.
+#ifndef KVX_KERNELS_ATTEND_MANY_H_
+#define KVX_KERNELS_ATTEND_MANY_H_
+
+#include "attend_plan.h"
+
+namespace kvx {
+
+// A token's row in LDS is its 2 DP bytes, in 16-byte chunks that are exchanged
+// within the row so that the rows of one read fall on different banks (256
+// bytes apart in 16ths): `chunk` of row `r` lies at chunk KeyChunk or ValueChunk.
+// Keys are read 16 bytes of 16 neighbouring rows at a time, values 64 bytes of
+// four neighbouring rows.
+template <int DP>
+__device__ __forceinline__ int KeyChunk(int r, int chunk) {
+  if constexpr (DP == 64) return chunk ^ (r / 2 % 8);   // two rows in 256 bytes
+  if constexpr (DP == 96) return chunk ^ (r / 4 % 4);   // rows 192 bytes apart
+  return chunk ^ (r % 16);
+}
+template <int DP>
+__device__ __forceinline__ int ValueChunk(int r, int chunk) {
+  if constexpr (DP == 64) return chunk ^ (r / 2 % 2 * 4);
+  if constexpr (DP == 96) return chunk;
+  return chunk ^ (r % 4 * 4);
+}
+
+// Places of a step's tokens: looked up three steps ahead, their scales two.
+struct Places {
+  int64_t at[kManyStep];  // element offset of the token's row, or -1
+  int32_t id[kManyStep];  // its block, or -1
+  float k_scale[kManyStep], v_scale[kManyStep];
+  uint64_t present;  // one bit a token
+};
+
+constexpr size_t ManyLds(const AttendLaunch& l, int dp) {
+  return 2 * kManyStep * 4 * dp + 4 * sizeof(Places) +
+         static_cast<size_t>(l.groups + l.batch.sequences) * sizeof(int);
+}
+
+template <class E, bool E4, int DP>
+__device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int worker) {
+  constexpr bool kScaleValues = E4 && std::is_same_v<E, F16>;  // as in AttendFew
+  using P = std::conditional_t<E4 && !kScaleValues, Bf16, E>;
+  using Scalar = typename E::Scalar;
+  constexpr int KS = DP / 16, DT = DP / 32, kRow = 2 * DP;  // bytes of a token's row
+  constexpr int kChunks = kManyStep * (DP / 8) / kAttendThreads;  // of a thread
+  constexpr int kTile = 2 * kManyStep * kRow;  // keys, then values
+  Places* places = reinterpret_cast<Places*>(lds + 2 * kTile);
+  int* sums = reinterpret_cast<int*>(places + 4);  // [groups + sequences]
+  const BatchView& b = a.batch;
+  const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+
+  const int units = a.groups + b.sequences;
+  for (int i = threadIdx.x; i < units; i += kAttendThreads) {
+    sums[i] = ManyWork(a, i, LoadManyUnit(a, i));
+  }
+  BlockSums(sums, units);
+  const int work = one(sums[units - 1]);
+  if (work == 0) return;
+  const Axis axis = ManyAxis(a, work);
+  if (worker >= axis.workers) return;
+  const int x_start = axis.Start(worker), x_end = axis.Start(worker + 1);
+  const int G = a.q_heads / a.k_heads;
+  const int lane = threadIdx.x % 64, wave = one(threadIdx.x / 64);
+  const int in32 = lane % 32, half = lane / 32;
+
+  // The end of a tile that the part starts with comes last, after the start of
+  // the one that it ends with: workgroups with equal tiles then read the same
+  // tokens at the same time.
+  int limit = x_end, put_off = 0;
+  for (int x = x_start; x < limit;) {
+    const int i = one(FirstAbove(sums, units, x / a.k_heads));
+    const int before = i > 0 ? one(sums[i - 1]) : 0;
+    const int per_head = one(sums[i]) - before;
+    const int h = (x - before * a.k_heads) / per_head;
+    const int at_unit = x - before * a.k_heads - h * per_head;
+    const ManyUnit u = LoadManyUnit(a, i);
+    const int rows = one(u.rows), begin = one(u.begin), end = one(u.end), first = one(u.first);
+    const int base = one(u.base);
+    const bool group = i < a.groups;
+    const int tile = one(TileAt(a, group, base, ManyTiles(u), at_unit));
+    const int tile_at = ManyCost(a, group, base, tile);
+    const int cost = ManyCost(a, group, base, tile + 1) - tile_at;
+    const int from = at_unit - tile_at, to = min(cost, from + (limit - x));
+    if (x == x_start && put_off == 0 && from > 0 && x + to - from < x_end) {
+      put_off = x + to - from;
+      x = put_off;
+      continue;
+    }
+    const int sequence = group ? min(max(one(a.group_starts[i]), 0), b.sequences - 1)
+                               : i - a.groups;
+    const SequenceSpan span = LoadSequence(b, sequence);
+    const bool grouped = group || LoadOwnKeys(a, sequence).grouped;
+    // Steps that the tile's rows see, and this part's share of them.
+    int steps = (end - begin + kManyStep - 1) / kManyStep;
+    if (!group && a.causal) {
+      const int last = min(rows, (tile + 1) * kManyRows) - 1;
+      const int seen = Visible(a, span, first + FastDivI(a.group_div, last));
+      steps = min(steps, (max(seen - begin, 0) + kManyStep - 1) / kManyStep);
+    }
+    steps = one(steps);
+    const int step0 = static_cast<int>(static_cast<int64_t>(from) * steps / cost);
+    const int step1 = static_cast<int>(static_cast<int64_t>(to) * steps / cost);
+
+    // Queries: row l % 32 of the wave's 32, as an operand.
+    const int row = tile * kManyRows + wave * 32 + in32;
+    const int t = FastDivI(a.group_div, row);
+    const int64_t token = first + t;
+    const int head = h * G + (row - t * G);
+    int seen = INT_MAX;
+    if (row < rows) {
+      if (!group) {
+        seen = Visible(a, span, first + t);
+      } else {
+        int s = static_cast<int>(token);
+        if (b.starts != nullptr) {
+          int lo = 0, hi = b.sequences;  // first s with starts[s + 1] > token
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (b.starts[mid + 1] > token) {
+              hi = mid;
+            } else {
+              lo = mid + 1;
+            }
+          }
+          s = min(lo, b.sequences - 1);
+        }
+        seen = min(Visible(a, LoadSequence(b, s), static_cast<int>(token)), end);
+      }
+    }
+    int least = seen, most_seen = row < rows ? seen : 0;
+#pragma unroll
+    for (int m = 32; m > 0; m /= 2) {
+      least = min(least, __shfl_xor(least, m));
+      most_seen = max(most_seen, __shfl_xor(most_seen, m));
+    }
+    least = one(least);
+    most_seen = one(most_seen);
+    u32x4 q[KS];
+    {
+      const Scalar* p = static_cast<const Scalar*>(a.q) + token * a.q_token + head * a.q_head +
+                        half * 8;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        q[ks] = u32x4{0, 0, 0, 0};
+        if (row < rows && ks * 16 + half * 8 < a.head_dim) {
+          q[ks] = *reinterpret_cast<const Bytes16*>(p + ks * 16);
+        }
+      }
+    }
+
+    const int32_t* table = b.tables + sequence * b.table_stride;
+    const int64_t row_stride = static_cast<int64_t>(a.k_heads) * a.head_dim;
+    // One wave looks up a step's 64 tokens, another one their scales. Loads
+    // return in order, so a lookup is issued before the step's tokens and put
+    // into LDS after its products: nobody waits for it.
+    int found = -1;
+    float found_k = 0.0f, found_v = 0.0f;
+    const auto find = [&](int step) {
+      const int p = begin + step * kManyStep + lane;
+      found = step < step1 && p < end ? table[FastDivI(a.block_div, p)] : -1;
+    };
+    const auto keep = [&](int step) {
+      Places& to = places[step & 3];
+      const int p = begin + step * kManyStep + lane;
+      const bool is = found >= 0 && found < b.num_blocks;
+      const int slot = p - FastDivI(a.block_div, p) * b.block_tokens;
+      to.at[lane] = is ? (static_cast<int64_t>(found) * b.block_tokens + slot) * row_stride +
+                             h * a.head_dim
+                       : -1;
+      to.id[lane] = is ? found : -1;
+      const uint64_t present = __ballot(is);
+      if (lane == 0) to.present = present;
+    };
+    const auto find_scales = [&](int step) {
+      const int id = places[step & 3].id[lane];
+      const int64_t at = static_cast<int64_t>(max(id, 0)) * a.k_heads + h;
+      found_k = a.k_scales[at];
+      found_v = a.v_scales[at];
+    };
+    const auto keep_scales = [&](int step) {
+      places[step & 3].k_scale[lane] = found_k;
+      places[step & 3].v_scale[lane] = found_v;
+    };
+    constexpr int W = E4 ? 2 : 4;
+    using Words = __attribute__((ext_vector_type(W))) uint32_t;
+    Words kw[kChunks], vw[kChunks];
+    const auto load = [&](int step) {
+      const Places& held = places[step & 3];
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int tok = chunk / (DP / 8), d = chunk % (DP / 8) * 8;
+        const int64_t at = held.at[tok];
+        kw[n] = vw[n] = Words(0);
+        if (at >= 0 && d < a.head_dim) {
+          if constexpr (E4) {
+            kw[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(a.k_pool) + at + d);
+            vw[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(a.v_pool) + at + d);
+          } else {
+            kw[n] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) + at + d);
+            vw[n] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.v_pool) + at + d);
+          }
+        }
+      }
+    };
+    const auto store = [&](int step) {
+      char* to = lds + (step & 1) * kTile;
+      const Places& held = places[step & 3];
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int tok = chunk / (DP / 8), d = chunk % (DP / 8) * 8;
+        u32x4 k, v;
+        if constexpr (E4) {
+          k = Widen<E>(kw[n]);
+          if constexpr (kScaleValues) {
+            v = WidenScaled<P>(vw[n], held.at[tok] >= 0 ? held.v_scale[tok] : 0.0f);
+          } else {
+            v = Widen<P>(vw[n]);
+          }
+        } else {
+          k = kw[n];
+          v = vw[n];
+        }
+        *reinterpret_cast<u32x4*>(to + tok * kRow + KeyChunk<DP>(tok, d / 8) * 16) = k;
+        *reinterpret_cast<u32x4*>(to + kTile / 2 + tok * kRow + ValueChunk<DP>(tok, d / 8) * 16) = v;
+      }
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16(0.0f);
+    float top = -__builtin_inff(), sum = 0.0f;
+    const float c = a.scale * kLog2e;
+    if (step0 < step1) {
+      if (wave < 3) {
+        find(step0 + wave);
+        keep(step0 + wave);
+      }
+      if constexpr (E4) {
+        if (wave < 2) {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          find_scales(step0 + wave);
+          keep_scales(step0 + wave);
+        }
+      }
+      __syncthreads();
+      load(step0);
+      store(step0);
+    }
+    for (int step = step0; step < step1; ++step) {
+      __syncthreads();
+      const bool finds = wave == (step & 3), finds_scales = E4 && wave == ((step + 1) & 3);
+      if (finds) find(step + 3);
+      if (finds_scales) find_scales(step + 2);
+      if (step + 1 < step1) load(step + 1);
+      const Places& here = places[step & 3];
+      const int p0 = begin + step * kManyStep;
+      if (p0 < most_seen) {
+        const char* keys = lds + (step & 1) * kTile;
+        const char* values = keys + kTile / 2;
+        f32x16 sc[2] = {f32x16(0.0f), f32x16(0.0f)};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x4 key = *reinterpret_cast<const u32x4*>(
+                keys + (u * 32 + in32) * kRow + KeyChunk<DP>(u * 32 + in32, ks * 2 + half) * 16);
+            sc[u] = Mma32<E>(key, q[ks], sc[u]);
+          }
+        }
+#if KVX_SCHED & 1
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int n = 0; n < 2 * KS - 6; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
+#endif
+        // Lane: row l % 32, tokens 32 u + 8 (i / 4) + 4 (l / 32) + i % 4.
+        if constexpr (E4) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const f32x4 f =
+                  *reinterpret_cast<const f32x4*>(&here.k_scale[u * 32 + i * 2 + half * 4]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sc[u][i + j] *= f[j];
+            }
+          }
+        }
+        const uint64_t present = here.present;
+        if (p0 + kManyStep > least || present != ~uint64_t{0}) {
+          // Token 32 u + n of the step is number n + 4 half of its lane's.
+          const int behind = seen - p0 - half * 4;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t there = static_cast<uint32_t>(present >> (u * 32)) >> (half * 4);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int n = (i / 4) * 8 + i % 4;
+              if (u * 32 + n >= behind || (there & (1u << n)) == 0) sc[u][i] = -__builtin_inff();
+            }
+          }
+        }
+        float most = sc[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) most = fmaxf(most, sc[i / 16][i % 16]);
+        most = Across32(most) * c;
+        // The maximum is only moved when it falls behind by 2^8.
+        if (__any(most > top + 8.0f)) {
+          const float now = fmaxf(top, most);
+          const float back = now == -__builtin_inff() ? 0.0f : now;
+          const float shrink = __builtin_amdgcn_exp2f(top - back);
+          top = now;
+          sum *= shrink;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] *= shrink;
+        }
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sc[u][i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], c, -base));
+            sum += sc[u][i];
+          }
+        }
+        if constexpr (E4 && !kScaleValues) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const f32x4 f =
+                  *reinterpret_cast<const f32x4*>(&here.v_scale[u * 32 + i * 2 + half * 4]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // A hidden token's scale may be anything.
+                sc[u][i + j] = sc[u][i + j] == 0.0f ? 0.0f : sc[u][i + j] * f[j];
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int u = kk / 2, i = kk % 2 * 8;
+          const u32x4 p = {Pack2<P>(sc[u][i], sc[u][i + 1]), Pack2<P>(sc[u][i + 2], sc[u][i + 3]),
+                           Pack2<P>(sc[u][i + 4], sc[u][i + 5]),
+                           Pack2<P>(sc[u][i + 6], sc[u][i + 7])};
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            // Row 4 half + l % 16 / 4 of 8, 8 bytes l % 4 of the 32 of l / 16 % 2.
+            const int r = kk * 16 + half * 4 + lane % 16 / 4;
+            const int chunk = dt * 4 + lane / 16 % 2 * 2 + lane % 4 / 2;
+            const char* v = values + r * kRow + ValueChunk<DP>(r, chunk) * 16 + lane % 2 * 8;
+            const u32x2 lo = ReadTransposed(v), hi = ReadTransposed(v + 8 * kRow);
+            o[dt] = Mma32<P>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[dt]);
+          }
+        }
+      }
+      if (step + 1 < step1) store(step + 1);
+      if (finds) keep(step + 3);
+      if (finds_scales) keep_scales(step + 2);
+    }
+
+    // Lane: row l % 32, dimensions 32 dt + 8 (i / 4) + 4 (l / 32) + i % 4.
+    sum += __shfl_xor(sum, 32);
+    const bool whole = from == 0 && to == cost;
+    if (row < rows) {
+      if (whole && !grouped) {
+        const float inverse = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+        Scalar* out = static_cast<Scalar*>(a.out) + token * a.out_token + head * a.out_head;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int d = dt * 32 + i * 2 + half * 4;
+            using Pair = u32x2 __attribute__((aligned(2)));
+            if (d < a.head_dim) {
+              *reinterpret_cast<Pair*>(out + d) =
+                  u32x2{Pack2<E>(o[dt][i] * inverse, o[dt][i + 1] * inverse),
+                        Pack2<E>(o[dt][i + 2] * inverse, o[dt][i + 3] * inverse)};
+            }
+          }
+        }
+        if (a.lse != nullptr && half == 0) {
+          a.lse[token * a.q_heads + head] = (top + log2f(sum)) / kLog2e;
+        }
+      } else {
+        const int64_t to_row = whole ? WholeRow(a, group, token, head)
+                                     : ManySlotRow(a, axis.Slot(worker, x)) + wave * 32 + in32;
+        if (half == 0) PartStats(a)[to_row] = f32x2{top, sum};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            *reinterpret_cast<f32x4*>(a.parts + to_row * DP + dt * 32 + i * 2 + half * 4) =
+                f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+          }
+        }
+      }
+    }
+    x += to - from;
+    if (x == x_end && put_off > 0) {
+      x = x_start;
+      limit = put_off;
+    }
+    __syncthreads();  // the next piece's tokens take this one's place in LDS
+  }
+}
+
+}  // namespace kvx
+
+#endif  // KVX_KERNELS_ATTEND_MANY_H_

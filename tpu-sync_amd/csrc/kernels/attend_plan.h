@@ -5,12 +5,35 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "attend.h"
 
 namespace kvx {
 
 constexpr int kAttendThreads = 256;
+constexpr int kWaves = kAttendThreads / 64;
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Rows may start at any element.
+using Bytes16 = u32x4 __attribute__((aligned(2)));
+using Bytes8 = u32x2 __attribute__((aligned(1)));
+
+// Raises a kernel's limit of dynamic LDS to the CU's 160 KiB, once a device.
+template <auto kernel>
+hipError_t AllowDynamicLds(size_t bytes) {
+  static std::atomic<uint64_t> allowed{0};
+  if (bytes <= 65536) return hipSuccess;
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  const uint64_t bit = uint64_t{1} << (device & 63);
+  if (e != hipSuccess || (allowed.load() & bit) != 0) return e;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 256);
+  if (e == hipSuccess) allowed.fetch_or(bit);
+  return e;
+}
 
 __device__ __forceinline__ int FastDivI(const FastDivU32& f, int n) {
   const uint32_t u = static_cast<uint32_t>(n);
@@ -21,7 +44,7 @@ __device__ __forceinline__ int FastDivI(const FastDivU32& f, int n) {
 // 2); c[i] must have been written by any thread before, and is visible to all
 // after.
 __device__ __forceinline__ void BlockSums(int* c, int n) {
-  __shared__ int waves[kAttendThreads / 64];
+  __shared__ int waves[kWaves];
   const int each = (n + kAttendThreads - 1) / kAttendThreads;
   const int i0 = threadIdx.x * each, i1 = min(i0 + each, n);
   __syncthreads();
@@ -103,37 +126,77 @@ __device__ __forceinline__ int Visible(const AttendLaunch& a, const SequenceSpan
   return a.causal ? min(max(q.length - q.count + (token - q.first) + 1, 0), all) : all;
 }
 
-// -- attend_few: every sequence's steps for each key head in turn make one
-// axis, which is cut into equal parts, one a workgroup.
+// Work of all sequences and key heads laid end to end and cut into parts of
+// `each`, one a worker.
+struct Axis {
+  int total, each, workers;
+  float inverse;  // 1 / each
+
+  __device__ Axis(int work, int most) : total(work) {
+    each = most > 0 ? max((work + most - 1) / most, 1) : 1;
+    workers = most > 0 ? (work + each - 1) / each : 0;
+    inverse = 1.0f / static_cast<float>(each);
+  }
+  __device__ __forceinline__ int Start(int w) const { return min(w * each, total); }
+  // The worker whose part holds x. The product is off by under one (x / each is
+  // below 2^12, its relative error below 2^-21).
+  __device__ __forceinline__ int Owner(int x) const {
+    const int w = static_cast<int>(static_cast<float>(x) * inverse);
+    const int rest = x - w * each;
+    return w + (rest >= each ? 1 : 0) - (rest < 0 ? 1 : 0);
+  }
+  // Worker w's slot for the piece that starts at x in its part: a part cuts at
+  // most the first and the last of its pieces.
+  __device__ __forceinline__ int Slot(int w, int x) const {
+    return x == w * each ? 2 * w : 2 * w + 1;
+  }
+};
+
+// -- Few rows: steps of kFewStep tokens; a worker is a wave.
 
 __device__ __forceinline__ int FewSteps(const OwnKeys& k) {
   if (k.rows == 0 || k.rows > kFewRows) return 0;
   return max(1, (k.end - k.begin + kFewStep - 1) / kFewStep);
 }
 
-struct FewAxis {
-  int total;    // steps of all sequences and key heads
-  int workers;  // workgroups that get a part
+__device__ __forceinline__ Axis FewAxis(const AttendLaunch& a, int steps) {
+  return Axis(steps * a.k_heads, a.few_grid * kWaves);
+}
 
-  __device__ FewAxis(const AttendLaunch& a, int steps)
-      : total(steps * a.k_heads), workers(min(a.few_grid, steps * a.k_heads)) {}
-  __device__ int Start(int w) const {
-    return static_cast<int>(static_cast<int64_t>(w) * total / workers);
-  }
-  // The workgroup whose part holds step x: the largest w with Start(w) <= x.
-  __device__ int Owner(int x) const {
-    return static_cast<int>(((static_cast<int64_t>(x) + 1) * workers - 1) / total);
-  }
-};
-
-// -- attend_many: items (row tile, part of the keys, key head) of groups and
-// of sequences with many rows.
+// -- Many rows: tiles of kManyRows rows of the groups, then of the sequences
+// with more than kFewRows rows; a worker is a workgroup. Under a causal mask
+// tile r sees 128 r / G keys more than the first, so the axis gives it
+// `base` + 2 r / G steps of 64: C(r) = r base + r (r - 1) / G is where it starts.
 
 struct ManyUnit {
   int first, rows;  // first token, and rows a key head
   int begin, end;   // keys
-  int length;       // 0: a group
+  int base;         // steps of the first tile
 };
+
+__device__ __forceinline__ int ManyTiles(const ManyUnit& u) {
+  return (u.rows + kManyRows - 1) / kManyRows;
+}
+
+__device__ __forceinline__ int ManyCost(const AttendLaunch& a, bool group, int base, int tile) {
+  const int more = group || !a.causal ? 0 : FastDivI(a.group_div, tile * (tile - 1));
+  return tile * base + more;
+}
+
+// The last of `tiles` tiles that starts at or before `at` of its unit's axis.
+__device__ __forceinline__ int TileAt(const AttendLaunch& a, bool group, int base, int tiles,
+                                      int at) {
+  int tile = 0;
+  while (tiles - tile > 1) {
+    const int mid = (tile + tiles) / 2;
+    if (ManyCost(a, group, base, mid) <= at) {
+      tile = mid;
+    } else {
+      tiles = mid;
+    }
+  }
+  return tile;
+}
 
 __device__ __forceinline__ ManyUnit LoadGroup(const AttendLaunch& a, int g) {
   ManyUnit u = {0, 0, 0, 0, 0};
@@ -142,51 +205,108 @@ __device__ __forceinline__ ManyUnit LoadGroup(const AttendLaunch& a, int g) {
   if (s0 == s1) return u;
   const SequenceSpan f = LoadSequence(a.batch, s0), l = LoadSequence(a.batch, s1 - 1);
   u.first = f.first;
-  u.rows = max(l.first + l.count - f.first, 0) * (a.q_heads / a.k_heads);
   u.end = PrefixLength(a, g);
-  if (u.end == 0) u.rows = 0;
+  if (u.end > 0) u.rows = max(l.first + l.count - f.first, 0) * (a.q_heads / a.k_heads);
+  u.base = (u.end + kManyStep - 1) / kManyStep + 1;
   return u;
 }
 
-__device__ __forceinline__ int ManyTiles(const ManyUnit& u) {
-  return (u.rows + kManyRows - 1) / kManyRows;
-}
-__device__ __forceinline__ int ManySteps(const ManyUnit& u) {
-  return max(1, (u.end - u.begin + kManyStep - 1) / kManyStep);
-}
-
-__device__ __forceinline__ ManyUnit LoadManySequence(const OwnKeys& k) {
-  ManyUnit u = {k.q.first, k.rows > kFewRows ? k.rows : 0, k.begin, k.end, k.q.length};
+__device__ __forceinline__ ManyUnit LoadManySequence(const AttendLaunch& a, const OwnKeys& k) {
+  ManyUnit u = {k.q.first, k.rows > kFewRows ? k.rows : 0, k.begin, k.end, 0};
+  const int ahead = a.causal ? min(k.q.length - k.q.count, k.end) : k.end;
+  u.base = max(ahead - k.begin, 0) / kManyStep + 2;
   return u;
 }
 
-// Parts that a unit's keys are split into: `each` steps a part where there are
-// too few tiles to fill the GPU (each > 0).
-__device__ __forceinline__ int ManyParts(int steps, int each) {
-  return each > 0 ? (steps + each - 1) / each : 1;
+__device__ __forceinline__ ManyUnit LoadManyUnit(const AttendLaunch& a, int i) {
+  return i < a.groups ? LoadGroup(a, i) : LoadManySequence(a, LoadOwnKeys(a, i - a.groups));
 }
 
-// Steps a part (0: no split) for `tiles` tiles with `steps` steps in all.
-__device__ __forceinline__ int ManyEach(const AttendLaunch& a, int tiles, int64_t steps) {
-  constexpr int kLeast = 8;
-  if (tiles >= a.many_target) return 0;
-  return max(kLeast, static_cast<int>((steps + a.many_target - 1) / a.many_target));
+__device__ __forceinline__ int ManyWork(const AttendLaunch& a, int i, const ManyUnit& u) {
+  return ManyCost(a, i < a.groups, u.base, ManyTiles(u));
 }
 
-// Slots of parts.
+// At least 8 steps a worker.
+__device__ __forceinline__ Axis ManyAxis(const AttendLaunch& a, int work) {
+  const int total = work * a.k_heads;
+  return Axis(total, min(a.many_grid, max(total / 8, 1)));
+}
+
+// Rows of `parts`: two slots a wave of few_rows rows, two slots a workgroup of
+// kManyRows rows; with groups a row for every (token, head) that was not cut,
+// of its own keys and of its group's.
 __device__ __forceinline__ int64_t FewSlotRow(const AttendLaunch& a, int slot) {
   return static_cast<int64_t>(slot) * a.few_rows;
 }
 __device__ __forceinline__ int64_t ManySlotRow(const AttendLaunch& a, int slot) {
-  return static_cast<int64_t>(2 * a.few_grid) * a.few_rows +
-         static_cast<int64_t>(slot) * kManyRows;
+  return 2ll * kWaves * a.few_grid * a.few_rows + static_cast<int64_t>(slot) * kManyRows;
 }
-// The row of a (token, head) that attend_few did not cut, of a grouped sequence.
-__device__ __forceinline__ int64_t WholeRow(const AttendLaunch& a, int64_t token, int head) {
-  return ManySlotRow(a, a.many_parts) + token * a.q_heads + head;
+__device__ __forceinline__ int64_t WholeRow(const AttendLaunch& a, bool group, int64_t token,
+                                            int head) {
+  return ManySlotRow(a, 2 * a.many_grid) + (group ? 1ll : 0ll) * a.batch.tokens * a.q_heads +
+         token * a.q_heads + head;
 }
 __device__ __forceinline__ f32x2* PartStats(const AttendLaunch& a) {
   return reinterpret_cast<f32x2*>(a.parts + a.part_rows * a.padded_dim);
+}
+
+// The plan that attend_join reads, in words.
+struct PlanView {
+  int* few;     // [sequences] inclusive sums of FewSteps
+  int* many;    // [groups + sequences] inclusive sums of ManyWork
+  int* todo;    // [sequences] inclusive sums of grouped sequences' row groups
+  int* first;   // [sequences] first token
+  int* rows;    // [sequences] rows a key head
+  int* group;   // [sequences] group or -1
+  int* base;    // [groups + sequences] ManyUnit::base
+  int* gfirst;  // [groups] first token
+
+  __device__ PlanView(const AttendLaunch& a, int* at) {
+    const int S = a.batch.sequences, units = S + a.groups;
+    few = at;
+    many = few + S;
+    todo = many + units;
+    first = todo + S;
+    rows = first + S;
+    group = rows + S;
+    base = group + S;
+    gfirst = base + units;
+  }
+};
+__host__ __device__ inline int PlanWords(const AttendLaunch& a) {
+  return 7 * a.batch.sequences + 3 * a.groups;
+}
+// Of those, the ones that are summed up in LDS.
+__host__ __device__ inline int PlanSumWords(const AttendLaunch& a) {
+  return 3 * a.batch.sequences + a.groups;
+}
+__device__ __forceinline__ int* Plan(const AttendLaunch& a) {
+  return reinterpret_cast<int*>(PartStats(a) + a.part_rows);
+}
+
+// Written by one workgroup of the kernel before attend_join. lds: PlanSumWords.
+__device__ __forceinline__ void WritePlan(const AttendLaunch& a, int* lds) {
+  const int S = a.batch.sequences, units = a.groups + S;
+  const PlanView here(a, lds), to(a, Plan(a));
+  for (int s = threadIdx.x; s < S; s += kAttendThreads) {
+    const OwnKeys k = LoadOwnKeys(a, s);
+    here.few[s] = FewSteps(k);
+    here.todo[s] = k.grouped ? (k.rows + a.join_rows - 1) / a.join_rows : 0;
+    to.first[s] = k.q.first;
+    to.rows[s] = k.rows;
+    to.group[s] = k.grouped ? GroupOf(a, s) : -1;
+  }
+  for (int i = threadIdx.x; i < units; i += kAttendThreads) {
+    const ManyUnit u = LoadManyUnit(a, i);
+    here.many[i] = ManyWork(a, i, u);
+    to.base[i] = u.base;
+    if (i < a.groups) to.gfirst[i] = u.first;
+  }
+  BlockSums(here.few, S);
+  BlockSums(here.many, units);
+  BlockSums(here.todo, S);
+  int* out = Plan(a);
+  for (int i = threadIdx.x; i < PlanSumWords(a); i += kAttendThreads) out[i] = lds[i];
 }
 
 // Maximum over the four 16-lane rows of a wave, lane by lane.
@@ -236,6 +356,20 @@ __device__ __forceinline__ u32x2 ReadTransposed(const void* p) {
   using Lds = __attribute__((address_space(3))) s16x4;
   return __builtin_bit_cast(
       u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p)));
+}
+
+// Eight e4m3 values times f as an operand, rounded to its type.
+template <class E>
+__device__ __forceinline__ u32x4 WidenScaled(u32x2 w, float f) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), false);
+    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), true);
+    r[2 * i] = Pack2<E>(lo[0] * f, lo[1] * f);
+    r[2 * i + 1] = Pack2<E>(hi[0] * f, hi[1] * f);
+  }
+  return r;
 }
 
 // Eight e4m3 values as an operand.
