@@ -1,5 +1,6 @@
 #include "attention_args.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <string>

@@ -7,15 +7,18 @@
 //
 // Pool of the inputs' type (append_kv_kernel): a workgroup takes a few tokens,
 // finds their sequences (all lengths at once, one a lane), puts places and
-// (cos, sin) into LDS and walks the tokens' key rows and value rows.
+// (cos, sin) into LDS; teams of lanes (head_row.h) take a token's key heads and
+// value heads in turn. Reading and writing the rows bounds it.
 //
 // e4m3 pool (append_e4m3_kernel): one fp32 scale per (block, head), so all
 // rows of a block and head have to be seen before the first is written. A
 // workgroup takes the new rows of one block, K or V, a wave the heads in turn:
 //   amax = max |x| over the finite new values
 //   new  = max(old, amax / 448),  old = 0 where no earlier token is in the block
-//   q    = e4m3(clamp(x / new, -448, 448)),
-// first reading the rows for amax, then again (from the cache) to store them.
+//   q    = e4m3(clamp(x / new, -448, 448)).
+// A wave holds kHeld rows a lane of one head in registers, all loaded before the
+// first is worked on; a block with more new rows is read once for amax and again
+// (from the cache) to be stored.
 // Earlier tokens of the block are stored again at old / new where new is
 // larger, so they keep their values within e4m3's rounding. Nothing is
 // accumulated over blocks or waves: the same call gives the same bytes.
@@ -29,7 +32,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxTokens = 16;  // of one workgroup, or of a pass over a block
+constexpr int kMaxTokens = 32;  // of one workgroup of append_kv_kernel
+constexpr int kEnough = 1024;  // workgroups
 
 __device__ __forceinline__ int FastDiv(const FastDivU32& f, int n) {
   const uint32_t u = static_cast<uint32_t>(n);
@@ -45,33 +49,32 @@ __device__ __forceinline__ int64_t RotationPosition(const AppendLaunch& a, int64
 
 template <class E, int VEC, int LPR>
 __global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch a,
-                                                             const int tokens_each) {
+                                                             const int tokens_each,
+                                                             const int teams_of_token) {
   extern __shared__ f32x2 cs[];  // [tokens_each][rotary_dim / 2]
   __shared__ int sequence[kMaxTokens], place[kMaxTokens];
   __shared__ int64_t row_at[kMaxTokens];  // first element of the token's rows, or -1
   using Scalar = typename E::Scalar;
-  constexpr int kRows = kThreads / LPR;
   const int pairs = a.rotary_dim / 2;
   const int t0 = blockIdx.x * tokens_each;
   const int nt = min(tokens_each, a.batch.tokens - t0);
-  // Rows of the workgroup: the tokens' keys, then their values, shared out
-  // over gridDim.y workgroups.
-  const int rows = nt * a.heads, step = kRows * gridDim.y;
-  int r = blockIdx.y * kRows + threadIdx.x / LPR;
   const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
-  Row<E, VEC, LPR> row;
-  int t = 0, h = 0;
-  const auto load = [&]() {
-    const int i = r < rows ? r : r - rows;
-    t = i / a.heads;
-    h = i - t * a.heads;
-    const int64_t token = t0 + t;
-    row.Load(lane, r < rows ? static_cast<const Scalar*>(a.k) + token * a.k_token + h * a.k_head
-                            : static_cast<const Scalar*>(a.v) + token * a.v_token + h * a.v_head);
+  // The team's first token and head; heads are shared out over the token's
+  // teams of gridDim.y workgroups.
+  const int team = threadIdx.x / LPR;
+  const int first = blockIdx.y * teams_of_token + team % teams_of_token;
+  const int step = teams_of_token * gridDim.y;
+  const int token_step = kThreads / LPR / teams_of_token;
+  RawRow<E, VEC, LPR> keys, values;
+  const auto load = [&](int t, int h) {
+    if (h >= a.heads) return;
+    keys.Load(lane, static_cast<const Scalar*>(a.k) + (t0 + t) * a.k_token + h * a.k_head, true);
+    values.Load(lane, static_cast<const Scalar*>(a.v) + (t0 + t) * a.v_token + h * a.v_head, false);
   };
-  if (r < 2 * rows) load();  // in flight while the places are found
-  float w[lane.kChunks][VEC], wo[lane.kChunks][VEC];
-  LoadWeights(lane, a.k_weight, a.weight_f32, w, wo);
+  int t = team / teams_of_token;
+  if (t < nt) load(t, first);  // in flight while the places are found
+  Weights<E, VEC, LPR> weights;
+  weights.Load(lane, a.k_weight, a.weight_f32);
 
   if (threadIdx.x < kMaxTokens) sequence[threadIdx.x] = -1;
   __syncthreads();
@@ -113,18 +116,20 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch 
     }
   }
   __syncthreads();
-  while (r < 2 * rows) {
+  for (; t < nt; t += token_step) {
+    const Factors<E, VEC, LPR> f(lane, cs + t * pairs, weights);
     const int64_t at = row_at[t];
-    const bool key = r < rows;
-    if (key) {
-      if (a.k_weight != nullptr) row.Norm(lane, w, wo, a.eps);
-      row.Rotate(lane, cs + t * pairs);
+    for (int h = first; h < a.heads;) {
+      const int64_t to = at + h * a.head_dim;
+      const Row<E, VEC, LPR> row(lane, keys, f, a.k_weight != nullptr, a.eps);
+      if (at >= 0) {
+        row.Store(lane, static_cast<Scalar*>(a.k_pool) + to);
+        values.Store(lane, static_cast<Scalar*>(a.v_pool) + to);
+      }
+      h += step;
+      load(t, h);
     }
-    if (at >= 0) {
-      row.Store(lane, static_cast<Scalar*>(key ? a.k_pool : a.v_pool) + at + h * a.head_dim);
-    }
-    r += step;
-    if (r < 2 * rows) load();
+    if (t + token_step < nt) load(t + token_step, first);
   }
 }
 
@@ -140,9 +145,11 @@ struct BlockRows {
 template <class E, int VEC, int LPR>
 struct E4m3Row {
   using Lane = RowLane<E, VEC, LPR>;
-  static __device__ __forceinline__ float Quantised(float x, float inverse) {
-    const float y = x * inverse;
-    return y > kE4m3Max ? kE4m3Max : y < -kE4m3Max ? -kE4m3Max : y;  // a NaN stays one
+  static __device__ __forceinline__ void Clamp(float* y) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      y[j] = y[j] > kE4m3Max ? kE4m3Max : y[j] < -kE4m3Max ? -kE4m3Max : y[j];  // NaN stays
+    }
   }
   static __device__ __forceinline__ void Store(uint8_t* p, const float* y) {
     if constexpr (VEC == 8) {
@@ -176,16 +183,18 @@ struct E4m3Row {
   }
 };
 
+constexpr int kHeld = 8;  // rows of one head that a lane holds
+
 template <class E, int VEC, int LPR>
-__global__ __launch_bounds__(kThreads) void append_e4m3_kernel(const AppendLaunch a) {
-  extern __shared__ f32x2 cs[];  // [kMaxTokens][rotary_dim / 2], then amax [heads]
+__global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLaunch a) {
+  extern __shared__ f32x2 cs[];  // [kRows][rotary_dim / 2], then amax [heads]
   __shared__ int counted[kThreads / 64];
   __shared__ BlockRows found;
   using Scalar = typename E::Scalar;
   using Q = E4m3Row<E, VEC, LPR>;
-  constexpr int kWaveRows = 64 / LPR;
+  constexpr int kWaveRows = 64 / LPR, kRows = kHeld * kWaveRows;
   const int pairs = a.rotary_dim / 2;
-  float* amax = reinterpret_cast<float*>(cs + kMaxTokens * pairs);
+  float* amax = reinterpret_cast<float*>(cs + kRows * pairs);
   const BatchView& b = a.batch;
   const int wave = threadIdx.x / 64, in_wave = threadIdx.x % 64;
 
@@ -247,15 +256,145 @@ __global__ __launch_bounds__(kThreads) void append_e4m3_kernel(const AppendLaunc
                    rows.id * (slot_bytes * b.block_tokens);
   float* scales = (key ? a.k_scales : a.v_scales) + static_cast<int64_t>(rows.id) * a.heads;
   const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
-  Row<E, VEC, LPR> row;
-  float w[lane.kChunks][VEC], wo[lane.kChunks][VEC];
-  LoadWeights(lane, key ? a.k_weight : nullptr, a.weight_f32, w, wo);
+  Weights<E, VEC, LPR> weights;
+  weights.Load(lane, key ? a.k_weight : nullptr, a.weight_f32);
   const int heads_step = kWaves * gridDim.z;
 
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int c0 = 0; c0 < rows.count; c0 += kMaxTokens) {
-      const int nc = min(kMaxTokens, rows.count - c0);
-      if (key && (pass == 0 || rows.count > kMaxTokens)) {
+  // One head of a chunk of rows, held.
+  const auto one_head = [&](auto held_rows, int pass, bool at_once, int c0, int nc, int h) {
+    constexpr int held = decltype(held_rows)::value;
+    // Row i of the chunk: lane group i % kWaveRows, register i / kWaveRows.
+    // Every lane takes part in the rows' sums; those behind the last row
+    // repeat it.
+    RawRow<E, VEC, LPR> raw[held];
+#pragma unroll
+    for (int n = 0; n < held; ++n) {
+      const int i = min(n * kWaveRows + in_wave / LPR, nc - 1);
+      raw[n].Load(lane, in + (rows.token + c0 + i) * token_stride + h * head_stride, key);
+    }
+    float x[held][lane.kChunks][VEC];
+    float largest = 0.0f;
+#pragma unroll
+    for (int n = 0; n < held; ++n) {
+      const auto keep = [&](const Row<E, VEC, LPR>& row) {
+#pragma unroll
+        for (int m = 0; m < lane.kChunks; ++m) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            x[n][m][j] = row.x[m][j];
+            largest = fmaxf(largest, fabsf(row.x[m][j]));
+          }
+        }
+      };
+      if (key) {
+        const int i = min(n * kWaveRows + in_wave / LPR, nc - 1);
+        const Factors<E, VEC, LPR> f(lane, cs + i * pairs, weights);
+        keep(Row<E, VEC, LPR>(lane, raw[n], f, a.k_weight != nullptr, a.eps));
+      } else {
+        keep(Row<E, VEC, LPR>(raw[n]));
+      }
+    }
+    // Infinities are no part of the largest value, and are clamped.
+    const bool endless = __any(largest == __builtin_inff());
+    if (endless) {
+      largest = 0.0f;
+#pragma unroll
+      for (int n = 0; n < held; ++n) {
+#pragma unroll
+        for (int m = 0; m < lane.kChunks; ++m) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float size = fabsf(x[n][m][j]);
+            largest = fmaxf(largest, size < __builtin_inff() ? size : 0.0f);
+          }
+        }
+      }
+    }
+    if (pass == 0 || at_once) {
+#pragma unroll
+      for (int m = 32; m > 0; m /= 2) largest = fmaxf(largest, __shfl_xor(largest, m));
+    }
+    if (pass == 0) {
+      if (in_wave == 0) amax[h] = fmaxf(amax[h], largest);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      return;
+    }
+    // The scale: found with the first rows, and kept in LDS for later ones as
+    // the largest value that it comes from, or as minus the scale that stays.
+    float from;
+    if (c0 == 0) {
+      float old = rows.slot > 0 ? scales[h] : 0.0f;
+      old = old > 0.0f ? old : 0.0f;
+      if (!at_once) largest = amax[h];
+      const float scale = fmaxf(old, largest / kE4m3Max);
+      const bool grown = scale > old;
+      if (grown && rows.slot > 0) {
+        const float ratio = old / scale;
+        for (int i = in_wave / LPR; i < rows.slot; i += kWaveRows) {
+          uint8_t* p = block + i * slot_bytes + h * a.head_dim;
+#pragma unroll
+          for (int n = 0; n < lane.kChunks; ++n) {
+            if (!lane.Has(n)) continue;
+            float y[VEC];
+            Q::Load(p + lane.Dim(n), y);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] *= ratio;
+            Q::Store(p + lane.Dim(n), y);
+          }
+        }
+      }
+      from = grown ? largest : -old;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (in_wave == 0) {
+        scales[h] = scale;
+        amax[h] = from;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+      from = amax[h];
+    }
+    // q = x / scale. A scale that comes from a largest value has been rounded,
+    // and rows of few bits often meet the middle between two codes, where that
+    // rounding would decide: their quotient is 0.875 x / (largest / 512), both
+    // exact, by its remainder.
+    const float part = from > 0.0f ? 0.875f : 1.0f;
+    const float whole = from > 0.0f ? from * (1.0f / 512) : -from;
+    const float inverse = whole > 0.0f ? fminf(1.0f / whole, 3.0e38f) : 0.0f;
+    // Infinities, and quotients that are not normal numbers throughout.
+    const bool clamp = endless || whole < 1.0e-30f;
+#pragma unroll
+    for (int n = 0; n < held; ++n) {
+      const int i = n * kWaveRows + in_wave / LPR;
+      if (i >= nc) continue;
+      uint8_t* p = block + (rows.slot + c0 + i) * slot_bytes + h * a.head_dim;
+#pragma unroll
+      for (int m = 0; m < lane.kChunks; ++m) {
+        if (!lane.Has(m)) continue;
+        float y[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = part * x[n][m][j] * inverse;
+        if (clamp) {
+          Q::Clamp(y);
+        } else {
+          // The quotient itself, by its remainder: bf16 rows often meet the
+          // middle between two codes, where the product's error decides.
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            y[j] = __builtin_fmaf(__builtin_fmaf(-y[j], whole, part * x[n][m][j]), inverse, y[j]);
+          }
+        }
+        Q::Store(p + lane.Dim(m), y);
+      }
+    }
+  };
+
+  // Passes: one that finds the largest values, one that stores; in one go where
+  // the new rows fit a wave's registers.
+  const bool at_once = rows.count <= kRows;
+  for (int pass = at_once ? 1 : 0; pass < 2; ++pass) {
+    for (int c0 = 0; c0 < rows.count; c0 += kRows) {
+      const int nc = min(kRows, rows.count - c0);
+      if (key && pairs > 0) {
         __syncthreads();
         for (int i = threadIdx.x; i < nc * pairs; i += kThreads) {
           const int ti = i / pairs;
@@ -265,72 +404,10 @@ __global__ __launch_bounds__(kThreads) void append_e4m3_kernel(const AppendLaunc
         __syncthreads();
       }
       for (int h = blockIdx.z * kWaves + wave; h < a.heads; h += heads_step) {
-        float scale = 0.0f, inverse = 0.0f;
-        if (pass == 1) {
-          float old = rows.slot > 0 ? scales[h] : 0.0f;
-          old = old > 0.0f ? old : 0.0f;
-          // After the first rows the table holds the new scale already.
-          scale = c0 == 0 ? fmaxf(old, amax[h] / kE4m3Max) : amax[h];
-          inverse = scale > 0.0f ? fminf(1.0f / scale, 3.0e38f) : 0.0f;
-          if (c0 == 0) {
-            if (scale > old && rows.slot > 0) {
-              const float ratio = old / scale;
-              for (int i = in_wave / LPR; i < rows.slot; i += kWaveRows) {
-                uint8_t* p = block + i * slot_bytes + h * a.head_dim;
-#pragma unroll
-                for (int n = 0; n < lane.kChunks; ++n) {
-                  if (!lane.Has(n)) continue;
-                  float y[VEC];
-                  Q::Load(p + lane.Dim(n), y);
-#pragma unroll
-                  for (int j = 0; j < VEC; ++j) y[j] *= ratio;
-                  Q::Store(p + lane.Dim(n), y);
-                }
-              }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (in_wave == 0) {
-              scales[h] = scale;
-              amax[h] = scale;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          }
-        }
-        float largest = 0.0f;
-        // Every lane takes part in the rows' sums, so all make the same steps.
-        for (int i0 = 0; i0 < nc; i0 += kWaveRows) {
-          const int i = min(i0 + in_wave / LPR, nc - 1);
-          row.Load(lane, in + (rows.token + c0 + i) * token_stride + h * head_stride);
-          if (key) {
-            if (a.k_weight != nullptr) row.Norm(lane, w, wo, a.eps);
-            row.Rotate(lane, cs + i * pairs);
-          }
-          if (pass == 0) {
-#pragma unroll
-            for (int n = 0; n < lane.kChunks; ++n) {
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) {
-                const float x = fabsf(row.x[n][j]);
-                largest = fmaxf(largest, x < __builtin_inff() ? x : 0.0f);
-              }
-            }
-          } else {
-            uint8_t* p = block + (rows.slot + c0 + i) * slot_bytes + h * a.head_dim;
-#pragma unroll
-            for (int n = 0; n < lane.kChunks; ++n) {
-              if (!lane.Has(n)) continue;
-              float y[VEC];
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) y[j] = Q::Quantised(row.x[n][j], inverse);
-              Q::Store(p + lane.Dim(n), y);
-            }
-          }
-        }
-        if (pass == 0) {
-#pragma unroll
-          for (int m = 32; m > 0; m /= 2) largest = fmaxf(largest, __shfl_xor(largest, m));
-          if (in_wave == 0) amax[h] = fmaxf(amax[h], largest);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (nc <= kWaveRows) {
+          one_head(std::integral_constant<int, 1>{}, pass, at_once, c0, nc, h);
+        } else {
+          one_head(std::integral_constant<int, kHeld>{}, pass, at_once, c0, nc, h);
         }
       }
     }
@@ -351,23 +428,20 @@ hipError_t Launch(const AppendLaunch& l, hipStream_t stream) {
                                             2 * static_cast<int64_t>(l.batch.sequences));
     // Few blocks: their heads spread over workgroups.
     int split = 1;
-    while (split * kWaves < l.heads && blocks * 2 * split < 512) ++split;
+    while (split * kWaves < l.heads && blocks * 2 * split < 1024) ++split;
     const dim3 grid(static_cast<unsigned>(blocks), 2, split);
-    const size_t lds = kMaxTokens * pairs + static_cast<size_t>(l.heads) * sizeof(float);
+    const size_t lds = kHeld * (64 / LPR) * pairs +
+                       static_cast<size_t>(l.heads) * sizeof(float);
     hipLaunchKernelGGL((append_e4m3_kernel<E, VEC, LPR>), grid, dim3(kThreads), lds, stream, l);
     return hipGetLastError();
   }
-  constexpr int kRows = kThreads / LPR;
-  int each = 1, split = 1;
-  if (tokens > 1024) {
-    while (each < kMaxTokens && each * l.heads < 64) each *= 2;
-  } else {
-    const int groups = (2 * l.heads + kRows - 1) / kRows;
-    while (split < groups && tokens * split < 512) ++split;
-  }
+  const int of_token = TeamsOfToken(l.heads, LPR);
+  int each = kThreads / LPR / of_token, split = 1;
+  while (each < kMaxTokens && tokens / each >= 2 * kEnough) each *= 2;
+  while (split * of_token < l.heads && static_cast<int64_t>(tokens) * split < 2048) ++split;
   const dim3 grid((tokens + each - 1) / each, split);
   hipLaunchKernelGGL((append_kv_kernel<E, VEC, LPR>), grid, dim3(kThreads), each * pairs, stream,
-                     l, each);
+                     l, each, of_token);
   return hipGetLastError();
 }
 

@@ -7,10 +7,12 @@
 // dimensions; the rest keep y. Everything between the load and the store is
 // fp32 (the angle is reduced in 64 bits), so a value is rounded once.
 //
-// A workgroup takes a few tokens: it puts their R/2 (cos, sin) into LDS once
-// for all heads (one sincos a token and pair instead of one a head), then its
-// waves walk the tokens' rows, 16-byte chunks across the lanes.
+// A workgroup takes a few tokens and puts their R/2 (cos, sin) into LDS, one
+// sincos a token and pair for all heads. Then teams of lanes (head_row.h) take a
+// token's heads in turn. Reading and writing the rows bounds it.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "head_row.h"
 #include "norm_rope.h"
@@ -19,7 +21,8 @@ namespace kvx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;  // of one workgroup
+constexpr int kMaxTokens = 32;  // of one workgroup
+constexpr int kEnough = 1024;  // workgroups
 
 __device__ __forceinline__ int64_t Position(const NormRopeLaunch& a, int64_t t) {
   return a.positions_64 ? static_cast<const int64_t*>(a.positions)[t]
@@ -28,82 +31,67 @@ __device__ __forceinline__ int64_t Position(const NormRopeLaunch& a, int64_t t) 
 
 template <class E, int VEC, int LPR>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeLaunch a,
-                                                             const int tokens_each) {
+                                                             const int tokens_each,
+                                                             const int teams_of_token) {
   extern __shared__ f32x2 cs[];  // [tokens_each][rotary_dim / 2]
   using Scalar = typename E::Scalar;
-  constexpr int kRows = kThreads / LPR;
   const int pairs = a.rotary_dim / 2;
   const int t0 = blockIdx.x * tokens_each;
   const int nt = min(tokens_each, a.tokens - t0);
-  const int heads = a.q.heads + a.k.heads;
-  // The heads of a token are shared out over gridDim.y workgroups.
-  const int step = kRows * gridDim.y;
-  int h = blockIdx.y * kRows + threadIdx.x / LPR, t = 0;
-  while (h >= heads) {
-    h -= heads;
-    ++t;
-  }
   const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
-  Row<E, VEC, LPR> row;
-  const auto load = [&]() {
-    const bool is_q = h < a.q.heads;
-    const int64_t token = t0 + t;
-    const int64_t at = is_q ? token * a.q.in_token + h * a.q.in_head
-                            : token * a.k.in_token + (h - a.q.heads) * a.k.in_head;
-    row.Load(lane, static_cast<const Scalar*>(is_q ? a.q.in : a.k.in) + at);
+  // The team's first token and head; heads are shared out over the token's
+  // teams of gridDim.y workgroups.
+  const int team = threadIdx.x / LPR;
+  const int first = blockIdx.y * teams_of_token + team % teams_of_token;
+  const int step = teams_of_token * gridDim.y;
+  const int token_step = kThreads / LPR / teams_of_token;
+  RawRow<E, VEC, LPR> raw;
+  const auto load = [&](const HeadRows& rows, int t, int h) {
+    if (h >= rows.heads) return;
+    raw.Load(lane, static_cast<const Scalar*>(rows.in) + (t0 + t) * rows.in_token + h * rows.in_head,
+             true);
   };
-  if (t < nt) load();  // in flight while the angles are computed
-  float wq[lane.kChunks][VEC], wqo[lane.kChunks][VEC], wk[lane.kChunks][VEC],
-      wko[lane.kChunks][VEC];
-  LoadWeights(lane, a.q.weight, a.weight_f32, wq, wqo);
-  LoadWeights(lane, a.k.weight, a.weight_f32, wk, wko);
+  int t = team / teams_of_token;
+  if (t < nt) load(a.q, t, first);  // in flight while the angles are computed
+  Weights<E, VEC, LPR> q_weights, k_weights;
+  q_weights.Load(lane, a.q.weight, a.weight_f32);
+  k_weights.Load(lane, a.k.weight, a.weight_f32);
   for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
     const int ti = i / pairs;
     cs[i] = Turn(Position(a, t0 + ti), a.inv_freq[i - ti * pairs]);
   }
   __syncthreads();
-  while (t < nt) {
-    const bool is_q = h < a.q.heads;
-    if ((is_q ? a.q.weight : a.k.weight) != nullptr) {
-      if (is_q) {
-        row.Norm(lane, wq, wqo, a.eps);
-      } else {
-        row.Norm(lane, wk, wko, a.eps);
-      }
+  const auto heads_of = [&](const HeadRows& rows, const Weights<E, VEC, LPR>& weights) {
+    const Factors<E, VEC, LPR> f(lane, cs + t * pairs, weights);
+    Scalar* out = static_cast<Scalar*>(rows.out) + (t0 + t) * rows.out_token;
+    for (int h = first; h < rows.heads;) {
+      const Row<E, VEC, LPR> row(lane, raw, f, rows.weight != nullptr, a.eps);
+      row.Store(lane, out + h * rows.out_head);
+      h += step;
+      load(rows, t, h);
     }
-    row.Rotate(lane, cs + t * pairs);
-    const int64_t token = t0 + t;
-    if (is_q) {
-      row.Store(lane, static_cast<Scalar*>(a.q.out) + token * a.q.out_token + h * a.q.out_head);
-    } else {
-      row.Store(lane, static_cast<Scalar*>(a.k.out) + token * a.k.out_token +
-                          (h - a.q.heads) * a.k.out_head);
-    }
-    h += step;
-    while (h >= heads) {
-      h -= heads;
-      ++t;
-    }
-    if (t < nt) load();
+  };
+  for (; t < nt; t += token_step) {
+    heads_of(a.q, q_weights);
+    load(a.k, t, first);
+    heads_of(a.k, k_weights);
+    if (t + token_step < nt) load(a.q, t + token_step, first);
   }
 }
 
 template <class E, int VEC, int LPR>
 hipError_t Launch(const NormRopeLaunch& l, hipStream_t stream) {
-  constexpr int kRows = kThreads / LPR;
-  const int heads = l.q.heads + l.k.heads;
-  // About 64 rows a workgroup, so the angles are shared out over many; with
-  // few tokens one each, and their heads spread over workgroups too.
-  int each = 1, split = 1;
-  if (l.tokens > 1024) {
-    while (each < kMaxTokens && each * heads < 64) each *= 2;
-  } else {
-    const int groups = (heads + kRows - 1) / kRows;
-    while (split < groups && l.tokens * split < 512) ++split;
-  }
+  const int heads = std::max(l.q.heads, l.k.heads);
+  const int of_token = TeamsOfToken(heads, LPR);
+  // Some tokens for every team or teams of one, so the angles' latency is paid
+  // once; with few tokens one, and their heads spread over workgroups too.
+  int each = kThreads / LPR / of_token, split = 1;
+  while (each < kMaxTokens && l.tokens / each >= 2 * kEnough) each *= 2;
+  while (split * of_token < heads && static_cast<int64_t>(l.tokens) * split < 2048) ++split;
   const dim3 grid((l.tokens + each - 1) / each, split);
   const size_t lds = static_cast<size_t>(each) * (l.rotary_dim / 2) * sizeof(f32x2);
-  hipLaunchKernelGGL((norm_rope_kernel<E, VEC, LPR>), grid, dim3(kThreads), lds, stream, l, each);
+  hipLaunchKernelGGL((norm_rope_kernel<E, VEC, LPR>), grid, dim3(kThreads), lds, stream, l, each,
+                     of_token);
   return hipGetLastError();
 }
 
