@@ -38,12 +38,7 @@ constexpr size_t FewLds(const AttendLaunch& l, int dp) {
 
 template <class E, bool E4, int DP, int RT, bool FULL>
 __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int workgroup) {
-  using P = std::conditional_t<E4 && !std::is_same_v<E, F16>, Bf16, E>;  // of the second product
   using Scalar = typename E::Scalar;
-  // e4m3 values: in bf16 they are exact and their scale goes to the
-  // exponentials; a scaled exponential would leave fp16's range, so there the
-  // scale goes to the values.
-  constexpr bool kScaleValues = E4 && std::is_same_v<E, F16>;
   constexpr int KS = DP / 32, DT = DP / 16, VST = FewValueStride(DP);
   const BatchView& b = a.batch;
   int* sums = reinterpret_cast<int*>(lds + kWaves * 32 * VST);  // [sequences]
@@ -210,13 +205,16 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           for (int rt = 0; rt < RT; ++rt) sc[rt][u] = Mma16<E>(key, q[rt][ks], sc[rt][u]);
         }
       }
-      float vs[8];  // scales of the values of the lane's tokens
-      float vl[2] = {vf[0], vf[1]};  // and of those that it loads
+      float vs[8];  // scales, or their rests, of the values of the lane's tokens
+      float power[2] = {1, 1};  // and powers of those that it loads
       if constexpr (E4) {
+        const float rest[2] = {ValueRest<E>(vf[0]), ValueRest<E>(vf[1])};
+        power[0] = ValuePower<E>(vf[0]);
+        power[1] = ValuePower<E>(vf[1]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float f = __shfl(kf[i / 4], quarter * 4 + i % 4);
-          if constexpr (!kScaleValues) vs[i] = __shfl(vf[i / 4], quarter * 4 + i % 4);
+          vs[i] = __shfl(rest[i / 4], quarter * 4 + i % 4);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) sc[rt][i / 4][i % 4] *= f;
         }
@@ -274,15 +272,15 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           e[i] = __builtin_amdgcn_exp2f(fmaf(sc[rt][i / 4][i % 4], c, -base));
           sum[rt] += e[i];
         }
-        if constexpr (E4 && !kScaleValues) {
+        if constexpr (E4) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             // A hidden token's scale may be anything.
             e[i] = e[i] == 0.0f ? 0.0f : e[i] * vs[i];
           }
         }
-        pw[rt] = u32x4{Pack2<P>(e[0], e[1]), Pack2<P>(e[2], e[3]), Pack2<P>(e[4], e[5]),
-                       Pack2<P>(e[6], e[7])};
+        pw[rt] = u32x4{Pack2<E>(e[0], e[1]), Pack2<E>(e[2], e[3]), Pack2<E>(e[4], e[5]),
+                       Pack2<E>(e[6], e[7])};
       }
       if ((valid[0] & valid[1]) != 0xffffu) {
 #pragma unroll
@@ -290,7 +288,6 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           if ((valid[u] >> in16 & 1) == 0) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) vw[u][ks] = Words(0);
-            vl[u] = 0.0f;
           }
         }
       }
@@ -299,10 +296,8 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           u32x4 value;
-          if constexpr (kScaleValues) {
-            value = WidenScaled<P>(vw[u][ks], vl[u]);
-          } else if constexpr (E4) {
-            value = Widen<P>(vw[u][ks]);
+          if constexpr (E4) {
+            value = Widen<E>(vw[u][ks], power[u]);
           } else {
             value = vw[u][ks];
           }
@@ -319,7 +314,7 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
         const u32x2 lo = ReadTransposed(p), hi = ReadTransposed(p + 16 * VST);
         const u32x4 value = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = Mma16<P>(value, pw[rt], o[rt][dt]);
+        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = Mma16<E>(value, pw[rt], o[rt][dt]);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }

@@ -57,8 +57,6 @@ constexpr size_t ManyLds(const AttendLaunch& l, int dp) {
 
 template <class E, bool E4, int DP>
 __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int worker) {
-  constexpr bool kScaleValues = E4 && std::is_same_v<E, F16>;  // as in AttendFew
-  using P = std::conditional_t<E4 && !kScaleValues, Bf16, E>;
   using Scalar = typename E::Scalar;
   constexpr int KS = DP / 16, DT = DP / 32, kRow = 2 * DP;  // bytes of a token's row
   constexpr int kChunks = kManyStep * (DP / 8) / kAttendThreads;  // of a thread
@@ -232,11 +230,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
         u32x4 k, v;
         if constexpr (E4) {
           k = Widen<E>(kw[n]);
-          if constexpr (kScaleValues) {
-            v = WidenScaled<P>(vw[n], held.at[tok] >= 0 ? held.v_scale[tok] : 0.0f);
-          } else {
-            v = Widen<P>(vw[n]);
-          }
+          v = Widen<E>(vw[n], ValuePower<E>(held.v_scale[tok]));
         } else {
           k = kw[n];
           v = vw[n];
@@ -288,15 +282,6 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
             sc[u] = Mma32<E>(key, q[ks], sc[u]);
           }
         }
-#if KVX_SCHED & 1
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-        for (int n = 0; n < 2 * KS - 6; ++n) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
-#endif
         // Lane: row l % 32, tokens 32 u + 8 (i / 4) + 4 (l / 32) + i % 4.
         if constexpr (E4) {
 #pragma unroll
@@ -347,7 +332,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
             sum += sc[u][i];
           }
         }
-        if constexpr (E4 && !kScaleValues) {
+        if constexpr (E4) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -357,7 +342,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 // A hidden token's scale may be anything.
-                sc[u][i + j] = sc[u][i + j] == 0.0f ? 0.0f : sc[u][i + j] * f[j];
+                sc[u][i + j] = sc[u][i + j] == 0.0f ? 0.0f : sc[u][i + j] * ValueRest<E>(f[j]);
               }
             }
           }
@@ -365,9 +350,9 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const int u = kk / 2, i = kk % 2 * 8;
-          const u32x4 p = {Pack2<P>(sc[u][i], sc[u][i + 1]), Pack2<P>(sc[u][i + 2], sc[u][i + 3]),
-                           Pack2<P>(sc[u][i + 4], sc[u][i + 5]),
-                           Pack2<P>(sc[u][i + 6], sc[u][i + 7])};
+          const u32x4 p = {Pack2<E>(sc[u][i], sc[u][i + 1]), Pack2<E>(sc[u][i + 2], sc[u][i + 3]),
+                           Pack2<E>(sc[u][i + 4], sc[u][i + 5]),
+                           Pack2<E>(sc[u][i + 6], sc[u][i + 7])};
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             // Row 4 half + l % 16 / 4 of 8, 8 bytes l % 4 of the 32 of l / 16 % 2.
@@ -375,7 +360,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
             const int chunk = dt * 4 + lane / 16 % 2 * 2 + lane % 4 / 2;
             const char* v = values + r * kRow + ValueChunk<DP>(r, chunk) * 16 + lane % 2 * 8;
             const u32x2 lo = ReadTransposed(v), hi = ReadTransposed(v + 8 * kRow);
-            o[dt] = Mma32<P>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[dt]);
+            o[dt] = Mma32<E>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[dt]);
           }
         }
       }

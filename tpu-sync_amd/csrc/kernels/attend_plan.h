@@ -358,25 +358,29 @@ __device__ __forceinline__ u32x2 ReadTransposed(const void* p) {
       u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(p)));
 }
 
-// Eight e4m3 values times f as an operand, rounded to its type.
+// Eight e4m3 values times a power of two as an operand.
 template <class E>
-__device__ __forceinline__ u32x4 WidenScaled(u32x2 w, float f) {
-  u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), false);
-    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), true);
-    r[2 * i] = Pack2<E>(lo[0] * f, lo[1] * f);
-    r[2 * i + 1] = Pack2<E>(hi[0] * f, hi[1] * f);
-  }
-  return r;
+__device__ __forceinline__ u32x4 Widen(u32x2 w, float power = 1.0f) {
+  return u32x4{FromE4m3<E>(w[0], false, power), FromE4m3<E>(w[0], true, power),
+               FromE4m3<E>(w[1], false, power), FromE4m3<E>(w[1], true, power)};
 }
 
-// Eight e4m3 values as an operand.
+// The scale of e4m3 values goes to the exponentials, so that the values stay
+// exact and a product is rounded once. In bf16 all of it does; an exponential,
+// up to 2^8, that takes it could leave fp16's range, so there the values take its
+// power of two, as far as they stay exact, and the exponentials the rest.
 template <class E>
-__device__ __forceinline__ u32x4 Widen(u32x2 w) {
-  return u32x4{FromE4m3<E>(w[0], false), FromE4m3<E>(w[0], true), FromE4m3<E>(w[1], false),
-               FromE4m3<E>(w[1], true)};
+__device__ __forceinline__ float ValuePower(float scale) {
+  if constexpr (!std::is_same_v<E, F16>) return 1.0f;
+  const float power = __builtin_bit_cast(
+      float, __builtin_bit_cast(uint32_t, scale) & 0x7f800000u);
+  return fminf(fmaxf(power, 1.0f / 256), 128.0f);
+}
+template <class E>
+__device__ __forceinline__ float ValueRest(float scale) {
+  if constexpr (!std::is_same_v<E, F16>) return scale;
+  return scale * __builtin_bit_cast(
+      float, 0x7f000000u - __builtin_bit_cast(uint32_t, ValuePower<E>(scale)));
 }
 
 }  // namespace kvx

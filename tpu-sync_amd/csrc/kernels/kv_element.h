@@ -85,22 +85,21 @@ __device__ __forceinline__ f32x2 Unpack2(uint32_t w) {
   return __builtin_convertvector(__builtin_bit_cast(typename E::V2, w), f32x2);
 }
 
-// The two e4m3 values in half `hi` of w, exact in either 16-bit type.
+// The two e4m3 values in half `hi` of w, times a power of two: exact in either
+// 16-bit type for powers from 2^-8 to 2^7.
 template <class E>
-__device__ __forceinline__ uint32_t FromE4m3(uint32_t w, bool hi);
-template <>
-__device__ __forceinline__ uint32_t FromE4m3<Bf16>(uint32_t w, bool hi) {
-  return hi ? __builtin_bit_cast(uint32_t,
-                                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
-            : __builtin_bit_cast(uint32_t,
-                                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-}
-template <>
-__device__ __forceinline__ uint32_t FromE4m3<F16>(uint32_t w, bool hi) {
-  return hi ? __builtin_bit_cast(uint32_t,
-                                 __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
-            : __builtin_bit_cast(uint32_t,
-                                 __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+__device__ __forceinline__ uint32_t FromE4m3(uint32_t w, bool hi, float power) {
+  if constexpr (std::is_same_v<E, F16>) {
+    return hi ? __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, true))
+              : __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, false));
+  } else {
+    return hi ? __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, true))
+              : __builtin_bit_cast(uint32_t,
+                                   __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, false));
+  }
 }
 
 struct SequenceSpan {
