@@ -424,6 +424,10 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
     *workspace_bytes = need;
     return OkStatus();
   }
+  if (!out->e4m3 && (reinterpret_cast<uintptr_t>(out->k_pool) |
+                     reinterpret_cast<uintptr_t>(out->v_pool)) % 16 != 0) {
+    return Bad("cache storages: must be aligned to 16 bytes");
+  }
   if (need > 0) {
     if (a.workspace_bytes < need) {
       return Bad("workspace: " + std::to_string(need) + " bytes are needed");

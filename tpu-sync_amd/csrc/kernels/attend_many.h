@@ -2,14 +2,25 @@
 // of sequences that share a prefix against that prefix.
 //
 // A workgroup takes a tile of 128 rows, 32 a wave, and steps through its keys
-// 64 at a time: the tile of K and V lies in LDS for all four waves, the next
-// one is on its way from memory in registers. Matrix instructions bound it,
-// so the layout keeps everything between the two products in place: S^T = K Q^T
-// in 32 x 32 x 16 products leaves lane l with the scores of row l % 32, so a
-// row's maximum takes one swap between the wave's halves, and the packed
-// exponentials are the operand of O^T = V^T P^T as they stand (the contraction
-// runs over tokens in the order that the scores lie in). V is transposed by
-// the LDS reads.
+// 64 at a time; K and V of a step lie in LDS for all four waves. Matrix
+// instructions bound it, so the layout keeps everything between the two products
+// in place: S^T = K Q^T in 32 x 32 x 16 products leaves lane l with the scores of
+// row l % 32, so a row's maximum takes one swap between the wave's halves, and
+// the packed exponentials are the operand of O^T = V^T P^T as they stand (the
+// contraction runs over tokens in the order that the scores lie in). V is
+// transposed by the LDS reads.
+//
+// A wave works in halves of a step: the scores of the next 32 tokens are on the
+// matrix cores while the exponentials of these are taken, and their operands are
+// read four products ahead. Tokens go from memory straight into LDS, each storage
+// refilled as soon as its last reader is past a barrier: keys run two steps
+// ahead, values one, so K and V need two buffers each and no registers. (e4m3
+// tokens are widened on the way, in registers.) 4099 new tokens of 32 heads on 8
+// over 7000 keys in bf16, D = 128: 730 us with tokens passing through registers
+// and a wave's products and exponentials in turn, 676 us without, 655 us with
+// operands read ahead and products given priority, 611 us with the places of
+// tokens kept as byte offsets (885 TFLOP/s, where an 8192^3 product of the library
+// reaches 1211).
 //
 // Work. The tiles of all groups and sequences make one axis, weighed by the
 // keys they see, and every workgroup gets an equal part of it: no tail of late
@@ -42,9 +53,26 @@ __device__ __forceinline__ int ValueChunk(int r, int chunk) {
   return chunk ^ (r % 4 * 4);
 }
 
+__device__ __forceinline__ uint32_t LdsAddress(char* p) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)p));
+}
+// Loads 16 bytes a lane straight into LDS, lane l's to address `to` + 16 l. The
+// compiler does not know of them: LdsArrived waits for all but the last N.
+__device__ __forceinline__ void ToLds16(const void* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(to), "v"(from)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void LdsArrived() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
 // Places of a step's tokens: looked up three steps ahead, their scales two.
 struct Places {
-  int64_t at[kManyStep];  // element offset of the token's row, or -1
+  int64_t at[kManyStep];  // byte offset of the token's row; without one, of the first
   int32_t id[kManyStep];  // its block, or -1
   float k_scale[kManyStep], v_scale[kManyStep];
   uint64_t present;  // one bit a token
@@ -65,7 +93,15 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
   int* sums = reinterpret_cast<int*>(places + 4);  // [groups + sequences]
   const BatchView& b = a.batch;
   const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  using Words = u32x2;  // e4m3 values of a chunk
+  const uint32_t lds_at = one(LdsAddress(lds));
 
+  // Dimensions behind the last one are never written.
+  if (!E4 && a.head_dim < DP) {
+    for (int i = threadIdx.x; i < 2 * kTile / 16; i += kAttendThreads) {
+      reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
+    }
+  }
   const int units = a.groups + b.sequences;
   for (int i = threadIdx.x; i < units; i += kAttendThreads) {
     sums[i] = ManyWork(a, i, LoadManyUnit(a, i));
@@ -181,9 +217,8 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
       const int p = begin + step * kManyStep + lane;
       const bool is = found >= 0 && found < b.num_blocks;
       const int slot = p - FastDivI(a.block_div, p) * b.block_tokens;
-      to.at[lane] = is ? (static_cast<int64_t>(found) * b.block_tokens + slot) * row_stride +
-                             h * a.head_dim
-                       : -1;
+      const int64_t row = is ? static_cast<int64_t>(found) * b.block_tokens + slot : 0;
+      to.at[lane] = (row * row_stride + h * a.head_dim) * (E4 ? 1 : 2);
       to.id[lane] = is ? found : -1;
       const uint64_t present = __ballot(is);
       if (lane == 0) to.present = present;
@@ -198,53 +233,133 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
       places[step & 3].k_scale[lane] = found_k;
       places[step & 3].v_scale[lane] = found_v;
     };
-    constexpr int W = E4 ? 2 : 4;
-    using Words = __attribute__((ext_vector_type(W))) uint32_t;
-    Words kw[kChunks], vw[kChunks];
-    const auto load = [&](int step) {
+    // Tokens of a step on their way into LDS: e4m3 ones widened in registers,
+    // others straight from memory, a wave's 64 chunks at a time. A token without
+    // a place reads the pool's first row, so that this needs no branch.
+    Words w[kChunks];
+    const auto load = [&](int step, const void* pool) {
+      const Places& held = places[step & 3];
+      int64_t at[kChunks];
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int d = chunk % (DP / 8) * 8;
+        at[n] = held.at[chunk / (DP / 8)] + (d < a.head_dim ? d : 0);
+      }
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        w[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(pool) + at[n]);
+      }
+    };
+    const auto store = [&](int step, auto is_key) {
+      char* to = lds + (is_key() ? 0 : kTile) + (step & 1) * (kTile / 2);
       const Places& held = places[step & 3];
 #pragma unroll
       for (int n = 0; n < kChunks; ++n) {
         const int chunk = threadIdx.x + n * kAttendThreads;
         const int tok = chunk / (DP / 8), d = chunk % (DP / 8) * 8;
-        const int64_t at = held.at[tok];
-        kw[n] = vw[n] = Words(0);
-        if (at >= 0 && d < a.head_dim) {
-          if constexpr (E4) {
-            kw[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(a.k_pool) + at + d);
-            vw[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(a.v_pool) + at + d);
-          } else {
-            kw[n] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) + at + d);
-            vw[n] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.v_pool) + at + d);
-          }
+        const int at = is_key() ? KeyChunk<DP>(tok, d / 8) : ValueChunk<DP>(tok, d / 8);
+        const bool is = (held.present >> tok & 1) != 0 && d < a.head_dim;
+        *reinterpret_cast<u32x4*>(to + tok * kRow + at * 16) =
+            Widen<E>(is ? w[n] : Words(0), is_key() ? 1.0f : ValuePower<E>(held.v_scale[tok]));
+      }
+    };
+    const auto fetch = [&](int step, const void* pool, auto is_key) {
+      const Places& held = places[step & 3];
+      const uint32_t to = lds_at + (is_key() ? 0 : kTile) + (step & 1) * (kTile / 2) + wave * 1024;
+      const auto from = [&](int n, int& d) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int tok = chunk / (DP / 8), c = chunk % (DP / 8);
+        d = (is_key() ? KeyChunk<DP>(tok, c) : ValueChunk<DP>(tok, c)) * 8;
+        return static_cast<const char*>(pool) + d * 2 + held.at[tok];
+      };
+      const char* at[kChunks];
+      int d[kChunks];
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) at[n] = from(n, d[n]);
+      if (a.head_dim == DP) {
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) ToLds16(at[n], to + n * kAttendThreads * 16);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kChunks; ++n) {
+          if (d[n] < a.head_dim) ToLds16(at[n], to + n * kAttendThreads * 16);
         }
       }
     };
-    const auto store = [&](int step) {
-      char* to = lds + (step & 1) * kTile;
+    // Values of tokens without a place are cleared once they are there (their
+    // scores are masked, whatever their keys are).
+    const auto clear = [&](int step) {
       const Places& held = places[step & 3];
+      if (held.present == ~uint64_t{0}) return;
 #pragma unroll
       for (int n = 0; n < kChunks; ++n) {
         const int chunk = threadIdx.x + n * kAttendThreads;
-        const int tok = chunk / (DP / 8), d = chunk % (DP / 8) * 8;
-        u32x4 k, v;
-        if constexpr (E4) {
-          k = Widen<E>(kw[n]);
-          v = Widen<E>(vw[n], ValuePower<E>(held.v_scale[tok]));
-        } else {
-          k = kw[n];
-          v = vw[n];
+        if ((held.present >> (chunk / (DP / 8)) & 1) == 0) {
+          *reinterpret_cast<u32x4*>(lds + kTile + (step & 1) * (kTile / 2) + chunk * 16) =
+              u32x4{0, 0, 0, 0};
         }
-        *reinterpret_cast<u32x4*>(to + tok * kRow + KeyChunk<DP>(tok, d / 8) * 16) = k;
-        *reinterpret_cast<u32x4*>(to + kTile / 2 + tok * kRow + ValueChunk<DP>(tok, d / 8) * 16) = v;
       }
     };
+    constexpr std::true_type kKeys{};
+    constexpr std::false_type kValues{};
 
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16(0.0f);
     float top = -__builtin_inff(), sum = 0.0f;
     const float c = a.scale * kLog2e;
+    // Scores of half a step. Lane: row l % 32, tokens 8 (i / 4) + 4 (l / 32) + i % 4.
+    const auto scores = [&](int step, int u) {
+      const char* keys = lds + (step & 1) * (kTile / 2);
+      f32x16 sc = f32x16(0.0f);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 key = *reinterpret_cast<const u32x4*>(
+            keys + (u * 32 + in32) * kRow + KeyChunk<DP>(u * 32 + in32, ks * 2 + half) * 16);
+        sc = Mma32<E>(key, q[ks], sc);
+      }
+      return sc;
+    };
+    // Scales and masks them, and moves the maximum.
+    const auto settle = [&](int step, int u, f32x16& sc) {
+      const Places& here = places[step & 3];
+      if constexpr (E4) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(&here.k_scale[u * 32 + i * 2 + half * 4]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i + j] *= f[j];
+        }
+      }
+      const int p0 = begin + step * kManyStep + u * 32;
+      const uint32_t present = static_cast<uint32_t>(here.present >> (u * 32));
+      if (p0 + 32 > least || present != ~uint32_t{0}) {
+        // Token n of the half is number n + 4 half of its lane's.
+        const int behind = seen - p0 - half * 4;
+        const uint32_t there = present >> (half * 4);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int n = (i / 4) * 8 + i % 4;
+          if (n >= behind || (there & (1u << n)) == 0) sc[i] = -__builtin_inff();
+        }
+      }
+      float most = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) most = fmaxf(most, sc[i]);
+      most = Across32(most) * c;
+      // The maximum is only moved when it falls behind by 2^8.
+      if (__any(most > top + 8.0f)) {
+        const float now = fmaxf(top, most);
+        const float back = now == -__builtin_inff() ? 0.0f : now;
+        const float shrink = __builtin_amdgcn_exp2f(top - back);
+        top = now;
+        sum *= shrink;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= shrink;
+      }
+    };
+    f32x16 sc;
     if (step0 < step1) {
       if (wave < 3) {
         find(step0 + wave);
@@ -258,115 +373,121 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
         }
       }
       __syncthreads();
-      load(step0);
-      store(step0);
-    }
-    for (int step = step0; step < step1; ++step) {
+      if constexpr (E4) {
+        load(step0, a.k_pool);
+        store(step0, kKeys);
+        load(step0 + 1, a.k_pool);
+        store(step0 + 1, kKeys);
+        load(step0, a.v_pool);
+        store(step0, kValues);
+      } else {
+        fetch(step0, a.k_pool, kKeys);
+        fetch(step0, a.v_pool, kValues);
+        fetch(step0 + 1, a.k_pool, kKeys);
+        LdsArrived<0>();
+        clear(step0);
+      }
       __syncthreads();
-      const bool finds = wave == (step & 3), finds_scales = E4 && wave == ((step + 1) & 3);
-      if (finds) find(step + 3);
-      if (finds_scales) find_scales(step + 2);
-      if (step + 1 < step1) load(step + 1);
-      const Places& here = places[step & 3];
-      const int p0 = begin + step * kManyStep;
-      if (p0 < most_seen) {
-        const char* keys = lds + (step & 1) * kTile;
-        const char* values = keys + kTile / 2;
-        f32x16 sc[2] = {f32x16(0.0f), f32x16(0.0f)};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u32x4 key = *reinterpret_cast<const u32x4*>(
-                keys + (u * 32 + in32) * kRow + KeyChunk<DP>(u * 32 + in32, ks * 2 + half) * 16);
-            sc[u] = Mma32<E>(key, q[ks], sc[u]);
-          }
-        }
-        // Lane: row l % 32, tokens 32 u + 8 (i / 4) + 4 (l / 32) + i % 4.
+      sc = scores(step0, 0);
+      settle(step0, 0, sc);
+      for (int step = step0; step < step1; ++step) {
+        if (step > step0) __syncthreads();
+        const bool finds = wave == (step & 3), finds_scales = E4 && wave == ((step + 1) & 3);
+        if (finds) find(step + 3);
+        if (finds_scales) find_scales(step + 2);
+        // Keys two steps ahead and values one: the keys of this step go when the
+        // scores of its second half are there, the values at its end.
         if constexpr (E4) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const f32x4 f =
-                  *reinterpret_cast<const f32x4*>(&here.k_scale[u * 32 + i * 2 + half * 4]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sc[u][i + j] *= f[j];
-            }
-          }
+          load(step + 2, a.k_pool);
+        } else {
+          fetch(step + 1, a.v_pool, kValues);
         }
-        const uint64_t present = here.present;
-        if (p0 + kManyStep > least || present != ~uint64_t{0}) {
-          // Token 32 u + n of the step is number n + 4 half of its lane's.
-          const int behind = seen - p0 - half * 4;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t there = static_cast<uint32_t>(present >> (u * 32)) >> (half * 4);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int n = (i / 4) * 8 + i % 4;
-              if (u * 32 + n >= behind || (there & (1u << n)) == 0) sc[u][i] = -__builtin_inff();
-            }
-          }
-        }
-        float most = sc[0][0];
-#pragma unroll
-        for (int i = 1; i < 32; ++i) most = fmaxf(most, sc[i / 16][i % 16]);
-        most = Across32(most) * c;
-        // The maximum is only moved when it falls behind by 2^8.
-        if (__any(most > top + 8.0f)) {
-          const float now = fmaxf(top, most);
-          const float back = now == -__builtin_inff() ? 0.0f : now;
-          const float shrink = __builtin_amdgcn_exp2f(top - back);
-          top = now;
-          sum *= shrink;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt] *= shrink;
-        }
-        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const Places& here = places[step & 3];
+        const char* values = lds + kTile + (step & 1) * (kTile / 2);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          // Exponentials and values of this half, while the matrix cores work on
+          // the next one's scores.
+          if (begin + step * kManyStep + u * 32 < most_seen) {
+            const float base = top == -__builtin_inff() ? 0.0f : top;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            f32x16 next = scores(step + u, 1 - u);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sc[u][i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], c, -base));
-            sum += sc[u][i];
-          }
-        }
-        if constexpr (E4) {
+            for (int i = 0; i < 16; ++i) {
+              sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -base));
+              sum += sc[i];
+            }
+            if constexpr (E4) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+              for (int i = 0; i < 16; i += 4) {
+                const f32x4 f =
+                    *reinterpret_cast<const f32x4*>(&here.v_scale[u * 32 + i * 2 + half * 4]);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const f32x4 f =
-                  *reinterpret_cast<const f32x4*>(&here.v_scale[u * 32 + i * 2 + half * 4]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                // A hidden token's scale may be anything.
-                sc[u][i + j] = sc[u][i + j] == 0.0f ? 0.0f : sc[u][i + j] * ValueRest<E>(f[j]);
+                for (int j = 0; j < 4; ++j) {
+                  // A hidden token's scale may be anything.
+                  sc[i + j] = sc[i + j] == 0.0f ? 0.0f : sc[i + j] * ValueRest<E>(f[j]);
+                }
               }
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+              const int i = kk * 8;
+              const u32x4 p = {Pack2<E>(sc[i], sc[i + 1]), Pack2<E>(sc[i + 2], sc[i + 3]),
+                               Pack2<E>(sc[i + 4], sc[i + 5]), Pack2<E>(sc[i + 6], sc[i + 7])};
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) {
+                // Row 4 half + l % 16 / 4 of 8, 8 bytes l % 4 of the 32 of l / 16 % 2.
+                const int r = u * 32 + kk * 16 + half * 4 + lane % 16 / 4;
+                const int chunk = dt * 4 + lane / 16 % 2 * 2 + lane % 4 / 2;
+                const char* v = values + r * kRow + ValueChunk<DP>(r, chunk) * 16 + lane % 2 * 8;
+                const u32x2 lo = ReadTransposed(v), hi = ReadTransposed(v + 8 * kRow);
+                o[dt] = Mma32<E>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[dt]);
+              }
+            }
+            // Operands are read four products ahead.
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int n = 0; n < KS - 4; ++n) {
+              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < DT * 2; ++n) {
+              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+            __builtin_amdgcn_s_setprio(0);
+            sc = next;
+            if (step + u < step1 && begin + step * kManyStep + u * 32 + 32 < most_seen) {
+              settle(step + u, 1 - u, sc);
+            }
+          }
+          if (u == 0) {
+            if constexpr (!E4) {
+              if (finds) keep(step + 3);
+              LdsArrived<kChunks>();  // all but the values: the next step's keys
+            }
+            __syncthreads();
+            if constexpr (E4) {
+              store(step + 2, kKeys);
+              load(step + 1, a.v_pool);
+            } else {
+              fetch(step + 2, a.k_pool, kKeys);
             }
           }
         }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const int u = kk / 2, i = kk % 2 * 8;
-          const u32x4 p = {Pack2<E>(sc[u][i], sc[u][i + 1]), Pack2<E>(sc[u][i + 2], sc[u][i + 3]),
-                           Pack2<E>(sc[u][i + 4], sc[u][i + 5]),
-                           Pack2<E>(sc[u][i + 6], sc[u][i + 7])};
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            // Row 4 half + l % 16 / 4 of 8, 8 bytes l % 4 of the 32 of l / 16 % 2.
-            const int r = kk * 16 + half * 4 + lane % 16 / 4;
-            const int chunk = dt * 4 + lane / 16 % 2 * 2 + lane % 4 / 2;
-            const char* v = values + r * kRow + ValueChunk<DP>(r, chunk) * 16 + lane % 2 * 8;
-            const u32x2 lo = ReadTransposed(v), hi = ReadTransposed(v + 8 * kRow);
-            o[dt] = Mma32<E>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, o[dt]);
-          }
+        if constexpr (E4) {
+          store(step + 1, kValues);
+          if (finds) keep(step + 3);
+          if (finds_scales) keep_scales(step + 2);
+        } else {
+          LdsArrived<kChunks>();  // all but the keys: the next step's values
+          clear(step + 1);
         }
       }
-      if (step + 1 < step1) store(step + 1);
-      if (finds) keep(step + 3);
-      if (finds_scales) keep_scales(step + 2);
+      if constexpr (!E4) LdsArrived<0>();
     }
 
     // Lane: row l % 32, dimensions 32 dt + 8 (i / 4) + 4 (l / 32) + i % 4.
