@@ -212,7 +212,7 @@ int64_t PlanAttend(AttendLaunch* l) {
   if (many_sequences || l->groups > 0) {
     const int64_t tiles = CeilDiv(T * G, kManyRows) * 2 + S + l->groups;
     const int64_t steps = tiles * l->k_heads * (CeilDiv(capacity, kManyStep) + 2);
-    l->many_grid = static_cast<int>(std::min<int64_t>(resident, std::max<int64_t>(steps / 8, 1)));
+    l->many_grid = static_cast<int>(std::min<int64_t>(resident, std::max<int64_t>(steps / kLeastPart, 1)));
   }
   if (l->groups == 0 && l->many_grid == 0 && capacity <= kFewStep) return 0;  // nothing to split
   // Rows that a workgroup joins at once: as many as it has teams of a row's

@@ -226,10 +226,15 @@ __device__ __forceinline__ int ManyWork(const AttendLaunch& a, int i, const Many
   return ManyCost(a, i < a.groups, u.base, ManyTiles(u));
 }
 
-// At least 8 steps a worker.
+// A worker's least part, in steps of 64 tokens: small calls spread over more
+// workgroups, though more of their tiles are cut and joined. 3141 shared tokens of
+// one sequence's 32 heads on 8, D = 64: 24.5 us with parts of 8 steps, 17.1 us of
+// 2, 17.2 us of 1; 3 chunks of 16 tokens over 4000 keys: 25.3, 21.9 and 27.0 us.
+// Large calls have larger parts anyway.
+constexpr int kLeastPart = 2;
 __device__ __forceinline__ Axis ManyAxis(const AttendLaunch& a, int work) {
   const int total = work * a.k_heads;
-  return Axis(total, min(a.many_grid, max(total / 8, 1)));
+  return Axis(total, min(a.many_grid, max(total / kLeastPart, 1)));
 }
 
 // Rows of `parts`: two slots a wave of few_rows rows, two slots a workgroup of
