@@ -286,6 +286,20 @@ void AttendArgs() {
   Refused(Attend([](A& a) { a.workspace = kHost; }), "workspace: host", "attend: host workspace");
   Refused(Attend([](A& a) { a.out = kDev1; }), "device 1", "attend: out on device 1");
 
+  // Storages that do not start on 16 bytes: attend reads them in such pieces.
+  kvx::PoolSource odd;
+  odd.find = [](const void* c, int64_t layer, int64_t shard, kvx::PoolStorage* out) {
+    const bool found = Find(c, layer, shard, out);
+    out->base += 8;
+    out->bytes -= out->block_bytes;
+    return found;
+  };
+  {
+    const kvx_attend_args good = GoodAttend();
+    kvx::AttendLaunch launch;
+    Refused(kvx::CheckAttend(odd, good, &launch, nullptr), "aligned to 16", "attend: odd storages");
+  }
+
   // The workspace's size is the same with and without addresses, and nothing
   // is needed where no row can be cut.
   kvx_attend_args a = GoodAttend();

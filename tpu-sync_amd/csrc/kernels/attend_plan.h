@@ -29,8 +29,13 @@ hipError_t AllowDynamicLds(size_t bytes) {
   hipError_t e = hipGetDevice(&device);
   const uint64_t bit = uint64_t{1} << (device & 63);
   if (e != hipSuccess || (allowed.load() & bit) != 0) return e;
+  // What the kernel's own arrays leave of a CU's.
+  hipFuncAttributes own;
+  e = hipFuncGetAttributes(&own, reinterpret_cast<const void*>(kernel));
+  if (e != hipSuccess) return e;
   e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 256);
+                          hipFuncAttributeMaxDynamicSharedMemorySize,
+                          160 * 1024 - static_cast<int>(own.sharedSizeBytes));
   if (e == hipSuccess) allowed.fetch_or(bit);
   return e;
 }
@@ -379,7 +384,7 @@ __device__ __forceinline__ float ValuePower(float scale) {
   if constexpr (!std::is_same_v<E, F16>) return 1.0f;
   const float power = __builtin_bit_cast(
       float, __builtin_bit_cast(uint32_t, scale) & 0x7f800000u);
-  return fminf(fmaxf(power, 1.0f / 256), 128.0f);
+  return fminf(fmaxf(power, 1.0f / 32768), 128.0f);
 }
 template <class E>
 __device__ __forceinline__ float ValueRest(float scale) {

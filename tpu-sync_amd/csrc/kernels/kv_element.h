@@ -86,7 +86,7 @@ __device__ __forceinline__ f32x2 Unpack2(uint32_t w) {
 }
 
 // The two e4m3 values in half `hi` of w, times a power of two: exact in either
-// 16-bit type for powers from 2^-8 to 2^7.
+// 16-bit type for powers from 2^-15 to 2^7.
 template <class E>
 __device__ __forceinline__ uint32_t FromE4m3(uint32_t w, bool hi, float power) {
   if constexpr (std::is_same_v<E, F16>) {
