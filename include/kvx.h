@@ -1119,7 +1119,8 @@ int kvx_manager_append_kv(kvx_manager* m, const kvx_append_kv_args* args, void* 
  * (non_causal: all of the sequence's). Scores, sums and partial results are
  * fp32; exponentials are rounded to the products' 16-bit type. A query that
  * sees nothing gets zeros and an lse of -inf. In a chunk, a value that is not
- * finite reaches the earlier queries of its own sequence too.
+ * finite reaches the earlier queries of its own sequence too. Storages of 16-bit
+ * types must start on 16 bytes; q and out may start at any element.
  *
  * Groups: the sequences [group_starts[g], group_starts[g + 1]) (ascending,
  * device int32) hold their first prefix_lengths[g] tokens in the same blocks,
