@@ -38,8 +38,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxTokens = 32;  // of one workgroup of append_kv_kernel
-constexpr int kEnough = 1024;  // workgroups
+// append_kv_kernel: a workgroup takes one token until there are kEnough
+// workgroups, then more, up to kMaxTokens. 2048 and 8192 tokens x 8 heads x 128:
+// 6.5 and 15.0 us; with 256 as enough 8.0 and 23.0 us, with 4096 6.5 and 16.2 us.
+constexpr int kMaxTokens = 32;
+constexpr int kEnough = 1024;
 
 __device__ __forceinline__ int FastDiv(const FastDivU32& f, int n) {
   const uint32_t u = static_cast<uint32_t>(n);

@@ -26,6 +26,10 @@
 
 namespace kvx {
 
+// Rows a key head up to which a wave works alone on a part of the keys. 64
+// sequences of 3000 to 4000 tokens, 32 query heads on one, D = 128: 40 us, as
+// tiles of 128 rows 69 us; 24 heads on one over 100 to 200 tokens: 18 and 37 us;
+// 4 new tokens of 32 heads on 4: 149 and 141 us.
 constexpr int kFewRows = 32;
 constexpr int kFewStep = 32;    // tokens of one step of a wave
 constexpr int kManyRows = 128;  // rows of one tile
