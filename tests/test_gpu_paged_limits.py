@@ -138,3 +138,28 @@ def test_e4m3_codes_of_values_are_exact(kvx, cuda, dtype, count, block, dim):
             got = cache[ids[j // block], :rows.shape[0]]
             assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
     mgr.close()
+
+
+def test_starts_and_groups_out_of_order(kvx, cuda):
+    """Starts that give the same tokens to thousands of sequences, and groups that
+    overlap: the work stays what the sizes allow, and nothing outside is touched."""
+    T, S, width = 4096, 4096, 64
+    caches = [torch.randn(70, 16, 1, 64, device=cuda).to(BF16) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
+    room = torch.full((T + 64, 8, 64), 5.0, device=cuda).to(BF16)
+    q = torch.randn(T, 8, 64, device=cuda).to(BF16)
+    tables = torch.randint(0, 70, (S, width), device=cuda, dtype=torch.int32)
+    lengths = torch.full((S,), 2**31 - 1, device=cuda, dtype=torch.int32)
+    back = torch.tensor([0, T] * (S // 2) + [0], device=cuda, dtype=torch.int32)
+    groups = torch.tensor([0, S] * 128 + [0], device=cuda, dtype=torch.int32)
+    prefixes = torch.full((256,), 2**31 - 1, device=cuda, dtype=torch.int32)
+    one = torch.arange(S + 1, device=cuda, dtype=torch.int32)
+    for starts, kw in ((back, {}), (one, dict(group_starts=groups, prefix_lengths=prefixes)),
+                       (back, dict(group_starts=groups, prefix_lengths=prefixes))):
+        mgr.attend(0, 1, q, tables, lengths, starts=starts, out=room[32:32 + T], **kw)
+        torch.cuda.synchronize()
+        assert bool((room[:32] == 5).all()) and bool((room[32 + T:] == 5).all())
+    # A valid call after it, through the same manager.
+    few = mgr.attend(0, 1, q[:2], tables[:2], ints([100, 30], cuda))
+    assert bool(torch.isfinite(few).all())
+    mgr.close()

@@ -392,9 +392,12 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
   // of 32, each for every key head, and squares of tiles.
   const int64_t tiles = 2 * (a.tokens * G / kManyRows + 1) + a.batch.sequences + a.groups;
   const int64_t steps = out->batch.capacity / kManyStep + 3 + a.tokens / kManyStep;
-  if (tiles > 65536 || tiles > INT32_MAX / 2 / c.heads / steps) {
+  const int64_t few = a.batch.sequences * (out->batch.capacity / kFewStep + 1);
+  if (tiles > 65536 || tiles > INT32_MAX / 2 / c.heads / steps || few > INT32_MAX / 2 / c.heads) {
     return Bad("tokens * table_width is too large for one call");
   }
+  out->most_few = static_cast<int32_t>(few);
+  out->most_many = static_cast<int32_t>(tiles * steps);
   if (a.batch.sequences == 0) out->batch.tokens = 0;
   out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
   out->group_div = MakeFastDivU32(static_cast<uint32_t>(G));

@@ -50,6 +50,7 @@ struct AttendLaunch {
   const void* v_pool = nullptr;
   const float* k_scales = nullptr;  // e4m3: [num_blocks][k_heads]
   const float* v_scales = nullptr;
+  int32_t most_few = 0, most_many = 0;  // steps of a key head that the sizes allow
   // Groups of sequences [group_starts[g], group_starts[g + 1]) whose first
   // prefix_lengths[g] tokens are in the same blocks.
   const int32_t* group_starts = nullptr;

@@ -59,7 +59,7 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
     lengths[s] = k.q.length;
     if (a.groups > 0) begins[s] = 2 * k.begin + (k.grouped ? 1 : 0);
   }
-  BlockSums(sums, b.sequences);
+  BlockSums(sums, b.sequences, a.most_few);
   const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   const int all = one(sums[b.sequences - 1]);
   if (all == 0) return;

@@ -121,7 +121,8 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
     const int head = h * G + (row - t * G);
 
     // The row's parts: workers [w0, w0 + own) of its own keys' axis and, of a
-    // group's, [v0, v0 + shared) of the prefix's.
+    // group's, [v0, v0 + shared) of the prefix's. (Starts or groups that are out
+    // of order may point behind the axes: bounded, their rows mean nothing.)
     const Axis& axis = is_few ? few : many;
     const int w0 = axis.Owner(x), own = axis.Owner(x + size - 1) - w0 + 1;
     if (g < 0 && own == 1) continue;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
     if (g >= 0) {
       const int at = before(plan.many, g), per_head = plan.many[g] - at;
       if (per_head > 0) {
-        shared_row = (static_cast<int>(token) - plan.gfirst[g]) * G + (row - t * G);
+        shared_row = max((static_cast<int>(token) - plan.gfirst[g]) * G + (row - t * G), 0);
         const int tile = shared_row / kManyRows, base = plan.base[g];
         y = at * a.k_heads + h * per_head + ManyCost(a, true, base, tile);
         v0 = many.Owner(y);
@@ -142,14 +143,15 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
       for (int n = mine; n < own + shared; n += at_once) {
         int64_t from;
         if (n >= own) {
-          const int w = v0 + n - own;
+          const int w = max(min(v0 + n - own, many.workers - 1), 0);
           from = shared == 1 ? WholeRow(a, true, token, head)
                              : ManySlotRow(a, n == own ? many.Slot(w, y) : 2 * w) +
                                    shared_row % kManyRows;
         } else if (own == 1) {
           from = WholeRow(a, false, token, head);
         } else {
-          const int w = w0 + n, slot = n == 0 ? axis.Slot(w, x) : 2 * w;
+          const int w = max(min(w0 + n, axis.workers - 1), 0);
+          const int slot = n == 0 ? axis.Slot(w, x) : 2 * w;
           from = is_few ? FewSlotRow(a, slot) + row : ManySlotRow(a, slot) + row % kManyRows;
         }
         const f32x2 st = PartStats(a)[from];

@@ -106,7 +106,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
   for (int i = threadIdx.x; i < units; i += kAttendThreads) {
     sums[i] = ManyWork(a, i, LoadManyUnit(a, i));
   }
-  BlockSums(sums, units);
+  BlockSums(sums, units, a.most_many);
   const int work = one(sums[units - 1]);
   if (work == 0) return;
   const Axis axis = ManyAxis(a, work);

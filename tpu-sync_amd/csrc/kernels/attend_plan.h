@@ -46,28 +46,36 @@ __device__ __forceinline__ int FastDivI(const FastDivU32& f, int n) {
 }
 
 // In-place inclusive sums of c[0..n) over the workgroup (n <= kMaxSequences *
-// 2); c[i] must have been written by any thread before, and is visible to all
-// after.
-__device__ __forceinline__ void BlockSums(int* c, int n) {
+// 2), none above `most`: a valid call's stay below it, and starts that are out of
+// order, whose tokens count for many sequences, cannot make more work or wrap
+// around. c[i] must have been written by any thread before, and is visible to
+// all after.
+__device__ __forceinline__ void BlockSums(int* c, int n, int most) {
   __shared__ int waves[kWaves];
+  const auto add = [&](int x, int y) {
+    const uint32_t sum = static_cast<uint32_t>(x) + static_cast<uint32_t>(y);
+    return static_cast<int>(min(sum, static_cast<uint32_t>(most)));
+  };
   const int each = (n + kAttendThreads - 1) / kAttendThreads;
   const int i0 = threadIdx.x * each, i1 = min(i0 + each, n);
   __syncthreads();
   int mine = 0;
-  for (int i = i0; i < i1; ++i) mine += c[i];
+  for (int i = i0; i < i1; ++i) mine = add(mine, c[i]);
   int sum = mine;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) {
     const int o = __shfl_up(sum, m);
-    if (lane >= m) sum += o;
+    if (lane >= m) sum = add(sum, o);
   }
   if (lane == 63) waves[wave] = sum;
+  // What the lanes before this one have.
+  int at = __shfl_up(sum, 1);
+  if (lane == 0) at = 0;
   __syncthreads();
-  int at = sum - mine;
-  for (int w = 0; w < wave; ++w) at += waves[w];
+  for (int w = 0; w < wave; ++w) at = add(at, waves[w]);
   for (int i = i0; i < i1; ++i) {
-    at += c[i];
+    at = add(at, c[i]);
     c[i] = at;
   }
   __syncthreads();
@@ -312,9 +320,9 @@ __device__ __forceinline__ void WritePlan(const AttendLaunch& a, int* lds) {
     to.base[i] = u.base;
     if (i < a.groups) to.gfirst[i] = u.first;
   }
-  BlockSums(here.few, S);
-  BlockSums(here.many, units);
-  BlockSums(here.todo, S);
+  BlockSums(here.few, S, a.most_few);
+  BlockSums(here.many, units, a.most_many);
+  BlockSums(here.todo, S, a.batch.tokens * (a.q_heads / a.k_heads) / a.join_rows + S);
   int* out = Plan(a);
   for (int i = threadIdx.x; i < PlanSumWords(a); i += kAttendThreads) out[i] = lds[i];
 }
