@@ -15,12 +15,12 @@
 // read four products ahead. Tokens go from memory straight into LDS, each storage
 // refilled as soon as its last reader is past a barrier: keys run two steps
 // ahead, values one, so K and V need two buffers each and no registers. (e4m3
-// tokens are widened on the way, in registers.) 4099 new tokens of 32 heads on 8
-// over 7000 keys in bf16, D = 128: 730 us with tokens passing through registers
-// and a wave's products and exponentials in turn, 676 us without, 655 us with
-// operands read ahead and products given priority, 611 us with the places of
-// tokens kept as byte offsets (885 TFLOP/s, where an 8192^3 product of the library
-// reaches 1211).
+// tokens are widened on the way, in registers.) 4099 new tokens of 5 sequences of
+// 2000 to 12000, 32 heads on 8, D = 128, bf16: 730 us with tokens passing through
+// registers and a wave's products and exponentials in turn, 676 us without, 655 us
+// with operands read ahead and products given priority, 611 to 625 us with the
+// places of tokens kept as byte offsets (865 to 885 TFLOP/s, where an 8192^3
+// product of the library reaches 1211).
 //
 // Work. The tiles of all groups and sequences make one axis, weighed by the
 // keys they see, and every workgroup gets an equal part of it: no tail of late
