@@ -163,3 +163,33 @@ def test_starts_and_groups_out_of_order(kvx, cuda):
     few = mgr.attend(0, 1, q[:2], tables[:2], ints([100, 30], cuda))
     assert bool(torch.isfinite(few).all())
     mgr.close()
+
+
+def test_captured_chunks_that_share_memory(kvx, cuda):
+    """Chunks, and sequences on a shared prefix, captured in two graphs that take
+    their workspaces from one pool, replayed in turn between eager calls."""
+    steps = [Step(kvx, cuda, [40, 3, 150], [500, 90, 150], 8, 2, 128, 16, BF16, BF16),
+             Step(kvx, cuda, [1] * 8, [700 + s for s in range(8)], 8, 2, 128, 16, F16, FP8,
+                  [(0, 8, 640)])]
+    graphs, pool = [], None
+    for step in steps:
+        args, kw = step.args(), step.kw()
+        want = step.mgr.attend(0, 1, step.q, *args, **kw)
+        held = torch.zeros_like(step.q)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            held.copy_(step.mgr.attend(0, 1, step.q, *args, **kw))
+        pool = graph.pool()
+        graphs.append((graph, held, want, args, kw))
+    for i in range(4):
+        for step, (graph, held, want, args, kw) in zip(steps, graphs):
+            graph.replay()
+            eager = step.mgr.attend(0, 1, step.q, *args, **kw)
+            if i % 2:
+                torch.cuda.synchronize()
+            assert torch.equal(held, want) and torch.equal(eager, want)
+            held.zero_()
+    del graphs, graph
+    for step in steps:
+        step.mgr.close()
