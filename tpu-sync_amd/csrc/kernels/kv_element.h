@@ -123,8 +123,8 @@ __device__ __forceinline__ SequenceSpan LoadSequence(const BatchView& b, int32_t
 
 // cos and sin of position * inv_freq. The product and its turns are taken in
 // two 64-bit words (each error term exact by a fused multiply-add) and reduced
-// there, so any position up to 2^53 keeps an angle good to the 2^-25 turns of
-// the 32-bit one that cos and sin then get.
+// there, so any position up to 2^53 keeps its angle; cos and sin get the nearest
+// 32-bit one, and what that leaves, up to 2^-26 turns, turns their result.
 __device__ __forceinline__ f32x2 Turn(int64_t position, float inv_freq) {
 // A product fused into the difference would bring its error term in twice.
 #pragma clang fp contract(off)
@@ -134,10 +134,12 @@ __device__ __forceinline__ f32x2 Turn(int64_t position, float inv_freq) {
   const double angle = p * f, angle_rest = fma(p, f, -angle);
   const double turns = angle * kTurn;
   const double rest = fma(angle, kTurn, -turns) + angle * kTurnRest + angle_rest * kTurn;
-  const float part = static_cast<float>((turns - rint(turns)) + rest);
+  const double within = (turns - rint(turns)) + rest;
+  const float part = static_cast<float>(within);
+  const float left = static_cast<float>(within - part) * 6.2831853f;
   float s, c;
   sincospif(2.0f * part, &s, &c);
-  return f32x2{c, s};
+  return f32x2{__builtin_fmaf(-left, s, c), __builtin_fmaf(left, c, s)};
 }
 
 }  // namespace kvx
