@@ -161,8 +161,8 @@ def norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps: f
         projection). ``k`` may be None.
       positions: int32 or int64 [tokens].
       inv_freq: fp32 [rotary_dim / 2] with rotary_dim <= head_dim; the angle of
-        pair i is position * inv_freq[i], exact to fp32 cos and sin for positions up to
-        2^53. Dimensions from rotary_dim on are not rotated. None: norm only.
+        pair i is position * inv_freq[i], exact for positions up to 2^53 before its
+        cos and sin are taken in fp32. Dimensions from rotary_dim on are not rotated. None: norm only.
       q_weight, k_weight: [head_dim], of the rows' type or fp32; None: no norm.
       interleaved: pairs are (2i, 2i + 1) instead of (i, i + rotary_dim / 2).
       out_q, out_k: results; the input itself, or apart from the inputs.
