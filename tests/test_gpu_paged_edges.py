@@ -1,0 +1,52 @@
+"""GPU: calls on the paged pool that other tests do not make: the same call on its
+own result."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_attend import BF16, F16, FP8, ints  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("counts,block,dim", [([1, 1], 16, 64), ([7, 30], 16, 128),
+                                              ([300, 9], 256, 128), ([5, 4], 8, 80)])
+def test_append_again_stores_the_same_codes(kvx, cuda, dtype, counts, block, dim):
+    """An e4m3 block that holds earlier tokens: the new ones come from the largest
+    value's exact quotient, by the call that raises the scale and by the same call
+    (a replay, a step that is taken back) after it. The largest value is 31 / 4 and
+    the others 93 / 2^n, so 448 x / largest = 21 x 2^(8 - n) is the middle between
+    two codes; by the scale, 31 / 1792 rounded down in its last bit, the quotient
+    is the next number above it."""
+    gen = torch.Generator(device=cuda).manual_seed(dim)
+    before = 3  # tokens of each sequence's first block, not of these calls
+    blocks = sum((before + n + block - 1) // block for n in counts)
+    caches = [torch.ones(blocks, block, 2, dim, device=cuda).to(FP8) for _ in range(2)]
+    scales = [torch.full((blocks, 2), 1 / 1024, device=cuda) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, scale_tables=scales)
+    tokens, table, starts, at = sum(counts), [], [0], 0
+    width = max((before + n + block - 1) // block for n in counts)
+    for n in counts:
+        need = (before + n + block - 1) // block
+        table.append(list(range(at, at + need)) + [-1] * (width - need))
+        at += need
+        starts.append(starts[-1] + n)
+    n = torch.randint(4, 13, (tokens, 2, dim), device=cuda, generator=gen)
+    x = 93 * torch.pow(2.0, -n) * (1 - 2 * (n % 2))
+    x[:, :, 0] = 31 / 4
+    k, v = x.to(dtype), (-x).to(dtype)
+    assert torch.equal(k.float(), x)
+    args = (ints(table, cuda), ints([before + n for n in counts], cuda))
+    held = []
+    for _ in range(3):
+        mgr.append_kv(0, 1, k, v, *args, starts=ints(starts, cuda))
+        held.append([c.view(torch.uint8).clone() for c in caches] + [s.clone() for s in scales])
+    for again in held[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(held[0], again))
+    want = (x.double() * 1792 / 31).to(FP8).view(torch.uint8)
+    for s, count in enumerate(counts):
+        rows = [caches[0][table[s][p // block], p % block]
+                for p in range(before, before + count)]
+        assert torch.equal(torch.stack(rows).view(torch.uint8), want[starts[s]:starts[s + 1]])
+    mgr.close()

@@ -336,7 +336,8 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
       float old = rows.slot > 0 ? scales[h] : 0.0f;
       old = old > 0.0f ? old : 0.0f;
       if (!at_once) largest = amax[h];
-      const float scale = fmaxf(old, largest / kE4m3Max);
+      const float wanted = largest / kE4m3Max;
+      const float scale = fmaxf(old, wanted);
       const bool grown = scale > old;
       if (grown && rows.slot > 0) {
         const float ratio = old / scale;
@@ -353,7 +354,9 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
           }
         }
       }
-      from = grown ? largest : -old;
+      // (Also where the scale already is what these rows want: the same call
+      // on its own result stores the same codes.)
+      from = wanted >= old ? largest : -old;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (in_wave == 0) {
         scales[h] = scale;
