@@ -1,5 +1,5 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
-own result."""
+own result, starts that are out of order."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -49,4 +49,27 @@ def test_append_again_stores_the_same_codes(kvx, cuda, dtype, counts, block, dim
         rows = [caches[0][table[s][p // block], p % block]
                 for p in range(before, before + count)]
         assert torch.equal(torch.stack(rows).view(torch.uint8), want[starts[s]:starts[s + 1]])
+    mgr.close()
+
+
+def test_append_to_e4m3_with_starts_out_of_order(kvx, cuda):
+    """Starts that give each of 2048 sequences the same 2099200 tokens, a block each,
+    over 2^32 blocks in all: each block is written once, by the first sequence."""
+    tokens, sequences = 2**21 + 2048, 4096
+    caches = [torch.zeros(tokens, 1, 1, 8, device=cuda).to(FP8) for _ in range(2)]
+    scales = [torch.zeros(tokens, 1, device=cuda) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, scale_tables=scales)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    k = torch.randn(tokens, 1, 8, device=cuda, generator=gen).to(BF16)
+    ids = torch.randperm(tokens, device=cuda, generator=gen).to(torch.int32)
+    back = torch.tensor([0, tokens] * (sequences // 2) + [0], dtype=torch.int32, device=cuda)
+    held = []
+    for n, starts in ((sequences, back), (1, ints([0, tokens], cuda))):
+        for t in caches + scales:
+            t.view(torch.uint8).zero_()
+        mgr.append_kv(0, 1, k, -k, ids[None].expand(n, tokens),
+                      torch.full((n,), tokens, dtype=torch.int32, device=cuda), starts=starts)
+        held.append([t.view(torch.uint8).clone() for t in caches + scales])
+    assert all(torch.equal(a, b) for a, b in zip(*held))
+    assert bool((scales[0] > 0).all())
     mgr.close()

@@ -209,7 +209,9 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
   const int wave = threadIdx.x / 64, in_wave = threadIdx.x % 64;
 
   // The block: the blockIdx.x-th of those that the sequences touch, in order.
+  // Sums stop at the grid's size, so that one sequence at most has it.
   if (threadIdx.x == 0) found.id = -1;
+  const auto add = [](int x, int y) { return AddUpTo(x, y, static_cast<int>(gridDim.x)); };
   const auto touched = [&](const SequenceSpan& q, int& lo, int& hi) {
     lo = max(q.length - q.count, 0);
     hi = min(q.length, b.capacity);
@@ -221,17 +223,19 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
   const int s0 = threadIdx.x * each, s1 = min(s0 + each, b.sequences);
   if (b.starts != nullptr) {
     int mine = 0, lo, hi;
-    for (int s = s0; s < s1; ++s) mine += touched(LoadSequence(b, s), lo, hi);
+    for (int s = s0; s < s1; ++s) mine = add(mine, touched(LoadSequence(b, s), lo, hi));
     int sum = mine;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
       const int o = __shfl_up(sum, m);
-      if (in_wave >= m) sum += o;
+      if (in_wave >= m) sum = add(sum, o);
     }
     if (in_wave == 63) counted[wave] = sum;
+    // What the lanes before this one have.
+    before = __shfl_up(sum, 1);
+    if (in_wave == 0) before = 0;
     __syncthreads();
-    before = sum - mine;
-    for (int w = 0; w < wave; ++w) before += counted[w];
+    for (int w = 0; w < wave; ++w) before = add(before, counted[w]);
   } else {
     before = s0;  // one token, so one block, a sequence
     __syncthreads();
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
       const int id = b.tables[s * b.table_stride + at];
       found.id = id < b.num_blocks ? id : -1;
     }
-    before += n;
+    before = add(before, n);
   }
   for (int h = threadIdx.x; h < a.heads; h += threads) amax[h] = 0.0f;
   __syncthreads();

@@ -46,16 +46,11 @@ __device__ __forceinline__ int FastDivI(const FastDivU32& f, int n) {
 }
 
 // In-place inclusive sums of c[0..n) over the workgroup (n <= kMaxSequences *
-// 2), none above `most`: a valid call's stay below it, and starts that are out of
-// order, whose tokens count for many sequences, cannot make more work or wrap
-// around. c[i] must have been written by any thread before, and is visible to
-// all after.
+// 2), none above `most` (AddUpTo). c[i] must have been written by any thread
+// before, and is visible to all after.
 __device__ __forceinline__ void BlockSums(int* c, int n, int most) {
   __shared__ int waves[kWaves];
-  const auto add = [&](int x, int y) {
-    const uint32_t sum = static_cast<uint32_t>(x) + static_cast<uint32_t>(y);
-    return static_cast<int>(min(sum, static_cast<uint32_t>(most)));
-  };
+  const auto add = [&](int x, int y) { return AddUpTo(x, y, most); };
   const int each = (n + kAttendThreads - 1) / kAttendThreads;
   const int i0 = threadIdx.x * each, i1 = min(i0 + each, n);
   __syncthreads();

@@ -20,6 +20,15 @@ constexpr bool Is16Bit(int32_t t) { return t == kBf16 || t == kF16; }
 constexpr int64_t ElementBytes(int32_t t) { return t == kF32 ? 4 : t == kE4m3 ? 1 : 2; }
 constexpr float kE4m3Max = 448.0f;
 
+// x + y, but at most `most`, for x and y of [0, most]. Work is summed up so
+// where it comes from device arrays: a valid call's sums stay below `most`, and
+// starts that are out of order, whose tokens count for many sequences, can
+// neither make more work nor wrap around to places that others have.
+constexpr int AddUpTo(int x, int y, int most) {
+  const uint32_t sum = static_cast<uint32_t>(x) + static_cast<uint32_t>(y);
+  return sum < static_cast<uint32_t>(most) ? static_cast<int>(sum) : most;
+}
+
 // The sequences of a call. Sequence s owns the new tokens [starts[s],
 // starts[s + 1]) (starts null: token s) and holds lengths[s] tokens with them,
 // token p in slot p % block_tokens of block tables[s][p / block_tokens]. The
