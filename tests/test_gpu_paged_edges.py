@@ -1,5 +1,5 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
-own result, starts that are out of order."""
+own result, starts that are out of order, interleaved heads."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -73,3 +73,18 @@ def test_append_to_e4m3_with_starts_out_of_order(kvx, cuda):
     assert all(torch.equal(a, b) for a, b in zip(*held))
     assert bool((scales[0] > 0).all())
     mgr.close()
+
+
+@pytest.mark.parametrize("dim", [64, 80, 5])
+def test_norm_rope_in_place_of_interleaved_heads(kvx, cuda, dim):
+    """A projection that lies as [tokens, heads, (q, k, v), head_dim]."""
+    gen = torch.Generator(device=cuda).manual_seed(dim)
+    qkv = torch.randn(33, 6, 3, dim, device=cuda, generator=gen).to(BF16)
+    held, pos = qkv.clone(), torch.arange(33, device=cuda) * 100
+    inv = torch.rand(dim // 2, device=cuda, generator=gen)
+    w = torch.rand(dim, device=cuda, generator=gen).to(BF16)
+    q, k = qkv[:, :, 0], qkv[:, :, 1]
+    want = kvx.norm_rope(q, k, pos, inv, q_weight=w, k_weight=w)
+    kvx.norm_rope(q, k, pos, inv, q_weight=w, k_weight=w, out_q=q, out_k=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    assert torch.equal(qkv[:, :, 2], held[:, :, 2])

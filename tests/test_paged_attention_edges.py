@@ -33,3 +33,7 @@ def run_check(name, tmp_path, library):
 
 def test_sums_of_work_do_not_wrap(tmp_path):
     assert "all passed" in run_check("paged_sums_check", tmp_path, library=False)
+
+
+def test_arguments_in_one_buffer(tmp_path):
+    assert "all passed" in run_check("attention_overlap_check", tmp_path, library=True)

@@ -60,22 +60,48 @@ bool Meet(uint64_t a, uint64_t a_bytes, uint64_t b, uint64_t b_bytes) {
   return a_bytes > 0 && b_bytes > 0 && a < b + b_bytes && b < a + a_bytes;
 }
 
+// Rows in bytes: `blocks` of them `period` apart, each of `rows` of `width`
+// bytes `step` apart (a stride of one row or block is 0).
+struct Lattice {
+  int64_t blocks = 1, period = 0, rows = 1, step = 0, width = 0;
+
+  explicit Lattice(const Rows& r) : width(r.dim * r.item) {
+    const int64_t t = r.tokens > 1 ? r.token_stride * r.item : 0;
+    const int64_t h = r.heads > 1 ? r.head_stride * r.item : 0;
+    const bool tokens_outside = t >= h;
+    blocks = tokens_outside ? r.tokens : r.heads;
+    period = tokens_outside ? t : h;
+    rows = tokens_outside ? r.heads : r.tokens;
+    step = tokens_outside ? h : t;
+  }
+  int64_t span() const { return (rows - 1) * step + width; }  // of a block
+};
+
+// Whether pieces of `a` and `b` bytes, each repeated `period` apart and the
+// latter `gap` behind the former, stay apart.
+bool Apart(int64_t a, int64_t b, int64_t period, int64_t gap) {
+  if (period <= 0) return false;
+  const int64_t at = (gap % period + period) % period;
+  return a <= at && at + b <= period;
+}
+
 bool Meet(const Rows& a, const Rows& b) {
   uint64_t x = 0, y = 0;
   if (a.empty() || b.empty() || !a.Extent(&x) || !b.Extent(&y)) return false;
   if (!Meet(a.at, x, b.at, y)) return false;
-  // Parts of one wider row (a fused projection): apart if no row of one
-  // reaches into a row of the other.
-  if (a.token_stride == b.token_stride && a.tokens > 1 && a.item == b.item) {
-    const int64_t period = a.token_stride * a.item;
-    const int64_t la = ((a.heads - 1) * a.head_stride + a.dim) * a.item;
-    const int64_t lb = ((b.heads - 1) * b.head_stride + b.dim) * b.item;
-    const int64_t gap = a.at <= b.at ? static_cast<int64_t>(b.at - a.at)
-                                     : static_cast<int64_t>(a.at - b.at);
-    const int64_t first = a.at <= b.at ? la : lb, second = a.at <= b.at ? lb : la;
-    if (gap < period && first <= gap && gap + second <= period) return false;
-  }
-  return true;
+  // Parts of one wider row (a fused projection): apart if no block of one
+  // reaches into a block of the other, or, with heads side by side ([q, k, v] of
+  // each), no row into a row.
+  const Lattice l(a), m(b);
+  const int64_t gap = static_cast<int64_t>(b.at - a.at);
+  const auto common = [](int64_t s, int64_t n, int64_t t, int64_t k) {
+    return n == 1 ? t : k == 1 || s == t ? s : 0;
+  };
+  const int64_t period = common(l.period, l.blocks, m.period, m.blocks);
+  if (Apart(l.span(), m.span(), period, gap)) return false;
+  const int64_t step = common(l.step, l.rows, m.step, m.rows);
+  return step <= 0 || l.period % step != 0 || m.period % step != 0 ||
+         !Apart(l.width, m.width, step, gap);
 }
 
 // Results may take the place of what they are computed from, row for row;
