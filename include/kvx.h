@@ -1130,7 +1130,9 @@ int kvx_manager_append_kv(kvx_manager* m, const kvx_append_kv_args* args, void* 
  * workspace: device memory of kvx_manager_attend_workspace bytes (a function of
  * the sizes alone, addresses may still be 0; starts only has to be set or not
  * set as in the call), 16-byte aligned; its contents mean nothing between calls.
- * Calls that can run at the same time need one each.
+ * Calls that can run at the same time need one each. out, lse and the workspace
+ * may not overlap each other, the cache or another argument (out may be q, with
+ * its strides).
  */
 typedef struct kvx_attend_args {
   kvx_paged_cache cache;

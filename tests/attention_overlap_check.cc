@@ -8,6 +8,7 @@
 #include <cstring>
 #include <functional>
 #include <set>
+#include <string>
 
 #include "attention_args.h"
 #include "device_memory.h"
@@ -142,11 +143,114 @@ void FusedProjections() {
   }
 }
 
+// 100 blocks of [16][2][64]: layers 0, 1 bf16; 2, 3 e4m3; 4, 5 their scales.
+bool Find(const void*, int64_t layer, int64_t shard, kvx::PoolStorage* out) {
+  if (layer < 0 || layer > 5 || shard != 0) return false;
+  const int64_t block[] = {4096, 4096, 2048, 2048, 8, 8};
+  *out = {At(2048 + layer), block[layer] * 100, block[layer]};
+  return true;
+}
+
+kvx::PoolSource Pool() {
+  kvx::PoolSource p;
+  p.find = Find;
+  return p;
+}
+
+kvx_paged_cache GoodCache(bool e4m3) {
+  kvx_paged_cache c;
+  std::memset(&c, 0, sizeof(c));
+  c.k_layer = e4m3 ? 2 : 0;
+  c.v_layer = e4m3 ? 3 : 1;
+  c.k_scale_layer = 4;
+  c.v_scale_layer = 5;
+  c.dtype = e4m3 ? KVX_E4M3 : KVX_BF16;
+  c.block_tokens = 16;
+  c.heads = 2;
+  c.head_dim = 64;
+  return c;
+}
+
+kvx_paged_batch GoodBatch() {
+  kvx_paged_batch b;
+  std::memset(&b, 0, sizeof(b));
+  b.tables = At(10);
+  b.table_stride = 64;
+  b.table_width = 20;
+  b.lengths = At(11);
+  b.starts = At(12);
+  b.sequences = 3;
+  return b;
+}
+
+kvx::Status Attend(bool e4m3, const std::function<void(kvx_attend_args&)>& change) {
+  kvx_attend_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.cache = GoodCache(e4m3);
+  a.batch = GoodBatch();
+  a.tokens = 10;
+  a.dtype = KVX_BF16;
+  a.q_heads = 8;
+  a.q = At(1);
+  a.out = At(2);
+  a.lse = At(3);
+  a.q_token_stride = a.out_token_stride = 512;
+  a.q_head_stride = a.out_head_stride = 64;
+  a.group_starts = At(20);
+  a.prefix_lengths = At(21);
+  a.groups = 2;
+  a.scale = 0.125f;
+  a.workspace = At(100);
+  a.workspace_bytes = 512 << 20;
+  change(a);
+  kvx::AttendLaunch l;
+  return kvx::CheckAttend(Pool(), a, &l, nullptr);
+}
+
+void AttendResults() {
+  using A = kvx_attend_args;
+  for (bool e4m3 : {false, true}) {
+    const auto run = [&](const std::function<void(A&)>& f) { return Attend(e4m3, f); };
+    Passes(run([](A&) {}), "attend");
+    Passes(run([](A& a) { a.out = a.q; }), "attend in place");
+    Passes(run([](A& a) { a.workspace = At(2048) - (512 << 20); }), "a workspace before the cache");
+    Passes(run([](A& a) { a.lse = a.out + 10 * 512 * 2; }), "lse behind out");
+    const uint64_t k = e4m3 ? At(2050) : At(2048), v = k + (1 << 20);
+    const uint64_t last = 100 * (e4m3 ? 2048 : 4096) - 16;
+    struct {
+      uint64_t at;
+      const char* name;
+    } others[] = {{k, "the cache"},        {v, "the cache"},          {k + last, "the cache"},
+                  {v + last, "the cache"}, {At(10), "tables"},        {At(10) + 512 + 64, "tables"},
+                  {At(11), "lengths"},     {At(12), "starts"},        {At(20), "group_starts"},
+                  {At(21), "prefix_lengths"}};
+    for (const auto& o : others) {
+      Refused(run([&](A& a) { a.out = o.at; }), (std::string("out: overlaps ") + o.name).c_str(),
+              "out");
+      Refused(run([&](A& a) { a.lse = o.at; }), (std::string("lse: overlaps ") + o.name).c_str(),
+              "lse");
+      Refused(run([&](A& a) { a.workspace = o.at; }),
+              (std::string("workspace: overlaps ") + o.name).c_str(), "workspace");
+    }
+    Refused(run([](A& a) { a.lse = a.out + 64; }), "lse: overlaps out", "lse on out");
+    Refused(run([](A& a) { a.lse = a.q + 64; }), "lse: overlaps q", "lse on q");
+    Refused(run([](A& a) { a.workspace = a.out + 64; }), "workspace: overlaps out", "parts on out");
+    Refused(run([](A& a) { a.workspace = a.q + 64; }), "workspace: overlaps", "parts on q");
+    Refused(run([](A& a) { a.workspace = a.lse; }), "workspace: overlaps lse", "parts on lse");
+  }
+  for (uint64_t at : {At(2052), At(2053) + 796}) {
+    Refused(Attend(true, [&](kvx_attend_args& a) { a.lse = at; }), "the cache's scales",
+            "lse on scales");
+    Passes(Attend(false, [&](kvx_attend_args& a) { a.lse = at; }), "no scales in use");
+  }
+}
+
 }  // namespace
 
 int main() {
   kvx::SetAddressQueryForTesting(FakeQuery);
   FusedProjections();
+  AttendResults();
   kvx::SetAddressQueryForTesting(nullptr);
   if (failures == 0) std::printf("attention overlap checks: all passed\n");
   return failures == 0 ? 0 : 1;

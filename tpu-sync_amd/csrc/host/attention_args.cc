@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "device_memory.h"
@@ -20,7 +21,7 @@ struct Rows {
   int64_t token_stride, head_stride;
   int64_t tokens, heads, dim, item;
 
-  bool empty() const { return tokens == 0 || heads == 0; }
+  bool empty() const { return tokens == 0 || heads == 0 || dim == 0; }
   // Bytes from the first to behind the last element; false on overflow.
   bool Extent(uint64_t* bytes) const {
     int64_t t = 0, h = 0, n = 0;
@@ -102,6 +103,29 @@ bool Meet(const Rows& a, const Rows& b) {
   const int64_t step = common(l.step, l.rows, m.step, m.rows);
   return step <= 0 || l.period % step != 0 || m.period % step != 0 ||
          !Apart(l.width, m.width, step, gap);
+}
+
+// An argument, with its extent.
+struct Named {
+  Rows rows;
+  const char* name;
+  uint64_t bytes = 0;
+
+  Named(const Rows& r, const char* n) : rows(r), name(n) {
+    if (r.empty() || !r.Extent(&bytes)) bytes = 0;
+  }
+};
+
+// `bytes` bytes at an address, without gaps.
+Rows Whole(uint64_t at, int64_t bytes) { return {at, 0, 0, bytes > 0 ? 1 : 0, 1, bytes, 1}; }
+
+Status CheckApart(const Named& written, std::initializer_list<Named> others) {
+  for (const Named& o : others) {
+    if (Meet(written.rows.at, written.bytes, o.rows.at, o.bytes) && Meet(written.rows, o.rows)) {
+      return Bad(std::string(written.name) + ": overlaps " + o.name);
+    }
+  }
+  return OkStatus();
 }
 
 // Results may take the place of what they are computed from, row for row;
@@ -194,11 +218,22 @@ Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t 
   return OkStatus();
 }
 
+// The arrays of a batch, checked before.
+Rows Tables(const kvx_paged_batch& b) {
+  return {b.tables, b.table_stride, 0, b.sequences, 1, b.table_width, 4};
+}
+Rows Lengths(const kvx_paged_batch& b) { return Whole(b.lengths, b.sequences * 4); }
+Rows Starts(const kvx_paged_batch& b) {
+  return Whole(b.starts, b.starts != 0 ? (b.sequences + 1) * 4 : 0);
+}
+
 struct Cache {
   PoolStorage k, v;
-  uint64_t k_scales = 0, v_scales = 0;
+  PoolStorage k_scales, v_scales;  // e4m3
   int64_t num_blocks = 0;
 };
+
+Rows Whole(const PoolStorage& s) { return Whole(s.base, s.bytes); }
 
 Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type, Cache* out) {
   if (!pool.device_backed) {
@@ -241,8 +276,8 @@ Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type,
       blocks = std::min(blocks, t.bytes / t.block_bytes);
     }
     if (s[0].base == s[1].base) return Bad("keys and values need scale tables of their own");
-    out->k_scales = s[0].base;
-    out->v_scales = s[1].base;
+    out->k_scales = s[0];
+    out->v_scales = s[1];
   } else if ((out->k.base | out->v.base) % 2 != 0) {
     return Bad("cache storages: unaligned address");
   }
@@ -348,8 +383,8 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
   out->v_head = a.v_head_stride;
   out->k_pool = reinterpret_cast<void*>(cache.k.base);
   out->v_pool = reinterpret_cast<void*>(cache.v.base);
-  out->k_scales = reinterpret_cast<float*>(cache.k_scales);
-  out->v_scales = reinterpret_cast<float*>(cache.v_scales);
+  out->k_scales = reinterpret_cast<float*>(cache.k_scales.base);
+  out->v_scales = reinterpret_cast<float*>(cache.v_scales.base);
   out->k_weight = reinterpret_cast<const void*>(a.k_weight);
   out->positions = reinterpret_cast<const void*>(a.positions);
   out->inv_freq = reinterpret_cast<const float*>(a.inv_freq);
@@ -394,11 +429,6 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
     }
     if (a.lse != 0) {
       KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
-      uint64_t bytes = 0;
-      if (!o.empty() && o.Extent(&bytes) &&
-          Meet(a.lse, static_cast<uint64_t>(a.tokens * a.q_heads) * 4, a.out, bytes)) {
-        return Bad("lse: overlaps out");
-      }
     }
   } else {
     // Sizes only: the address arguments may still be unset.
@@ -436,8 +466,8 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
   out->out_head = a.out_head_stride;
   out->k_pool = reinterpret_cast<const void*>(cache.k.base);
   out->v_pool = reinterpret_cast<const void*>(cache.v.base);
-  out->k_scales = reinterpret_cast<const float*>(cache.k_scales);
-  out->v_scales = reinterpret_cast<const float*>(cache.v_scales);
+  out->k_scales = reinterpret_cast<const float*>(cache.k_scales.base);
+  out->v_scales = reinterpret_cast<const float*>(cache.v_scales.base);
   out->group_starts = reinterpret_cast<const int32_t*>(a.group_starts);
   out->prefix_lengths = reinterpret_cast<const int32_t*>(a.prefix_lengths);
   out->groups = a.groups;
@@ -465,7 +495,26 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
     KVX_RETURN_IF_ERROR(ranges.Check(a.workspace, static_cast<uint64_t>(need), "workspace"));
     out->parts = reinterpret_cast<float*>(a.workspace);
   }
-  return OkStatus();
+  // What is written may meet nothing else (`out` may be q).
+  const Named results = {o, "out"}, queries = {q, "q"};
+  const Named lse = {Whole(a.lse, a.lse != 0 ? a.tokens * a.q_heads * 4 : 0), "lse"};
+  const Named workspace = {Whole(a.workspace, need), "workspace"};
+  const int64_t groups = a.batch.sequences > 0 ? a.groups : 0;
+  const std::initializer_list<Named> others = {
+      {Whole(cache.k), "the cache"},
+      {Whole(cache.v), "the cache"},
+      {Whole(cache.k_scales), "the cache's scales"},
+      {Whole(cache.v_scales), "the cache's scales"},
+      {Tables(a.batch), "tables"},
+      {Lengths(a.batch), "lengths"},
+      {Starts(a.batch), "starts"},
+      {Whole(a.group_starts, groups > 0 ? (groups + 1) * 4 : 0), "group_starts"},
+      {Whole(a.prefix_lengths, groups * 4), "prefix_lengths"}};
+  for (const Named* written : {&results, &lse, &workspace}) {
+    KVX_RETURN_IF_ERROR(CheckApart(*written, others));
+  }
+  KVX_RETURN_IF_ERROR(CheckApart(lse, {results, queries}));
+  return CheckApart(workspace, {results, queries, lse});
 }
 
 }  // namespace kvx
