@@ -1089,7 +1089,8 @@ typedef struct kvx_paged_batch {
  * clamped to +-448 scales, and earlier tokens are stored again under a scale
  * that grew. A block that takes new tokens must belong to one sequence of the
  * call, and a token to one slot: with the same block or slot twice, which of
- * the values remain is not defined.
+ * the values remain is not defined. No argument may lie in the cache or its
+ * scales.
  */
 typedef struct kvx_append_kv_args {
   kvx_paged_cache cache;

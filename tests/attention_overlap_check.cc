@@ -245,12 +245,71 @@ void AttendResults() {
   }
 }
 
+kvx::Status Append(bool e4m3, const std::function<void(kvx_append_kv_args&)>& change) {
+  kvx_append_kv_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.cache = GoodCache(e4m3);
+  a.batch = GoodBatch();
+  a.tokens = 10;
+  a.dtype = KVX_BF16;
+  a.rotary_dim = 64;
+  a.k = At(1);
+  a.v = At(2);
+  a.k_token_stride = a.v_token_stride = 128;
+  a.k_head_stride = a.v_head_stride = 64;
+  a.k_weight = At(3);
+  a.weight_dtype = KVX_F32;
+  a.inv_freq = At(4);
+  a.positions = At(5);
+  a.positions_64 = 1;
+  change(a);
+  kvx::AppendLaunch l;
+  return kvx::CheckAppendKv(Pool(), a, &l);
+}
+
+void AppendInputs() {
+  using A = kvx_append_kv_args;
+  struct {
+    const char* name;
+    std::function<void(A&, uint64_t)> put;
+  } const inputs[] = {
+      {"k", [](A& a, uint64_t at) { a.k = at; }},
+      {"v", [](A& a, uint64_t at) { a.v = at; }},
+      {"tables", [](A& a, uint64_t at) { a.batch.tables = at; }},
+      {"lengths", [](A& a, uint64_t at) { a.batch.lengths = at; }},
+      {"starts", [](A& a, uint64_t at) { a.batch.starts = at; }},
+      {"k_weight", [](A& a, uint64_t at) { a.k_weight = at; }},
+      {"inv_freq", [](A& a, uint64_t at) { a.inv_freq = at; }},
+      {"positions", [](A& a, uint64_t at) { a.positions = at; }},
+  };
+  for (bool e4m3 : {false, true}) {
+    Passes(Append(e4m3, [](A&) {}), "append");
+    const uint64_t k = e4m3 ? At(2050) : At(2048), v = k + (1 << 20);
+    const uint64_t last = 100 * (e4m3 ? 2048 : 4096) - 8;
+    for (const auto& in : inputs) {
+      const std::string on = std::string(in.name) + ": overlaps the cache";
+      for (uint64_t at : {k, v, k + last, v + last}) {
+        Refused(Append(e4m3, [&](A& a) { in.put(a, at); }), on.c_str(), "append from the cache");
+      }
+      for (uint64_t at : {At(2052), At(2053), At(2053) + 792}) {
+        if (e4m3) {
+          Refused(Append(true, [&](A& a) { in.put(a, at); }), (on + "'s scales").c_str(),
+                  "append from the scales");
+        } else {
+          Passes(Append(false, [&](A& a) { in.put(a, at); }), "no scales in use");
+        }
+      }
+    }
+  }
+}
+
 }  // namespace
 
 int main() {
   kvx::SetAddressQueryForTesting(FakeQuery);
   FusedProjections();
   AttendResults();
+  AppendInputs();
   kvx::SetAddressQueryForTesting(nullptr);
   if (failures == 0) std::printf("attention overlap checks: all passed\n");
   return failures == 0 ? 0 : 1;

@@ -119,10 +119,10 @@ struct Named {
 // `bytes` bytes at an address, without gaps.
 Rows Whole(uint64_t at, int64_t bytes) { return {at, 0, 0, bytes > 0 ? 1 : 0, 1, bytes, 1}; }
 
-Status CheckApart(const Named& written, std::initializer_list<Named> others) {
+Status CheckApart(const Named& a, std::initializer_list<Named> others) {
   for (const Named& o : others) {
-    if (Meet(written.rows.at, written.bytes, o.rows.at, o.bytes) && Meet(written.rows, o.rows)) {
-      return Bad(std::string(written.name) + ": overlaps " + o.name);
+    if (Meet(a.rows.at, a.bytes, o.rows.at, o.bytes) && Meet(a.rows, o.rows)) {
+      return Bad(std::string(a.name) + ": overlaps " + o.name);
     }
   }
   return OkStatus();
@@ -357,15 +357,6 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
   const Rows v = {a.v, a.v_token_stride, a.v_head_stride, a.tokens, c.heads, c.head_dim, 2};
   KVX_RETURN_IF_ERROR(CheckRows(&ranges, k, "k"));
   KVX_RETURN_IF_ERROR(CheckRows(&ranges, v, "v"));
-  for (const Rows* r : {&k, &v}) {
-    uint64_t bytes = 0;
-    if (r->empty() || !r->Extent(&bytes)) continue;
-    for (const PoolStorage* s : {&cache.k, &cache.v}) {
-      if (Meet(r->at, bytes, s->base, static_cast<uint64_t>(s->bytes))) {
-        return Bad(std::string(r == &k ? "k" : "v") + ": overlaps the cache");
-      }
-    }
-  }
   *out = AppendLaunch{};
   KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
                                  &out->batch));
@@ -373,6 +364,25 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
                                     a.positions_64 != 0, a.tokens));
   KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.k_weight, a.weight_dtype, a.dtype, c.head_dim, a.eps,
                                   "k_weight"));
+  // What is written may meet nothing that is read.
+  const std::initializer_list<Named> read = {
+      {k, "k"},
+      {v, "v"},
+      {Tables(a.batch), "tables"},
+      {Lengths(a.batch), "lengths"},
+      {Starts(a.batch), "starts"},
+      {Whole(a.k_weight, a.k_weight != 0 ? c.head_dim * ElementBytes(a.weight_dtype) : 0),
+       "k_weight"},
+      {Whole(a.inv_freq, a.tokens > 0 ? a.rotary_dim * 2 : 0), "inv_freq"},
+      {Whole(a.positions,
+             a.rotary_dim > 0 && a.positions != 0 ? a.tokens * (a.positions_64 != 0 ? 8 : 4) : 0),
+       "positions"}};
+  for (const Named& r : read) {
+    KVX_RETURN_IF_ERROR(CheckApart(r, {{Whole(cache.k), "the cache"},
+                                       {Whole(cache.v), "the cache"},
+                                       {Whole(cache.k_scales), "the cache's scales"},
+                                       {Whole(cache.v_scales), "the cache's scales"}}));
+  }
   if (a.batch.sequences == 0) out->batch.tokens = 0;
   out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
   out->k = reinterpret_cast<const void*>(a.k);
