@@ -143,6 +143,44 @@ void FusedProjections() {
   }
 }
 
+void NormInputs() {
+  using A = kvx_norm_rope_args;
+  const auto weighted = [](const std::function<void(A&)>& change) {
+    return Norm([&](A& a) {
+      a.q_weight = At(7);
+      a.k_weight = At(8);
+      a.weight_dtype = KVX_F32;
+      change(a);
+    });
+  };
+  Passes(weighted([](A&) {}), "norm");
+  // Rows of 512 elements 1024 apart: the weights between the first two.
+  Passes(weighted([](A& a) {
+           a.q_out_token_stride = 1024;
+           a.q_weight = a.q_out + 512 * 2;
+         }),
+         "a weight between rows");
+  for (uint64_t off : {0, 9 * 512 * 2 + 510 * 2}) {
+    for (bool q : {true, false}) {
+      const char* name = q ? "q_out" : "k_out";
+      const auto on = [&](uint64_t A::*input, const char* what) {
+        const std::string message = std::string(name) + ": overlaps " + what;
+        Refused(weighted([&](A& a) { a.*input = (q ? a.q_out : a.k_out) + off; }), message.c_str(),
+                "norm onto its inputs");
+      };
+      on(&A::q_weight, "q_weight");
+      on(&A::k_weight, "k_weight");
+      on(&A::inv_freq, "inv_freq");
+      on(&A::positions, "positions");
+    }
+  }
+  Passes(weighted([](A& a) {
+           a.rotary_dim = 0;
+           a.positions = a.inv_freq = a.q_out;
+         }),
+         "nothing rotated");
+}
+
 // 100 blocks of [16][2][64]: layers 0, 1 bf16; 2, 3 e4m3; 4, 5 their scales.
 bool Find(const void*, int64_t layer, int64_t shard, kvx::PoolStorage* out) {
   if (layer < 0 || layer > 5 || shard != 0) return false;
@@ -308,6 +346,7 @@ void AppendInputs() {
 int main() {
   kvx::SetAddressQueryForTesting(FakeQuery);
   FusedProjections();
+  NormInputs();
   AttendResults();
   AppendInputs();
   kvx::SetAddressQueryForTesting(nullptr);

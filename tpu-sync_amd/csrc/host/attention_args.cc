@@ -319,6 +319,15 @@ Status CheckNormRope(const kvx_norm_rope_args& a, NormRopeLaunch* out) {
                                   "q_weight"));
   KVX_RETURN_IF_ERROR(CheckWeight(&ranges, a.k_weight, a.weight_dtype, a.dtype, a.head_dim, a.eps,
                                   "k_weight"));
+  const int64_t weight_bytes = a.head_dim * ElementBytes(a.weight_dtype);
+  const int64_t rotated = a.rotary_dim > 0 ? a.tokens : 0;
+  for (const Named& written : {Named(qo, "q_out"), Named(ko, "k_out")}) {
+    KVX_RETURN_IF_ERROR(CheckApart(
+        written, {{Whole(a.q_weight, a.q_weight != 0 ? weight_bytes : 0), "q_weight"},
+                  {Whole(a.k_weight, a.k_weight != 0 ? weight_bytes : 0), "k_weight"},
+                  {Whole(a.inv_freq, a.tokens > 0 ? a.rotary_dim * 2 : 0), "inv_freq"},
+                  {Whole(a.positions, rotated * (a.positions_64 != 0 ? 8 : 4)), "positions"}}));
+  }
   const auto rows = [](const Rows& in, const Rows& o, uint64_t weight) {
     HeadRows r;
     r.in = reinterpret_cast<const void*>(in.at);
