@@ -1,5 +1,6 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
-own result, starts that are out of order, interleaved heads."""
+own result, starts that are out of order, interleaved heads, inputs that are
+differentiated."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -88,3 +89,36 @@ def test_norm_rope_in_place_of_interleaved_heads(kvx, cuda, dim):
     kvx.norm_rope(q, k, pos, inv, q_weight=w, k_weight=w, out_q=q, out_k=k)
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
     assert torch.equal(qkv[:, :, 2], held[:, :, 2])
+
+
+def test_inputs_that_are_differentiated_are_refused(kvx, cuda):
+    from torch.autograd import forward_ad
+    caches = [torch.zeros(4, 16, 2, 64, device=cuda).to(BF16) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
+    pos, args = ints([0, 1, 2], cuda), (ints([[0, 1, 2, 3]], cuda), ints([3], cuda))
+    good = dict(x=torch.ones(3, 2, 64, device=cuda).to(BF16), inv=torch.ones(32, device=cuda),
+                w=torch.ones(64, device=cuda))
+
+    def calls(x, inv, w):
+        kw = dict(starts=ints([0, 3], cuda))
+        yield lambda: kvx.norm_rope(x, None, pos, inv, q_weight=w)
+        yield lambda: mgr.append_kv(0, 1, x, x, *args, inv_freq=inv, k_weight=w, **kw)
+        if inv is good["inv"] and w is good["w"]:
+            yield lambda: mgr.attend(0, 1, x, *args, **kw)
+
+    for call in calls(**good):
+        call()
+    for name, t in good.items():
+        leaf = t.clone().requires_grad_()
+        for call in calls(**{**good, name: leaf}):
+            with pytest.raises(ValueError, match="requires gradients"):
+                call()
+            with torch.no_grad():
+                call()
+        with forward_ad.dual_level():
+            for call in calls(**{**good, name: forward_ad.make_dual(t, torch.ones_like(t))}):
+                with pytest.raises(ValueError, match="has a tangent"):
+                    call()
+            for call in calls(**good):
+                call()
+    mgr.close()

@@ -6,6 +6,10 @@ import subprocess
 
 import pytest
 
+torch = pytest.importorskip("torch")
+
+from fake_device import FakeDeviceTensor  # noqa: E402
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -37,3 +41,26 @@ def test_sums_of_work_do_not_wrap(tmp_path):
 
 def test_arguments_in_one_buffer(tmp_path):
     assert "all passed" in run_check("attention_overlap_check", tmp_path, library=True)
+
+
+def test_frequencies_that_require_gradients_are_refused(kvx):
+    def fake(*shape, dtype=torch.bfloat16, **kw):
+        return FakeDeviceTensor(torch.zeros(shape, dtype=dtype, **kw))
+
+    q, pos = fake(3, 4, 64), fake(3, dtype=torch.int64)
+    inv = fake(32, dtype=torch.float32, requires_grad=True)
+    with pytest.raises(ValueError, match="inv_freq requires gradients: there is no backward"):
+        kvx.norm_rope(q, None, pos, inv, out_q=fake(3, 4, 64), stream=0)
+
+
+def test_tangents_are_refused(kvx):
+    from torch.autograd import forward_ad
+    module = __import__(kvx.__name__ + ".paged_attention", fromlist=["paged_attention"])
+    module._load_torch()
+    x = torch.ones(4)
+    module._refuse_gradients(x, "x")
+    with forward_ad.dual_level():
+        module._refuse_gradients(x, "x")
+        with pytest.raises(ValueError, match="x has a tangent"):
+            module._refuse_gradients(forward_ad.make_dual(x, torch.ones(4)), "x")
+    module._refuse_gradients(x, "x")

@@ -8,8 +8,9 @@ their argument handling is here. The three are a step's work around the cache:
     mgr.append_kv(2 * i, 2 * i + 1, k, v, tables, lengths, inv_freq=inv_freq, k_weight=wk)
     out = mgr.attend(2 * i, 2 * i + 1, q, tables, lengths)
 
-They are serving operators with no backward pass: tensors that require
-gradients are refused while gradients are recorded. Calls are enqueued on
+They are serving operators with no derivatives: tensors that require gradients
+are refused while gradients are recorded, and so are dual tensors of forward-mode
+differentiation. Calls are enqueued on
 ``stream`` (default: torch's current stream), allocate their outputs and
 workspace from torch's allocator on that stream, and can be captured into a
 graph. This module only passes pointers; the checks behind it are libkvx's.
@@ -33,7 +34,7 @@ for _pack, _args in ((_NORM_ROPE, _capi.NormRopeArgs), (_APPEND_KV, _capi.Append
     assert _pack.size == ctypes.sizeof(_args)
 
 _TYPES = {}
-_torch = None
+_torch = _forward_ad = None
 
 
 def _current_stream(device):
@@ -41,9 +42,11 @@ def _current_stream(device):
 
 
 def _load_torch():
-    global _torch, _current_stream
+    global _torch, _forward_ad, _current_stream
     if _torch is None:
         import torch
+        from torch.autograd import forward_ad
+        _forward_ad = forward_ad
         # The handle alone, without a Stream object around it, where torch has it.
         _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
         _TYPES.update({torch.bfloat16: _capi.BF16, torch.float16: _capi.F16,
@@ -63,6 +66,15 @@ def _on_device(t, device):
     return getattr(t, "is_cuda", False) and (t.device.index or 0) == device
 
 
+def _refuse_gradients(t, what):
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise ValueError(f"{what} requires gradients: there is no backward pass")
+    # Outside of a dual level (-1) no tensor has a tangent to look for.
+    if (getattr(_forward_ad, "_current_level", 0) >= 0
+            and _forward_ad.unpack_dual(t).tangent is not None):
+        raise ValueError(f"{what} has a tangent: there is no forward-mode derivative")
+
+
 def _rows(t, what, device, dtype=None, shape=None):
     """Checks a [tokens, heads, head_dim] tensor whose last dimension is
     contiguous; returns its address and (token, head) strides."""
@@ -75,8 +87,7 @@ def _rows(t, what, device, dtype=None, shape=None):
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if shape is not None and got != shape:
         raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(got)}")
-    if t.requires_grad and _torch.is_grad_enabled():
-        raise ValueError(f"{what} requires gradients: there is no backward pass")
+    _refuse_gradients(t, what)
     token, head, last = t.stride()
     if last != 1 and got[2] != 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
@@ -101,8 +112,7 @@ def _weight(t, what, device, dtype, n):
     if t is None:
         return 0, 0
     ptr = _vector(t, what, device, (dtype, _torch.float32), n)
-    if t.requires_grad and _torch.is_grad_enabled():
-        raise ValueError(f"{what} requires gradients: there is no backward pass")
+    _refuse_gradients(t, what)
     return ptr, _TYPES[t.dtype]
 
 
@@ -115,6 +125,7 @@ def _rotation(device, inv_freq, positions, tokens, head_dim):
         raise ValueError(f"inv_freq must have 1 to {head_dim // 2} elements, "
                          f"got {tuple(inv_freq.shape)}")
     at = _vector(inv_freq, "inv_freq", device, (_torch.float32,), n)
+    _refuse_gradients(inv_freq, "inv_freq")
     if positions is None:
         return 2 * n, at, 0, 0
     where = _vector(positions, "positions", device, (_torch.int64, _torch.int32), tokens)
