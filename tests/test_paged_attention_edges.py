@@ -1,6 +1,8 @@
 """The paged operators' checks and arithmetic on the CPU where calls are unusual:
 programs of their own that include the library's sources' headers."""
+import glob
 import os
+import re
 import shutil
 import subprocess
 
@@ -64,3 +66,19 @@ def test_tangents_are_refused(kvx):
         with pytest.raises(ValueError, match="x has a tangent"):
             module._refuse_gradients(forward_ad.make_dual(x, torch.ones(4)), "x")
     module._refuse_gradients(x, "x")
+
+
+def test_inline_assembly_does_not_write_m0():
+    """The compiler uses m0 too and reserves it, so that a clobber says nothing: a
+    load into LDS gets its address by an operand that the compiler puts there."""
+    kernels = os.path.join(ROOT, "tpu-sync_amd", "csrc", "kernels")
+    found = 0
+    for path in glob.glob(os.path.join(kernels, "*")):
+        with open(path) as f:
+            for statement in re.findall(r"asm volatile\((.*?)\);", f.read(), re.S):
+                code, operands = statement.split(":", 1)
+                assert "m0" not in code, f"{path}: {statement}"
+                if "_lds_" in code:
+                    found += 1
+                    assert '"{m0}"' in operands, f"{path}: {statement}"
+    assert found > 0

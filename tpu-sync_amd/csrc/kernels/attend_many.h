@@ -57,13 +57,11 @@ __device__ __forceinline__ uint32_t LdsAddress(char* p) {
   return static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)p));
 }
-// Loads 16 bytes a lane straight into LDS, lane l's to address `to` + 16 l. The
-// compiler does not know of them: LdsArrived waits for all but the last N.
+// Loads 16 bytes a lane straight into LDS, lane l's to address `to` + 16 l, which
+// is taken from m0 (the compiler's to write, a wait state ahead). The compiler
+// does not know of the loads: LdsArrived waits for all but the last N.
 __device__ __forceinline__ void ToLds16(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(to), "v"(from)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(to) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void LdsArrived() {
