@@ -1,12 +1,14 @@
 // Checks AddUpTo (kernels/kv_element.h), the sums by which the paged operators'
 // kernels share out work that device arrays name, on the CPU: with starts that
 // give thousands of sequences the same millions of tokens, each place of the grid
-// still belongs to one sequence at most.
+// still belongs to one sequence at most. And WorkerAt (kernels/attend.h), the
+// order in which a grid's workgroups take attention's parts.
 #include <climits>
 #include <cstdint>
 #include <cstdio>
 #include <vector>
 
+#include "attend.h"
 #include "kv_element.h"
 
 using kvx::AddUpTo;
@@ -15,7 +17,44 @@ static_assert(AddUpTo(0, 0, 0) == 0 && AddUpTo(3, 4, 8) == 7 && AddUpTo(4, 4, 8)
 static_assert(AddUpTo(8, 8, 8) == 8 && AddUpTo(INT_MAX, INT_MAX, INT_MAX) == INT_MAX, "");
 static_assert(AddUpTo(INT_MAX, 1, INT_MAX) == INT_MAX, "");
 
+// Every worker has one place, an XCD's (every eighth place) are neighbours, and no
+// XCD has more than its share: a grid that was sized for longer sequences than
+// the call has leaves no XCD idle.
+bool Places(int grid, int workers) {
+  std::vector<int> place(workers, -1);
+  int of[8] = {0}, low[8], high[8];
+  for (int x = 0; x < 8; ++x) {
+    low[x] = INT_MAX;
+    high[x] = -1;
+  }
+  for (int p = 0; p < grid; ++p) {
+    const int w = kvx::WorkerAt(p, workers);
+    if (w < 0) continue;
+    if (w >= workers || place[w] >= 0) return false;
+    place[w] = p;
+    ++of[p % 8];
+    low[p % 8] = w < low[p % 8] ? w : low[p % 8];
+    high[p % 8] = w > high[p % 8] ? w : high[p % 8];
+  }
+  for (int w = 0; w < workers; ++w) {
+    if (place[w] < 0) return false;
+  }
+  for (int x = 0; x < 8; ++x) {
+    if (of[x] > (workers + 7) / 8) return false;
+    if (of[x] > 0 && high[x] - low[x] + 1 != of[x]) return false;
+  }
+  return true;
+}
+
 int main() {
+  for (int grid : {256, 512}) {
+    for (int workers = 0; workers <= grid; ++workers) {
+      if (!Places(grid, workers)) {
+        std::printf("FAIL: %d workers in a grid of %d\n", workers, grid);
+        return 1;
+      }
+    }
+  }
   // Sequence 2 k has all of `each` tokens, sequence 2 k + 1 none; a block a token.
   for (int each : {1, 4096, (1 << 20) + 1, (1 << 21) + 2048, 1 << 29}) {
     const int grid = each;

@@ -38,6 +38,18 @@ constexpr int kMaxSequences = 4096;
 constexpr int kMaxGroups = 256;
 constexpr int kMaxHeadDim = 256;
 
+// The worker at a place of a grid whose places go to the XCDs in turn, or -1:
+// an XCD's workers are neighbours, and every XCD has its share of them, however
+// many the lengths leave of the grid that the table's width allows. (Shared out
+// over that grid, a prompt of 128 tokens, 32 heads on 8, in a table of 8192 had two
+// XCDs: 31.3 us, here 24.2.)
+constexpr int kXcds = 8;
+constexpr int WorkerAt(int place, int workers) {
+  const int each = (workers + kXcds - 1) / kXcds;
+  const int at = place / kXcds, worker = place % kXcds * each + at;
+  return at < each && worker < workers ? worker : -1;
+}
+
 struct AttendLaunch {
   BatchView batch;
   FastDivU32 block_div;  // by batch.block_tokens

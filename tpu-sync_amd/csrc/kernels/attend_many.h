@@ -82,7 +82,7 @@ constexpr size_t ManyLds(const AttendLaunch& l, int dp) {
 }
 
 template <class E, bool E4, int DP>
-__device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int worker) {
+__device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int place) {
   using Scalar = typename E::Scalar;
   constexpr int KS = DP / 16, DT = DP / 32, kRow = 2 * DP;  // bytes of a token's row
   constexpr int kChunks = kManyStep * (DP / 8) / kAttendThreads;  // of a thread
@@ -108,7 +108,8 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
   const int work = one(sums[units - 1]);
   if (work == 0) return;
   const Axis axis = ManyAxis(a, work);
-  if (worker >= axis.workers) return;
+  const int worker = WorkerAt(place, axis.workers);
+  if (worker < 0) return;
   const int x_start = axis.Start(worker), x_end = axis.Start(worker + 1);
   const int G = a.q_heads / a.k_heads;
   const int lane = threadIdx.x % 64, wave = one(threadIdx.x / 64);

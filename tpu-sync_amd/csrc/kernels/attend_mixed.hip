@@ -10,7 +10,6 @@
 namespace kvx {
 namespace {
 
-constexpr int kXcds = 8;
 constexpr int kRound = 256;  // CUs
 
 // A kind's workgroups, in whole rounds.
@@ -33,9 +32,7 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void attend_mixe
   const bool is_many = round < 2 * both ? round % 2 == 0 : many > few;
   const int mine = (round < 2 * both ? round / 2 : round - both) * kRound + block % kRound;
   if (is_many) {
-    // An XCD's workgroups take neighbouring parts.
-    const int worker = mine % kXcds * (many / kXcds) + mine / kXcds;
-    if (worker < a.many_grid) AttendMany<E, E4, DP>(a, lds, worker);
+    AttendMany<E, E4, DP>(a, lds, mine);
   } else {
     if (mine < a.few_grid) AttendFew<E, E4, DP, RT, FULL>(a, lds, mine);
   }
