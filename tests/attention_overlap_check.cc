@@ -1,5 +1,5 @@
-// Which of the paged operators' arguments may lie in one buffer, on the CPU, no
-// GPU calls: a pool and an address map of their own making stand in for the
+// Which of the paged operators' arguments may lie in one buffer, or be empty, on
+// the CPU, no GPU calls: a pool and an address map of their own making stand in for the
 // manager and the HIP runtime. Arguments that share no element pass, however
 // they are interleaved; a result on anything else that the call reads or writes
 // is refused with INVALID_ARGUMENT and a message that names both.
@@ -341,6 +341,22 @@ void AppendInputs() {
   }
 }
 
+// A table without a column, as torch makes it: no address, a stride of 1.
+void NoTable() {
+  for (int64_t sequences : {1, 3}) {
+    const auto change = [&](auto& a) {
+      a.batch.sequences = sequences;
+      a.batch.tables = 0;
+      a.batch.table_width = 0;
+      a.batch.table_stride = 1;
+    };
+    for (bool e4m3 : {false, true}) {
+      Passes(Append(e4m3, change), "append without a table");
+      Passes(Attend(e4m3, change), "attend without a table");
+    }
+  }
+}
+
 }  // namespace
 
 int main() {
@@ -349,6 +365,7 @@ int main() {
   NormInputs();
   AttendResults();
   AppendInputs();
+  NoTable();
   kvx::SetAddressQueryForTesting(nullptr);
   if (failures == 0) std::printf("attention overlap checks: all passed\n");
   return failures == 0 ? 0 : 1;

@@ -1,6 +1,6 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
 own result, starts that are out of order, interleaved heads, inputs that are
-differentiated."""
+differentiated, tables without a column."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -121,4 +121,25 @@ def test_inputs_that_are_differentiated_are_refused(kvx, cuda):
                     call()
             for call in calls(**good):
                 call()
+    mgr.close()
+
+
+@pytest.mark.parametrize("cache", [BF16, FP8])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [3, 0, 40], [200]])
+def test_tables_without_a_column(kvx, cuda, cache, counts):
+    """No token has a place: nothing is stored, and every query sees nothing."""
+    caches = [torch.full((4, 16, 2, 64), 7.0, device=cuda).to(cache) for _ in range(2)]
+    kw = {}
+    if cache == FP8:
+        kw = dict(scale_tables=[torch.ones(4, 2, device=cuda) for _ in range(2)])
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, **kw)
+    n, tokens = len(counts), sum(counts)
+    starts = ints([sum(counts[:i]) for i in range(n + 1)], cuda)
+    args = (torch.empty((n, 0), dtype=torch.int32, device=cuda), ints(counts, cuda))
+    k = torch.ones(tokens, 2, 64, device=cuda).to(BF16)
+    mgr.append_kv(0, 1, k, k, *args, starts=starts)
+    assert all(bool((c.float() == 7).all()) for c in caches)
+    out, lse = mgr.attend(0, 1, torch.ones(tokens, 8, 64, device=cuda).to(BF16), *args,
+                          starts=starts, return_lse=True)
+    assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
     mgr.close()

@@ -199,7 +199,7 @@ Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t 
         __builtin_add_overflow(words, b.table_width, &words) || words > INT64_MAX / 4) {
       return Bad("tables: size overflows");
     }
-    KVX_RETURN_IF_ERROR(CheckWords(ranges, b.tables, words, "tables"));
+    if (b.table_width > 0) KVX_RETURN_IF_ERROR(CheckWords(ranges, b.tables, words, "tables"));
     KVX_RETURN_IF_ERROR(CheckWords(ranges, b.lengths, b.sequences, "lengths"));
     if (b.starts != 0) {
       KVX_RETURN_IF_ERROR(CheckWords(ranges, b.starts, b.sequences + 1, "starts"));
