@@ -1,6 +1,7 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
 own result, starts that are out of order, interleaved heads, inputs that are
-differentiated, tables without a column."""
+differentiated, tables without a column, queries that see nothing beside
+values that are not finite."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -142,4 +143,45 @@ def test_tables_without_a_column(kvx, cuda, cache, counts):
     out, lse = mgr.attend(0, 1, torch.ones(tokens, 8, 64, device=cuda).to(BF16), *args,
                           starts=starts, return_lse=True)
     assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
+    mgr.close()
+
+
+@pytest.mark.parametrize("cache", [BF16, FP8])
+@pytest.mark.parametrize("counts,lengths,prefix", [
+    ([1, 1, 1], [90, 0, 70], 64),  # padded with an empty sequence, within a group
+    ([1] * 40, [5000] + [0] * 38 + [4992], 4992),  # cut into many parts
+    ([2, 3, 2], [66, 0, 65], 64),
+    ([4], [2], 0),  # the first two of a chunk are before its sequence
+    ([40], [3], 0), ([50, 300], [20, 200], 0)])
+def test_queries_that_see_nothing_beside_infinities(kvx, cuda, cache, counts, lengths, prefix):
+    """Zeros and an lse of -inf, whatever values are masked."""
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    blocks = [(n + 15) // 16 for n in lengths]
+    width = max(blocks)
+    caches = [torch.randn(sum(blocks) + 1, 16, 2, 64, device=cuda, generator=gen) for _ in range(2)]
+    caches[1][:, 1] = float("nan") if cache == FP8 else float("inf")
+    kw = {}
+    if cache == FP8:
+        kw = dict(scale_tables=[torch.ones(sum(blocks) + 1, 2, device=cuda) for _ in range(2)])
+    mgr = kvx.KVCacheManager([c.to(cache) for c in caches], host_blocks_to_allocate=1, **kw)
+    tables, at = [], 0
+    for n in blocks:
+        tables.append(list(range(at, at + n)) + [-1] * (width - n))
+        at += n
+    call = dict(starts=ints([sum(counts[:i]) for i in range(len(counts) + 1)], cuda))
+    if prefix:
+        for t, n in zip(tables[1:], lengths[1:]):
+            if n:
+                t[:prefix // 16] = tables[0][:prefix // 16]
+        call.update(group_starts=ints([0, len(counts)], cuda),
+                    prefix_lengths=ints([prefix], cuda))
+    q = torch.randn(sum(counts), 8, 64, device=cuda, generator=gen).to(BF16)
+    out, lse = mgr.attend(0, 1, q, ints(tables, cuda), ints(lengths, cuda), return_lse=True, **call)
+    first = 0
+    for count, n in zip(counts, lengths):
+        none = slice(first, first + max(count - n, 0))
+        assert bool((out[none] == 0).all()) and bool(torch.isneginf(lse[none]).all())
+        seen = slice(none.stop, first + count)
+        assert bool(torch.isfinite(lse[seen]).all())
+        first += count
     mgr.close()

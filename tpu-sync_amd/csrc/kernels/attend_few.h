@@ -355,13 +355,13 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
       const int head = h * G + (row - t * G);
       if (row < rows) {
         if (whole && !grouped) {
-          const float inverse = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+          const float inverse = 1.0f / l;
           Scalar* out = static_cast<Scalar*>(a.out) + token * a.out_token + head * a.out_head;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const int d = dt * 16 + quarter * 4;
             using Pair = u32x2 __attribute__((aligned(2)));
-            const f32x4 v = o[rt][dt] * inverse;
+            const f32x4 v = Finished(o[rt][dt], l, inverse);
             if (FULL || d < a.head_dim) {
               *reinterpret_cast<Pair*>(out + d) = u32x2{Pack2<E>(v[0], v[1]), Pack2<E>(v[2], v[3])};
             }

@@ -322,6 +322,12 @@ __device__ __forceinline__ void WritePlan(const AttendLaunch& a, int* lds) {
   for (int i = threadIdx.x; i < PlanSumWords(a); i += kAttendThreads) out[i] = lds[i];
 }
 
+// o / l, and zeros of a row that sees nothing (l = 0): values that it does not see
+// have met exponentials of 0, which leaves NaN of those that are not finite.
+__device__ __forceinline__ f32x4 Finished(f32x4 o, float l, float inverse) {
+  return l == 0.0f ? f32x4{0, 0, 0, 0} : o * inverse;
+}
+
 // Maximum over the four 16-lane rows of a wave, lane by lane.
 __device__ __forceinline__ float Across32(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
