@@ -1,8 +1,9 @@
-// Which of the paged operators' arguments may lie in one buffer, or be empty, on
-// the CPU, no GPU calls: a pool and an address map of their own making stand in for the
-// manager and the HIP runtime. Arguments that share no element pass, however
-// they are interleaved; a result on anything else that the call reads or writes
-// is refused with INVALID_ARGUMENT and a message that names both.
+// Which of the paged operators' arguments may lie in one buffer, be empty or be
+// too many, on the CPU, no GPU calls: a pool and an address map of their own
+// making stand in for the manager and the HIP runtime. Arguments that share no
+// element pass, however they are interleaved; a result on anything else that the
+// call reads or writes is refused with INVALID_ARGUMENT and a message that names
+// both.
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -357,6 +358,51 @@ void NoTable() {
   }
 }
 
+// Grids of 2^32 threads and more, which no launch takes, are refused before it.
+void LargestGrids() {
+  const auto norm = [](int64_t tokens) {
+    return Norm([&](kvx_norm_rope_args& a) {
+      a.tokens = tokens;
+      a.q_heads = 1;
+      a.k_heads = 0;
+      a.k = a.k_out = 0;
+      a.head_dim = 1;
+      a.rotary_dim = 0;
+      a.q = At(0);
+      a.q_out = At(1536);
+      a.q_token_stride = a.q_out_token_stride = a.q_head_stride = a.q_out_head_stride = 1;
+    });
+  };
+  Passes(norm((1ll << 29) - 32), "norm of 2^29 - 32 rows");
+  Refused(norm((1ll << 29) - 31), "too many tokens", "norm of 2^29 - 31 rows");
+  // Blocks of one slot [1][1][1], e4m3: a workgroup of 64 threads each.
+  kvx::PoolSource pool;
+  pool.find = [](const void*, int64_t layer, int64_t, kvx::PoolStorage* out) {
+    const int64_t block = layer < 4 ? 1 : 4;
+    *out = {At(2048 + layer * 16), block * 1000, block};
+    return true;
+  };
+  const auto append = [&](int64_t tokens, int32_t type) {
+    kvx_append_kv_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.cache = GoodCache(true);
+    a.cache.block_tokens = a.cache.heads = a.cache.head_dim = 1;
+    a.batch = GoodBatch();
+    a.tokens = tokens;
+    a.dtype = type;
+    a.k = At(0);
+    a.v = At(1024);
+    a.k_token_stride = a.v_token_stride = a.k_head_stride = a.v_head_stride = 1;
+    a.batch.tables = At(4000);
+    a.batch.lengths = At(4001);
+    a.batch.starts = At(4002);
+    kvx::AppendLaunch l;
+    return kvx::CheckAppendKv(pool, a, &l);
+  };
+  Passes(append((1ll << 26) - 1, KVX_BF16), "append to 2^26 - 1 blocks");
+  Refused(append(1ll << 26, KVX_F16), "too many tokens", "append to 2^26 blocks");
+}
+
 }  // namespace
 
 int main() {
@@ -366,6 +412,7 @@ int main() {
   AttendResults();
   AppendInputs();
   NoTable();
+  LargestGrids();
   kvx::SetAddressQueryForTesting(nullptr);
   if (failures == 0) std::printf("attention overlap checks: all passed\n");
   return failures == 0 ? 0 : 1;

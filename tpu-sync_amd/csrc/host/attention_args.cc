@@ -148,6 +148,13 @@ Status CheckTokens(int64_t tokens, int64_t heads, int64_t dim) {
   return OkStatus();
 }
 
+Status CheckGrid(int64_t workgroups, int64_t threads) {
+  return GridFits(workgroups, threads) ? OkStatus() : Bad("too many tokens for one call");
+}
+Status CheckRowGrid(int64_t tokens) {
+  return CheckGrid((tokens + kMostRowTokens - 1) / kMostRowTokens, kRowThreads);
+}
+
 Status CheckRotation(DeviceRangeChecker* ranges, int64_t rotary, int64_t dim, uint64_t inv_freq,
                      uint64_t positions, bool positions_64, int64_t tokens) {
   if (rotary < 0 || rotary % 2 != 0 || rotary > dim) {
@@ -296,6 +303,7 @@ Status CheckNormRope(const kvx_norm_rope_args& a, NormRopeLaunch* out) {
   KVX_RETURN_IF_ERROR(CheckTokens(a.tokens, static_cast<int64_t>(a.q_heads) + a.k_heads,
                                   a.head_dim));
   if (a.q_heads < 0 || a.k_heads < 0) return Bad("negative number of heads");
+  KVX_RETURN_IF_ERROR(CheckRowGrid(a.tokens));
   DeviceRangeChecker ranges(a.device);
   const int64_t item = ElementBytes(a.dtype);
   const Rows q = {a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.q_heads, a.head_dim, item};
@@ -416,7 +424,7 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
   out->positions_64 = a.positions_64 != 0;
   out->interleaved = a.interleaved != 0;
   out->eps = a.eps;
-  return OkStatus();
+  return out->e4m3 ? CheckGrid(MostBlocks(*out), BlockThreads(*out)) : CheckRowGrid(a.tokens);
 }
 
 Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunch* out,

@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "kv_element.h"
@@ -38,6 +39,16 @@ struct AppendLaunch {
   bool interleaved = false;
   float eps = 0;
 };
+
+// The e4m3 kernel's workgroups, one for every block that the tokens can touch
+// (whole ones, and a first and a last part of each sequence), and its threads.
+inline int64_t MostBlocks(const AppendLaunch& l) {
+  const int64_t tokens = l.batch.tokens, sequences = l.batch.sequences;
+  return l.batch.starts == nullptr
+             ? sequences
+             : std::min(tokens, tokens / l.batch.block_tokens + 2 * sequences);
+}
+inline int BlockThreads(const AppendLaunch& l) { return 64 * std::min(l.heads, kRowThreads / 64); }
 
 // Every address range must have been checked.
 hipError_t LaunchAppendKv(const AppendLaunch& l, hipStream_t stream);

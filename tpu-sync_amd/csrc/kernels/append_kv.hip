@@ -36,12 +36,12 @@
 namespace kvx {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kRowThreads;
 constexpr int kWaves = kThreads / 64;
 // append_kv_kernel: a workgroup takes one token until there are kEnough
 // workgroups, then more, up to kMaxTokens. 2048 and 8192 tokens x 8 heads x 128:
 // 6.5 and 15.0 us; with 256 as enough 8.0 and 23.0 us, with 4096 6.5 and 16.2 us.
-constexpr int kMaxTokens = 32;
+constexpr int kMaxTokens = kMostRowTokens;
 constexpr int kEnough = 1024;
 
 __device__ __forceinline__ int FastDiv(const FastDivU32& f, int n) {
@@ -436,16 +436,10 @@ hipError_t Launch(const AppendLaunch& l, hipStream_t stream) {
   const size_t pairs = static_cast<size_t>(l.rotary_dim / 2) * sizeof(f32x2);
   const int tokens = l.batch.tokens;
   if (l.e4m3) {
-    // A block for every one that the tokens can touch: whole ones, and a first
-    // and a last part of each sequence.
-    const int64_t blocks =
-        l.batch.starts == nullptr
-            ? l.batch.sequences
-            : std::min<int64_t>(tokens, tokens / l.batch.block_tokens +
-                                            2 * static_cast<int64_t>(l.batch.sequences));
+    const int64_t blocks = MostBlocks(l);
     // Few blocks: their heads spread over workgroups.
     int split = 1;
-    const int waves = std::min(kWaves, l.heads);
+    const int waves = BlockThreads(l) / 64;
     while (split * waves < l.heads && blocks * 2 * split < 1024) ++split;
     const dim3 grid(static_cast<unsigned>(blocks), 2, split);
     const size_t lds = kHeld * (64 / LPR) * pairs +

@@ -20,6 +20,14 @@ constexpr bool Is16Bit(int32_t t) { return t == kBf16 || t == kF16; }
 constexpr int64_t ElementBytes(int32_t t) { return t == kF32 ? 4 : t == kE4m3 ? 1 : 2; }
 constexpr float kE4m3Max = 448.0f;
 
+// A launch counts the threads of a grid's dimension in 32 bits.
+constexpr bool GridFits(int64_t workgroups, int64_t threads) {
+  return workgroups <= UINT32_MAX / threads;
+}
+// Of the kernels that take up to so many tokens a workgroup of so many threads.
+constexpr int kRowThreads = 256;
+constexpr int kMostRowTokens = 32;
+
 // x + y, but at most `most`, for x and y of [0, most]. Work is summed up so
 // where it comes from device arrays: a valid call's sums stay below `most`, and
 // starts that are out of order, whose tokens count for many sequences, can

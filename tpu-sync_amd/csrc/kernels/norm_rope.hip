@@ -22,11 +22,11 @@
 namespace kvx {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kRowThreads;
 // A workgroup takes one token until there are kEnough workgroups, then more, up
 // to kMaxTokens. 2048 and 8192 tokens x 40 heads x 128: 12.6 and 31.1 us; with
 // 256 as enough 17.8 and 58.9 us, with 4096 the same as here.
-constexpr int kMaxTokens = 32;
+constexpr int kMaxTokens = kMostRowTokens;
 constexpr int kEnough = 1024;
 
 __device__ __forceinline__ int64_t Position(const NormRopeLaunch& a, int64_t t) {
