@@ -1,7 +1,7 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
 own result, starts that are out of order, interleaved heads, inputs that are
 differentiated, tables without a column, queries that see nothing beside
-values that are not finite."""
+values that are not finite, rows of nothing but infinities."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -184,4 +184,26 @@ def test_queries_that_see_nothing_beside_infinities(kvx, cuda, cache, counts, le
         seen = slice(none.stop, first + count)
         assert bool(torch.isfinite(lse[seen]).all())
         first += count
+    mgr.close()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("count,dim", [(1, 64), (16, 128), (40, 80), (3, 5)])
+def test_append_of_infinities_alone(kvx, cuda, dtype, count, dim):
+    """No finite value but 0 gives a scale of 0 and infinities are clamped to 448
+    scales: their codes are +-448, which stand for 0, and not NaN."""
+    block, blocks = 16, (count + 15) // 16
+    caches = [torch.ones(blocks, block, 2, dim, device=cuda).to(FP8) for _ in range(2)]
+    scales = [torch.ones(blocks, 2, device=cuda) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, scale_tables=scales)
+    x = torch.zeros(count, 2, dim, device=cuda)
+    x[:, 0, 1], x[:, 0, 3], x[:, 1, 2] = float("inf"), float("-inf"), float("nan")
+    mgr.append_kv(0, 1, x.to(dtype), (-x).to(dtype), ints([list(range(blocks))], cuda),
+                  ints([count], cuda), starts=ints([0, count], cuda))
+    for cache, table, sign in zip(caches, scales, (1, -1)):
+        assert bool((table == 0).all())
+        got = cache.reshape(-1, 2, dim)[:count].float()
+        want = (x * sign).clamp(-448, 448)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
     mgr.close()

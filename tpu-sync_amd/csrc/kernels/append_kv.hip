@@ -391,6 +391,11 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
 #pragma unroll
         for (int j = 0; j < VEC; ++j) y[j] = part * x[n][m][j] * inverse;
         if (clamp) {
+          // A scale of 0 belongs to zeros, infinities and NaN, which stay.
+          if (whole <= 0.0f) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] = x[n][m][j];
+          }
           Q::Clamp(y);
         } else {
           // The quotient itself, by its remainder: bf16 rows often meet the
