@@ -1,7 +1,8 @@
 """GPU: calls on the paged pool that other tests do not make: the same call on its
 own result, starts that are out of order, interleaved heads, inputs that are
-differentiated, tables without a column, queries that see nothing beside
-values that are not finite, rows of nothing but infinities."""
+differentiated, tables without a column, queries that see nothing beside values
+that are not finite, rows of nothing but infinities, thousands of sequences around
+64 KiB of LDS, one token far above thousands."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -206,4 +207,61 @@ def test_append_of_infinities_alone(kvx, cuda, dtype, count, dim):
         want = (x * sign).clamp(-448, 448)
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+    mgr.close()
+
+
+@pytest.mark.parametrize("sequences", [2130, 2250, 2340])
+def test_sequences_whose_plan_and_arrays_pass_64_kib(kvx, cuda, sequences):
+    """28 bytes a sequence are under 64 KiB of LDS, with the joining kernel's own
+    6 KiB over it."""
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    caches = [torch.randn(40, 16, 1, 64, device=cuda, generator=gen).to(BF16) for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
+    tables = torch.randint(0, 40, (sequences, 8), device=cuda, dtype=torch.int32, generator=gen)
+    lengths = torch.randint(1, 129, (sequences,), device=cuda, dtype=torch.int32, generator=gen)
+    q = torch.randn(sequences, 2, 64, device=cuda, generator=gen).to(BF16)
+    out = mgr.attend(0, 1, q, tables, lengths)
+    for s in range(0, sequences, 97):
+        one = mgr.attend(0, 1, q[s:s + 1], tables[s:s + 1], lengths[s:s + 1])
+        # Two roundings of the same sums, which parts of other sizes add up.
+        assert bool(((out[s] - one[0]).float().abs() <= 2.0**-6 * one[0].float().abs() + 0.01).all())
+    mgr.close()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (BF16, FP8), (F16, FP8)])
+@pytest.mark.parametrize("count,sequences", [(1, 1100), (40, 600)])
+@pytest.mark.parametrize("drop", [8.0, 12.0, 14.0])
+def test_many_tokens_far_below_the_largest(kvx, cuda, dtype, cache, count, sequences, drop):
+    """One token's score is `drop` above those of 16383 others, whose exponentials
+    are then 2^-11 to 2^-20 of its own (below fp16's normal numbers) and add up to 5
+    to 1 % of it. They have the values 1, it has 0: the result is their share.
+    So many sequences over the same blocks that one worker goes through each."""
+    n, dim, block = 16384, 64, 64
+    code = 16 if cache == FP8 else 1  # the value 1 at a scale of 1 / code
+    k, v = torch.zeros(n, dim, device=cuda), torch.full((n, dim), float(code), device=cuda)
+    k[0, 0], v[0] = drop * code, 0.0
+    pool = [x.reshape(n // block, block, 1, dim).to(cache) for x in (k, v)]
+    assert all(torch.equal(x.float().reshape(n, dim), y) for x, y in zip(pool, (k, v)))
+    kw = {}
+    if cache == FP8:
+        kw = dict(scale_tables=[torch.full((n // block, 1), 1 / code, device=cuda)
+                                for _ in range(2)])
+    mgr = kvx.KVCacheManager(pool, host_blocks_to_allocate=1, **kw)
+    q = torch.zeros(count * sequences, 1, dim, device=cuda)
+    q[:, 0, 0] = 1.0
+    table = torch.arange(n // block, dtype=torch.int32, device=cuda)
+    out = mgr.attend(0, 1, q.to(dtype), table[None].expand(sequences, -1),
+                     torch.full((sequences,), n, dtype=torch.int32, device=cuda), scale=1.0,
+                     starts=torch.arange(sequences + 1, dtype=torch.int32, device=cuda) * count)
+    others = torch.arange(n - count, n, device=cuda).double()[None, :, None, None]
+    size = torch.exp(torch.tensor(-drop, dtype=torch.float64)).item()
+    want = others * size / (1 + others * size)
+    # Each exponential is off by half a step of its type, in fp16 by up to 2^-25 of
+    # the largest; in fp32 its exponent by 64 half steps and its sums by n. The
+    # result has half a step of its own.
+    half = torch.finfo(dtype).eps / 2
+    low = others * 2.0**-25 if dtype == F16 else 0.0
+    room = want * (2 * half + (n + 128) * 2.0**-24) + low
+    off = (out.double().reshape(sequences, count, 1, dim) - want).abs()
+    assert bool((off <= room).all()), f"{float((off / want).max())} off"
     mgr.close()

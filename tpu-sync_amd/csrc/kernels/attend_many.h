@@ -432,6 +432,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
               const int i = kk * 8;
+              // Rounded to operands, as in attend_few.h.
               const u32x4 p = {Pack2<E>(sc[i], sc[i + 1]), Pack2<E>(sc[i + 2], sc[i + 3]),
                                Pack2<E>(sc[i + 4], sc[i + 5]), Pack2<E>(sc[i + 6], sc[i + 7])};
 #pragma unroll
