@@ -360,13 +360,13 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
       const int head = h * G + (row - t * G);
       if (row < rows) {
         if (whole && !grouped) {
-          const float inverse = 1.0f / l;
+          const float inverse = InverseSum(l);
           Scalar* out = static_cast<Scalar*>(a.out) + token * a.out_token + head * a.out_head;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const int d = dt * 16 + quarter * 4;
             using Pair = u32x2 __attribute__((aligned(2)));
-            const f32x4 v = Finished(o[rt][dt], l, inverse);
+            const f32x4 v = Seen(o[rt][dt], l) * inverse;
             if (FULL || d < a.head_dim) {
               *reinterpret_cast<Pair*>(out + d) = u32x2{Pack2<E>(v[0], v[1]), Pack2<E>(v[2], v[3])};
             }
@@ -378,7 +378,8 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           const int64_t to = whole ? WholeRow(a, false, token, head) : FewSlotRow(a, slot) + row;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            *reinterpret_cast<f32x4*>(a.parts + to * DP + dt * 16 + quarter * 4) = o[rt][dt];
+            *reinterpret_cast<f32x4*>(a.parts + to * DP + dt * 16 + quarter * 4) =
+                Seen(o[rt][dt], l);
           }
           if (quarter == 0) PartStats(a)[to] = f32x2{top[rt], l};
         }

@@ -20,8 +20,6 @@ struct Merged {
   f32x4 v = {0, 0, 0, 0};
 
   __device__ __forceinline__ void Add(float pm, float pl, f32x4 pv) {
-    // A part of which the row sees nothing adds nothing, whatever its values are.
-    if (pl == 0.0f) pv = f32x4{0, 0, 0, 0};
     const float now = fmaxf(m, pm);
     const float back = now == -__builtin_inff() ? 0.0f : now;
     const float f = __builtin_amdgcn_exp2f(m - back), g = __builtin_amdgcn_exp2f(pm - back);
@@ -170,7 +168,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(const Atten
         sum.Add(st[0], st[1], part_v[other]);
       }
       if (has_row && d < a.head_dim) {
-        const f32x4 v = Finished(sum.v, sum.l, 1.0f / sum.l);
+        const f32x4 v = sum.v * InverseSum(sum.l);
         using Pair = u32x2 __attribute__((aligned(2)));
         *reinterpret_cast<Pair*>(static_cast<Scalar*>(a.out) + token * a.out_token +
                                  head * a.out_head + d) =

@@ -495,7 +495,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
     const bool whole = from == 0 && to == cost;
     if (row < rows) {
       if (whole && !grouped) {
-        const float inverse = 1.0f / sum;
+        const float inverse = InverseSum(sum);
         Scalar* out = static_cast<Scalar*>(a.out) + token * a.out_token + head * a.out_head;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
@@ -504,8 +504,8 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
             const int d = dt * 32 + i * 2 + half * 4;
             using Pair = u32x2 __attribute__((aligned(2)));
             if (d < a.head_dim) {
-              const f32x4 v = Finished(
-                  f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]}, sum, inverse);
+              const f32x4 v =
+                  Seen(f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]}, sum) * inverse;
               *reinterpret_cast<Pair*>(out + d) = u32x2{Pack2<E>(v[0], v[1]), Pack2<E>(v[2], v[3])};
             }
           }
@@ -522,7 +522,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             *reinterpret_cast<f32x4*>(a.parts + to_row * DP + dt * 32 + i * 2 + half * 4) =
-                f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+                Seen(f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]}, sum);
           }
         }
       }

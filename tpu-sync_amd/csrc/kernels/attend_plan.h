@@ -322,10 +322,14 @@ __device__ __forceinline__ void WritePlan(const AttendLaunch& a, int* lds) {
   for (int i = threadIdx.x; i < PlanSumWords(a); i += kAttendThreads) out[i] = lds[i];
 }
 
-// o / l, and zeros of a row that sees nothing (l = 0): values that it does not see
-// have met exponentials of 0, which leaves NaN of those that are not finite.
-__device__ __forceinline__ f32x4 Finished(f32x4 o, float l, float inverse) {
-  return l == 0.0f ? f32x4{0, 0, 0, 0} : o * inverse;
+// o, or zeros where a row or its part sees nothing (l = 0): values that it does
+// not see have met exponentials of 0, which leaves NaN of those that are not finite.
+__device__ __forceinline__ f32x4 Seen(f32x4 o, float l) {
+  return l == 0.0f ? f32x4{0, 0, 0, 0} : o;
+}
+// 1 / l, and 0 of 0.
+__device__ __forceinline__ float InverseSum(float l) {
+  return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
 }
 
 // Maximum over the four 16-lane rows of a wave, lane by lane.
