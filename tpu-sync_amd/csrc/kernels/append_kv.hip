@@ -9,8 +9,9 @@
 // finds their sequences (all lengths at once, one a lane), puts places and
 // (cos, sin) into LDS; teams of lanes (head_row.h) take a token's key heads and
 // value heads in turn. Reading and writing the rows bounds it: 16384 tokens x 8
-// heads x 128, normed, 26 us (5.1 TB/s both ways); one token of each of 64
-// sequences 4 us, which is the launch and its dependent loads.
+// heads x 128, normed, 34.5 us from cold caches (3.9 TB/s both ways), 26.3 us
+// again and again on rows that the last-level cache holds; one token of each of
+// 64 sequences 4.1 us, which is the launch and its dependent loads.
 //
 // e4m3 pool (append_e4m3_kernel): one fp32 scale per (block, head), so all
 // rows of a block and head have to be seen before the first is written. A
@@ -22,9 +23,10 @@
 // before the first is worked on (one, where there is one new token), so that the
 // rows are read once; a block with more new rows is read once for amax and again
 // (from the cache) to be stored. Registers decide: 8201 tokens x 8 heads x 128
-// take 23 us with 8 rows held by 2 waves a SIMD, 32 us with 4 by 3, 61 us with 4
-// by 4 (spilled). Workgroups have as many waves as heads, up to four: 85624
-// tokens of one head, normed, 41 us; with three waves idle 76 us.
+// took 23 us with 8 rows held by 2 waves a SIMD (256 registers), 32 us with 4 by
+// 3, 61 us with 4 by 4 (spilled); 25.4 us since codes are exact quotients.
+// Workgroups have as many waves as heads, up to four: 85624 tokens of one head,
+// normed, 41 us; with three waves idle 76 us.
 // Earlier tokens of the block are stored again at old / new where new is
 // larger, so they keep their values within e4m3's rounding. Nothing is
 // accumulated over blocks or waves: the same call gives the same bytes.

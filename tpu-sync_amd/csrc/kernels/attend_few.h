@@ -20,10 +20,10 @@
 // no wave waits for another. What a part cuts is at its two ends and goes to
 // slots 2w and 2w + 1 of `parts`; what it holds whole goes straight to the
 // output, or, where a group's prefix comes on top, to its own row of `parts`.
-// 64 sequences of 65 to 8192 tokens, 32 heads on 8, D = 128, bf16: 209 us for 1.09
+// 64 sequences of 65 to 8192 tokens, 32 heads on 8, D = 128, bf16: 210 us for 1.09
 // GB (5.2 TB/s; 256-byte rows of one head at random 16-token blocks are read at 5.6
-// to 6.0 by a kernel that does nothing else), in e4m3 on one key head 45 us for 266
-// MB (5.9 TB/s). Three waves a SIMD instead of two: the same, e4m3 4 % slower.
+// to 6.0 by a kernel that does nothing else), in e4m3 on one key head 46 us for 266
+// MB (5.7 TB/s). Three waves a SIMD instead of two: the same, e4m3 4 % slower.
 #ifndef KVX_KERNELS_ATTEND_FEW_H_
 #define KVX_KERNELS_ATTEND_FEW_H_
 

@@ -7,7 +7,7 @@
 // / 4 threads, so a row of many parts (one long sequence) is read at once; parts
 // are merged in a fixed order. Rows that were finished are not visited. Reading
 // the parts bounds it where there are many (67 MB written and read for 4099 new
-// tokens of 32 heads: 42 us), its launch and the plan's loads where there are few
+// tokens of 32 heads: 37 us), its launch and the plan's loads where there are few
 // (one sequence of 700 tokens: 6 us).
 #include <algorithm>
 

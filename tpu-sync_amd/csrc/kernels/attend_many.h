@@ -18,9 +18,11 @@
 // tokens are widened on the way, in registers.) 4099 new tokens of 5 sequences of
 // 2000 to 12000, 32 heads on 8, D = 128, bf16: 730 us with tokens passing through
 // registers and a wave's products and exponentials in turn, 676 us without, 655 us
-// with operands read ahead and products given priority, 611 to 625 us with the
-// places of tokens kept as byte offsets (865 to 885 TFLOP/s, where an 8192^3
-// product of the library reaches 1211).
+// with operands read ahead and products given priority, 626 to 639 us with the
+// places of tokens kept as byte offsets (back to back, 37 us of joining among them:
+// 845 to 862 TFLOP/s, where an 8192^3 product of the library reaches 1211). Matrix
+// cores are busy for 46 % of the CUs' cycles and other vector instructions for
+// 51 %, so the two hardly overlap.
 //
 // Work. The tiles of all groups and sequences make one axis, weighed by the
 // keys they see, and every workgroup gets an equal part of it: no tail of late

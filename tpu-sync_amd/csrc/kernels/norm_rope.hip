@@ -10,8 +10,9 @@
 // A workgroup takes a few tokens and puts their R/2 (cos, sin) into LDS, one
 // sincos a token and pair for all heads. Then teams of lanes (head_row.h) take a
 // token's heads in turn. Reading and writing the rows bounds it: 8192 tokens x 40
-// heads x 128 in bf16, 31 us (5.4 TB/s both ways); 64 tokens 4.9 us, the launch
-// and a chain of dependent loads.
+// heads x 128 in bf16, 39.3 us from cold caches (4.3 TB/s both ways), 31.1 us again
+// and again on rows that the last-level cache holds in part; 64 tokens 4.9 us, the
+// launch and a chain of dependent loads.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
