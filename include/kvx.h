@@ -1007,6 +1007,12 @@ int kvx_scatter_blocks(uint64_t storage_table, int64_t num_storages,
 #define KVX_F16 1
 #define KVX_F32 2
 #define KVX_E4M3 3 /* OCP e4m3 with one fp32 scale a (block, head) */
+/* OCP e2m1, two values a byte (the first in its low half), with one e8m0 scale (a
+ * byte e for 2^(e - 127), 255: NaN) for 32 neighbouring dimensions of a token's
+ * head. A head's tokens of a block lie together: storages [blocks][heads]
+ * [block_tokens][head_dim / 2], scale tables [blocks][heads][block_tokens][head_dim /
+ * 32], head_dim a multiple of 32, storages aligned to 16 bytes. */
+#define KVX_FP4 4
 
 /*
  * RMS norm and position rotation of query and key heads in one pass, for each
@@ -1054,9 +1060,9 @@ typedef struct kvx_paged_cache {
   int64_t k_layer;
   int64_t v_layer;
   int64_t shard;
-  int64_t k_scale_layer; /* KVX_E4M3: tables [blocks][heads] fp32 */
+  int64_t k_scale_layer; /* KVX_E4M3: tables [blocks][heads] fp32; KVX_FP4: above */
   int64_t v_scale_layer;
-  int32_t dtype; /* the tensors' type or KVX_E4M3 */
+  int32_t dtype; /* the tensors' type, KVX_E4M3 or KVX_FP4 */
   int32_t block_tokens;
   int32_t heads;
   int32_t head_dim;
@@ -1087,7 +1093,12 @@ typedef struct kvx_paged_batch {
  *   max(old, largest finite |x| of its new tokens / 448),
  * old = 0 unless the block holds earlier tokens of the sequence; values are
  * clamped to +-448 scales, and earlier tokens are stored again under a scale
- * that grew. A block that takes new tokens must belong to one sequence of the
+ * that grew. In a KVX_FP4 cache the scale s of 32 values is the smallest power of
+ * two, of 2^-125 to 2^125 (2^13 for fp16 tensors), with
+ *   largest finite |x| <= 7 s,
+ * and the codes are the nearest to x / s (even ones in the middle), at most 6;
+ * infinities get +-6, and a NaN makes its 32 values NaN. Other tokens are not
+ * touched. A block that takes new tokens must belong to one sequence of the
  * call, and a token to one slot: with the same block or slot twice, which of
  * the values remain is not defined. No argument may lie in the cache or its
  * scales.
@@ -1121,7 +1132,9 @@ int kvx_manager_append_kv(kvx_manager* m, const kvx_append_kv_args* args, void* 
  * fp32; exponentials are rounded to the products' 16-bit type. A query that
  * sees nothing gets zeros and an lse of -inf. In a chunk, a value that is not
  * finite reaches the earlier queries of its own sequence too. Storages of 16-bit
- * types must start on 16 bytes; q and out may start at any element.
+ * types must start on 16 bytes; q and out may start at any element. fp16 queries
+ * take scales of a KVX_FP4 cache above 2^13 as 2^13 and round its values below
+ * 2^-24 (fp16 tensors store none of them).
  *
  * Groups: the sequences [group_starts[g], group_starts[g + 1]) (ascending,
  * device int32) hold their first prefix_lengths[g] tokens in the same blocks,

@@ -216,7 +216,7 @@ class PushItemC(ctypes.Structure):
     _fields_ = [(k, ctypes.c_int64) for k in ("layer", "shard", "k", "staging_offset", "size")]
 
 
-BF16, F16, F32, E4M3 = 0, 1, 2, 3  # KVX_BF16 ...
+BF16, F16, F32, E4M3, FP4 = 0, 1, 2, 3, 4  # KVX_BF16 ...
 
 
 class NormRopeArgs(ctypes.Structure):

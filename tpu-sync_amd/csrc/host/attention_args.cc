@@ -236,9 +236,13 @@ Rows Starts(const kvx_paged_batch& b) {
 
 struct Cache {
   PoolStorage k, v;
-  PoolStorage k_scales, v_scales;  // e4m3
+  PoolStorage k_scales, v_scales;  // e4m3 and 4 bits
   int64_t num_blocks = 0;
 };
+
+int32_t KindOf(int32_t cache_type) {
+  return cache_type == kE4m3 ? kPoolE4m3 : cache_type == kFp4 ? kPoolFp4 : kPoolSame;
+}
 
 Rows Whole(const PoolStorage& s) { return Whole(s.base, s.bytes); }
 
@@ -247,8 +251,8 @@ Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type,
     return FailedPreconditionError("needs a device-backed KVCacheManagerBase");
   }
   if (!Is16Bit(type)) return Bad("dtype must be KVX_BF16 or KVX_F16");
-  if (c.dtype != type && c.dtype != kE4m3) {
-    return Bad("the cache must be of the tensors' type or KVX_E4M3");
+  if (c.dtype != type && c.dtype != kE4m3 && c.dtype != kFp4) {
+    return Bad("the cache must be of the tensors' type, KVX_E4M3 or KVX_FP4");
   }
   if (c.heads < 1 || c.heads > 1024) return Bad("heads must be 1..1024");
   if (c.head_dim < 1 || c.head_dim > kMaxHeadDim) return Bad("head_dim must be 1..256");
@@ -257,34 +261,46 @@ Status FindCache(const PoolSource& pool, const kvx_paged_cache& c, int32_t type,
       !pool.find(pool.context, c.v_layer, c.shard, &out->v)) {
     return OutOfRangeError("layer or shard index out of range");
   }
-  const int64_t block = static_cast<int64_t>(c.block_tokens) * c.heads * c.head_dim *
-                        ElementBytes(c.dtype);
+  const bool fp4 = c.dtype == kFp4;
+  if (fp4 && c.head_dim % kFp4Group != 0) {
+    return Bad("head_dim must be a multiple of 32 in a KVX_FP4 cache");
+  }
+  const int64_t values = static_cast<int64_t>(c.block_tokens) * c.heads * c.head_dim;
+  const int64_t block = fp4 ? values / 2 : values * ElementBytes(c.dtype);
   if (out->k.block_bytes != block || out->v.block_bytes != block) {
     return Bad("blocks of " + std::to_string(out->k.block_bytes) + " and " +
                std::to_string(out->v.block_bytes) + " bytes do not hold [" +
                std::to_string(c.block_tokens) + ", " + std::to_string(c.heads) + ", " +
-               std::to_string(c.head_dim) + "] of " + std::to_string(ElementBytes(c.dtype)) +
-               " bytes");
+               std::to_string(c.head_dim) + "] of " +
+               (fp4 ? "4 bits" : std::to_string(ElementBytes(c.dtype)) + " bytes"));
   }
   int64_t blocks = std::min(out->k.bytes, out->v.bytes) / block;
-  if (c.dtype == kE4m3) {
+  if (c.dtype == kE4m3 || fp4) {
     PoolStorage s[2];
     if (!pool.find(pool.context, c.k_scale_layer, c.shard, &s[0]) ||
         !pool.find(pool.context, c.v_scale_layer, c.shard, &s[1])) {
       return OutOfRangeError("scale layer or shard index out of range");
     }
     for (const PoolStorage& t : s) {
-      if (t.block_bytes != static_cast<int64_t>(c.heads) * 4) {
+      if (fp4 && t.block_bytes != values / kFp4Group) {
+        return Bad("scale tables must hold one byte for 32 values: " +
+                   std::to_string(values / kFp4Group) + " bytes a block, not " +
+                   std::to_string(t.block_bytes));
+      }
+      if (!fp4 && t.block_bytes != static_cast<int64_t>(c.heads) * 4) {
         return Bad("scale tables must hold one fp32 a (block, head): " +
                    std::to_string(c.heads * 4) + " bytes a block, not " +
                    std::to_string(t.block_bytes));
       }
-      if (t.base % 4 != 0) return Bad("scale tables: unaligned address");
+      if (!fp4 && t.base % 4 != 0) return Bad("scale tables: unaligned address");
       blocks = std::min(blocks, t.bytes / t.block_bytes);
     }
     if (s[0].base == s[1].base) return Bad("keys and values need scale tables of their own");
     out->k_scales = s[0];
     out->v_scales = s[1];
+    if (fp4 && (out->k.base | out->v.base) % 16 != 0) {
+      return Bad("cache storages: must be aligned to 16 bytes");
+    }
   } else if ((out->k.base | out->v.base) % 2 != 0) {
     return Bad("cache storages: unaligned address");
   }
@@ -410,8 +426,8 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
   out->v_head = a.v_head_stride;
   out->k_pool = reinterpret_cast<void*>(cache.k.base);
   out->v_pool = reinterpret_cast<void*>(cache.v.base);
-  out->k_scales = reinterpret_cast<float*>(cache.k_scales.base);
-  out->v_scales = reinterpret_cast<float*>(cache.v_scales.base);
+  out->k_scales = reinterpret_cast<void*>(cache.k_scales.base);
+  out->v_scales = reinterpret_cast<void*>(cache.v_scales.base);
   out->k_weight = reinterpret_cast<const void*>(a.k_weight);
   out->positions = reinterpret_cast<const void*>(a.positions);
   out->inv_freq = reinterpret_cast<const float*>(a.inv_freq);
@@ -419,12 +435,12 @@ Status CheckAppendKv(const PoolSource& pool, const kvx_append_kv_args& a, Append
   out->head_dim = c.head_dim;
   out->rotary_dim = a.rotary_dim;
   out->type = a.dtype;
-  out->e4m3 = c.dtype == kE4m3;
+  out->pool = KindOf(c.dtype);
   out->weight_f32 = a.weight_dtype == kF32;
   out->positions_64 = a.positions_64 != 0;
   out->interleaved = a.interleaved != 0;
   out->eps = a.eps;
-  return out->e4m3 ? CheckGrid(MostBlocks(*out), BlockThreads(*out)) : CheckRowGrid(a.tokens);
+  return out->pool == kPoolE4m3 ? CheckGrid(MostBlocks(*out), BlockThreads(*out)) : CheckRowGrid(a.tokens);
 }
 
 Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunch* out,
@@ -493,8 +509,8 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
   out->out_head = a.out_head_stride;
   out->k_pool = reinterpret_cast<const void*>(cache.k.base);
   out->v_pool = reinterpret_cast<const void*>(cache.v.base);
-  out->k_scales = reinterpret_cast<const float*>(cache.k_scales.base);
-  out->v_scales = reinterpret_cast<const float*>(cache.v_scales.base);
+  out->k_scales = reinterpret_cast<const void*>(cache.k_scales.base);
+  out->v_scales = reinterpret_cast<const void*>(cache.v_scales.base);
   out->group_starts = reinterpret_cast<const int32_t*>(a.group_starts);
   out->prefix_lengths = reinterpret_cast<const int32_t*>(a.prefix_lengths);
   out->groups = a.groups;
@@ -502,7 +518,7 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
   out->k_heads = c.heads;
   out->head_dim = c.head_dim;
   out->type = a.dtype;
-  out->e4m3 = c.dtype == kE4m3;
+  out->pool = KindOf(c.dtype);
   out->causal = a.non_causal == 0;
   out->scale = a.scale;
   const int64_t need = out->batch.tokens == 0 ? 0 : PlanAttend(out);
@@ -510,7 +526,7 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
     *workspace_bytes = need;
     return OkStatus();
   }
-  if (!out->e4m3 && (reinterpret_cast<uintptr_t>(out->k_pool) |
+  if (out->pool == kPoolSame && (reinterpret_cast<uintptr_t>(out->k_pool) |
                      reinterpret_cast<uintptr_t>(out->v_pool)) % 16 != 0) {
     return Bad("cache storages: must be aligned to 16 bytes");
   }

@@ -20,20 +20,19 @@ struct AppendLaunch {
   const void* k = nullptr;
   const void* v = nullptr;
   int64_t k_token = 0, k_head = 0, v_token = 0, v_head = 0;
-  // Storages [num_blocks][block_tokens][heads][head_dim]; in e4m3 with scales
-  // [num_blocks][heads].
+  // Storages and their scales, laid out as PoolKind says.
   void* k_pool = nullptr;
   void* v_pool = nullptr;
-  float* k_scales = nullptr;
-  float* v_scales = nullptr;
+  void* k_scales = nullptr;
+  void* v_scales = nullptr;
   const void* k_weight = nullptr;   // [head_dim], or null: no norm
   const void* positions = nullptr;  // of the rotation; null: the places in the cache
   const float* inv_freq = nullptr;  // [rotary_dim / 2]
   int32_t heads = 0;
   int32_t head_dim = 0;
   int32_t rotary_dim = 0;
-  int32_t type = kBf16;  // of k and v (and of the pool unless it is e4m3)
-  bool e4m3 = false;
+  int32_t type = kBf16;  // of k and v (and of a kPoolSame pool)
+  int32_t pool = kPoolSame;  // PoolKind
   bool weight_f32 = false;
   bool positions_64 = false;
   bool interleaved = false;

@@ -58,13 +58,89 @@ __device__ __forceinline__ int64_t RotationPosition(const AppendLaunch& a, int64
                         : static_cast<const int32_t*>(a.positions)[token];
 }
 
+// A row's codes and scales in a 4-bit pool. A lane holds 8 neighbouring values
+// and four lanes a group (VEC 8), or a lane one value and half a wave a group.
 template <class E, int VEC, int LPR>
+struct Fp4Row {
+  using Lane = RowLane<E, VEC, LPR>;
+  static __device__ __forceinline__ uint32_t GroupMost(uint32_t m) {
+    if constexpr (VEC == 8) {
+      const auto most = [&m](auto control) {
+        m = max(m, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(
+                       0, static_cast<int>(m), decltype(control)::value, 0xf, 0xf, true)));
+      };
+      most(std::integral_constant<int, 0xb1>{});  // lanes 1 0 3 2
+      most(std::integral_constant<int, 0x4e>{});  // lanes 2 3 0 1
+    } else {
+#pragma unroll
+      for (int i = 1; i < 32; i *= 2) {
+        m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), i)));
+      }
+    }
+    return m;
+  }
+  // Every lane of a wave takes part.
+  static __device__ __forceinline__ void Store(const Lane& l, const float (*x)[VEC], bool stores,
+                                               uint8_t* codes, uint8_t* scales) {
+    constexpr uint32_t kEndless = 0x7f800000u;
+#pragma unroll
+    for (int n = 0; n < Lane::kChunks; ++n) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        m = max(m, __builtin_bit_cast(uint32_t, x[n][j]) & 0x7fffffffu);
+      }
+      m = GroupMost(m);
+      // Infinities are no part of the largest value, and are clamped.
+      if (__any(m == kEndless)) {
+        uint32_t finite = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const uint32_t u = __builtin_bit_cast(uint32_t, x[n][j]) & 0x7fffffffu;
+          finite = max(finite, u < kEndless ? u : 0u);
+        }
+        finite = GroupMost(finite);
+        if (m == kEndless) m = finite;
+      }
+      // The smallest power of two s with m <= 7 s: 6 is the largest code, and up to 7
+      // it is the nearest one. Bounded, so that 6 s is finite and the smallest code
+      // no subnormal number. A NaN makes NaN of its group.
+      constexpr uint32_t top = std::is_same_v<E, F16> ? kFp4MostF16 : kFp4Most;
+      const uint32_t code = m > kEndless
+                                ? 255u
+                                : min(max((m + 0x1fffffu) >> 23, kFp4Least + 2) - 2, top);
+      const float scale = __builtin_bit_cast(float, code << 23);
+      const bool writes = stores && l.Has(n);
+      // The quotient by a power of two is exact, and the instruction rounds to the
+      // nearest code, to the even one in the middle, and to 6 above it.
+      if constexpr (VEC == 8) {
+        uint32_t w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[n][0], x[n][1], scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[n][2], x[n][3], scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[n][4], x[n][5], scale, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[n][6], x[n][7], scale, 3);
+        if (writes) *reinterpret_cast<uint32_t*>(codes + l.Dim(n) / 2) = w;
+      } else {
+        const float other = __shfl_xor(x[n][0], 1);
+        const uint32_t w =
+            __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[n][0], other, scale, 0);
+        if (writes && l.Dim(n) % 2 == 0) codes[l.Dim(n) / 2] = static_cast<uint8_t>(w);
+      }
+      if (writes && l.Dim(n) % kFp4Group == 0) {
+        scales[l.Dim(n) / kFp4Group] = static_cast<uint8_t>(code);
+      }
+    }
+  }
+};
+
+template <class E, int VEC, int LPR, bool FP4>
 __global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch a,
                                                              const int tokens_each,
                                                              const int teams_of_token) {
   extern __shared__ f32x2 cs[];  // [tokens_each][rotary_dim / 2]
   __shared__ int sequence[kMaxTokens], place[kMaxTokens];
-  __shared__ int64_t row_at[kMaxTokens];  // first element of the token's rows, or -1
+  // First element of the token's rows (in 4 bits its first head's row), or -1.
+  __shared__ int64_t row_at[kMaxTokens];
   using Scalar = typename E::Scalar;
   const int pairs = a.rotary_dim / 2;
   const int t0 = blockIdx.x * tokens_each;
@@ -114,8 +190,12 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch 
       const int b = FastDiv(a.block_div, p);
       const int id = a.batch.tables[s * a.batch.table_stride + b];
       if (id >= 0 && id < a.batch.num_blocks) {
-        at = (static_cast<int64_t>(id) * a.batch.block_tokens + (p - b * a.batch.block_tokens)) *
-             a.heads * a.head_dim;
+        const int slot = p - b * a.batch.block_tokens;
+        if constexpr (FP4) {
+          at = static_cast<int64_t>(id) * a.heads * a.batch.block_tokens + slot;
+        } else {
+          at = (static_cast<int64_t>(id) * a.batch.block_tokens + slot) * a.heads * a.head_dim;
+        }
       }
     }
     row_at[threadIdx.x] = at;
@@ -131,9 +211,17 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(const AppendLaunch 
     const Factors<E, VEC, LPR> f(lane, cs + t * pairs, weights);
     const int64_t at = row_at[t];
     for (int h = first; h < a.heads;) {
-      const int64_t to = at + h * a.head_dim;
+      const int64_t to = at + h * (FP4 ? a.batch.block_tokens : a.head_dim);
       const Row<E, VEC, LPR> row(lane, keys, f, a.k_weight != nullptr, a.eps);
-      if (at >= 0) {
+      if constexpr (FP4) {
+        const int64_t codes = to * (a.head_dim / 2), scales = to * (a.head_dim / kFp4Group);
+        using Q = Fp4Row<E, VEC, LPR>;
+        Q::Store(lane, row.x, at >= 0, static_cast<uint8_t*>(a.k_pool) + codes,
+                 static_cast<uint8_t*>(a.k_scales) + scales);
+        Q::Store(lane, Row<E, VEC, LPR>(values).x, at >= 0,
+                 static_cast<uint8_t*>(a.v_pool) + codes,
+                 static_cast<uint8_t*>(a.v_scales) + scales);
+      } else if (at >= 0) {
         row.Store(lane, static_cast<Scalar*>(a.k_pool) + to);
         values.Store(lane, static_cast<Scalar*>(a.v_pool) + to);
       }
@@ -270,7 +358,8 @@ __global__ __launch_bounds__(kThreads, 2) void append_e4m3_kernel(const AppendLa
   const int64_t slot_bytes = static_cast<int64_t>(a.heads) * a.head_dim;
   uint8_t* block = static_cast<uint8_t*>(key ? a.k_pool : a.v_pool) +
                    rows.id * (slot_bytes * b.block_tokens);
-  float* scales = (key ? a.k_scales : a.v_scales) + static_cast<int64_t>(rows.id) * a.heads;
+  float* scales = static_cast<float*>(key ? a.k_scales : a.v_scales) +
+                  static_cast<int64_t>(rows.id) * a.heads;
   const RowLane<E, VEC, LPR> lane(a.head_dim, a.rotary_dim, a.interleaved);
   Weights<E, VEC, LPR> weights;
   weights.Load(lane, key ? a.k_weight : nullptr, a.weight_f32);
@@ -442,7 +531,7 @@ template <class E, int VEC, int LPR>
 hipError_t Launch(const AppendLaunch& l, hipStream_t stream) {
   const size_t pairs = static_cast<size_t>(l.rotary_dim / 2) * sizeof(f32x2);
   const int tokens = l.batch.tokens;
-  if (l.e4m3) {
+  if (l.pool == kPoolE4m3) {
     const int64_t blocks = MostBlocks(l);
     // Few blocks: their heads spread over workgroups.
     int split = 1;
@@ -459,8 +548,9 @@ hipError_t Launch(const AppendLaunch& l, hipStream_t stream) {
   while (each < kMaxTokens && tokens / each >= 2 * kEnough) each *= 2;
   while (split * of_token < l.heads && static_cast<int64_t>(tokens) * split < 2048) ++split;
   const dim3 grid((tokens + each - 1) / each, split);
-  hipLaunchKernelGGL((append_kv_kernel<E, VEC, LPR>), grid, dim3(kThreads), each * pairs, stream,
-                     l, each, of_token);
+  constexpr auto same = append_kv_kernel<E, VEC, LPR, false>, fp4 = append_kv_kernel<E, VEC, LPR, true>;
+  hipLaunchKernelGGL(l.pool == kPoolFp4 ? fp4 : same, grid, dim3(kThreads), each * pairs, stream, l,
+                     each, of_token);
   return hipGetLastError();
 }
 

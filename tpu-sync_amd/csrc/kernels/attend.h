@@ -58,10 +58,10 @@ struct AttendLaunch {
   void* out = nullptr;
   float* lse = nullptr;  // [tokens][q_heads] or null
   int64_t q_token = 0, q_head = 0, out_token = 0, out_head = 0;
-  const void* k_pool = nullptr;  // [num_blocks][block_tokens][k_heads][head_dim]
+  const void* k_pool = nullptr;  // laid out as PoolKind says
   const void* v_pool = nullptr;
-  const float* k_scales = nullptr;  // e4m3: [num_blocks][k_heads]
-  const float* v_scales = nullptr;
+  const void* k_scales = nullptr;
+  const void* v_scales = nullptr;
   int32_t most_few = 0, most_many = 0;  // steps of a key head that the sizes allow
   // Groups of sequences [group_starts[g], group_starts[g + 1]) whose first
   // prefix_lengths[g] tokens are in the same blocks.
@@ -70,7 +70,7 @@ struct AttendLaunch {
   int32_t groups = 0;
   int32_t q_heads = 0, k_heads = 0, head_dim = 0;
   int32_t type = kBf16;  // of q and out
-  bool e4m3 = false;
+  int32_t pool = kPoolSame;  // PoolKind
   bool causal = true;
   float scale = 1.0f;
   // Parts of split rows, part_rows rows of padded_dim floats relative to their

@@ -27,7 +27,7 @@
 #ifndef KVX_KERNELS_ATTEND_FEW_H_
 #define KVX_KERNELS_ATTEND_FEW_H_
 
-#include "attend_plan.h"
+#include "pool_lane.h"
 
 namespace kvx {
 
@@ -40,15 +40,13 @@ constexpr size_t FewLds(const AttendLaunch& l, int dp) {
          (l.groups > 0 ? 3 : 2) * sizeof(int) * static_cast<size_t>(l.batch.sequences);
 }
 
-template <class E, bool E4, int DP, int RT, bool FULL>
+template <class E, int POOL, int DP, int RT, bool FULL>
 __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int workgroup) {
   using Scalar = typename E::Scalar;
   constexpr int KS = DP / 32, DT = DP / 16, VST = FewValueStride(DP);
-  // The order in which a product goes through the dimensions is free: a lane
-  // takes 16 e4m3 ones in a row for two products where they come in pairs. 128
-  // sequences of 8 query heads on one, 300 to 16384 tokens, D = 128: 56 us (4.7
-  // TB/s); with 8 in a row 76 us.
-  constexpr bool kWide = E4 && FULL && KS % 2 == 0;
+  constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
+  using Pool = PoolLane<E, POOL, DP, FULL>;
+  using Words = typename Pool::Words;
   const BatchView& b = a.batch;
   int* sums = reinterpret_cast<int*>(lds + kWaves * 32 * VST);  // [sequences]
   int* lengths = sums + b.sequences;
@@ -70,12 +68,9 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
   const int x_first = axis.Start(worker), x_end = axis.Start(worker + 1);
 
   const int in16 = lane % 16, quarter = lane / 16;
-  const auto dim_of = [&](int ks) {
-    return kWide ? ks / 2 * 64 + quarter * 16 + ks % 2 * 8 : ks * 32 + quarter * 8;
-  };
+  const auto dim_of = [&](int ks) { return Pool::DimOf(quarter, ks); };
   char* mine = lds + wave * 32 * VST;
   const int G = a.q_heads / a.k_heads;
-  const int64_t row_stride = static_cast<int64_t>(a.k_heads) * a.head_dim;
   const float c = a.scale * kLog2e;
 
   for (int x = x_first; x < x_end;) {
@@ -136,6 +131,7 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
         if (step < step1 && p < end) id[u] = table[FastDivI(a.block_div, p)];
       }
     };
+    const Pool pool(lane, h, a);
     int64_t at[2];
     bool has[2];
     const auto place = [&](int step, const int (&id)[2]) {
@@ -146,50 +142,30 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
         has[u] = id[u] >= 0 && id[u] < b.num_blocks;
         // A token without a place reads the pool's first row (it is masked, and
         // its values are cleared), so that loads need no branch.
-        const int64_t row = static_cast<int64_t>(id[u]) * b.block_tokens + slot;
-        at[u] = (has[u] ? row : 0) * row_stride + h * a.head_dim + quarter * (kWide ? 16 : 8);
+        at[u] = pool.At(id[u], slot, has[u]);
       }
     };
-    constexpr int W = E4 ? 2 : 4;
-    using Words = __attribute__((ext_vector_type(W))) uint32_t;
-    const auto load = [&](const void* pool, Words (&w)[2][KS]) {
+    const auto load = [&](const void* from, Words (&w)[2][KS]) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) pool.Load(from, at[u], w[u]);
+    };
+    const auto scales_of = [&](const void* scales, const int (&id)[2], float (&f)[2]) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if constexpr (kWide) {
-#pragma unroll
-          for (int ks = 0; ks < KS; ks += 2) {
-            using Wide = u32x4 __attribute__((aligned(1)));
-            const u32x4 x = *reinterpret_cast<const Wide*>(static_cast<const uint8_t*>(pool) +
-                                                           at[u] + ks * 32);
-            w[u][ks] = Words{x[0], x[1]};
-            w[u][ks + 1] = Words{x[2], x[3]};
-          }
-          continue;
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          if constexpr (!FULL) w[u][ks] = Words(0);
-          if (FULL || ks * 32 + quarter * 8 < a.head_dim) {
-            if constexpr (E4) {
-              w[u][ks] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(pool) +
-                                                          at[u] + ks * 32);
-            } else {
-              w[u][ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(pool) +
-                                                           at[u] + ks * 32);
-            }
-          }
-        }
+        f[u] = static_cast<const float*>(
+            scales)[(has[u] ? static_cast<int64_t>(id[u]) : 0) * a.k_heads + h];
       }
     };
-    const auto scales_of = [&](const float* scales, const int (&id)[2], float (&f)[2]) {
+    // In 4 bits, those of the lane's own dimensions.
+    constexpr int kCodes = F4 ? Pool::kScales : 1;
+    const auto codes_of = [&](const void* scales, uint32_t (&f)[2][kCodes]) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f[u] = scales[(has[u] ? static_cast<int64_t>(id[u]) : 0) * a.k_heads + h];
-      }
+      for (int u = 0; u < 2; ++u) pool.LoadScales(scales, at[u], f[u]);
     };
 
     Words kw[2][KS], vw[2][KS];
     float kf[2] = {1, 1}, vf[2] = {1, 1};
+    [[maybe_unused]] uint32_t kc[2][kCodes], vc[2][kCodes];
     uint32_t valid[2], valid_next[2];
     int id[2], id_first[2];
     const auto note = [&](uint32_t (&v)[2]) {
@@ -207,6 +183,10 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
       scales_of(a.k_scales, id_first, kf);
       scales_of(a.v_scales, id_first, vf);
     }
+    if constexpr (F4) {
+      codes_of(a.k_scales, kc);
+      codes_of(a.v_scales, vc);
+    }
     load(a.v_pool, vw);
 
     for (int step = step0; step < step1; ++step) {
@@ -221,6 +201,8 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           u32x4 key;
           if constexpr (E4) {
             key = Widen<E>(kw[u][ks]);
+          } else if constexpr (F4) {
+            key = pool.FromCodes(kw[u][ks], kc[u], ks);
           } else {
             key = kw[u][ks];
           }
@@ -254,6 +236,7 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
       } else {
         find(step + 2, id);
         load(a.k_pool, kw);
+        if constexpr (F4) codes_of(a.k_scales, kc);
       }
       if (p0 + 32 > seen_by_all || (valid[0] & valid[1]) != 0xffffu) {
 #pragma unroll
@@ -316,6 +299,10 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           if ((valid[u] >> in16 & 1) == 0) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) vw[u][ks] = Words(0);
+            if constexpr (F4) {
+#pragma unroll
+              for (int i = 0; i < kCodes; ++i) vc[u][i] = 0;
+            }
           }
         }
       }
@@ -326,6 +313,8 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           u32x4 value;
           if constexpr (E4) {
             value = Widen<E>(vw[u][ks], power[u]);
+          } else if constexpr (F4) {
+            value = pool.FromCodes(vw[u][ks], vc[u], ks);
           } else {
             value = vw[u][ks];
           }
@@ -333,6 +322,7 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
         }
       }
       load(a.v_pool, vw);
+      if constexpr (F4) codes_of(a.v_scales, vc);
       valid[0] = valid_next[0];
       valid[1] = valid_next[1];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -83,9 +83,11 @@ constexpr size_t ManyLds(const AttendLaunch& l, int dp) {
          static_cast<size_t>(l.groups + l.batch.sequences) * sizeof(int);
 }
 
-template <class E, bool E4, int DP>
+template <class E, int POOL, int DP>
 __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int place) {
   using Scalar = typename E::Scalar;
+  constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
+  constexpr bool kWidens = E4 || F4;  // tokens pass through registers
   constexpr int KS = DP / 16, DT = DP / 32, kRow = 2 * DP;  // bytes of a token's row
   constexpr int kChunks = kManyStep * (DP / 8) / kAttendThreads;  // of a thread
   constexpr int kTile = 2 * kManyStep * kRow;  // keys, then values
@@ -93,11 +95,15 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
   int* sums = reinterpret_cast<int*>(places + 4);  // [groups + sequences]
   const BatchView& b = a.batch;
   const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  using Words = u32x2;  // e4m3 values of a chunk
+  // Chunks of 8 dimensions that a thread loads at once: all of a 4-bit scale's where
+  // a token has enough of them for that.
+  constexpr int kRun = !F4 ? 1 : DP % 128 == 0 ? 4 : DP == 64 ? 2 : 1;
+  constexpr int kLoads = kChunks / kRun;
+  using Words = std::conditional_t<F4, __attribute__((ext_vector_type(kRun))) uint32_t, u32x2>;
   const uint32_t lds_at = one(LdsAddress(lds));
 
   // Dimensions behind the last one are never written.
-  if (!E4 && a.head_dim < DP) {
+  if (!kWidens && a.head_dim < DP) {
     for (int i = threadIdx.x; i < 2 * kTile / 16; i += kAttendThreads) {
       reinterpret_cast<u32x4*>(lds)[i] = u32x4{0, 0, 0, 0};
     }
@@ -218,8 +224,13 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
       const int p = begin + step * kManyStep + lane;
       const bool is = found >= 0 && found < b.num_blocks;
       const int slot = p - FastDivI(a.block_div, p) * b.block_tokens;
-      const int64_t row = is ? static_cast<int64_t>(found) * b.block_tokens + slot : 0;
-      to.at[lane] = (row * row_stride + h * a.head_dim) * (E4 ? 1 : 2);
+      if constexpr (F4) {
+        to.at[lane] = ((static_cast<int64_t>(is ? found : 0) * a.k_heads + h) * b.block_tokens +
+                       (is ? slot : 0)) * (a.head_dim / 2);
+      } else {
+        const int64_t row = is ? static_cast<int64_t>(found) * b.block_tokens + slot : 0;
+        to.at[lane] = (row * row_stride + h * a.head_dim) * (E4 ? 1 : 2);
+      }
       to.id[lane] = is ? found : -1;
       const uint64_t present = __ballot(is);
       if (lane == 0) to.present = present;
@@ -227,8 +238,8 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
     const auto find_scales = [&](int step) {
       const int id = places[step & 3].id[lane];
       const int64_t at = static_cast<int64_t>(max(id, 0)) * a.k_heads + h;
-      found_k = a.k_scales[at];
-      found_v = a.v_scales[at];
+      found_k = static_cast<const float*>(a.k_scales)[at];
+      found_v = static_cast<const float*>(a.v_scales)[at];
     };
     const auto keep_scales = [&](int step) {
       places[step & 3].k_scale[lane] = found_k;
@@ -237,32 +248,54 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
     // Tokens of a step on their way into LDS: e4m3 ones widened in registers,
     // others straight from memory, a wave's 64 chunks at a time. A token without
     // a place reads the pool's first row, so that this needs no branch.
-    Words w[kChunks];
-    const auto load = [&](int step, const void* pool) {
+    Words w[kLoads];
+    uint32_t codes[kLoads];  // of 4-bit scales
+    constexpr int kOfToken = DP / 8 / kRun;  // loads
+    const auto load = [&](int step, const void* pool, const void* scales) {
       const Places& held = places[step & 3];
-      int64_t at[kChunks];
+      int64_t at[kLoads];
+      int d[kLoads];
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
+      for (int n = 0; n < kLoads; ++n) {
         const int chunk = threadIdx.x + n * kAttendThreads;
-        const int d = chunk % (DP / 8) * 8;
-        at[n] = held.at[chunk / (DP / 8)] + (d < a.head_dim ? d : 0);
+        d[n] = chunk % kOfToken * (8 * kRun);
+        if (d[n] >= a.head_dim) d[n] = 0;
+        at[n] = held.at[chunk / kOfToken];
       }
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
-        w[n] = *reinterpret_cast<const Bytes8*>(static_cast<const uint8_t*>(pool) + at[n]);
+      for (int n = 0; n < kLoads; ++n) {
+        const uint8_t* p = static_cast<const uint8_t*>(pool) + at[n];
+        if constexpr (F4) {
+          // A row has a scale for every 16 of its bytes.
+          codes[n] = static_cast<const uint8_t*>(scales)[at[n] / (kFp4Group / 2) + d[n] / kFp4Group];
+          using Unaligned = Words __attribute__((aligned(4)));
+          w[n] = *reinterpret_cast<const Unaligned*>(p + d[n] / 2);
+        } else {
+          w[n] = *reinterpret_cast<const Bytes8*>(p + d[n]);
+        }
       }
     };
     const auto store = [&](int step, auto is_key) {
       char* to = lds + (is_key() ? 0 : kTile) + (step & 1) * (kTile / 2);
       const Places& held = places[step & 3];
 #pragma unroll
-      for (int n = 0; n < kChunks; ++n) {
+      for (int n = 0; n < kLoads; ++n) {
         const int chunk = threadIdx.x + n * kAttendThreads;
-        const int tok = chunk / (DP / 8), d = chunk % (DP / 8) * 8;
-        const int at = is_key() ? KeyChunk<DP>(tok, d / 8) : ValueChunk<DP>(tok, d / 8);
+        const int tok = chunk / kOfToken, d = chunk % kOfToken * (8 * kRun);
         const bool is = (held.present >> tok & 1) != 0 && d < a.head_dim;
-        *reinterpret_cast<u32x4*>(to + tok * kRow + at * 16) =
-            Widen<E>(is ? w[n] : Words(0), is_key() ? 1.0f : ValuePower<E>(held.v_scale[tok]));
+        if (!is) w[n] = Words(0);
+        const uint32_t scale = F4 && is ? Fp4Scale<E>(codes[n]) : 0u;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          const int at = is_key() ? KeyChunk<DP>(tok, d / 8 + i) : ValueChunk<DP>(tok, d / 8 + i);
+          u32x4 value;
+          if constexpr (F4) {
+            value = FromFp4<E>(w[n][i], scale);
+          } else {
+            value = Widen<E>(w[n], is_key() ? 1.0f : ValuePower<E>(held.v_scale[tok]));
+          }
+          *reinterpret_cast<u32x4*>(to + tok * kRow + at * 16) = value;
+        }
       }
     };
     const auto fetch = [&](int step, const void* pool, auto is_key) {
@@ -374,12 +407,12 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
         }
       }
       __syncthreads();
-      if constexpr (E4) {
-        load(step0, a.k_pool);
+      if constexpr (kWidens) {
+        load(step0, a.k_pool, a.k_scales);
         store(step0, kKeys);
-        load(step0 + 1, a.k_pool);
+        load(step0 + 1, a.k_pool, a.k_scales);
         store(step0 + 1, kKeys);
-        load(step0, a.v_pool);
+        load(step0, a.v_pool, a.v_scales);
         store(step0, kValues);
       } else {
         fetch(step0, a.k_pool, kKeys);
@@ -398,8 +431,8 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
         if (finds_scales) find_scales(step + 2);
         // Keys two steps ahead and values one: the keys of this step go when the
         // scores of its second half are there, the values at its end.
-        if constexpr (E4) {
-          load(step + 2, a.k_pool);
+        if constexpr (kWidens) {
+          load(step + 2, a.k_pool, a.k_scales);
         } else {
           fetch(step + 1, a.v_pool, kValues);
         }
@@ -467,20 +500,20 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
             }
           }
           if (u == 0) {
-            if constexpr (!E4) {
+            if constexpr (!kWidens) {
               if (finds) keep(step + 3);
               LdsArrived<kChunks>();  // all but the values: the next step's keys
             }
             __syncthreads();
-            if constexpr (E4) {
+            if constexpr (kWidens) {
               store(step + 2, kKeys);
-              load(step + 1, a.v_pool);
+              load(step + 1, a.v_pool, a.v_scales);
             } else {
               fetch(step + 2, a.k_pool, kKeys);
             }
           }
         }
-        if constexpr (E4) {
+        if constexpr (kWidens) {
           store(step + 1, kValues);
           if (finds) keep(step + 3);
           if (finds_scales) keep_scales(step + 2);
@@ -489,7 +522,7 @@ __device__ __forceinline__ void AttendMany(const AttendLaunch& a, char* lds, int
           clear(step + 1);
         }
       }
-      if constexpr (!E4) LdsArrived<0>();
+      if constexpr (!kWidens) LdsArrived<0>();
     }
 
     // Lane: row l % 32, dimensions 32 dt + 8 (i / 4) + 4 (l / 32) + i % 4.

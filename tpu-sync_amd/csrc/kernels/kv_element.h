@@ -14,11 +14,23 @@ enum ElementType : int32_t {
   kF16 = 1,
   kF32 = 2,
   kE4m3 = 3,  // OCP e4m3 (no infinities, largest value 448)
+  kFp4 = 4,   // OCP e2m1 with one e8m0 scale for 32 neighbouring values
 };
 
 constexpr bool Is16Bit(int32_t t) { return t == kBf16 || t == kF16; }
-constexpr int64_t ElementBytes(int32_t t) { return t == kF32 ? 4 : t == kE4m3 ? 1 : 2; }
+constexpr int64_t ElementBytes(int32_t t) { return t == kF32 ? 4 : t == kE4m3 ? 1 : 2; }  // not kFp4
 constexpr float kE4m3Max = 448.0f;
+constexpr int kFp4Group = 32;  // values that share a scale
+
+// How a pool is held, next to tensors of a 16-bit type.
+enum PoolKind : int {
+  kPoolSame = 0,  // [blocks][tokens][heads][dim] of the tensors' type
+  kPoolE4m3 = 1,  // the same in e4m3, scales [blocks][heads] fp32
+  // e2m1 codes [blocks][heads][tokens][dim / 2] and e8m0 scales [blocks][heads]
+  // [tokens][dim / 32]. A head's tokens of a block lie together: a row is 64 bytes at
+  // 128 dimensions, half a cache line, which heads side by side would each read whole.
+  kPoolFp4 = 2,
+};
 
 // A launch counts the threads of a grid's dimension in 32 bits.
 constexpr bool GridFits(int64_t workgroups, int64_t threads) {
@@ -117,6 +129,38 @@ __device__ __forceinline__ uint32_t FromE4m3(uint32_t w, bool hi, float power) {
               : __builtin_bit_cast(uint32_t,
                                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, false));
   }
+}
+
+// Eight e2m1 values times a scale, given as the bits of a float whose exponent is
+// the e8m0 code (255 makes NaN of all): exact in bf16, and in fp16 for scales of
+// 2^-23 to 2^13.
+template <class E>
+__device__ __forceinline__ u32x4 FromFp4(uint32_t w, uint32_t scale) {
+  const float f = __builtin_bit_cast(float, scale);
+  if constexpr (std::is_same_v<E, F16>) {
+    return u32x4{
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3))};
+  } else {
+    return u32x4{
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3))};
+  }
+}
+
+// The scale of an e8m0 code for FromFp4. In fp16 a scale above 2^13, whose values
+// could leave the type's range, counts as 2^13; append_kv stores none from fp16.
+constexpr uint32_t kFp4MostF16 = 127 + 13, kFp4Most = 127 + 125, kFp4Least = 127 - 125;
+template <class E>
+__device__ __forceinline__ uint32_t Fp4Scale(uint32_t code) {
+  if constexpr (std::is_same_v<E, F16>) {
+    code = code > kFp4MostF16 && code != 255 ? kFp4MostF16 : code;
+  }
+  return code << 23;
 }
 
 struct SequenceSpan {

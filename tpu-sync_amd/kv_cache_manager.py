@@ -490,7 +490,10 @@ class KVCacheManager:
 
         The storages k_layer and v_layer must be [blocks, tokens, heads,
         head_dim] tensors of k's type, or float8_e4m3fn with one scale table
-        [blocks, heads] a KV storage (scale_tables, in the storages' order).
+        [blocks, heads] a KV storage (scale_tables, in the storages' order), or
+        float4_e2m1fn_x2 [blocks, heads, tokens, head_dim / 2] with scale tables
+        float8_e8m0fnu [blocks, heads, tokens, head_dim / 32], head_dim a
+        multiple of 32.
 
         Args:
           k, v: [tokens, heads, head_dim], bf16 or fp16, last dimension
@@ -509,7 +512,10 @@ class KVCacheManager:
         token past its table or with a block id outside the pool is dropped. A
         block that takes tokens must belong to one sequence of the call. In a
         float8 storage the scale of a (block, head) grows with its largest
-        value, and earlier tokens of the block are stored again under it.
+        value, and earlier tokens of the block are stored again under it. In a
+        4-bit storage 32 neighbouring dimensions of a token's head share a power
+        of two, the smallest under which none of them is above 7 (the largest
+        code is 6, the nearest one up to there).
         """
         from . import paged_attention
         paged_attention.append_kv(self, k_layer, v_layer, k, v, tables, lengths, starts=starts,

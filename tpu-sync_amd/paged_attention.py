@@ -50,7 +50,8 @@ def _load_torch():
         # The handle alone, without a Stream object around it, where torch has it.
         _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
         _TYPES.update({torch.bfloat16: _capi.BF16, torch.float16: _capi.F16,
-                       torch.float32: _capi.F32, torch.float8_e4m3fn: _capi.E4M3})
+                       torch.float32: _capi.F32, torch.float8_e4m3fn: _capi.E4M3,
+                       torch.float4_e2m1fn_x2: _capi.FP4})
         _torch = torch
     return _torch
 
@@ -219,6 +220,19 @@ def norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps: f
     return out_q, out_k
 
 
+def _check_scales(layers, tables, shard_idx, kind, fp4_shape):
+    """Checks the types of scale tables, and the shape of a 4-bit cache's (the
+    library checks bytes, which bytes in another order would have too)."""
+    for layer in tables:
+        t = layers[layer][shard_idx]
+        if kind == _torch.float8_e4m3fn:
+            if t.dtype != _torch.float32:
+                raise ValueError("scale tables must be float32")
+        elif t.dtype != _torch.float8_e8m0fnu or tuple(t.shape[1:]) != fp4_shape:
+            raise ValueError(f"scale tables must be float8_e8m0fnu [blocks, heads, tokens, "
+                             f"head_dim / 32] ({fp4_shape}), got {t.dtype} {tuple(t.shape[1:])}")
+
+
 def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
     """Two of the manager's storages as the fields of kvx_paged_cache."""
     torch = _torch
@@ -233,22 +247,25 @@ def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
         t = layers[layer][shard_idx]
         if len(t.shape) != 4:
             raise ValueError("the cache's storages must be [blocks, tokens, heads, head_dim] "
-                             f"tensors, got {tuple(t.shape)}")
-        if t.dtype not in (dtype, torch.float8_e4m3fn):
-            raise ValueError(f"the cache must be {dtype} or float8_e4m3fn, got {t.dtype}")
+                             "tensors (in 4 bits [blocks, heads, tokens, head_dim / 2]), "
+                             f"got {tuple(t.shape)}")
+        if t.dtype not in (dtype, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            raise ValueError(f"the cache must be {dtype}, float8_e4m3fn or float4_e2m1fn_x2, "
+                             f"got {t.dtype}")
         shapes.append((t.dtype,) + tuple(t.shape[1:]))
     if shapes[0] != shapes[1]:
         raise ValueError("the key and value storages must have the same type and block shape")
     kind, block_tokens, heads, head_dim = shapes[0]
+    if kind == torch.float4_e2m1fn_x2:
+        heads, block_tokens, head_dim = block_tokens, heads, 2 * head_dim
     k_scales = v_scales = 0
-    if kind == torch.float8_e4m3fn:
+    if kind != dtype:
         # Scale tables follow the KV storages, one a storage.
         if len(layers) != 2 * n:
-            raise ValueError("a float8 cache needs one scale table a KV storage "
+            raise ValueError(f"a {str(kind)[6:]} cache needs one scale table a KV storage "
                              f"({n}), got {len(layers) - n}")
-        for layer in (n + k_layer, n + v_layer):
-            if layers[layer][shard_idx].dtype != torch.float32:
-                raise ValueError("scale tables must be float32")
+        _check_scales(layers, (n + k_layer, n + v_layer), shard_idx, kind,
+                      (heads, block_tokens, head_dim // 32))
         k_scales, v_scales = n + k_layer, n + v_layer
     return (k_layer, v_layer, shard_idx, k_scales, v_scales, _TYPES[kind], block_tokens, heads,
             head_dim)
