@@ -1172,6 +1172,91 @@ typedef struct kvx_attend_args {
 int kvx_manager_attend_workspace(kvx_manager* m, const kvx_attend_args* args, int64_t* bytes);
 int kvx_manager_attend(kvx_manager* m, const kvx_attend_args* args, void* stream);
 
+/*
+ * What attention each cached token got, for the eviction of those that got little.
+ * For the tokens j of a sequence from begins[s] on and every head of the cache:
+ *   weights[block of j][head][slot of j] =
+ *       decay * (the same, 0 for the call's own tokens) +
+ *       sum over the query rows of the head that see j of exp(scale q.k_j - lse).
+ * lse is what kvx_manager_attend returns for the same queries. decay 0 does not read
+ * what was there. Sums are fp32 and taken in one order whatever the lengths, so the same
+ * call gives the same bytes. Other entries of the table are left alone; a token that has
+ * no place is skipped. A block that holds a token from begins[s] on must belong to one
+ * sequence of the call (those of a shared prefix lie before begins). A sequence without
+ * query rows is left alone.
+ */
+typedef struct kvx_weigh_args {
+  kvx_paged_cache cache; /* v_layer and v_scale_layer are not used */
+  kvx_paged_batch batch;
+  int64_t tokens;
+  int32_t dtype; /* KVX_BF16 or KVX_F16 */
+  int32_t q_heads;
+  uint64_t q; /* as in kvx_attend_args */
+  int64_t q_token_stride, q_head_stride;
+  uint64_t lse;     /* fp32 [tokens][q_heads] */
+  uint64_t weights; /* fp32 [blocks][heads][block_tokens], written */
+  int64_t blocks;   /* of the table: at least the cache's */
+  uint64_t begins;  /* int32 [sequences] or 0 */
+  int32_t non_causal;
+  float scale; /* positive */
+  float decay; /* 0..1 */
+  int32_t reserved;
+} kvx_weigh_args;
+
+int kvx_manager_weigh(kvx_manager* m, const kvx_weigh_args* args, void* stream);
+
+/*
+ * The tokens of each sequence and head that stay within `budget`. Of a sequence that
+ * holds more, the first f = min(begins[s], budget) stay, the last min(recent, budget -
+ * f), and of the others those with the largest weights, the earlier one of two that are
+ * equal (NaN, and a token without a place, come last). kept [sequences][heads][budget]
+ * gets their positions, ascending; behind a shorter sequence's tokens -1. new_lengths
+ * (may be 0) gets min(length, budget); a length is at most table_width * block_tokens.
+ * batch.starts must be 0.
+ */
+typedef struct kvx_choose_kept_args {
+  int32_t device;
+  int32_t heads;
+  int32_t block_tokens;
+  int32_t reserved;
+  int64_t blocks;   /* of the table of weights */
+  uint64_t weights; /* fp32 [blocks][heads][block_tokens] */
+  kvx_paged_batch batch;
+  uint64_t begins;      /* int32 [sequences] or 0 */
+  uint64_t kept;        /* int32 [sequences][heads][budget], written */
+  uint64_t new_lengths; /* int32 [sequences] or 0, written */
+  int64_t budget;       /* 0..2^30 */
+  int64_t recent;       /* not negative */
+} kvx_choose_kept_args;
+
+int kvx_choose_kept(const kvx_choose_kept_args* args, void* stream);
+
+/*
+ * Moves kept tokens to the front of their sequences, in place: for every sequence, head
+ * and i < budget with kept[s][head][i] = p >= 0, the key and value (with their scales in
+ * a KVX_FP4 cache) and the weight (weights may be 0) of position p go to position i.
+ * Positions ascend, so p >= i, and -1 stands behind them alone; of others the values
+ * are not defined. A position that has no place moves nothing. In a KVX_E4M3 cache a
+ * (block, head) that takes a token from elsewhere gets the largest scale of the tokens
+ * that it then holds, under which all of them are stored again. What lies behind the
+ * kept tokens is left as it is (under the block's scale). A block that takes a token
+ * must belong to one sequence of the call. No argument may lie in the cache or its
+ * scales, nor in the weights.
+ */
+typedef struct kvx_compact_args {
+  kvx_paged_cache cache; /* head_dim a multiple of 8, 16-bit storages on 16 bytes */
+  uint64_t tables;       /* int32 [sequences][table_width] */
+  int64_t table_stride;
+  int64_t table_width;
+  int64_t sequences;
+  uint64_t kept; /* int32 [sequences][heads][budget] */
+  int64_t budget;
+  uint64_t weights; /* fp32 [blocks][heads][block_tokens] or 0 */
+  int64_t blocks;   /* of the table of weights: at least the cache's */
+} kvx_compact_args;
+
+int kvx_manager_compact(kvx_manager* m, const kvx_compact_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,8 +10,9 @@ from .kv_cache_manager import (KVCacheManager, LogicalBlockManager, RaidenFuture
                                probe_stream_queues, measure_link_peaks)
 from .kv_cache_store import (BlockStatus, KVCacheMetadata, KVCacheMetadataShmRegion,
                              KVCacheStore, LRUCache, RaidenBlockId, RaidenId)
-from . import copy_plan, paged_attention, pool_layout, tiling, transport
+from . import copy_plan, eviction, paged_attention, pool_layout, tiling, transport
 from .paged_attention import norm_rope
+from .eviction import choose_kept
 from .pool_layout import PoolSpec, RegionSpec
 from .weight_synchronizer import (StridedEntry, StridedPlan, WeightSynchronizer,
                                   column_split_entries, compute_nd_shard_slices, copy_strided)
@@ -21,7 +22,7 @@ __all__ = ["KVCacheManager", "LogicalBlockManager", "RaidenFuture", "KvxError", 
            "KVCacheMetadata", "KVCacheMetadataShmRegion", "WeightSynchronizer",
            "StridedEntry", "StridedPlan", "copy_strided", "column_split_entries",
            "compute_nd_shard_slices", "pool_layout", "copy_plan", "tiling", "transport", "PoolSpec", "RegionSpec",
-           "paged_attention", "norm_rope", "library_path"]
+           "paged_attention", "norm_rope", "eviction", "choose_kept", "library_path"]
 
 
 def library_path() -> str:

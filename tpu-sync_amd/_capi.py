@@ -275,6 +275,33 @@ class AttendArgs(ctypes.Structure):
                    ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64)])
 
 
+class WeighArgs(ctypes.Structure):
+    _fields_ = ([("cache", PagedCache), ("batch", PagedBatch), ("tokens", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "q_heads")]
+                + [("q", ctypes.c_uint64)]
+                + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride")]
+                + [("lse", ctypes.c_uint64), ("weights", ctypes.c_uint64),
+                   ("blocks", ctypes.c_int64), ("begins", ctypes.c_uint64),
+                   ("non_causal", ctypes.c_int32), ("scale", ctypes.c_float),
+                   ("decay", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
+class ChooseKeptArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("device", "heads", "block_tokens", "reserved")]
+                + [("blocks", ctypes.c_int64), ("weights", ctypes.c_uint64),
+                   ("batch", PagedBatch)]
+                + [(n, ctypes.c_uint64) for n in ("begins", "kept", "new_lengths")]
+                + [(n, ctypes.c_int64) for n in ("budget", "recent")])
+
+
+class CompactArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCache), ("tables", ctypes.c_uint64),
+                ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int64),
+                ("sequences", ctypes.c_int64), ("kept", ctypes.c_uint64),
+                ("budget", ctypes.c_int64), ("weights", ctypes.c_uint64),
+                ("blocks", ctypes.c_int64)]
+
+
 # kvx_ready_fn(user, code)
 READY_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_int32)
 
@@ -518,6 +545,9 @@ PROTOTYPES = {
     "kvx_manager_append_kv": (_int, [_vp, ctypes.POINTER(AppendKvArgs), _vp]),
     "kvx_manager_attend_workspace": (_int, [_vp, ctypes.POINTER(AttendArgs), _i64p]),
     "kvx_manager_attend": (_int, [_vp, ctypes.POINTER(AttendArgs), _vp]),
+    "kvx_manager_weigh": (_int, [_vp, ctypes.POINTER(WeighArgs), _vp]),
+    "kvx_choose_kept": (_int, [ctypes.POINTER(ChooseKeptArgs), _vp]),
+    "kvx_manager_compact": (_int, [_vp, ctypes.POINTER(CompactArgs), _vp]),
 }
 
 _lib = None

@@ -1,42 +1,13 @@
 // extern "C" entry points of the operators that fill and read the paged pool:
 // checks (host/attention_args.cc), then launches on the caller's stream.
-#include "../host/attention_args.h"
-#include "../host/hip_util.h"
-#include "capi_internal.h"
+#include "pool_source.h"
 
 namespace {
 
 using kvx_capi::Done;
 using kvx_capi::Fail;
-
-bool FindStorage(const void* context, int64_t layer, int64_t shard, kvx::PoolStorage* out) {
-  const auto* m = static_cast<const kvx::KVCacheManager*>(context);
-  if (layer < 0 || shard < 0) return false;
-  out->block_bytes = 0;
-  if (!m->DeviceStorage(static_cast<size_t>(layer), static_cast<size_t>(shard), &out->base,
-                        &out->bytes)) {
-    return false;
-  }
-  out->block_bytes = m->LayerBlockByteSize(static_cast<size_t>(layer));
-  return out->block_bytes > 0;
-}
-
-kvx::PoolSource Source(const kvx_manager* m) {
-  kvx::PoolSource p;
-  p.device = m->impl->device();
-  p.device_backed = m->impl->device_backed();
-  p.context = m->impl.get();
-  p.find = FindStorage;
-  return p;
-}
-
-// Runs `launch` with `device` current.
-template <class F>
-int OnDevice(int device, F launch) {
-  kvx::DeviceGuard dg(device);
-  if (!dg.ok()) return Fail(KVX_INTERNAL, "hipSetDevice failed");
-  return Done(kvx::HipStatus(launch(), "kernel launch"));
-}
+using kvx_capi::OnDevice;
+using kvx_capi::Source;
 
 }  // namespace
 

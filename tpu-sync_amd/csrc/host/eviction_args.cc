@@ -1,0 +1,186 @@
+#include "eviction_args.h"
+
+#include <algorithm>
+
+#include <climits>
+#include <cmath>
+
+#include "paged_args.h"
+
+namespace kvx {
+namespace {
+
+using namespace paged;
+
+constexpr int64_t kMostBudget = int64_t{1} << 30;
+
+// A table of weights fp32 [blocks][heads][block_tokens].
+Status CheckTable(DeviceRangeChecker* ranges, uint64_t at, int64_t blocks, int64_t heads,
+                  int64_t block_tokens, Rows* out) {
+  if (blocks < 1 || blocks > INT32_MAX) return Bad("weights: blocks must be 1..2^31 - 1");
+  int64_t bytes = 0;
+  if (__builtin_mul_overflow(blocks, heads * block_tokens * 4, &bytes)) {
+    return Bad("weights: size overflows");
+  }
+  KVX_RETURN_IF_ERROR(CheckWords(ranges, at, bytes / 4, "weights"));
+  *out = Whole(at, bytes);
+  return OkStatus();
+}
+
+}  // namespace
+
+Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* out) {
+  Cache cache;
+  KVX_RETURN_IF_ERROR(FindCache(pool, a.cache, a.dtype, &cache, false));
+  const kvx_paged_cache& c = a.cache;
+  KVX_RETURN_IF_ERROR(CheckTokens(a.tokens, a.q_heads, c.head_dim));
+  if (c.head_dim % 8 != 0) return Bad("head_dim must be a multiple of 8");
+  if (a.q_heads < 1 || a.q_heads % c.heads != 0) {
+    return Bad("q_heads must be a multiple of the cache's heads");
+  }
+  if (!std::isfinite(a.scale) || a.scale <= 0) return Bad("scale must be finite and positive");
+  if (!(a.decay >= 0 && a.decay <= 1)) return Bad("decay must be 0..1");
+  DeviceRangeChecker ranges(pool.device);
+  const Rows q = {a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.q_heads, c.head_dim, 2};
+  KVX_RETURN_IF_ERROR(CheckRows(&ranges, q, "q"));
+  *out = WeighLaunch{};
+  AttendLaunch& l = out->attend;
+  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
+                                 &l.batch));
+  if (a.tokens > 0) KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
+  if (a.begins != 0 && a.batch.sequences > 0) {
+    KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.begins, a.batch.sequences, "begins"));
+  }
+  Rows table;
+  KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, c.heads, c.block_tokens, &table));
+  if (a.blocks < cache.num_blocks) return Bad("weights: fewer blocks than the cache's");
+  l.pool = KindOf(c.dtype);
+  if (l.pool == kPoolSame && cache.k.base % 16 != 0) {
+    return Bad("cache storages: must be aligned to 16 bytes");
+  }
+  // Work is counted in 32 bits: steps of 32 tokens, tiles of 128, for every head.
+  const int64_t few = a.batch.sequences * (l.batch.capacity / kFewStep + 1);
+  if (few > INT32_MAX / 2 / c.heads) return Bad("sequences * table_width is too large for one call");
+  KVX_RETURN_IF_ERROR(CheckApart(
+      {table, "weights"},
+      {{q, "q"},
+       {Whole(cache.k), "the cache"},
+       {Whole(cache.k_scales), "the cache's scales"},
+       {Tables(a.batch), "tables"},
+       {Lengths(a.batch), "lengths"},
+       {Starts(a.batch), "starts"},
+       {Whole(a.lse, a.tokens * a.q_heads * 4), "lse"},
+       {Whole(a.begins, a.begins != 0 ? a.batch.sequences * 4 : 0), "begins"}}));
+  if (a.batch.sequences == 0) l.batch.tokens = 0;
+  l.block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
+  l.group_div = MakeFastDivU32(static_cast<uint32_t>(a.q_heads / c.heads));
+  l.q = reinterpret_cast<const void*>(a.q);
+  l.q_token = a.q_token_stride;
+  l.q_head = a.q_head_stride;
+  l.k_pool = reinterpret_cast<const void*>(cache.k.base);
+  l.k_scales = reinterpret_cast<const void*>(cache.k_scales.base);
+  l.most_few = l.most_many = static_cast<int32_t>(few);
+  l.q_heads = a.q_heads;
+  l.k_heads = c.heads;
+  l.head_dim = c.head_dim;
+  l.type = a.dtype;
+  l.causal = a.non_causal == 0;
+  l.scale = a.scale;
+  out->lse = reinterpret_cast<const float*>(a.lse);
+  out->weights = reinterpret_cast<float*>(a.weights);
+  out->begins = reinterpret_cast<const int32_t*>(a.begins);
+  out->decay = a.decay;
+  if (l.batch.tokens > 0) PlanWeigh(out);
+  return OkStatus();
+}
+
+Status CheckChooseKept(const kvx_choose_kept_args& a, ChooseLaunch* out) {
+  if (a.heads < 1 || a.heads > 1024) return Bad("heads must be 1..1024");
+  if (a.block_tokens < 1 || a.block_tokens > (1 << 20)) return Bad("block_tokens must be 1..2^20");
+  if (a.budget < 0 || a.budget > kMostBudget) return Bad("budget must be 0..2^30");
+  if (a.recent < 0) return Bad("recent must not be negative");
+  if (a.batch.starts != 0) return Bad("starts: not used here");
+  DeviceRangeChecker ranges(a.device);
+  Rows table;
+  KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, a.heads, a.block_tokens, &table));
+  *out = ChooseLaunch{};
+  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.batch.sequences, a.block_tokens, a.blocks,
+                                 &out->batch));
+  const int64_t S = a.batch.sequences, words = S * a.heads * a.budget;
+  if (S > 0 && a.begins != 0) KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.begins, S, "begins"));
+  if (words > 0) KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.kept, words, "kept"));
+  if (S > 0 && a.new_lengths != 0) {
+    KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.new_lengths, S, "new_lengths"));
+  }
+  KVX_RETURN_IF_ERROR(CheckGrid(S * a.heads, kChooseThreads));
+  const Named kept = {Whole(a.kept, words * 4), "kept"};
+  const Named cut = {Whole(a.new_lengths, a.new_lengths != 0 ? S * 4 : 0), "new_lengths"};
+  for (const Named* written : {&kept, &cut}) {
+    KVX_RETURN_IF_ERROR(CheckApart(
+        *written, {{table, "weights"},
+                   {Tables(a.batch), "tables"},
+                   {Lengths(a.batch), "lengths"},
+                   {Whole(a.begins, a.begins != 0 ? S * 4 : 0), "begins"}}));
+  }
+  KVX_RETURN_IF_ERROR(CheckApart(cut, {kept}));
+  out->block_div = MakeFastDivU32(static_cast<uint32_t>(a.block_tokens));
+  out->weights = reinterpret_cast<const float*>(a.weights);
+  out->begins = reinterpret_cast<const int32_t*>(a.begins);
+  out->kept = reinterpret_cast<int32_t*>(a.kept);
+  out->new_lengths = reinterpret_cast<int32_t*>(a.new_lengths);
+  out->heads = a.heads;
+  out->budget = static_cast<int32_t>(a.budget);
+  out->recent = static_cast<int32_t>(std::min(a.recent, kMostBudget));
+  return OkStatus();
+}
+
+Status CheckCompact(const PoolSource& pool, const kvx_compact_args& a, CompactLaunch* out) {
+  Cache cache;
+  const kvx_paged_cache& c = a.cache;
+  KVX_RETURN_IF_ERROR(FindCache(pool, c, Is16Bit(c.dtype) ? c.dtype : kBf16, &cache));
+  if (c.head_dim % 8 != 0) return Bad("head_dim must be a multiple of 8");
+  if (a.budget < 0 || a.budget > kMostBudget) return Bad("budget must be 0..2^30");
+  if (KindOf(c.dtype) == kPoolSame && (cache.k.base | cache.v.base) % 16 != 0) {
+    return Bad("cache storages: must be aligned to 16 bytes");
+  }
+  DeviceRangeChecker ranges(pool.device);
+  *out = CompactLaunch{};
+  kvx_paged_batch batch = {a.tables, a.table_stride, a.table_width, 0, 0, a.sequences};
+  batch.lengths = a.kept;  // not read; checked with what follows
+  const int64_t words = a.sequences * c.heads * a.budget;
+  if (a.sequences < 0 || a.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
+  if (words == 0) return OkStatus();
+  KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.kept, words, "kept"));
+  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, batch, a.sequences, c.block_tokens, cache.num_blocks,
+                                 &out->batch));
+  KVX_RETURN_IF_ERROR(CheckGrid(a.sequences * c.heads, kCompactThreads));
+  Rows table = Whole(0, 0);
+  if (a.weights != 0) {
+    KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, c.heads, c.block_tokens, &table));
+    if (a.blocks < cache.num_blocks) return Bad("weights: fewer blocks than the cache's");
+  }
+  const Named weights = {table, "the weights"};
+  for (const Named& read : {Named(Tables(batch), "tables"), Named(Whole(a.kept, words * 4), "kept"),
+                            weights}) {
+    KVX_RETURN_IF_ERROR(CheckApart(read, {{Whole(cache.k), "the cache"},
+                                          {Whole(cache.v), "the cache"},
+                                          {Whole(cache.k_scales), "the cache's scales"},
+                                          {Whole(cache.v_scales), "the cache's scales"}}));
+  }
+  KVX_RETURN_IF_ERROR(CheckApart(weights, {{Tables(batch), "tables"},
+                                           {Whole(a.kept, words * 4), "kept"}}));
+  out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
+  out->kept = reinterpret_cast<const int32_t*>(a.kept);
+  out->budget = static_cast<int32_t>(a.budget);
+  out->k_pool = reinterpret_cast<void*>(cache.k.base);
+  out->v_pool = reinterpret_cast<void*>(cache.v.base);
+  out->k_scales = reinterpret_cast<void*>(cache.k_scales.base);
+  out->v_scales = reinterpret_cast<void*>(cache.v_scales.base);
+  out->weights = reinterpret_cast<float*>(a.weights);
+  out->heads = c.heads;
+  out->head_dim = c.head_dim;
+  out->pool = KindOf(c.dtype);
+  return OkStatus();
+}
+
+}  // namespace kvx

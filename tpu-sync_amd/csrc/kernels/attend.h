@@ -87,6 +87,9 @@ struct AttendLaunch {
   int32_t join_rows = 0;  // rows that one of them joins at once
 };
 
+// Widths that the kernels are compiled for.
+constexpr int PaddedDim(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+
 // Sizes of the launches of a call (from its shapes only). Returns the bytes of
 // `parts`.
 int64_t PlanAttend(AttendLaunch* l);
@@ -97,6 +100,8 @@ hipError_t LaunchAttend(const AttendLaunch& l, hipStream_t stream);
 // The parts, by translation unit.
 hipError_t LaunchAttendFew(const AttendLaunch& l, hipStream_t stream);
 hipError_t LaunchAttendMixed(const AttendLaunch& l, hipStream_t stream);
+hipError_t LaunchAttendMixedE4m3(const AttendLaunch& l, hipStream_t stream);
+hipError_t LaunchAttendMixedFp4(const AttendLaunch& l, hipStream_t stream);
 hipError_t LaunchAttendJoin(const AttendLaunch& l, hipStream_t stream);
 
 }  // namespace kvx

@@ -202,7 +202,7 @@ int64_t PlanAttend(AttendLaunch* l) {
   const int64_t T = l->batch.tokens, S = l->batch.sequences;
   const int64_t capacity = std::max(l->batch.capacity, 1);
   const bool single = l->batch.starts == nullptr;
-  l->padded_dim = l->head_dim <= 64 ? 64 : l->head_dim <= 96 ? 96 : l->head_dim <= 128 ? 128 : 256;
+  l->padded_dim = PaddedDim(l->head_dim);
   l->few_grid = l->few_rows = l->many_grid = l->join_grid = l->join_rows = 0;
   l->part_rows = 0;
   const int resident = (l->padded_dim > 128 ? 1 : 2) * kCus;  // workgroups

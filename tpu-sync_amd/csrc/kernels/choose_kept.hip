@@ -1,0 +1,165 @@
+// Which tokens of each sequence and key head stay within a budget.
+//
+// With L tokens held, L > budget: the first F = min(begin, budget) stay, the last R =
+// min(recent, budget - F) stay, and of those between, the N = budget - F - R with the
+// largest weights, the earlier one first where weights are equal. Positions come out
+// in ascending order.
+//
+// A workgroup takes one sequence and key head. Weights become unsigned numbers in the
+// same order (NaN, and tokens without a place, below all). The N-th largest is found by
+// its digits from the top, 11, 11 and 10 bits: a histogram in LDS of the digit among
+// those that agree in the digits before, then the digit in which the count from above
+// reaches N. With the N-th largest T known, waves count what is above and what equals it
+// in their ranges of positions, and write the positions that stay in a second pass, so
+// nothing depends on the order of atomic additions. Numbers are kept in LDS between
+// passes where they fit.
+#include "evict.h"
+
+#include <algorithm>
+
+#include "attend_plan.h"
+
+namespace kvx {
+namespace {
+
+constexpr int kWavesHere = kChooseThreads / 64;
+constexpr int kBins = 2048;
+// Numbers held in LDS: what its 160 KiB leave beside the histogram.
+constexpr int kHeldMost = 36864;
+
+__device__ __forceinline__ uint32_t Ordered(float x) {
+  if (x != x) return 0;
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);  // -0 is 0
+  return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+
+__global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const ChooseLaunch a,
+                                                                     const int held_most) {
+  extern __shared__ uint32_t held[];  // [held_most]
+  __shared__ int bins[kBins];
+  __shared__ int wave_sums[kWavesHere], wave_more[kWavesHere];
+  __shared__ int found_bin, found_above;
+  const BatchView& b = a.batch;
+  const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int length = min(max(b.lengths[s], 0), b.capacity);
+  int* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  if (h == 0 && threadIdx.x == 0 && a.new_lengths != nullptr) {
+    a.new_lengths[s] = min(length, a.budget);
+  }
+  if (length <= a.budget) {
+    for (int i = threadIdx.x; i < a.budget; i += kChooseThreads) kept[i] = i < length ? i : -1;
+    return;
+  }
+  const int begin = a.begins != nullptr ? max(a.begins[s], 0) : 0;
+  const int first = min(begin, a.budget), recent = min(a.recent, a.budget - first);
+  const int wanted = a.budget - first - recent;
+  for (int i = threadIdx.x; i < first; i += kChooseThreads) kept[i] = i;
+  for (int i = threadIdx.x; i < recent; i += kChooseThreads) {
+    kept[a.budget - recent + i] = length - recent + i;
+  }
+  if (wanted == 0) return;
+  const int count = length - recent - first;  // above `wanted`
+  const int32_t* table = b.tables + s * b.table_stride;
+  const bool holds = count <= held_most;
+  const auto load = [&](int i) {
+    const int p = first + i, at = FastDivI(a.block_div, p), id = table[at];
+    if (id < 0 || id >= b.num_blocks) return 0u;
+    return Ordered(a.weights[(static_cast<int64_t>(id) * a.heads + h) * b.block_tokens +
+                             (p - at * b.block_tokens)]);
+  };
+  const auto number = [&](int i) { return holds ? held[i] : load(i); };
+
+  // Digits of the number that is the wanted-th largest.
+  uint32_t digits = 0;
+  int above = 0;  // numbers that are larger in the digits so far
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t mask = pass == 2 ? 1023u : 2047u;
+    for (int i = threadIdx.x; i < kBins; i += kChooseThreads) bins[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kChooseThreads) {
+      uint32_t u;
+      if (pass == 0) {
+        u = load(i);
+        if (holds) held[i] = u;
+      } else {
+        u = number(i);
+        if (((u ^ digits) >> (pass == 1 ? 21 : 10)) != 0) continue;
+      }
+      atomicAdd(&bins[u >> shift & mask], 1);
+    }
+    __syncthreads();
+    // Counts from the top: thread t has bins from the top 2t and 2t + 1.
+    const int top = kBins - 1 - 2 * static_cast<int>(threadIdx.x);
+    const int n0 = bins[top], n1 = bins[top - 1];
+    int sum = n0 + n1;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const int o = __shfl_up(sum, m);
+      if (lane >= m) sum += o;
+    }
+    if (lane == 63) wave_sums[wave] = sum;
+    __syncthreads();
+    int before = above + sum - n0 - n1;
+    for (int w = 0; w < wave; ++w) before += wave_sums[w];
+    if (before < wanted && before + n0 >= wanted) {
+      found_bin = top;
+      found_above = before;
+    } else if (before + n0 < wanted && before + n0 + n1 >= wanted) {
+      found_bin = top - 1;
+      found_above = before + n0;
+    }
+    __syncthreads();
+    digits |= static_cast<uint32_t>(found_bin) << shift;
+    above = found_above;
+  }
+
+  // A wave's range of positions: what is above and what equals the number.
+  const int each = (count + kWavesHere * 64 - 1) / (kWavesHere * 64) * 64;
+  const int i0 = min(wave * each, count), i1 = min(i0 + each, count);
+  int more = 0, equal = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 64) {
+    const uint32_t u = i < i1 ? number(i) : 0u;
+    more += __popcll(__ballot(i < i1 && u > digits));
+    equal += __popcll(__ballot(i < i1 && u == digits));
+  }
+  if (lane == 0) {
+    wave_more[wave] = more;
+    wave_sums[wave] = equal;
+  }
+  __syncthreads();
+  more = equal = 0;
+  for (int w = 0; w < wave; ++w) {
+    more += wave_more[w];
+    equal += wave_sums[w];
+  }
+  const int of_equal = wanted - above;  // so many of those that equal it stay
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  for (int i = i0 + lane; i - lane < i1; i += 64) {
+    const uint32_t u = i < i1 ? number(i) : 0u;
+    const uint64_t larger = __ballot(i < i1 && u > digits);
+    const uint64_t same = __ballot(i < i1 && u == digits);
+    const int mine = equal + __popcll(same & below);
+    const bool stays = (larger >> lane & 1) != 0 || ((same >> lane & 1) != 0 && mine < of_equal);
+    if (stays) {
+      kept[first + more + __popcll(larger & below) + min(mine, of_equal)] = first + i;
+    }
+    more += __popcll(larger);
+    equal += __popcll(same);
+  }
+}
+
+}  // namespace
+
+hipError_t LaunchChooseKept(const ChooseLaunch& l, hipStream_t stream) {
+  const int held = std::min(l.batch.capacity, kHeldMost);
+  const size_t lds = static_cast<size_t>(held) * sizeof(uint32_t);
+  const hipError_t e = AllowDynamicLds<choose_kept_kernel>(lds + kBins * sizeof(int) + 1024);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(choose_kept_kernel, dim3(l.batch.sequences * l.heads), dim3(kChooseThreads),
+                     lds, stream, l, held);
+  return hipGetLastError();
+}
+
+}  // namespace kvx

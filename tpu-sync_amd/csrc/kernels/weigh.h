@@ -1,0 +1,30 @@
+// Host-side interface of the kernels that add up what attention each cached token
+// got (gfx950).
+#ifndef KVX_KERNELS_WEIGH_H_
+#define KVX_KERNELS_WEIGH_H_
+
+#include "attend.h"
+
+namespace kvx {
+
+struct WeighLaunch {
+  // Queries, keys, batch, scale and types (no values, no groups, no results).
+  AttendLaunch attend;
+  const float* lse = nullptr;       // [tokens][q_heads]
+  float* weights = nullptr;         // [num_blocks][k_heads][block_tokens]
+  const int32_t* begins = nullptr;  // [sequences]: first token weighed, or null: 0
+  float decay = 1.0f;
+};
+
+// Tokens of a tile of the kernel for many rows.
+constexpr int WeighTile(int padded_dim) { return padded_dim <= 128 ? 256 : 128; }
+
+// Sizes of the launches of a call (from its shapes only).
+void PlanWeigh(WeighLaunch* l);
+
+// Every address range must have been checked and PlanWeigh called.
+hipError_t LaunchWeigh(const WeighLaunch& l, hipStream_t stream);
+
+}  // namespace kvx
+
+#endif  // KVX_KERNELS_WEIGH_H_

@@ -1,0 +1,522 @@
+// The attention that each cached token got, added to a table of what it got before:
+//   w_j = decay w_j + sum over the rows of its key head that see it of
+//         e^{scale q.k_j - lse},
+// w_j = 0 before where the token is one of the call's own. lse is what attention
+// returns for the row, so that the exponentials of a row add up to 1. Everything
+// after the product is fp32.
+//
+// Tokens take the place of the output's columns, S = Q K^T, so a lane holds one
+// token's scores against several rows: the sum over rows stays in the lane but for
+// swaps at the end, and every token is added up by one wave in a fixed order.
+//
+// weigh_few (up to kFewRows rows a key head): as attend_few a wave takes an equal part
+// of the axis of all sequences' steps of 32 tokens; keys go from memory straight into
+// operands. Reading them bounds it.
+//
+// weigh_many (chunks): a workgroup takes WeighTile tokens of one sequence and key
+// head, keeps their keys in registers and goes through the rows that see them, 64 at a
+// time in LDS. The products and the exponentials (16 a lane for 8 products at D = 128)
+// bound it.
+#include "weigh.h"
+
+#include <algorithm>
+
+#include "attend_many.h"
+#include "pool_lane.h"
+
+namespace kvx {
+namespace {
+
+struct WeighKeys {
+  SequenceSpan q;
+  int rows, begin, end;
+};
+
+__device__ __forceinline__ WeighKeys LoadWeighKeys(const WeighLaunch& w, int s) {
+  WeighKeys k;
+  k.q = LoadSequence(w.attend.batch, s);
+  k.rows = k.q.count * (w.attend.q_heads / w.attend.k_heads);
+  k.end = min(k.q.length, w.attend.batch.capacity);
+  k.begin = w.begins != nullptr ? min(max(w.begins[s], 0), k.end) : 0;
+  return k;
+}
+
+__device__ __forceinline__ float Plus16(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) +
+         __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+__device__ __forceinline__ float Plus32(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) +
+         __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
+// -- Few rows.
+
+__device__ __forceinline__ int WeighSteps(const WeighKeys& k) {
+  if (k.rows == 0 || k.rows > kFewRows) return 0;
+  return (k.end - k.begin + kFewStep - 1) / kFewStep;
+}
+
+template <class E, int POOL, int DP, int RT, bool FULL>
+__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_kernel(
+    const WeighLaunch w) {
+  extern __shared__ int sums[];  // [sequences]
+  using Scalar = typename E::Scalar;
+  using Pool = PoolLane<E, POOL, DP, FULL>;
+  using Words = typename Pool::Words;
+  constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
+  constexpr int KS = Pool::KS, kCodes = F4 ? Pool::kScales : 1;
+  const AttendLaunch& a = w.attend;
+  const BatchView& b = a.batch;
+  for (int s = threadIdx.x; s < b.sequences; s += kAttendThreads) {
+    sums[s] = WeighSteps(LoadWeighKeys(w, s));
+  }
+  BlockSums(sums, b.sequences, a.most_few);
+  const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int all = one(sums[b.sequences - 1]);
+  if (all == 0) return;
+  const Axis axis = FewAxis(a, all);
+  const int lane = threadIdx.x % 64;
+  const int worker = static_cast<int>(blockIdx.x) * kWaves + one(threadIdx.x / 64);
+  if (worker >= axis.workers) return;
+  const int x_end = axis.Start(worker + 1);
+  const int in16 = lane % 16, quarter = lane / 16;
+  const int G = a.q_heads / a.k_heads;
+  const float c = a.scale * kLog2e;
+
+  for (int x = axis.Start(worker); x < x_end;) {
+    const int s = one(FirstAbove(sums, b.sequences, x / a.k_heads));
+    const int before = s > 0 ? one(sums[s - 1]) : 0;
+    const int steps = one(sums[s]) - before;
+    const int off = x - before * a.k_heads;
+    const int h = off / steps, step0 = off - h * steps;
+    const int step1 = min(steps, step0 + (x_end - x));
+    const WeighKeys k = LoadWeighKeys(w, s);
+    const int begin = one(k.begin), end = one(k.end), rows = one(k.rows);
+    const SequenceSpan span = {one(k.q.first), one(k.q.count), one(k.q.length)};
+    const int old_end = span.length - span.count;  // tokens that had a weight before
+
+    // Queries: row l % 16 of each row tile; and of the rows that this lane gets
+    // scores of, 4 (l / 16) + i, the log of their sums and the tokens that they see.
+    u32x4 q[RT][KS];
+    float base[RT][4];
+    int seen[RT][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = rt * 16 + in16, t = FastDivI(a.group_div, r);
+      const int64_t token = span.first + t;
+      const Scalar* p = static_cast<const Scalar*>(a.q) + token * a.q_token +
+                        (h * G + (r - t * G)) * a.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = Pool::DimOf(quarter, ks);
+        q[rt][ks] = u32x4{0, 0, 0, 0};
+        if (r < rows && (FULL || d < a.head_dim)) {
+          q[rt][ks] = *reinterpret_cast<const Bytes16*>(p + d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = rt * 16 + quarter * 4 + i, at = FastDivI(a.group_div, row);
+        base[rt][i] = 0.0f;
+        seen[rt][i] = 0;
+        if (row < rows) {
+          base[rt][i] = w.lse[(span.first + at) * static_cast<int64_t>(a.q_heads) + h * G +
+                              (row - at * G)] * kLog2e;
+          seen[rt][i] = Visible(a, span, span.first + at);
+        }
+      }
+    }
+
+    const Pool pool(lane, h, a);
+    const int32_t* table = b.tables + s * b.table_stride;
+    const auto find = [&](int step, int (&id)[2]) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int p = begin + step * kFewStep + u * 16 + in16;
+        id[u] = -1;
+        if (step < step1 && p < end) id[u] = table[FastDivI(a.block_div, p)];
+      }
+    };
+    int64_t at[2];
+    // The weight of the lane's own token: 16 (l / 16) + l % 16 of the step, l < 32.
+    float* mine = nullptr;
+    float held = 0.0f;
+    const auto place = [&](int step, const int (&id)[2]) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int p = begin + step * kFewStep + u * 16 + in16;
+        const int slot = p - FastDivI(a.block_div, p) * b.block_tokens;
+        const bool has = id[u] >= 0 && id[u] < b.num_blocks;
+        at[u] = pool.At(id[u], slot, has);
+        if (quarter == u) {
+          mine = has ? w.weights + (static_cast<int64_t>(id[u]) * a.k_heads + h) * b.block_tokens +
+                           slot
+                     : nullptr;
+          held = 0.0f;
+          if (has && p < old_end && w.decay != 0.0f) held = *mine;
+        }
+      }
+    };
+    Words kw[2][KS];
+    float kf[2] = {1, 1};
+    [[maybe_unused]] uint32_t kc[2][kCodes];
+    int id[2], id_now[2];
+    const auto load = [&](const int (&of)[2]) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        pool.Load(a.k_pool, at[u], kw[u]);
+        if constexpr (E4) {
+          const bool has = of[u] >= 0 && of[u] < b.num_blocks;
+          kf[u] = static_cast<const float*>(
+              a.k_scales)[(has ? static_cast<int64_t>(of[u]) : 0) * a.k_heads + h];
+        }
+        if constexpr (F4) pool.LoadScales(a.k_scales, at[u], kc[u]);
+      }
+    };
+    find(step0, id_now);
+    find(step0 + 1, id);
+    place(step0, id_now);
+    load(id_now);
+    for (int step = step0; step < step1; ++step) {
+      const int p0 = begin + step * kFewStep;
+      f32x4 sc[RT][2];
+      float factor[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        factor[u] = E4 ? c * kf[u] : c;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          u32x4 key;
+          if constexpr (E4) {
+            key = Widen<E>(kw[u][ks]);
+          } else if constexpr (F4) {
+            key = pool.FromCodes(kw[u][ks], kc[u], ks);
+          } else {
+            key = kw[u][ks];
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt][u] = Mma16<E>(q[rt][ks], key, sc[rt][u]);
+        }
+      }
+      float* const to = mine;
+      const float was = held;
+      id_now[0] = id[0];
+      id_now[1] = id[1];
+      place(step + 1, id_now);
+      find(step + 2, id);
+      load(id_now);
+      float got[2] = {0, 0};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int p = p0 + u * 16 + in16;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(sc[rt][u][i], factor[u], -base[rt][i]));
+            got[u] += p < seen[rt][i] ? e : 0.0f;
+          }
+        }
+        got[u] = Plus32(Plus16(got[u]));
+      }
+      if (quarter < 2 && to != nullptr) *to = fmaf(w.decay, was, quarter == 0 ? got[0] : got[1]);
+    }
+    x += step1 - step0;
+  }
+}
+
+// -- Many rows.
+
+constexpr int kWeighRows = 64;  // of a stage
+
+template <class E, int POOL, int DP>
+__global__ __launch_bounds__(kAttendThreads, 2) void weigh_many_kernel(const WeighLaunch w) {
+  extern __shared__ __align__(16) char lds[];
+  using Scalar = typename E::Scalar;
+  constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
+  constexpr int KS = DP / 16, kRow = 2 * DP, kTokens = WeighTile(DP);
+  constexpr int CT = kTokens / 128;  // tiles of 32 tokens a wave
+  constexpr int kChunks = kWeighRows * (DP / 8) / kAttendThreads;  // of a thread
+  struct Rows {
+    float base[kWeighRows];
+    int seen[kWeighRows];
+  };
+  Rows* row_data = reinterpret_cast<Rows*>(lds + 2 * kWeighRows * kRow);
+  int* sums = reinterpret_cast<int*>(row_data + 2);  // [sequences]
+  const AttendLaunch& a = w.attend;
+  const BatchView& b = a.batch;
+  for (int s = threadIdx.x; s < b.sequences; s += kAttendThreads) {
+    const WeighKeys k = LoadWeighKeys(w, s);
+    sums[s] = k.rows > kFewRows ? (k.end - k.begin + kTokens - 1) / kTokens : 0;
+  }
+  BlockSums(sums, b.sequences, a.most_many);
+  const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int tiles = one(sums[b.sequences - 1]) * a.k_heads;
+  const int lane = threadIdx.x % 64, wave = one(threadIdx.x / 64);
+  const int in32 = lane % 32, half = lane / 32;
+  const int G = a.q_heads / a.k_heads;
+  const float c = a.scale * kLog2e;
+
+  for (int x = blockIdx.x; x < tiles; x += gridDim.x) {
+    const int s = one(FirstAbove(sums, b.sequences, x / a.k_heads));
+    const int before = s > 0 ? one(sums[s - 1]) : 0;
+    const int of_head = one(sums[s]) - before;
+    const int off = x - before * a.k_heads;
+    const int h = off / of_head, tile = off - h * of_head;
+    const WeighKeys k = LoadWeighKeys(w, s);
+    const int end = one(k.end), rows = one(k.rows);
+    const SequenceSpan span = {one(k.q.first), one(k.q.count), one(k.q.length)};
+    const int j0 = one(k.begin) + tile * kTokens;
+    const int old_end = span.length - span.count;
+
+    // Keys: token l % 32 of each of the wave's tiles, as an operand.
+    const int32_t* table = b.tables + s * b.table_stride;
+    u32x4 key[CT][KS];
+    float factor[CT];
+    float* mine[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int p = j0 + (wave * CT + ct) * 32 + in32;
+      const int at = FastDivI(a.block_div, p), slot = p - at * b.block_tokens;
+      const int id = p < end ? table[at] : -1;
+      const bool has = id >= 0 && id < b.num_blocks;
+      const int64_t of_block = static_cast<int64_t>(has ? id : 0);
+      // Places in layouts with a head's tokens together, and with a token's heads.
+      const int64_t by_head = (of_block * a.k_heads + h) * b.block_tokens + (has ? slot : 0);
+      const int64_t by_token = (of_block * b.block_tokens + (has ? slot : 0)) * a.k_heads + h;
+      mine[ct] = has ? w.weights + by_head : nullptr;
+      factor[ct] = c;
+      if constexpr (E4) factor[ct] *= static_cast<const float*>(a.k_scales)[of_block * a.k_heads + h];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d = ks * 16 + half * 8;
+        key[ct][ks] = u32x4{0, 0, 0, 0};
+        if (!has || d >= a.head_dim) continue;
+        if constexpr (F4) {
+          const uint32_t code = static_cast<const uint8_t*>(
+              a.k_scales)[by_head * (a.head_dim / kFp4Group) + d / kFp4Group];
+          key[ct][ks] = FromFp4<E>(
+              *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.k_pool) +
+                                                 by_head * (a.head_dim / 2) + d / 2),
+              Fp4Scale<E>(code));
+        } else if constexpr (E4) {
+          key[ct][ks] = Widen<E>(*reinterpret_cast<const Bytes8*>(
+              static_cast<const uint8_t*>(a.k_pool) + by_token * a.head_dim + d));
+        } else {
+          key[ct][ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) +
+                                                          by_token * a.head_dim + d);
+        }
+      }
+    }
+
+    // Rows, from the first that sees the tile's first token.
+    const int first_token = a.causal ? max(j0 - old_end, 0) : 0;
+    const int row0 = one(min(first_token * G, rows)) / kWeighRows * kWeighRows;
+    u32x4 hold[kChunks];
+    float hold_base = 0.0f;
+    int hold_seen = 0;
+    const auto load = [&](int from) {
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int r = from + chunk / (DP / 8), d = chunk % (DP / 8) * 8;
+        const int t = FastDivI(a.group_div, r);
+        hold[n] = u32x4{0, 0, 0, 0};
+        if (r < rows && d < a.head_dim) {
+          hold[n] = *reinterpret_cast<const Bytes16*>(
+              static_cast<const Scalar*>(a.q) + static_cast<int64_t>(span.first + t) * a.q_token +
+              (h * G + (r - t * G)) * a.q_head + d);
+        }
+      }
+      if (threadIdx.x < kWeighRows) {
+        const int r = from + threadIdx.x, t = FastDivI(a.group_div, r);
+        hold_base = 0.0f;
+        hold_seen = 0;
+        if (r < rows) {
+          hold_base = w.lse[(span.first + t) * static_cast<int64_t>(a.q_heads) + h * G +
+                            (r - t * G)] * kLog2e;
+          hold_seen = Visible(a, span, span.first + t);
+        }
+      }
+    };
+    const auto store = [&](int buffer) {
+#pragma unroll
+      for (int n = 0; n < kChunks; ++n) {
+        const int chunk = threadIdx.x + n * kAttendThreads;
+        const int r = chunk / (DP / 8);
+        *reinterpret_cast<u32x4*>(lds + buffer * (kWeighRows * kRow) + r * kRow +
+                                  KeyChunk<DP>(r, chunk % (DP / 8)) * 16) = hold[n];
+      }
+      if (threadIdx.x < kWeighRows) {
+        row_data[buffer].base[threadIdx.x] = hold_base;
+        row_data[buffer].seen[threadIdx.x] = hold_seen;
+      }
+    };
+
+    float got[CT] = {};
+    load(row0);
+    int buffer = 0;
+    for (int r0 = row0; r0 < rows; r0 += kWeighRows) {
+      store(buffer);
+      __syncthreads();
+      if (r0 + kWeighRows < rows) load(r0 + kWeighRows);
+      const Rows& here = row_data[buffer];
+      // Whether every row sees every token of the wave.
+      const int last = min(j0 + (wave + 1) * CT * 32, end);
+      const bool plain =
+          r0 + kWeighRows <= rows && Visible(a, span, span.first + FastDivI(a.group_div, r0)) >= last;
+#pragma unroll
+      for (int rt = 0; rt < kWeighRows / 32; ++rt) {
+        f32x16 sc[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sc[ct] = f32x16(0.0f);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int r = rt * 32 + in32;
+          const u32x4 row = *reinterpret_cast<const u32x4*>(
+              lds + buffer * (kWeighRows * kRow) + r * kRow + KeyChunk<DP>(r, ks * 2 + half) * 16);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) sc[ct] = Mma32<E>(row, key[ct][ks], sc[ct]);
+        }
+        // Lane: token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4. Sums of 16 first:
+        // thousands of rows lose less so.
+        float some[CT] = {};
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 base = *reinterpret_cast<const f32x4*>(&here.base[rt * 32 + i * 2 + half * 4]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              sc[ct][i + j] =
+                  __builtin_amdgcn_exp2f(fmaf(sc[ct][i + j], factor[ct], -base[j]));
+            }
+          }
+          if (!plain) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int seen = here.seen[rt * 32 + i * 2 + half * 4 + j];
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct) {
+                if (j0 + (wave * CT + ct) * 32 + in32 >= seen) sc[ct][i + j] = 0.0f;
+              }
+            }
+          }
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) some[ct] += sc[ct][i + j];
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) got[ct] += some[ct];
+      }
+      // (The other buffer's readers are past the barrier above.)
+      buffer ^= 1;
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float sum = Plus32(got[ct]);
+      if (half == 0 && mine[ct] != nullptr) {
+        const int p = j0 + (wave * CT + ct) * 32 + in32;
+        const float was = p < old_end && w.decay != 0.0f ? *mine[ct] : 0.0f;
+        *mine[ct] = fmaf(w.decay, was, sum);
+      }
+    }
+    __syncthreads();  // the next tile's rows take this one's place in LDS
+  }
+}
+
+template <class E, int POOL, int DP, int RT, bool FULL>
+hipError_t Few(const WeighLaunch& l, hipStream_t stream) {
+  const size_t lds = static_cast<size_t>(l.attend.batch.sequences) * sizeof(int);
+  hipLaunchKernelGGL((weigh_few_kernel<E, POOL, DP, RT, FULL>), dim3(l.attend.few_grid),
+                     dim3(kAttendThreads), lds, stream, l);
+  return hipGetLastError();
+}
+
+template <class E, int POOL, int DP>
+hipError_t Both(const WeighLaunch& l, hipStream_t stream) {
+  const AttendLaunch& a = l.attend;
+  hipError_t e = hipSuccess;
+  if (a.few_grid > 0) {
+    if (a.head_dim != DP) {
+      e = Few<E, POOL, DP, 2, false>(l, stream);
+    } else {
+      e = a.few_rows <= 16 ? Few<E, POOL, DP, 1, true>(l, stream)
+                           : Few<E, POOL, DP, 2, true>(l, stream);
+    }
+  }
+  if (e != hipSuccess || a.many_grid == 0) return e;
+  const size_t lds = 2 * kWeighRows * (2 * DP + 8) +
+                     static_cast<size_t>(a.batch.sequences) * sizeof(int);
+  constexpr auto kernel = weigh_many_kernel<E, POOL, DP>;
+  e = AllowDynamicLds<kernel>(lds + 1024);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3(a.many_grid), dim3(kAttendThreads), lds, stream, l);
+  return hipGetLastError();
+}
+
+template <class E, int POOL>
+hipError_t PickDim(const WeighLaunch& l, hipStream_t stream) {
+  switch (l.attend.padded_dim) {
+    case 64:
+      return Both<E, POOL, 64>(l, stream);
+    case 96:
+      return Both<E, POOL, 96>(l, stream);
+    case 128:
+      return Both<E, POOL, 128>(l, stream);
+    default:
+      return Both<E, POOL, 256>(l, stream);
+  }
+}
+
+template <class E>
+hipError_t PickPool(const WeighLaunch& l, hipStream_t stream) {
+  switch (l.attend.pool) {
+    case kPoolE4m3:
+      return PickDim<E, kPoolE4m3>(l, stream);
+    case kPoolFp4:
+      return PickDim<E, kPoolFp4>(l, stream);
+    default:
+      return PickDim<E, kPoolSame>(l, stream);
+  }
+}
+
+}  // namespace
+
+void PlanWeigh(WeighLaunch* l) {
+  AttendLaunch& a = l->attend;
+  const int64_t G = a.q_heads / a.k_heads, T = a.batch.tokens, S = a.batch.sequences;
+  const int64_t capacity = std::max(a.batch.capacity, 1);
+  const bool single = a.batch.starts == nullptr;
+  a.padded_dim = PaddedDim(a.head_dim);
+  constexpr int kCus = 256;
+  const int resident = (a.padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
+  a.few_grid = a.few_rows = a.many_grid = 0;
+  if (G <= kFewRows) {
+    a.few_rows = static_cast<int>(single ? G : std::min<int64_t>(T * G, kFewRows));
+    const int64_t steps = S * a.k_heads * ((capacity + kFewStep - 1) / kFewStep);
+    a.few_grid = static_cast<int>(std::min<int64_t>(resident, (steps + kWaves - 1) / kWaves));
+  }
+  if (single ? G > kFewRows : T * G > kFewRows) {
+    const int tile = WeighTile(a.padded_dim);
+    // Sequences with more than kFewRows rows there are at most T * G / kFewRows.
+    const int64_t many = std::min(S, T * G / kFewRows);
+    const int64_t tiles = many * a.k_heads * ((capacity + tile - 1) / tile);
+    a.many_grid = static_cast<int>(std::min<int64_t>(2 * kCus, tiles));
+  }
+}
+
+hipError_t LaunchWeigh(const WeighLaunch& l, hipStream_t stream) {
+  return l.attend.type == kBf16 ? PickPool<Bf16>(l, stream) : PickPool<F16>(l, stream);
+}
+
+}  // namespace kvx

@@ -554,6 +554,56 @@ class KVCacheManager:
                                       scale=scale, causal=causal, out=out, return_lse=return_lse,
                                       shard_idx=shard_idx, stream=stream)
 
+    # -- eviction ------------------------------------------------------------
+    def weigh(self, k_layer: int, q, tables, lengths, lse, weights, *, starts=None, begins=None,
+              decay: float = 1.0, scale: Optional[float] = None, causal: bool = True,
+              shard_idx: int = 0, stream=None) -> None:
+        """Adds what attention each cached token got from ``q`` to ``weights``.
+
+        q, tables, lengths, starts, scale and causal are those of an ``attend`` that
+        returned ``lse``. weights is float32 [blocks, heads, tokens]: for token j
+        of a sequence, its block and slot, and each of the storage's heads,
+          weights = decay * weights + sum over the head's queries of
+                    exp(scale * q.k_j - lse),
+        where the call's own tokens had none before (so a block's entries need no
+        clearing when it is handed out). decay=0 keeps this call's alone. Tokens
+        before ``begins[s]`` (int32 [sequences]; a prefix shared with others) are
+        left out; a block that holds later ones must belong to one sequence.
+        """
+        from . import eviction
+        eviction.weigh(self, k_layer, q, tables, lengths, lse, weights, starts=starts,
+                       begins=begins, decay=decay, scale=scale, causal=causal,
+                       shard_idx=shard_idx, stream=stream)
+
+    def compact(self, k_layer: int, v_layer: int, kept, tables, *, weights=None,
+                shard_idx: int = 0, stream=None) -> None:
+        """Moves kept tokens to the front of their sequences, in place.
+
+        kept: int32 [sequences, heads, budget] of ``choose_kept``: place i of
+        sequence s and a head gets the key, the value and, with ``weights``, the
+        weight of position kept[s, head, i]. Positions ascend, -1 at the end. Heads
+        of one sequence keep tokens of their own; their keys have been rotated, so
+        attention does not mind their order. The next tokens are appended at the
+        new lengths, with their true ``positions``. In a float8 storage tokens
+        that meet in a block get the largest of their scales. Blocks from the first
+        place that takes another token on must belong to one sequence.
+        """
+        from . import eviction
+        eviction.compact(self, k_layer, v_layer, kept, tables, weights=weights,
+                         shard_idx=shard_idx, stream=stream)
+
+    def evict(self, k_layer: int, v_layer: int, weights, tables, lengths, budget: int, *,
+              recent: int = 0, begins=None, shard_idx: int = 0, stream=None):
+        """Cuts every sequence to ``budget`` tokens: ``choose_kept``, then
+        ``compact``. Returns the new lengths, int32 [sequences] on the device: the
+        lesser of each length and the budget. Blocks behind them are free."""
+        from . import eviction
+        kept, cut = eviction.choose_kept(weights, tables, lengths, budget, recent=recent,
+                                         begins=begins, stream=stream)
+        eviction.compact(self, k_layer, v_layer, kept, tables, weights=weights,
+                         shard_idx=shard_idx, stream=stream)
+        return cut
+
     # -- staging slots and host blocks --------------------------------------
     def configure_host_staging_slots(self, num_slots: int, max_major_per_slot: int) -> None:
         _capi.check(_capi.load().kvx_manager_configure_host_staging_slots(

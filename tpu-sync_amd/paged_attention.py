@@ -234,13 +234,21 @@ def _check_scales(layers, tables, shard_idx, kind, fp4_shape):
 
 
 def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
-    """Two of the manager's storages as the fields of kvx_paged_cache."""
+    """Two of the manager's storages as the fields of kvx_paged_cache; without
+    v_layer the keys' alone, without dtype of any type."""
     torch = _torch
     if mgr._device is None:
         raise _capi.KvxError(9, "needs a device-backed KVCacheManagerBase", "KVCacheManager")
     layers = mgr._tensors
     n = mgr.num_kv_layers
     shapes = []
+    if v_layer is None:
+        v_layer = k_layer
+    if dtype is None:
+        allowed = "bfloat16, float16"
+        types = (torch.bfloat16, torch.float16)
+    else:
+        allowed, types = dtype, (dtype,)
     for layer in (k_layer, v_layer):
         if not 0 <= layer < n or not 0 <= shard_idx < len(layers[layer]):
             raise _capi.KvxError(11, "layer or shard index out of range", "KVCacheManager")
@@ -249,8 +257,8 @@ def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
             raise ValueError("the cache's storages must be [blocks, tokens, heads, head_dim] "
                              "tensors (in 4 bits [blocks, heads, tokens, head_dim / 2]), "
                              f"got {tuple(t.shape)}")
-        if t.dtype not in (dtype, torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
-            raise ValueError(f"the cache must be {dtype}, float8_e4m3fn or float4_e2m1fn_x2, "
+        if t.dtype not in types + (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+            raise ValueError(f"the cache must be {allowed}, float8_e4m3fn or float4_e2m1fn_x2, "
                              f"got {t.dtype}")
         shapes.append((t.dtype,) + tuple(t.shape[1:]))
     if shapes[0] != shapes[1]:
@@ -259,7 +267,7 @@ def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
     if kind == torch.float4_e2m1fn_x2:
         heads, block_tokens, head_dim = block_tokens, heads, 2 * head_dim
     k_scales = v_scales = 0
-    if kind != dtype:
+    if kind in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
         # Scale tables follow the KV storages, one a storage.
         if len(layers) != 2 * n:
             raise ValueError(f"a {str(kind)[6:]} cache needs one scale table a KV storage "
@@ -284,18 +292,24 @@ def _cache(mgr, k_layer, v_layer, shard_idx, dtype):
     return found
 
 
-def _batch(device, tables, lengths, starts, tokens):
-    """The fields of kvx_paged_batch."""
+def _tables(device, tables):
+    """(address, row stride, width) of block tables."""
     if not _on_device(tables, device):
         raise ValueError(_off_device(tables, "tables", device))
     shape = tables.shape
     if len(shape) != 2 or tables.dtype != _torch.int32:
         raise ValueError(f"tables must be an int32 [sequences, blocks] tensor, got "
                          f"{tables.dtype} {tuple(shape)}")
-    n, width = shape
     row, last = tables.stride()
-    if last != 1 and width > 1:
+    if last != 1 and shape[1] > 1:
         raise ValueError("tables must be contiguous in their last dimension")
+    return tables.data_ptr(), row, shape[1]
+
+
+def _batch(device, tables, lengths, starts, tokens):
+    """The fields of kvx_paged_batch."""
+    tables_at, row, width = _tables(device, tables)
+    n = tables.shape[0]
     lengths_at = _vector(lengths, "lengths", device, (_torch.int32,), n)
     starts_at = 0
     if starts is not None:
@@ -303,7 +317,7 @@ def _batch(device, tables, lengths, starts, tokens):
     elif tokens != n:
         raise ValueError(f"without starts there is one token a sequence: {tokens} tokens, "
                          f"{n} sequences")
-    return tables.data_ptr(), row, width, lengths_at, starts_at, n
+    return tables_at, row, width, lengths_at, starts_at, n
 
 
 def append_kv(mgr, k_layer, v_layer, k, v, tables, lengths, *, starts, inv_freq, positions,
