@@ -1249,7 +1249,8 @@ typedef struct kvx_compact_args {
   int64_t table_stride;
   int64_t table_width;
   int64_t sequences;
-  uint64_t kept; /* int32 [sequences][heads][budget] */
+  uint64_t kept; /* int32 [sequences][heads][budget] at any strides */
+  int64_t kept_sequence_stride, kept_head_stride, kept_place_stride;
   int64_t budget;
   uint64_t weights; /* fp32 [blocks][heads][block_tokens] or 0 */
   int64_t blocks;   /* of the table of weights: at least the cache's */

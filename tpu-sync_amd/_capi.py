@@ -298,6 +298,8 @@ class CompactArgs(ctypes.Structure):
     _fields_ = [("cache", PagedCache), ("tables", ctypes.c_uint64),
                 ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int64),
                 ("sequences", ctypes.c_int64), ("kept", ctypes.c_uint64),
+                ("kept_sequence_stride", ctypes.c_int64), ("kept_head_stride", ctypes.c_int64),
+                ("kept_place_stride", ctypes.c_int64),
                 ("budget", ctypes.c_int64), ("weights", ctypes.c_uint64),
                 ("blocks", ctypes.c_int64)]
 

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include <climits>
+#include <utility>
 #include <cmath>
 
 #include "paged_args.h"
@@ -145,14 +146,24 @@ Status CheckCompact(const PoolSource& pool, const kvx_compact_args& a, CompactLa
   }
   DeviceRangeChecker ranges(pool.device);
   *out = CompactLaunch{};
-  kvx_paged_batch batch = {a.tables, a.table_stride, a.table_width, 0, 0, a.sequences};
-  batch.lengths = a.kept;  // not read; checked with what follows
-  const int64_t words = a.sequences * c.heads * a.budget;
   if (a.sequences < 0 || a.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
-  if (words == 0) return OkStatus();
+  if (a.kept_sequence_stride < 0 || a.kept_head_stride < 0 || a.kept_place_stride < 0) {
+    return Bad("kept: negative stride");
+  }
+  if (a.sequences == 0 || a.budget == 0) return OkStatus();
+  int64_t words = 1;
+  for (const auto& [n, stride] : {std::pair<int64_t, int64_t>{a.sequences, a.kept_sequence_stride},
+                                  {c.heads, a.kept_head_stride},
+                                  {a.budget, a.kept_place_stride}}) {
+    int64_t more = 0;
+    if (__builtin_mul_overflow(n - 1, stride, &more) ||
+        __builtin_add_overflow(words, more, &words) || words > INT64_MAX / 4) {
+      return Bad("kept: size overflows");
+    }
+  }
   KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.kept, words, "kept"));
-  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, batch, a.sequences, c.block_tokens, cache.num_blocks,
-                                 &out->batch));
+  const kvx_paged_batch batch = {a.tables, a.table_stride, a.table_width, 0, 0, a.sequences};
+  KVX_RETURN_IF_ERROR(CheckTables(&ranges, batch, c.block_tokens, cache.num_blocks, &out->batch));
   KVX_RETURN_IF_ERROR(CheckGrid(a.sequences * c.heads, kCompactThreads));
   Rows table = Whole(0, 0);
   if (a.weights != 0) {
@@ -171,6 +182,9 @@ Status CheckCompact(const PoolSource& pool, const kvx_compact_args& a, CompactLa
                                            {Whole(a.kept, words * 4), "kept"}}));
   out->block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
   out->kept = reinterpret_cast<const int32_t*>(a.kept);
+  out->kept_sequence = a.kept_sequence_stride;
+  out->kept_head = a.kept_head_stride;
+  out->kept_place = a.kept_place_stride;
   out->budget = static_cast<int32_t>(a.budget);
   out->k_pool = reinterpret_cast<void*>(cache.k.base);
   out->v_pool = reinterpret_cast<void*>(cache.v.base);

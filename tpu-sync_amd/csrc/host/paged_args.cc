@@ -102,12 +102,9 @@ Status CheckWords(DeviceRangeChecker* ranges, uint64_t at, int64_t n, const char
   return ranges->Check(at, static_cast<uint64_t>(n) * 4, what);
 }
 
-Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t tokens,
-                  int64_t block_tokens, int64_t num_blocks, BatchView* out) {
+Status CheckTables(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t block_tokens,
+                   int64_t num_blocks, BatchView* out) {
   if (b.sequences < 0 || b.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
-  if (b.starts == 0 && tokens != b.sequences) {
-    return Bad("without starts there is one token a sequence: tokens must equal sequences");
-  }
   if (b.table_width < 0 || b.table_stride < 0) return Bad("negative table width or stride");
   if (block_tokens < 1) return Bad("block_tokens must be positive");
   if (b.table_width > kMostTokens / block_tokens) {
@@ -120,21 +117,33 @@ Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t 
       return Bad("tables: size overflows");
     }
     if (b.table_width > 0) KVX_RETURN_IF_ERROR(CheckWords(ranges, b.tables, words, "tables"));
+  }
+  out->tables = reinterpret_cast<const int32_t*>(b.tables);
+  out->table_stride = b.table_stride;
+  out->table_width = static_cast<int32_t>(b.table_width);
+  out->sequences = static_cast<int32_t>(b.sequences);
+  out->block_tokens = static_cast<int32_t>(block_tokens);
+  out->capacity = static_cast<int32_t>(b.table_width * block_tokens);
+  out->num_blocks = static_cast<int32_t>(num_blocks);
+  return OkStatus();
+}
+
+Status CheckBatch(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t tokens,
+                  int64_t block_tokens, int64_t num_blocks, BatchView* out) {
+  if (b.sequences < 0 || b.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
+  if (b.starts == 0 && tokens != b.sequences) {
+    return Bad("without starts there is one token a sequence: tokens must equal sequences");
+  }
+  KVX_RETURN_IF_ERROR(CheckTables(ranges, b, block_tokens, num_blocks, out));
+  if (b.sequences > 0) {
     KVX_RETURN_IF_ERROR(CheckWords(ranges, b.lengths, b.sequences, "lengths"));
     if (b.starts != 0) {
       KVX_RETURN_IF_ERROR(CheckWords(ranges, b.starts, b.sequences + 1, "starts"));
     }
   }
-  out->tables = reinterpret_cast<const int32_t*>(b.tables);
   out->lengths = reinterpret_cast<const int32_t*>(b.lengths);
   out->starts = reinterpret_cast<const int32_t*>(b.starts);
-  out->table_stride = b.table_stride;
-  out->table_width = static_cast<int32_t>(b.table_width);
-  out->sequences = static_cast<int32_t>(b.sequences);
   out->tokens = static_cast<int32_t>(tokens);
-  out->block_tokens = static_cast<int32_t>(block_tokens);
-  out->capacity = static_cast<int32_t>(b.table_width * block_tokens);
-  out->num_blocks = static_cast<int32_t>(num_blocks);
   return OkStatus();
 }
 

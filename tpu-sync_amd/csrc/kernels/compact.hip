@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_kernel(const CompactLaunc
   char* pool = static_cast<char*>(key ? a.k_pool : a.v_pool) + blockIdx.z * slice_bytes;
   uint8_t* scales = static_cast<uint8_t*>(key ? a.k_scales : a.v_scales);
   const int32_t* table = a.batch.tables + s * a.batch.table_stride;
-  const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  const int32_t* kept = a.kept + s * a.kept_sequence + h * a.kept_head;
   const int pieces = slice_bytes / 16, items = places * pieces;
   const int rounds = (a.budget + places - 1) / places;
   // One workgroup of each row takes what lies beside it.
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_kernel(const CompactLaunc
     next_from = next_to = -1;
     const int i = r * places + static_cast<int>(threadIdx.x);
     if (static_cast<int>(threadIdx.x) < places && r < rounds && i < a.budget) {
-      const int p = kept[i];
+      const int p = kept[i * a.kept_place];
       if (p >= 0 && p != i) {
         x = RowAt<FP4>(a, table, h, p);
         y = RowAt<FP4>(a, table, h, i);
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
   uint8_t* pool = static_cast<uint8_t*>(key ? a.k_pool : a.v_pool);
   float* scales = static_cast<float*>(key ? a.k_scales : a.v_scales);
   const int32_t* table = a.batch.tables + s * a.batch.table_stride;
-  const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  const int32_t* kept = a.kept + s * a.kept_sequence + h * a.kept_head;
   const int B = a.batch.block_tokens, pieces = a.head_dim / 8;
   const bool takes_weight = a.weights != nullptr && key;
   // A group: the blocks that a round holds, or one that takes several rounds.
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
     }
     __syncthreads();
     for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
-      const int p = kept[i];
+      const int p = kept[i * a.kept_place];
       const int id = block_of(p);
       if (id >= 0) {
         const int g = FastDivI(a.block_div, i - begin);
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
         int64_t x = -1, y = -1;
         float ratio = 1.0f;
         if (i < end) {
-          const int p = kept[i], id = block_of(p), into = block_of(i);
+          const int p = kept[i * a.kept_place], id = block_of(p), into = block_of(i);
           const int g = FastDivI(a.block_div, i - begin);
           if (id >= 0 && into >= 0 && moves[g] != 0) {
             const auto row = [&](int of, int at) {
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
         }
       }
       if (takes_weight && threadIdx.x < kScaledRows && from[threadIdx.x] >= 0) {
-        weight = a.weights[WeightAt<false>(a, h, from[threadIdx.x], kept[i])];
+        weight = a.weights[WeightAt<false>(a, h, from[threadIdx.x], kept[i * a.kept_place])];
         weight_to = WeightAt<false>(a, h, to[threadIdx.x], i);
       }
       // Every wave has this round's rows before one of them is written over.

@@ -28,6 +28,7 @@ struct CompactLaunch {
   BatchView batch;  // tables alone
   FastDivU32 block_div;
   const int32_t* kept = nullptr;  // [sequences][heads][budget]
+  int64_t kept_sequence = 0, kept_head = 0, kept_place = 0;  // its strides
   int32_t budget = 0;
   // Storages and their scales, laid out as PoolKind says.
   void* k_pool = nullptr;

@@ -18,7 +18,7 @@ from .kv_cache_manager import _stream_ptr
 
 _WEIGH = struct.Struct(base._CACHE + base._BATCH + "q2iQ2q2QqQi2fi")
 _CHOOSE = struct.Struct("4iqQ" + base._BATCH + "3Q2q")
-_COMPACT = struct.Struct(base._CACHE + "Q3qQqQq")
+_COMPACT = struct.Struct(base._CACHE + "Q3qQ4qQq")
 for _pack, _args in ((_WEIGH, _capi.WeighArgs), (_CHOOSE, _capi.ChooseKeptArgs),
                      (_COMPACT, _capi.CompactArgs)):
     assert _pack.size == ctypes.sizeof(_args)
@@ -129,10 +129,9 @@ def compact(mgr, k_layer, v_layer, kept, tables, *, weights, shard_idx, stream) 
     cache = base._cache(mgr, k_layer, v_layer, shard_idx, None)
     if not base._on_device(kept, device):
         raise ValueError(base._off_device(kept, "kept", device))
-    if (kept.dtype != torch.int32 or len(kept.shape) != 3 or kept.shape[1] != cache[7]
-            or not kept.is_contiguous()):
-        raise ValueError(f"kept must be a contiguous int32 [sequences, {cache[7]}, budget] tensor, "
-                         f"got {kept.dtype} {tuple(kept.shape)}")
+    if kept.dtype != torch.int32 or len(kept.shape) != 3 or kept.shape[1] != cache[7]:
+        raise ValueError(f"kept must be an int32 [sequences, {cache[7]}, budget] tensor, got "
+                         f"{kept.dtype} {tuple(kept.shape)}")
     sequences, _, budget = kept.shape
     tables_at, row, width = base._tables(device, tables)
     if tables.shape[0] != sequences:
@@ -142,7 +141,8 @@ def compact(mgr, k_layer, v_layer, kept, tables, *, weights, shard_idx, stream) 
         blocks = mgr._tensors[k_layer][shard_idx].shape[0]
         weights_at, blocks = _weights(weights, device, blocks, cache[7], cache[6])
     args = _capi.CompactArgs.from_buffer_copy(_COMPACT.pack(
-        *cache, tables_at, row, width, sequences, kept.data_ptr(), budget, weights_at, blocks))
+        *cache, tables_at, row, width, sequences, kept.data_ptr(), *kept.stride(), budget, weights_at,
+        blocks))
     handle = base._current_stream(device) if stream is None else _stream_ptr(stream)
     rc = _capi.load().kvx_manager_compact(mgr._h, args, handle)
     if rc:
