@@ -1183,7 +1183,8 @@ int kvx_manager_attend(kvx_manager* m, const kvx_attend_args* args, void* stream
  * call gives the same bytes. Other entries of the table are left alone; a token that has
  * no place is skipped. A block that holds a token from begins[s] on must belong to one
  * sequence of the call (those of a shared prefix lie before begins). A sequence without
- * query rows is left alone.
+ * query rows is left alone. workspace: as for kvx_manager_attend; without starts and
+ * with up to 32 query heads a key head none is needed.
  */
 typedef struct kvx_weigh_args {
   kvx_paged_cache cache; /* v_layer and v_scale_layer are not used */
@@ -1201,8 +1202,11 @@ typedef struct kvx_weigh_args {
   float scale; /* positive */
   float decay; /* 0..1 */
   int32_t reserved;
+  uint64_t workspace;
+  int64_t workspace_bytes;
 } kvx_weigh_args;
 
+int kvx_manager_weigh_workspace(kvx_manager* m, const kvx_weigh_args* args, int64_t* bytes);
 int kvx_manager_weigh(kvx_manager* m, const kvx_weigh_args* args, void* stream);
 
 /*

@@ -283,7 +283,8 @@ class WeighArgs(ctypes.Structure):
                 + [("lse", ctypes.c_uint64), ("weights", ctypes.c_uint64),
                    ("blocks", ctypes.c_int64), ("begins", ctypes.c_uint64),
                    ("non_causal", ctypes.c_int32), ("scale", ctypes.c_float),
-                   ("decay", ctypes.c_float), ("reserved", ctypes.c_int32)])
+                   ("decay", ctypes.c_float), ("reserved", ctypes.c_int32),
+                   ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64)])
 
 
 class ChooseKeptArgs(ctypes.Structure):
@@ -547,6 +548,7 @@ PROTOTYPES = {
     "kvx_manager_append_kv": (_int, [_vp, ctypes.POINTER(AppendKvArgs), _vp]),
     "kvx_manager_attend_workspace": (_int, [_vp, ctypes.POINTER(AttendArgs), _i64p]),
     "kvx_manager_attend": (_int, [_vp, ctypes.POINTER(AttendArgs), _vp]),
+    "kvx_manager_weigh_workspace": (_int, [_vp, ctypes.POINTER(WeighArgs), _i64p]),
     "kvx_manager_weigh": (_int, [_vp, ctypes.POINTER(WeighArgs), _vp]),
     "kvx_choose_kept": (_int, [ctypes.POINTER(ChooseKeptArgs), _vp]),
     "kvx_manager_compact": (_int, [_vp, ctypes.POINTER(CompactArgs), _vp]),

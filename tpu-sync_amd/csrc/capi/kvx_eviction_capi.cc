@@ -13,12 +13,20 @@ using kvx_capi::Source;
 
 extern "C" {
 
+int kvx_manager_weigh_workspace(kvx_manager* m, const kvx_weigh_args* args, int64_t* bytes) {
+  if (m == nullptr || args == nullptr || bytes == nullptr) {
+    return Fail(KVX_INVALID_ARGUMENT, "null manager, arguments or output");
+  }
+  kvx::WeighLaunch l;
+  return kvx_capi::Done(kvx::CheckWeigh(Source(m), *args, &l, bytes));
+}
+
 int kvx_manager_weigh(kvx_manager* m, const kvx_weigh_args* args, void* stream) {
   if (m == nullptr || args == nullptr) {
     return Fail(KVX_INVALID_ARGUMENT, "null manager or arguments");
   }
   kvx::WeighLaunch l;
-  const kvx::Status st = kvx::CheckWeigh(Source(m), *args, &l);
+  const kvx::Status st = kvx::CheckWeigh(Source(m), *args, &l, nullptr);
   if (!st.ok()) return Fail(st);
   if (l.attend.batch.tokens == 0) return KVX_OK;
   return OnDevice(m->impl->device(),

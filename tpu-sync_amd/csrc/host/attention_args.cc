@@ -210,17 +210,7 @@ Status CheckAttend(const PoolSource& pool, const kvx_attend_args& a, AttendLaunc
       KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
     }
   } else {
-    // Sizes only: the address arguments may still be unset.
-    if (a.batch.sequences < 0 || a.batch.sequences > kMaxSequences) {
-      return Bad("sequences must be 0..4096");
-    }
-    if (a.batch.table_width < 0 || a.batch.table_width > kMostTokens / c.block_tokens) {
-      return Bad("table_width * block_tokens must be at most 2^30");
-    }
-    out->batch.starts = reinterpret_cast<const int32_t*>(a.batch.starts);
-    out->batch.sequences = static_cast<int32_t>(a.batch.sequences);
-    out->batch.tokens = static_cast<int32_t>(a.tokens);
-    out->batch.capacity = static_cast<int32_t>(a.batch.table_width * c.block_tokens);
+    KVX_RETURN_IF_ERROR(CheckSizes(a.batch, a.tokens, c.block_tokens, &out->batch));
   }
   const int64_t G = a.q_heads / c.heads;
   // Work is counted in 32 bits: tiles by steps of 64 tokens, sequences by steps

@@ -30,7 +30,8 @@ Status CheckTable(DeviceRangeChecker* ranges, uint64_t at, int64_t blocks, int64
 
 }  // namespace
 
-Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* out) {
+Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* out,
+                  int64_t* workspace_bytes) {
   Cache cache;
   KVX_RETURN_IF_ERROR(FindCache(pool, a.cache, a.dtype, &cache, false));
   const kvx_paged_cache& c = a.cache;
@@ -43,44 +44,47 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
   if (!(a.decay >= 0 && a.decay <= 1)) return Bad("decay must be 0..1");
   DeviceRangeChecker ranges(pool.device);
   const Rows q = {a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.q_heads, c.head_dim, 2};
-  KVX_RETURN_IF_ERROR(CheckRows(&ranges, q, "q"));
+  Rows table = Whole(0, 0);
   *out = WeighLaunch{};
   AttendLaunch& l = out->attend;
-  KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
-                                 &l.batch));
-  if (a.tokens > 0) KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
-  if (a.begins != 0 && a.batch.sequences > 0) {
-    KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.begins, a.batch.sequences, "begins"));
-  }
-  Rows table;
-  KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, c.heads, c.block_tokens, &table));
-  if (a.blocks < cache.num_blocks) return Bad("weights: fewer blocks than the cache's");
   l.pool = KindOf(c.dtype);
-  if (l.pool == kPoolSame && cache.k.base % 16 != 0) {
-    return Bad("cache storages: must be aligned to 16 bytes");
+  if (workspace_bytes == nullptr) {
+    KVX_RETURN_IF_ERROR(CheckRows(&ranges, q, "q"));
+    KVX_RETURN_IF_ERROR(CheckBatch(&ranges, a.batch, a.tokens, c.block_tokens, cache.num_blocks,
+                                   &l.batch));
+    if (a.tokens > 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.lse, a.tokens * a.q_heads, "lse"));
+    }
+    if (a.begins != 0 && a.batch.sequences > 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.begins, a.batch.sequences, "begins"));
+    }
+    KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, c.heads, c.block_tokens, &table));
+    if (a.blocks < cache.num_blocks) return Bad("weights: fewer blocks than the cache's");
+    if (l.pool == kPoolSame && cache.k.base % 16 != 0) {
+      return Bad("cache storages: must be aligned to 16 bytes");
+    }
+  } else {
+    KVX_RETURN_IF_ERROR(CheckSizes(a.batch, a.tokens, c.block_tokens, &l.batch));
   }
-  // Work is counted in 32 bits: steps of 32 tokens, tiles of 128, for every head.
+  // Work is counted in 32 bits, for every head: steps of 32 tokens, and tiles of 128 by
+  // stages of 64 rows.
+  const int64_t G = a.q_heads / c.heads;
   const int64_t few = a.batch.sequences * (l.batch.capacity / kFewStep + 1);
-  if (few > INT32_MAX / 2 / c.heads) return Bad("sequences * table_width is too large for one call");
-  KVX_RETURN_IF_ERROR(CheckApart(
-      {table, "weights"},
-      {{q, "q"},
-       {Whole(cache.k), "the cache"},
-       {Whole(cache.k_scales), "the cache's scales"},
-       {Tables(a.batch), "tables"},
-       {Lengths(a.batch), "lengths"},
-       {Starts(a.batch), "starts"},
-       {Whole(a.lse, a.tokens * a.q_heads * 4), "lse"},
-       {Whole(a.begins, a.begins != 0 ? a.batch.sequences * 4 : 0), "begins"}}));
+  const int64_t tiles = l.batch.capacity / kWeighTile + 1;
+  const int64_t stages = a.tokens * G / kWeighRows + 1 + a.batch.sequences;
+  if (few > INT32_MAX / 2 / c.heads || stages > INT32_MAX / 2 / c.heads / tiles) {
+    return Bad("tokens * table_width is too large for one call");
+  }
+  l.most_few = static_cast<int32_t>(few);
+  l.most_many = static_cast<int32_t>(tiles * stages);
   if (a.batch.sequences == 0) l.batch.tokens = 0;
   l.block_div = MakeFastDivU32(static_cast<uint32_t>(c.block_tokens));
-  l.group_div = MakeFastDivU32(static_cast<uint32_t>(a.q_heads / c.heads));
+  l.group_div = MakeFastDivU32(static_cast<uint32_t>(G));
   l.q = reinterpret_cast<const void*>(a.q);
   l.q_token = a.q_token_stride;
   l.q_head = a.q_head_stride;
   l.k_pool = reinterpret_cast<const void*>(cache.k.base);
   l.k_scales = reinterpret_cast<const void*>(cache.k_scales.base);
-  l.most_few = l.most_many = static_cast<int32_t>(few);
   l.q_heads = a.q_heads;
   l.k_heads = c.heads;
   l.head_dim = c.head_dim;
@@ -91,8 +95,32 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
   out->weights = reinterpret_cast<float*>(a.weights);
   out->begins = reinterpret_cast<const int32_t*>(a.begins);
   out->decay = a.decay;
-  if (l.batch.tokens > 0) PlanWeigh(out);
-  return OkStatus();
+  const int64_t need = l.batch.tokens == 0 ? 0 : PlanWeigh(out);
+  if (workspace_bytes != nullptr) {
+    *workspace_bytes = need;
+    return OkStatus();
+  }
+  if (need > 0) {
+    if (a.workspace_bytes < need) {
+      return Bad("workspace: " + std::to_string(need) + " bytes are needed");
+    }
+    if (a.workspace % 16 != 0) return Bad("workspace: must be aligned to 16 bytes");
+    KVX_RETURN_IF_ERROR(ranges.Check(a.workspace, static_cast<uint64_t>(need), "workspace"));
+    out->parts = reinterpret_cast<float*>(a.workspace);
+  }
+  const Named weights = {table, "weights"}, workspace = {Whole(a.workspace, need), "workspace"};
+  for (const Named* written : {&weights, &workspace}) {
+    KVX_RETURN_IF_ERROR(CheckApart(
+        *written, {{q, "q"},
+                   {Whole(cache.k), "the cache"},
+                   {Whole(cache.k_scales), "the cache's scales"},
+                   {Tables(a.batch), "tables"},
+                   {Lengths(a.batch), "lengths"},
+                   {Starts(a.batch), "starts"},
+                   {Whole(a.lse, a.tokens * a.q_heads * 4), "lse"},
+                   {Whole(a.begins, a.begins != 0 ? a.batch.sequences * 4 : 0), "begins"}}));
+  }
+  return CheckApart(workspace, {weights});
 }
 
 Status CheckChooseKept(const kvx_choose_kept_args& a, ChooseLaunch* out) {

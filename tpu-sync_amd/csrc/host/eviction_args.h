@@ -10,7 +10,9 @@
 namespace kvx {
 
 // attend.batch.tokens == 0 on success: nothing to do.
-Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* out);
+// With `workspace_bytes`, sizes the workspace and leaves addresses unchecked.
+Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* out,
+                  int64_t* workspace_bytes);
 // batch.sequences == 0 on success: nothing to do.
 Status CheckChooseKept(const kvx_choose_kept_args& a, ChooseLaunch* out);
 Status CheckCompact(const PoolSource& pool, const kvx_compact_args& a, CompactLaunch* out);

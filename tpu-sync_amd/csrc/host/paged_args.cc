@@ -102,6 +102,18 @@ Status CheckWords(DeviceRangeChecker* ranges, uint64_t at, int64_t n, const char
   return ranges->Check(at, static_cast<uint64_t>(n) * 4, what);
 }
 
+Status CheckSizes(const kvx_paged_batch& b, int64_t tokens, int64_t block_tokens, BatchView* out) {
+  if (b.sequences < 0 || b.sequences > kMaxSequences) return Bad("sequences must be 0..4096");
+  if (b.table_width < 0 || b.table_width > kMostTokens / block_tokens) {
+    return Bad("table_width * block_tokens must be at most 2^30");
+  }
+  out->starts = reinterpret_cast<const int32_t*>(b.starts);
+  out->sequences = static_cast<int32_t>(b.sequences);
+  out->tokens = static_cast<int32_t>(tokens);
+  out->capacity = static_cast<int32_t>(b.table_width * block_tokens);
+  return OkStatus();
+}
+
 Status CheckTables(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t block_tokens,
                    int64_t num_blocks, BatchView* out) {
   if (b.sequences < 0 || b.sequences > kMaxSequences) return Bad("sequences must be 0..4096");

@@ -85,6 +85,8 @@ Status CheckTokens(int64_t tokens, int64_t heads, int64_t dim);
 Status CheckGrid(int64_t workgroups, int64_t threads);
 Status CheckWords(DeviceRangeChecker* ranges, uint64_t at, int64_t n, const char* what);
 
+// A batch's sizes alone: the addresses may still be unset.
+Status CheckSizes(const kvx_paged_batch& b, int64_t tokens, int64_t block_tokens, BatchView* out);
 // The tables of a batch alone, and all of it.
 Status CheckTables(DeviceRangeChecker* ranges, const kvx_paged_batch& b, int64_t block_tokens,
                    int64_t num_blocks, BatchView* out);

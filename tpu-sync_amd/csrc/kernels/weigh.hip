@@ -13,7 +13,7 @@
 // of the axis of all sequences' steps of 32 tokens; keys go from memory straight into
 // operands. Reading them bounds it.
 //
-// weigh_many (chunks): a workgroup takes WeighTile tokens of one sequence and key
+// weigh_many (chunks): a workgroup takes kWeighTile tokens of one sequence and key
 // head, keeps their keys in registers and goes through the rows that see them, 64 at a
 // time in LDS. The products and the exponentials (16 a lane for 8 products at D = 128)
 // bound it.
@@ -232,18 +232,90 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_k
   }
 }
 
-// -- Many rows.
+// -- Many rows: tiles of kWeighTile tokens of the sequences with more than kFewRows rows,
+// each of as many stages of kWeighRows rows as see it.
 
-constexpr int kWeighRows = 64;  // of a stage
+struct WeighUnit {
+  int rows;
+  int begin, end;  // tokens
+  int old_end;     // tokens that are not the call's own
+  int tiles;
+  // Tiles that all rows see, of `stages` each; the others have 2 G less each than the
+  // one before, the first of them `later`.
+  int full, stages, later;
+};
+
+__device__ __forceinline__ WeighUnit LoadWeighUnit(const WeighLaunch& w, int s) {
+  const WeighKeys k = LoadWeighKeys(w, s);
+  const int G = w.attend.q_heads / w.attend.k_heads;
+  WeighUnit u;
+  u.rows = k.rows;
+  u.begin = k.begin;
+  u.end = k.end;
+  u.old_end = k.q.length - k.q.count;
+  u.tiles = k.rows > kFewRows ? (k.end - k.begin + kWeighTile - 1) / kWeighTile : 0;
+  u.stages = (k.rows + kWeighRows - 1) / kWeighRows;
+  u.full = u.tiles;
+  u.later = 0;
+  if (w.attend.causal) {
+    u.full = u.old_end < u.begin ? 0 : min((u.old_end - u.begin) / kWeighTile + 1, u.tiles);
+    // The first token of the next tile is so many behind the first of the call's own.
+    const int behind = u.begin + u.full * kWeighTile - u.old_end;
+    u.later = u.full < u.tiles ? u.stages - behind * G / kWeighRows : 0;
+  }
+  return u;
+}
+
+// Where tile i starts on its sequence's and head's axis.
+__device__ __forceinline__ int WeighCost(const WeighLaunch& w, const WeighUnit& u, int i) {
+  if (i <= u.full) return i * u.stages;
+  const int n = i - u.full;
+  static_assert(kWeighTile == 2 * kWeighRows, "2 G stages a tile");
+  return u.full * u.stages + n * u.later - n * (n - 1) * (w.attend.q_heads / w.attend.k_heads);
+}
+
+// The tile that holds `at`.
+__device__ __forceinline__ int WeighTileAt(const WeighLaunch& w, const WeighUnit& u, int at) {
+  if (at < u.full * u.stages) return at / u.stages;
+  int tile = u.full, tiles = u.tiles;
+  while (tiles - tile > 1) {
+    const int mid = (tile + tiles) / 2;
+    if (WeighCost(w, u, mid) <= at) {
+      tile = mid;
+    } else {
+      tiles = mid;
+    }
+  }
+  return tile;
+}
+
+// Sums of all sequences' costs into LDS.
+__device__ __forceinline__ void WeighSums(const WeighLaunch& w, int* sums) {
+  for (int s = threadIdx.x; s < w.attend.batch.sequences; s += kAttendThreads) {
+    const WeighUnit u = LoadWeighUnit(w, s);
+    sums[s] = WeighCost(w, u, u.tiles);
+  }
+  BlockSums(sums, w.attend.batch.sequences, w.attend.most_many);
+}
+
+// A worker's least part, in stages.
+constexpr int kLeastStages = 4;
+__device__ __forceinline__ Axis WeighAxis(const WeighLaunch& w, int work) {
+  const int total = work * w.attend.k_heads;
+  return Axis(total, min(w.attend.many_grid, max(total / kLeastStages, 1)));
+}
+
+constexpr int kAhead = 4;  // products that operands are read ahead
 
 template <class E, int POOL, int DP>
-__global__ __launch_bounds__(kAttendThreads, 2) void weigh_many_kernel(const WeighLaunch w) {
+__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_kernel(
+    const WeighLaunch w) {
   extern __shared__ __align__(16) char lds[];
   using Scalar = typename E::Scalar;
   constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
-  constexpr int KS = DP / 16, kRow = 2 * DP, kTokens = WeighTile(DP);
-  constexpr int CT = kTokens / 128;  // tiles of 32 tokens a wave
-  constexpr int kChunks = kWeighRows * (DP / 8) / kAttendThreads;  // of a thread
+  constexpr int KS = DP / 16, kRow = 2 * DP;
+  constexpr int kChunks = DP / 32;  // of a thread: every fourth of a row
+  static_assert(kWeighRows * 4 == kAttendThreads);
   struct Rows {
     float base[kWeighRows];
     int seen[kWeighRows];
@@ -252,186 +324,253 @@ __global__ __launch_bounds__(kAttendThreads, 2) void weigh_many_kernel(const Wei
   int* sums = reinterpret_cast<int*>(row_data + 2);  // [sequences]
   const AttendLaunch& a = w.attend;
   const BatchView& b = a.batch;
-  for (int s = threadIdx.x; s < b.sequences; s += kAttendThreads) {
-    const WeighKeys k = LoadWeighKeys(w, s);
-    sums[s] = k.rows > kFewRows ? (k.end - k.begin + kTokens - 1) / kTokens : 0;
-  }
-  BlockSums(sums, b.sequences, a.most_many);
   const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int tiles = one(sums[b.sequences - 1]) * a.k_heads;
+  WeighSums(w, sums);
+  const int work = one(sums[b.sequences - 1]);
+  if (work == 0) return;
+  const Axis axis = WeighAxis(w, work);
+  // The workgroups of one XCD take neighbouring parts, so its L2 serves a head's rows to
+  // all of them.
+  const int worker = WorkerAt(blockIdx.x, axis.workers);
+  if (worker < 0) return;
+  const int x_end = axis.Start(worker + 1);
   const int lane = threadIdx.x % 64, wave = one(threadIdx.x / 64);
   const int in32 = lane % 32, half = lane / 32;
   const int G = a.q_heads / a.k_heads;
   const float c = a.scale * kLog2e;
+  // Where the lane's part of a row's operands is in a stage.
+  int row_at[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    row_at[ks] = in32 * kRow + KeyChunk<DP>(in32, ks * 2 + half) * 16;
+  }
 
-  for (int x = blockIdx.x; x < tiles; x += gridDim.x) {
+  for (int x = axis.Start(worker); x < x_end;) {
     const int s = one(FirstAbove(sums, b.sequences, x / a.k_heads));
     const int before = s > 0 ? one(sums[s - 1]) : 0;
-    const int of_head = one(sums[s]) - before;
-    const int off = x - before * a.k_heads;
-    const int h = off / of_head, tile = off - h * of_head;
-    const WeighKeys k = LoadWeighKeys(w, s);
-    const int end = one(k.end), rows = one(k.rows);
-    const SequenceSpan span = {one(k.q.first), one(k.q.count), one(k.q.length)};
-    const int j0 = one(k.begin) + tile * kTokens;
-    const int old_end = span.length - span.count;
+    const int per_head = one(sums[s]) - before;
+    const int h = (x - before * a.k_heads) / per_head;
+    const int at_unit = x - before * a.k_heads - h * per_head;
+    const WeighUnit u = LoadWeighUnit(w, s);
+    const int tile = one(WeighTileAt(w, u, at_unit));
+    const int tile_at = one(WeighCost(w, u, tile));
+    const int stages = one(WeighCost(w, u, tile + 1)) - tile_at;
+    // The part's stages: the last of them end with the last row.
+    const int stage0 = at_unit - tile_at, stage1 = min(stages, stage0 + (x_end - x));
+    const int end = one(u.end), old_end = one(u.old_end);
+    const int row0 = (one(u.stages) - stages + stage0) * kWeighRows;
+    const int rows = min(one(u.rows), row0 + (stage1 - stage0) * kWeighRows);
+    const SequenceSpan span = LoadSequence(b, s);
+    const int j0 = one(u.begin) + tile * kWeighTile;
 
-    // Keys: token l % 32 of each of the wave's tiles, as an operand.
-    const int32_t* table = b.tables + s * b.table_stride;
-    u32x4 key[CT][KS];
-    float factor[CT];
-    float* mine[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int p = j0 + (wave * CT + ct) * 32 + in32;
+    // Keys: token l % 32 of the wave's, as an operand.
+    const int p = j0 + wave * 32 + in32;
+    u32x4 key[KS];
+    float factor = c;
+    float* mine;
+    {
       const int at = FastDivI(a.block_div, p), slot = p - at * b.block_tokens;
-      const int id = p < end ? table[at] : -1;
+      const int id = p < end ? b.tables[s * b.table_stride + at] : -1;
       const bool has = id >= 0 && id < b.num_blocks;
       const int64_t of_block = static_cast<int64_t>(has ? id : 0);
       // Places in layouts with a head's tokens together, and with a token's heads.
       const int64_t by_head = (of_block * a.k_heads + h) * b.block_tokens + (has ? slot : 0);
       const int64_t by_token = (of_block * b.block_tokens + (has ? slot : 0)) * a.k_heads + h;
-      mine[ct] = has ? w.weights + by_head : nullptr;
-      factor[ct] = c;
-      if constexpr (E4) factor[ct] *= static_cast<const float*>(a.k_scales)[of_block * a.k_heads + h];
+      mine = has ? w.weights + by_head : nullptr;
+      if constexpr (E4) factor *= static_cast<const float*>(a.k_scales)[of_block * a.k_heads + h];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = ks * 16 + half * 8;
-        key[ct][ks] = u32x4{0, 0, 0, 0};
+        key[ks] = u32x4{0, 0, 0, 0};
         if (!has || d >= a.head_dim) continue;
         if constexpr (F4) {
           const uint32_t code = static_cast<const uint8_t*>(
               a.k_scales)[by_head * (a.head_dim / kFp4Group) + d / kFp4Group];
-          key[ct][ks] = FromFp4<E>(
+          key[ks] = FromFp4<E>(
               *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.k_pool) +
                                                  by_head * (a.head_dim / 2) + d / 2),
               Fp4Scale<E>(code));
         } else if constexpr (E4) {
-          key[ct][ks] = Widen<E>(*reinterpret_cast<const Bytes8*>(
+          key[ks] = Widen<E>(*reinterpret_cast<const Bytes8*>(
               static_cast<const uint8_t*>(a.k_pool) + by_token * a.head_dim + d));
         } else {
-          key[ct][ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) +
-                                                          by_token * a.head_dim + d);
+          key[ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) +
+                                                      by_token * a.head_dim + d);
         }
       }
     }
 
-    // Rows, from the first that sees the tile's first token.
-    const int first_token = a.causal ? max(j0 - old_end, 0) : 0;
-    const int row0 = one(min(first_token * G, rows)) / kWeighRows * kWeighRows;
+    // Four threads load a row of every stage, and step from one to the next without a
+    // division.
+    const int step_tokens = kWeighRows / G, step_heads = kWeighRows - step_tokens * G;
+    const int my_row = threadIdx.x / 4, my_chunk = threadIdx.x % 4;
+    int t = FastDivI(a.group_div, row0 + my_row), of_token = row0 + my_row - t * G;
+    const Scalar* from = static_cast<const Scalar*>(a.q) +
+                         static_cast<int64_t>(span.first + t) * a.q_token +
+                         (h * G + of_token) * a.q_head + my_chunk * 8;
     u32x4 hold[kChunks];
     float hold_base = 0.0f;
     int hold_seen = 0;
-    const auto load = [&](int from) {
+    const auto load = [&](int r0) {
+      const bool has = r0 + my_row < rows;
 #pragma unroll
       for (int n = 0; n < kChunks; ++n) {
-        const int chunk = threadIdx.x + n * kAttendThreads;
-        const int r = from + chunk / (DP / 8), d = chunk % (DP / 8) * 8;
-        const int t = FastDivI(a.group_div, r);
         hold[n] = u32x4{0, 0, 0, 0};
-        if (r < rows && d < a.head_dim) {
-          hold[n] = *reinterpret_cast<const Bytes16*>(
-              static_cast<const Scalar*>(a.q) + static_cast<int64_t>(span.first + t) * a.q_token +
-              (h * G + (r - t * G)) * a.q_head + d);
+        if (has && (my_chunk + n * 4) * 8 < a.head_dim) {
+          hold[n] = *reinterpret_cast<const Bytes16*>(from + n * 32);
         }
       }
-      if (threadIdx.x < kWeighRows) {
-        const int r = from + threadIdx.x, t = FastDivI(a.group_div, r);
-        hold_base = 0.0f;
-        hold_seen = 0;
-        if (r < rows) {
-          hold_base = w.lse[(span.first + t) * static_cast<int64_t>(a.q_heads) + h * G +
-                            (r - t * G)] * kLog2e;
-          hold_seen = Visible(a, span, span.first + t);
-        }
+      hold_base = 0.0f;
+      hold_seen = 0;
+      if (has && my_chunk == 0) {
+        hold_base = w.lse[(span.first + t) * static_cast<int64_t>(a.q_heads) + h * G + of_token] *
+                    kLog2e;
+        hold_seen = Visible(a, span, span.first + t);
+      }
+      t += step_tokens;
+      of_token += step_heads;
+      from += step_tokens * a.q_token + step_heads * a.q_head;
+      if (of_token >= G) {  // from a token's heads to the next one's
+        ++t;
+        of_token -= G;
+        from += a.q_token - G * a.q_head;
       }
     };
-    const auto store = [&](int buffer) {
+    const auto store = [&](auto buffer) {
 #pragma unroll
       for (int n = 0; n < kChunks; ++n) {
-        const int chunk = threadIdx.x + n * kAttendThreads;
-        const int r = chunk / (DP / 8);
-        *reinterpret_cast<u32x4*>(lds + buffer * (kWeighRows * kRow) + r * kRow +
-                                  KeyChunk<DP>(r, chunk % (DP / 8)) * 16) = hold[n];
+        *reinterpret_cast<u32x4*>(lds + buffer() * (kWeighRows * kRow) + my_row * kRow +
+                                  KeyChunk<DP>(my_row, my_chunk + n * 4) * 16) = hold[n];
       }
-      if (threadIdx.x < kWeighRows) {
-        row_data[buffer].base[threadIdx.x] = hold_base;
-        row_data[buffer].seen[threadIdx.x] = hold_seen;
+      if (my_chunk == 0) {
+        row_data[buffer()].base[my_row] = hold_base;
+        row_data[buffer()].seen[my_row] = hold_seen;
       }
     };
 
-    float got[CT] = {};
-    load(row0);
-    int buffer = 0;
-    for (int r0 = row0; r0 < rows; r0 += kWeighRows) {
+    float got = 0.0f;
+    // The last token of the wave that counts: rows that see it see all of them.
+    const int last = min(j0 + wave * 32 + 32, end);
+    // Scores of 32 rows of a stage. Lane: token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4.
+    const auto scores = [&](auto buffer, auto rt) {
+      const char* at = lds + buffer() * (kWeighRows * kRow) + rt() * 32 * kRow;
+      f32x16 sc = f32x16(0.0f);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        sc = Mma32<E>(*reinterpret_cast<const u32x4*>(at + row_at[ks]), key[ks], sc);
+      }
+      return sc;
+    };
+    const auto raise = [&](auto buffer, auto rt, f32x16& sc) {
+      const float* base = &row_data[buffer()].base[rt() * 32 + half * 4];
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 of = *reinterpret_cast<const f32x4*>(base + i * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i + j], factor, -of[j]));
+        }
+      }
+    };
+    const auto add = [&](auto buffer, auto rt, f32x16& sc, bool plain) {
+      if (!plain) {
+        const int* seen = &row_data[buffer()].seen[rt() * 32 + half * 4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (p >= seen[i / 4 * 8 + i % 4]) sc[i] = 0.0f;
+        }
+      }
+      // Sums of 16 first: thousands of rows lose less so.
+      float some[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) some[j] = (sc[j] + sc[4 + j]) + (sc[8 + j] + sc[12 + j]);
+      got += (some[0] + some[1]) + (some[2] + some[3]);
+    };
+    const auto stage = [&](int r0, auto buffer) {
       store(buffer);
       __syncthreads();
       if (r0 + kWeighRows < rows) load(r0 + kWeighRows);
-      const Rows& here = row_data[buffer];
-      // Whether every row sees every token of the wave.
-      const int last = min(j0 + (wave + 1) * CT * 32, end);
-      const bool plain =
-          r0 + kWeighRows <= rows && Visible(a, span, span.first + FastDivI(a.group_div, r0)) >= last;
+      const bool plain = r0 + kWeighRows <= rows &&
+                         Visible(a, span, span.first + FastDivI(a.group_div, r0)) >= last;
+      constexpr std::integral_constant<int, 0> kFirst{};
+      constexpr std::integral_constant<int, 1> kSecond{};
+      // The second rows' products beside the first ones' exponentials.
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 sc = scores(buffer, kFirst);
+      f32x16 next = scores(buffer, kSecond);
+      raise(buffer, kFirst, sc);
+      raise(buffer, kSecond, next);
+      // Operands are read kAhead products ahead.
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-      for (int rt = 0; rt < kWeighRows / 32; ++rt) {
-        f32x16 sc[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) sc[ct] = f32x16(0.0f);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int r = rt * 32 + in32;
-          const u32x4 row = *reinterpret_cast<const u32x4*>(
-              lds + buffer * (kWeighRows * kRow) + r * kRow + KeyChunk<DP>(r, ks * 2 + half) * 16);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) sc[ct] = Mma32<E>(row, key[ct][ks], sc[ct]);
-        }
-        // Lane: token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4. Sums of 16 first:
-        // thousands of rows lose less so.
-        float some[CT] = {};
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const f32x4 base = *reinterpret_cast<const f32x4*>(&here.base[rt * 32 + i * 2 + half * 4]);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              sc[ct][i + j] =
-                  __builtin_amdgcn_exp2f(fmaf(sc[ct][i + j], factor[ct], -base[j]));
-            }
-          }
-          if (!plain) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int seen = here.seen[rt * 32 + i * 2 + half * 4 + j];
-#pragma unroll
-              for (int ct = 0; ct < CT; ++ct) {
-                if (j0 + (wave * CT + ct) * 32 + in32 >= seen) sc[ct][i + j] = 0.0f;
-              }
-            }
-          }
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) some[ct] += sc[ct][i + j];
-          }
-        }
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) got[ct] += some[ct];
+      for (int n = 0; n < KS; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      // (The other buffer's readers are past the barrier above.)
-      buffer ^= 1;
-    }
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const float sum = Plus32(got[ct]);
-      if (half == 0 && mine[ct] != nullptr) {
-        const int p = j0 + (wave * CT + ct) * 32 + in32;
-        const float was = p < old_end && w.decay != 0.0f ? *mine[ct] : 0.0f;
-        *mine[ct] = fmaf(w.decay, was, sum);
+      for (int n = 0; n < KS; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 32 / KS, 0);
+      }
+      add(buffer, kFirst, sc, plain);
+      add(buffer, kSecond, next, plain);
+    };
+    load(row0);
+    // (A buffer's readers are past the barrier of the stage in between.)
+    for (int r0 = row0; r0 < rows; r0 += 2 * kWeighRows) {
+      stage(r0, std::integral_constant<int, 0>{});
+      if (r0 + kWeighRows < rows) stage(r0 + kWeighRows, std::integral_constant<int, 1>{});
+    }
+    got = Plus32(got);
+    if (half == 0) {
+      if (stage0 > 0 || stage1 < stages) {
+        w.parts[axis.Slot(worker, x) * kWeighTile + wave * 32 + in32] = got;
+      } else if (mine != nullptr) {
+        const float was = p < old_end && w.decay != 0.0f ? *mine : 0.0f;
+        *mine = fmaf(w.decay, was, got);
       }
     }
+    x += stage1 - stage0;
     __syncthreads();  // the next tile's rows take this one's place in LDS
   }
+}
+
+// Adds up the parts of tiles that were cut, in order: a workgroup takes the tile that a
+// worker's start is in, if it is the first one in it.
+__global__ __launch_bounds__(kAttendThreads) void weigh_join_kernel(const WeighLaunch w) {
+  extern __shared__ int sums[];  // [sequences]
+  const AttendLaunch& a = w.attend;
+  const BatchView& b = a.batch;
+  WeighSums(w, sums);
+  const int work = sums[b.sequences - 1];
+  if (work == 0) return;
+  const Axis axis = WeighAxis(w, work);
+  constexpr int kTiles = kAttendThreads / kWeighTile;  // of a workgroup
+  const int cut = static_cast<int>(blockIdx.x) * kTiles + threadIdx.x / kWeighTile + 1;
+  if (cut >= axis.workers) return;
+  const int x = axis.Start(cut);
+  const int s = FirstAbove(sums, b.sequences, x / a.k_heads);
+  const int before = s > 0 ? sums[s - 1] : 0, per_head = sums[s] - before;
+  const int h = (x - before * a.k_heads) / per_head;
+  const int unit = before * a.k_heads + h * per_head;
+  const WeighUnit u = LoadWeighUnit(w, s);
+  const int tile = WeighTileAt(w, u, x - unit);
+  const int first = unit + WeighCost(w, u, tile), last = unit + WeighCost(w, u, tile + 1);
+  if (x == first || x - axis.each > first) return;
+  const int in_tile = threadIdx.x % kWeighTile;
+  float sum = 0.0f;
+  for (int n = axis.Owner(first); n <= axis.Owner(last - 1); ++n) {
+    const int slot = n < cut ? axis.Slot(n, first) : 2 * n;
+    sum += w.parts[slot * kWeighTile + in_tile];
+  }
+  const int p = u.begin + tile * kWeighTile + in_tile;
+  if (p >= u.end) return;
+  const int at = FastDivI(a.block_div, p), id = b.tables[s * b.table_stride + at];
+  if (id < 0 || id >= b.num_blocks) return;
+  float* mine = w.weights + (static_cast<int64_t>(id) * a.k_heads + h) * b.block_tokens +
+                (p - at * b.block_tokens);
+  *mine = fmaf(w.decay, p < u.old_end && w.decay != 0.0f ? *mine : 0.0f, sum);
 }
 
 template <class E, int POOL, int DP, int RT, bool FULL>
@@ -461,6 +600,12 @@ hipError_t Both(const WeighLaunch& l, hipStream_t stream) {
   e = AllowDynamicLds<kernel>(lds + 1024);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3(a.many_grid), dim3(kAttendThreads), lds, stream, l);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.many_grid == 1) return e;  // one worker cuts nothing
+  const int cuts = a.many_grid - 1, of_group = kAttendThreads / kWeighTile;
+  hipLaunchKernelGGL(weigh_join_kernel, dim3((cuts + of_group - 1) / of_group),
+                     dim3(kAttendThreads), static_cast<size_t>(a.batch.sequences) * sizeof(int),
+                     stream, l);
   return hipGetLastError();
 }
 
@@ -492,27 +637,29 @@ hipError_t PickPool(const WeighLaunch& l, hipStream_t stream) {
 
 }  // namespace
 
-void PlanWeigh(WeighLaunch* l) {
+int64_t PlanWeigh(WeighLaunch* l) {
   AttendLaunch& a = l->attend;
   const int64_t G = a.q_heads / a.k_heads, T = a.batch.tokens, S = a.batch.sequences;
   const int64_t capacity = std::max(a.batch.capacity, 1);
   const bool single = a.batch.starts == nullptr;
   a.padded_dim = PaddedDim(a.head_dim);
   constexpr int kCus = 256;
-  const int resident = (a.padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
   a.few_grid = a.few_rows = a.many_grid = 0;
   if (G <= kFewRows) {
     a.few_rows = static_cast<int>(single ? G : std::min<int64_t>(T * G, kFewRows));
     const int64_t steps = S * a.k_heads * ((capacity + kFewStep - 1) / kFewStep);
+    const int resident = (a.padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
     a.few_grid = static_cast<int>(std::min<int64_t>(resident, (steps + kWaves - 1) / kWaves));
   }
   if (single ? G > kFewRows : T * G > kFewRows) {
-    const int tile = WeighTile(a.padded_dim);
-    // Sequences with more than kFewRows rows there are at most T * G / kFewRows.
-    const int64_t many = std::min(S, T * G / kFewRows);
-    const int64_t tiles = many * a.k_heads * ((capacity + tile - 1) / tile);
-    a.many_grid = static_cast<int>(std::min<int64_t>(2 * kCus, tiles));
+    // Stages of the sequences with more than kFewRows rows (at most T * G / kFewRows).
+    const int64_t units = std::min(S, T * G / kFewRows);
+    const int64_t stages = (T * G + kWeighRows - 1) / kWeighRows + units;
+    const int64_t work = stages * a.k_heads * ((capacity + kWeighTile - 1) / kWeighTile);
+    a.many_grid = static_cast<int>(std::min<int64_t>(
+        (a.padded_dim > 128 ? 2 : 3) * kCus, std::max<int64_t>(work / kLeastStages, 1)));
   }
+  return 2ll * a.many_grid * kWeighTile * static_cast<int64_t>(sizeof(float));
 }
 
 hipError_t LaunchWeigh(const WeighLaunch& l, hipStream_t stream) {

@@ -16,7 +16,7 @@ from typing import Tuple
 from . import _capi, paged_attention as base
 from .kv_cache_manager import _stream_ptr
 
-_WEIGH = struct.Struct(base._CACHE + base._BATCH + "q2iQ2q2QqQi2fi")
+_WEIGH = struct.Struct(base._CACHE + base._BATCH + "q2iQ2q2QqQi2fiQq")
 _CHOOSE = struct.Struct("4iqQ" + base._BATCH + "3Q2q")
 _COMPACT = struct.Struct(base._CACHE + "Q3qQ4qQq")
 for _pack, _args in ((_WEIGH, _capi.WeighArgs), (_CHOOSE, _capi.ChooseKeptArgs),
@@ -75,9 +75,18 @@ def weigh(mgr, k_layer, q, tables, lengths, lse, weights, *, starts, begins, dec
     args = _capi.WeighArgs.from_buffer_copy(_WEIGH.pack(
         *cache, *batch, tokens, base._TYPES[q.dtype], q_heads, q_at, q_token, q_head,
         lse.data_ptr(), weights_at, table_blocks, _begins(begins, device, batch[5]), not causal,
-        dim ** -0.5 if scale is None else scale, decay, 0))
+        dim ** -0.5 if scale is None else scale, decay, 0, 0, 0))
+    lib = _capi.load()
+    if starts is not None or q_heads > 32 * cache[7]:  # single tokens need no workspace
+        need = ctypes.c_int64()
+        rc = lib.kvx_manager_weigh_workspace(mgr._h, args, need)
+        if rc:
+            _capi.check(rc, "KVCacheManager weigh")
+        if need.value:
+            workspace = base._empty(stream, q.device, need.value, torch.uint8)
+            args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
     handle = base._current_stream(device) if stream is None else _stream_ptr(stream)
-    rc = _capi.load().kvx_manager_weigh(mgr._h, args, handle)
+    rc = lib.kvx_manager_weigh(mgr._h, args, handle)
     if rc:
         _capi.check(rc, "KVCacheManager weigh")
 
