@@ -66,11 +66,11 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
   } else {
     KVX_RETURN_IF_ERROR(CheckSizes(a.batch, a.tokens, c.block_tokens, &l.batch));
   }
-  // Work is counted in 32 bits, for every head: steps of 32 tokens, and tiles of 128 by
+  // Work is counted in 32 bits, for every head: steps of 32 tokens, and tiles by
   // stages of 64 rows.
   const int64_t G = a.q_heads / c.heads;
   const int64_t few = a.batch.sequences * (l.batch.capacity / kFewStep + 1);
-  const int64_t tiles = l.batch.capacity / kWeighTile + 1;
+  const int64_t tiles = l.batch.capacity / WeighTile(PaddedDim(c.head_dim)) + 1;
   const int64_t stages = a.tokens * G / kWeighRows + 1 + a.batch.sequences;
   if (few > INT32_MAX / 2 / c.heads || stages > INT32_MAX / 2 / c.heads / tiles) {
     return Bad("tokens * table_width is too large for one call");

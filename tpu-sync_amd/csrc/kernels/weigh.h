@@ -14,11 +14,13 @@ struct WeighLaunch {
   float* weights = nullptr;         // [num_blocks][k_heads][block_tokens]
   const int32_t* begins = nullptr;  // [sequences]: first token weighed, or null: 0
   float decay = 1.0f;
-  // Sums of cut tiles: two slots of kWeighTile floats a worker.
+  // Sums of cut tiles: two slots of WeighTile floats a worker.
   float* parts = nullptr;
 };
 
-constexpr int kWeighTile = 128;  // tokens of a tile of the kernel for many rows
+// Tokens of a tile of the kernel for many rows: 64 for every wave, whose keys fill half
+// of its registers.
+constexpr int WeighTile(int padded_dim) { return padded_dim <= 128 ? 256 : 128; }
 constexpr int kWeighRows = 64;   // rows that they meet at once
 
 // Sizes of the launches of a call (from its shapes only). Returns the bytes of `parts`.

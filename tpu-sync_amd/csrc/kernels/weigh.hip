@@ -13,7 +13,7 @@
 // of the axis of all sequences' steps of 32 tokens; keys go from memory straight into
 // operands. Reading them bounds it.
 //
-// weigh_many (chunks): a workgroup takes kWeighTile tokens of one sequence and key
+// weigh_many (chunks): a workgroup takes WeighTile tokens of one sequence and key
 // head, keeps their keys in registers and goes through the rows that see them, 64 at a
 // time in LDS. The products and the exponentials (16 a lane for 8 products at D = 128)
 // bound it.
@@ -61,10 +61,9 @@ __device__ __forceinline__ int WeighSteps(const WeighKeys& k) {
   return (k.end - k.begin + kFewStep - 1) / kFewStep;
 }
 
+// `group`: number of the workgroup; sums: [sequences] in LDS.
 template <class E, int POOL, int DP, int RT, bool FULL>
-__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_kernel(
-    const WeighLaunch w) {
-  extern __shared__ int sums[];  // [sequences]
+__device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int group) {
   using Scalar = typename E::Scalar;
   using Pool = PoolLane<E, POOL, DP, FULL>;
   using Words = typename Pool::Words;
@@ -81,7 +80,7 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_k
   if (all == 0) return;
   const Axis axis = FewAxis(a, all);
   const int lane = threadIdx.x % 64;
-  const int worker = static_cast<int>(blockIdx.x) * kWaves + one(threadIdx.x / 64);
+  const int worker = group * kWaves + one(threadIdx.x / 64);
   if (worker >= axis.workers) return;
   const int x_end = axis.Start(worker + 1);
   const int in16 = lane % 16, quarter = lane / 16;
@@ -232,7 +231,7 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_k
   }
 }
 
-// -- Many rows: tiles of kWeighTile tokens of the sequences with more than kFewRows rows,
+// -- Many rows: tiles of WeighTile tokens of the sequences with more than kFewRows rows,
 // each of as many stages of kWeighRows rows as see it.
 
 struct WeighUnit {
@@ -240,47 +239,47 @@ struct WeighUnit {
   int begin, end;  // tokens
   int old_end;     // tokens that are not the call's own
   int tiles;
-  // Tiles that all rows see, of `stages` each; the others have 2 G less each than the
-  // one before, the first of them `later`.
-  int full, stages, later;
+  // Tiles that all rows see, of `stages` each; the others have `less` stages less each
+  // than the one before, the first of them `later`.
+  int full, stages, later, less;
 };
 
 __device__ __forceinline__ WeighUnit LoadWeighUnit(const WeighLaunch& w, int s) {
   const WeighKeys k = LoadWeighKeys(w, s);
-  const int G = w.attend.q_heads / w.attend.k_heads;
+  const int G = w.attend.q_heads / w.attend.k_heads, tile = WeighTile(w.attend.padded_dim);
   WeighUnit u;
+  u.less = tile / kWeighRows * G;
   u.rows = k.rows;
   u.begin = k.begin;
   u.end = k.end;
   u.old_end = k.q.length - k.q.count;
-  u.tiles = k.rows > kFewRows ? (k.end - k.begin + kWeighTile - 1) / kWeighTile : 0;
+  u.tiles = k.rows > kFewRows ? (k.end - k.begin + tile - 1) / tile : 0;
   u.stages = (k.rows + kWeighRows - 1) / kWeighRows;
   u.full = u.tiles;
   u.later = 0;
   if (w.attend.causal) {
-    u.full = u.old_end < u.begin ? 0 : min((u.old_end - u.begin) / kWeighTile + 1, u.tiles);
+    u.full = u.old_end < u.begin ? 0 : min((u.old_end - u.begin) / tile + 1, u.tiles);
     // The first token of the next tile is so many behind the first of the call's own.
-    const int behind = u.begin + u.full * kWeighTile - u.old_end;
+    const int behind = u.begin + u.full * tile - u.old_end;
     u.later = u.full < u.tiles ? u.stages - behind * G / kWeighRows : 0;
   }
   return u;
 }
 
 // Where tile i starts on its sequence's and head's axis.
-__device__ __forceinline__ int WeighCost(const WeighLaunch& w, const WeighUnit& u, int i) {
+__device__ __forceinline__ int WeighCost(const WeighUnit& u, int i) {
   if (i <= u.full) return i * u.stages;
   const int n = i - u.full;
-  static_assert(kWeighTile == 2 * kWeighRows, "2 G stages a tile");
-  return u.full * u.stages + n * u.later - n * (n - 1) * (w.attend.q_heads / w.attend.k_heads);
+  return u.full * u.stages + n * u.later - n * (n - 1) / 2 * u.less;
 }
 
 // The tile that holds `at`.
-__device__ __forceinline__ int WeighTileAt(const WeighLaunch& w, const WeighUnit& u, int at) {
+__device__ __forceinline__ int WeighTileAt(const WeighUnit& u, int at) {
   if (at < u.full * u.stages) return at / u.stages;
   int tile = u.full, tiles = u.tiles;
   while (tiles - tile > 1) {
     const int mid = (tile + tiles) / 2;
-    if (WeighCost(w, u, mid) <= at) {
+    if (WeighCost(u, mid) <= at) {
       tile = mid;
     } else {
       tiles = mid;
@@ -293,7 +292,7 @@ __device__ __forceinline__ int WeighTileAt(const WeighLaunch& w, const WeighUnit
 __device__ __forceinline__ void WeighSums(const WeighLaunch& w, int* sums) {
   for (int s = threadIdx.x; s < w.attend.batch.sequences; s += kAttendThreads) {
     const WeighUnit u = LoadWeighUnit(w, s);
-    sums[s] = WeighCost(w, u, u.tiles);
+    sums[s] = WeighCost(u, u.tiles);
   }
   BlockSums(sums, w.attend.batch.sequences, w.attend.most_many);
 }
@@ -306,14 +305,14 @@ __device__ __forceinline__ Axis WeighAxis(const WeighLaunch& w, int work) {
 }
 
 constexpr int kAhead = 4;  // products that operands are read ahead
+constexpr int WeighGroups(int padded_dim) { return padded_dim <= 64 ? 3 : 2; }  // of a CU
 
 template <class E, int POOL, int DP>
-__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_kernel(
-    const WeighLaunch w) {
-  extern __shared__ __align__(16) char lds[];
+__device__ __forceinline__ void WeighMany(const WeighLaunch& w, char* lds, int place) {
   using Scalar = typename E::Scalar;
   constexpr bool E4 = POOL == kPoolE4m3, F4 = POOL == kPoolFp4;
-  constexpr int KS = DP / 16, kRow = 2 * DP;
+  constexpr int KS = DP / 16, kRow = 2 * DP, kTile = WeighTile(DP);
+  constexpr int CT = kTile / 128;    // 32s of tokens of a wave
   constexpr int kChunks = DP / 32;  // of a thread: every fourth of a row
   static_assert(kWeighRows * 4 == kAttendThreads);
   struct Rows {
@@ -331,7 +330,7 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
   const Axis axis = WeighAxis(w, work);
   // The workgroups of one XCD take neighbouring parts, so its L2 serves a head's rows to
   // all of them.
-  const int worker = WorkerAt(blockIdx.x, axis.workers);
+  const int worker = WorkerAt(place, axis.workers);
   if (worker < 0) return;
   const int x_end = axis.Start(worker + 1);
   const int lane = threadIdx.x % 64, wave = one(threadIdx.x / 64);
@@ -352,23 +351,24 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
     const int h = (x - before * a.k_heads) / per_head;
     const int at_unit = x - before * a.k_heads - h * per_head;
     const WeighUnit u = LoadWeighUnit(w, s);
-    const int tile = one(WeighTileAt(w, u, at_unit));
-    const int tile_at = one(WeighCost(w, u, tile));
-    const int stages = one(WeighCost(w, u, tile + 1)) - tile_at;
+    const int tile = one(WeighTileAt(u, at_unit));
+    const int tile_at = one(WeighCost(u, tile));
+    const int stages = one(WeighCost(u, tile + 1)) - tile_at;
     // The part's stages: the last of them end with the last row.
     const int stage0 = at_unit - tile_at, stage1 = min(stages, stage0 + (x_end - x));
     const int end = one(u.end), old_end = one(u.old_end);
     const int row0 = (one(u.stages) - stages + stage0) * kWeighRows;
     const int rows = min(one(u.rows), row0 + (stage1 - stage0) * kWeighRows);
     const SequenceSpan span = LoadSequence(b, s);
-    const int j0 = one(u.begin) + tile * kWeighTile;
+    const int j0 = one(u.begin) + tile * kTile + wave * (CT * 32);  // the wave's
 
-    // Keys: token l % 32 of the wave's, as an operand.
-    const int p = j0 + wave * 32 + in32;
-    u32x4 key[KS];
-    float factor = c;
-    float* mine;
-    {
+    // Keys: token l % 32 of each of the wave's 32s, as an operand.
+    u32x4 key[CT][KS];
+    float factor[CT];
+    float* mine[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int p = j0 + ct * 32 + in32;
       const int at = FastDivI(a.block_div, p), slot = p - at * b.block_tokens;
       const int id = p < end ? b.tables[s * b.table_stride + at] : -1;
       const bool has = id >= 0 && id < b.num_blocks;
@@ -376,26 +376,29 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
       // Places in layouts with a head's tokens together, and with a token's heads.
       const int64_t by_head = (of_block * a.k_heads + h) * b.block_tokens + (has ? slot : 0);
       const int64_t by_token = (of_block * b.block_tokens + (has ? slot : 0)) * a.k_heads + h;
-      mine = has ? w.weights + by_head : nullptr;
-      if constexpr (E4) factor *= static_cast<const float*>(a.k_scales)[of_block * a.k_heads + h];
+      mine[ct] = has ? w.weights + by_head : nullptr;
+      factor[ct] = c;
+      if constexpr (E4) {
+        factor[ct] *= static_cast<const float*>(a.k_scales)[of_block * a.k_heads + h];
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d = ks * 16 + half * 8;
-        key[ks] = u32x4{0, 0, 0, 0};
+        key[ct][ks] = u32x4{0, 0, 0, 0};
         if (!has || d >= a.head_dim) continue;
         if constexpr (F4) {
           const uint32_t code = static_cast<const uint8_t*>(
               a.k_scales)[by_head * (a.head_dim / kFp4Group) + d / kFp4Group];
-          key[ks] = FromFp4<E>(
+          key[ct][ks] = FromFp4<E>(
               *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.k_pool) +
                                                  by_head * (a.head_dim / 2) + d / 2),
               Fp4Scale<E>(code));
         } else if constexpr (E4) {
-          key[ks] = Widen<E>(*reinterpret_cast<const Bytes8*>(
+          key[ct][ks] = Widen<E>(*reinterpret_cast<const Bytes8*>(
               static_cast<const uint8_t*>(a.k_pool) + by_token * a.head_dim + d));
         } else {
-          key[ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) +
-                                                      by_token * a.head_dim + d);
+          key[ct][ks] = *reinterpret_cast<const Bytes16*>(static_cast<const Scalar*>(a.k_pool) +
+                                                          by_token * a.head_dim + d);
         }
       }
     }
@@ -448,43 +451,61 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
       }
     };
 
-    float got = 0.0f;
+    float got[CT] = {};
     // The last token of the wave that counts: rows that see it see all of them.
-    const int last = min(j0 + wave * 32 + 32, end);
-    // Scores of 32 rows of a stage. Lane: token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4.
-    const auto scores = [&](auto buffer, auto rt) {
-      const char* at = lds + buffer() * (kWeighRows * kRow) + rt() * 32 * kRow;
-      f32x16 sc = f32x16(0.0f);
+    const int last = min(j0 + CT * 32, end);
+    // 32 rows of a stage. Lane: token l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4.
+    const auto tile_of = [&](auto buffer, int rt, bool plain) {
+      const char* at = lds + buffer() * (kWeighRows * kRow) + rt * 32 * kRow;
+      const Rows& here = row_data[buffer()];
+      const int r = rt * 32 + half * 4;
+      f32x16 sc[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) sc[ct] = f32x16(0.0f);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        sc = Mma32<E>(*reinterpret_cast<const u32x4*>(at + row_at[ks]), key[ks], sc);
+        const u32x4 row = *reinterpret_cast<const u32x4*>(at + row_at[ks]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sc[ct] = Mma32<E>(row, key[ct][ks], sc[ct]);
       }
-      return sc;
-    };
-    const auto raise = [&](auto buffer, auto rt, f32x16& sc) {
-      const float* base = &row_data[buffer()].base[rt() * 32 + half * 4];
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const f32x4 of = *reinterpret_cast<const f32x4*>(base + i * 2);
+        const f32x4 base = *reinterpret_cast<const f32x4*>(&here.base[r + i * 2]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sc[i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i + j], factor, -of[j]));
+        for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[ct][i + j] = __builtin_amdgcn_exp2f(fmaf(sc[ct][i + j], factor[ct], -base[j]));
+          }
         }
       }
-    };
-    const auto add = [&](auto buffer, auto rt, f32x16& sc, bool plain) {
+      // Operands are read ahead of their products.
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int n = 0; n < KS; ++n) {
+        __builtin_amdgcn_sched_group_barrier(0x8, CT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
       if (!plain) {
-        const int* seen = &row_data[buffer()].seen[rt() * 32 + half * 4];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (p >= seen[i / 4 * 8 + i % 4]) sc[i] = 0.0f;
+          const int seen = here.seen[r + i / 4 * 8 + i % 4];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            if (j0 + ct * 32 + in32 >= seen) sc[ct][i] = 0.0f;
+          }
         }
       }
       // Sums of 16 first: thousands of rows lose less so.
-      float some[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) some[j] = (sc[j] + sc[4 + j]) + (sc[8 + j] + sc[12 + j]);
-      got += (some[0] + some[1]) + (some[2] + some[3]);
+      for (int ct = 0; ct < CT; ++ct) {
+        float some[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          some[j] = (sc[ct][j] + sc[ct][4 + j]) + (sc[ct][8 + j] + sc[ct][12 + j]);
+        }
+        got[ct] += (some[0] + some[1]) + (some[2] + some[3]);
+      }
     };
     const auto stage = [&](int r0, auto buffer) {
       store(buffer);
@@ -492,29 +513,8 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
       if (r0 + kWeighRows < rows) load(r0 + kWeighRows);
       const bool plain = r0 + kWeighRows <= rows &&
                          Visible(a, span, span.first + FastDivI(a.group_div, r0)) >= last;
-      constexpr std::integral_constant<int, 0> kFirst{};
-      constexpr std::integral_constant<int, 1> kSecond{};
-      // The second rows' products beside the first ones' exponentials.
-      __builtin_amdgcn_sched_barrier(0);
-      f32x16 sc = scores(buffer, kFirst);
-      f32x16 next = scores(buffer, kSecond);
-      raise(buffer, kFirst, sc);
-      raise(buffer, kSecond, next);
-      // Operands are read kAhead products ahead.
-      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-      for (int n = 0; n < KS; ++n) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-#pragma unroll
-      for (int n = 0; n < KS; ++n) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 32 / KS, 0);
-      }
-      add(buffer, kFirst, sc, plain);
-      add(buffer, kSecond, next, plain);
+      for (int rt = 0; rt < kWeighRows / 32; ++rt) tile_of(buffer, rt, plain);
     };
     load(row0);
     // (A buffer's readers are past the barrier of the stage in between.)
@@ -522,13 +522,16 @@ __global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 2) void weigh_many_
       stage(r0, std::integral_constant<int, 0>{});
       if (r0 + kWeighRows < rows) stage(r0 + kWeighRows, std::integral_constant<int, 1>{});
     }
-    got = Plus32(got);
-    if (half == 0) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float sum = Plus32(got[ct]);
+      if (half != 0) continue;
       if (stage0 > 0 || stage1 < stages) {
-        w.parts[axis.Slot(worker, x) * kWeighTile + wave * 32 + in32] = got;
-      } else if (mine != nullptr) {
-        const float was = p < old_end && w.decay != 0.0f ? *mine : 0.0f;
-        *mine = fmaf(w.decay, was, got);
+        w.parts[axis.Slot(worker, x) * kTile + (wave * CT + ct) * 32 + in32] = sum;
+      } else if (mine[ct] != nullptr) {
+        const float was =
+            j0 + ct * 32 + in32 < old_end && w.decay != 0.0f ? *mine[ct] : 0.0f;
+        *mine[ct] = fmaf(w.decay, was, sum);
       }
     }
     x += stage1 - stage0;
@@ -546,31 +549,50 @@ __global__ __launch_bounds__(kAttendThreads) void weigh_join_kernel(const WeighL
   const int work = sums[b.sequences - 1];
   if (work == 0) return;
   const Axis axis = WeighAxis(w, work);
-  constexpr int kTiles = kAttendThreads / kWeighTile;  // of a workgroup
-  const int cut = static_cast<int>(blockIdx.x) * kTiles + threadIdx.x / kWeighTile + 1;
-  if (cut >= axis.workers) return;
+  const int tokens = WeighTile(a.padded_dim), in_tile = threadIdx.x;
+  const int cut = static_cast<int>(blockIdx.x) + 1;
+  if (cut >= axis.workers || in_tile >= tokens) return;
   const int x = axis.Start(cut);
   const int s = FirstAbove(sums, b.sequences, x / a.k_heads);
   const int before = s > 0 ? sums[s - 1] : 0, per_head = sums[s] - before;
   const int h = (x - before * a.k_heads) / per_head;
   const int unit = before * a.k_heads + h * per_head;
   const WeighUnit u = LoadWeighUnit(w, s);
-  const int tile = WeighTileAt(w, u, x - unit);
-  const int first = unit + WeighCost(w, u, tile), last = unit + WeighCost(w, u, tile + 1);
+  const int tile = WeighTileAt(u, x - unit);
+  const int first = unit + WeighCost(u, tile), last = unit + WeighCost(u, tile + 1);
   if (x == first || x - axis.each > first) return;
-  const int in_tile = threadIdx.x % kWeighTile;
   float sum = 0.0f;
   for (int n = axis.Owner(first); n <= axis.Owner(last - 1); ++n) {
     const int slot = n < cut ? axis.Slot(n, first) : 2 * n;
-    sum += w.parts[slot * kWeighTile + in_tile];
+    sum += w.parts[slot * tokens + in_tile];
   }
-  const int p = u.begin + tile * kWeighTile + in_tile;
+  const int p = u.begin + tile * tokens + in_tile;
   if (p >= u.end) return;
   const int at = FastDivI(a.block_div, p), id = b.tables[s * b.table_stride + at];
   if (id < 0 || id >= b.num_blocks) return;
   float* mine = w.weights + (static_cast<int64_t>(id) * a.k_heads + h) * b.block_tokens +
                 (p - at * b.block_tokens);
   *mine = fmaf(w.decay, p < u.old_end && w.decay != 0.0f ? *mine : 0.0f, sum);
+}
+
+template <class E, int POOL, int DP, int RT, bool FULL>
+__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_kernel(
+    const WeighLaunch w) {
+  extern __shared__ int sums[];
+  WeighFew<E, POOL, DP, RT, FULL>(w, sums, blockIdx.x);
+}
+
+// Chunks, and what few rows there are beside them.
+template <class E, int POOL, int DP, bool FULL>
+__global__ __launch_bounds__(kAttendThreads, WeighGroups(DP)) void weigh_mixed_kernel(
+    const WeighLaunch w) {
+  extern __shared__ __align__(16) char lds[];
+  const int place = static_cast<int>(blockIdx.x);
+  if (place < w.attend.many_grid) {
+    WeighMany<E, POOL, DP>(w, lds, place);
+  } else {
+    WeighFew<E, POOL, DP, 2, FULL>(w, reinterpret_cast<int*>(lds), place - w.attend.many_grid);
+  }
 }
 
 template <class E, int POOL, int DP, int RT, bool FULL>
@@ -581,32 +603,32 @@ hipError_t Few(const WeighLaunch& l, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <class E, int POOL, int DP, bool FULL>
+hipError_t Mixed(const WeighLaunch& l, hipStream_t stream) {
+  const AttendLaunch& a = l.attend;
+  const size_t lds = 2 * kWeighRows * (2 * DP + 8) +
+                     static_cast<size_t>(a.batch.sequences) * sizeof(int);
+  constexpr auto kernel = weigh_mixed_kernel<E, POOL, DP, FULL>;
+  hipError_t e = AllowDynamicLds<kernel>(lds + 1024);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3(a.many_grid + a.few_grid), dim3(kAttendThreads), lds, stream, l);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.many_grid == 1) return e;  // one worker cuts nothing
+  hipLaunchKernelGGL(weigh_join_kernel, dim3(a.many_grid - 1), dim3(kAttendThreads),
+                     static_cast<size_t>(a.batch.sequences) * sizeof(int), stream, l);
+  return hipGetLastError();
+}
+
 template <class E, int POOL, int DP>
 hipError_t Both(const WeighLaunch& l, hipStream_t stream) {
   const AttendLaunch& a = l.attend;
-  hipError_t e = hipSuccess;
-  if (a.few_grid > 0) {
-    if (a.head_dim != DP) {
-      e = Few<E, POOL, DP, 2, false>(l, stream);
-    } else {
-      e = a.few_rows <= 16 ? Few<E, POOL, DP, 1, true>(l, stream)
-                           : Few<E, POOL, DP, 2, true>(l, stream);
-    }
+  const bool full = a.head_dim == DP;
+  if (a.many_grid > 0) {
+    return full ? Mixed<E, POOL, DP, true>(l, stream) : Mixed<E, POOL, DP, false>(l, stream);
   }
-  if (e != hipSuccess || a.many_grid == 0) return e;
-  const size_t lds = 2 * kWeighRows * (2 * DP + 8) +
-                     static_cast<size_t>(a.batch.sequences) * sizeof(int);
-  constexpr auto kernel = weigh_many_kernel<E, POOL, DP>;
-  e = AllowDynamicLds<kernel>(lds + 1024);
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3(a.many_grid), dim3(kAttendThreads), lds, stream, l);
-  e = hipGetLastError();
-  if (e != hipSuccess || a.many_grid == 1) return e;  // one worker cuts nothing
-  const int cuts = a.many_grid - 1, of_group = kAttendThreads / kWeighTile;
-  hipLaunchKernelGGL(weigh_join_kernel, dim3((cuts + of_group - 1) / of_group),
-                     dim3(kAttendThreads), static_cast<size_t>(a.batch.sequences) * sizeof(int),
-                     stream, l);
-  return hipGetLastError();
+  if (!full) return Few<E, POOL, DP, 2, false>(l, stream);
+  return a.few_rows <= 16 ? Few<E, POOL, DP, 1, true>(l, stream)
+                          : Few<E, POOL, DP, 2, true>(l, stream);
 }
 
 template <class E, int POOL>
@@ -652,14 +674,15 @@ int64_t PlanWeigh(WeighLaunch* l) {
     a.few_grid = static_cast<int>(std::min<int64_t>(resident, (steps + kWaves - 1) / kWaves));
   }
   if (single ? G > kFewRows : T * G > kFewRows) {
+    const int tile = WeighTile(a.padded_dim);
     // Stages of the sequences with more than kFewRows rows (at most T * G / kFewRows).
     const int64_t units = std::min(S, T * G / kFewRows);
     const int64_t stages = (T * G + kWeighRows - 1) / kWeighRows + units;
-    const int64_t work = stages * a.k_heads * ((capacity + kWeighTile - 1) / kWeighTile);
+    const int64_t work = stages * a.k_heads * ((capacity + tile - 1) / tile);
     a.many_grid = static_cast<int>(std::min<int64_t>(
-        (a.padded_dim > 128 ? 2 : 3) * kCus, std::max<int64_t>(work / kLeastStages, 1)));
+        WeighGroups(a.padded_dim) * kCus, std::max<int64_t>(work / kLeastStages, 1)));
   }
-  return 2ll * a.many_grid * kWeighTile * static_cast<int64_t>(sizeof(float));
+  return 2ll * a.many_grid * WeighTile(a.padded_dim) * static_cast<int64_t>(sizeof(float));
 }
 
 hipError_t LaunchWeigh(const WeighLaunch& l, hipStream_t stream) {
