@@ -27,6 +27,11 @@
 namespace kvx {
 namespace {
 
+// Workgroups of a CU with few rows.
+constexpr int WeighFewGroups(int padded_dim, int row_tiles, bool full) {
+  return padded_dim > 128 ? 1 : row_tiles == 1 && full ? 4 : 2;
+}
+
 struct WeighKeys {
   SequenceSpan q;
   int rows, begin, end;
@@ -142,24 +147,26 @@ __device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int gr
       }
     };
     int64_t at[2];
-    // The weight of the lane's own token: 16 (l / 16) + l % 16 of the step, l < 32.
-    float* mine = nullptr;
+    // The weight of the lane's own token: 16 (l / 16) + l % 16 of the step, l < 32. The
+    // load needs no branch: what has no weight yet reads some, and does not use it.
+    int64_t mine = 0;
+    bool writes = false, adds = false;
     float held = 0.0f;
     const auto place = [&](int step, const int (&id)[2]) {
+      int64_t to[2];
+      bool has[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int p = begin + step * kFewStep + u * 16 + in16;
         const int slot = p - FastDivI(a.block_div, p) * b.block_tokens;
-        const bool has = id[u] >= 0 && id[u] < b.num_blocks;
-        at[u] = pool.At(id[u], slot, has);
-        if (quarter == u) {
-          mine = has ? w.weights + (static_cast<int64_t>(id[u]) * a.k_heads + h) * b.block_tokens +
-                           slot
-                     : nullptr;
-          held = 0.0f;
-          if (has && p < old_end && w.decay != 0.0f) held = *mine;
-        }
+        has[u] = id[u] >= 0 && id[u] < b.num_blocks;
+        at[u] = pool.At(id[u], slot, has[u]);
+        to[u] = has[u] ? (static_cast<int64_t>(id[u]) * a.k_heads + h) * b.block_tokens + slot : 0;
       }
+      mine = quarter == 1 ? to[1] : to[0];
+      writes = quarter < 2 && (quarter == 1 ? has[1] : has[0]);
+      adds = w.decay != 0.0f && begin + step * kFewStep + quarter * 16 + in16 < old_end;
+      held = w.weights[mine];
     };
     Words kw[2][KS];
     float kf[2] = {1, 1};
@@ -204,8 +211,9 @@ __device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int gr
           for (int rt = 0; rt < RT; ++rt) sc[rt][u] = Mma16<E>(q[rt][ks], key, sc[rt][u]);
         }
       }
-      float* const to = mine;
-      const float was = held;
+      const int64_t to = mine;
+      const bool writes_now = writes;
+      const float was = adds ? held : 0.0f;
       id_now[0] = id[0];
       id_now[1] = id[1];
       place(step + 1, id_now);
@@ -225,7 +233,7 @@ __device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int gr
         }
         got[u] = Plus32(Plus16(got[u]));
       }
-      if (quarter < 2 && to != nullptr) *to = fmaf(w.decay, was, quarter == 0 ? got[0] : got[1]);
+      if (writes_now) w.weights[to] = fmaf(w.decay, was, quarter == 0 ? got[0] : got[1]);
     }
     x += step1 - step0;
   }
@@ -298,7 +306,7 @@ __device__ __forceinline__ void WeighSums(const WeighLaunch& w, int* sums) {
 }
 
 // A worker's least part, in stages.
-constexpr int kLeastStages = 4;
+constexpr int kLeastStages = 1;
 __device__ __forceinline__ Axis WeighAxis(const WeighLaunch& w, int work) {
   const int total = work * w.attend.k_heads;
   return Axis(total, min(w.attend.many_grid, max(total / kLeastStages, 1)));
@@ -576,22 +584,25 @@ __global__ __launch_bounds__(kAttendThreads) void weigh_join_kernel(const WeighL
 }
 
 template <class E, int POOL, int DP, int RT, bool FULL>
-__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void weigh_few_kernel(
+__global__ __launch_bounds__(kAttendThreads, WeighFewGroups(DP, RT, FULL)) void weigh_few_kernel(
     const WeighLaunch w) {
   extern __shared__ int sums[];
   WeighFew<E, POOL, DP, RT, FULL>(w, sums, blockIdx.x);
 }
+
+// Places that WorkerAt needs for the workers of a grid.
+__host__ __device__ inline int Places(int grid) { return (grid + kXcds - 1) / kXcds * kXcds; }
 
 // Chunks, and what few rows there are beside them.
 template <class E, int POOL, int DP, bool FULL>
 __global__ __launch_bounds__(kAttendThreads, WeighGroups(DP)) void weigh_mixed_kernel(
     const WeighLaunch w) {
   extern __shared__ __align__(16) char lds[];
-  const int place = static_cast<int>(blockIdx.x);
-  if (place < w.attend.many_grid) {
+  const int place = static_cast<int>(blockIdx.x), many = Places(w.attend.many_grid);
+  if (place < many) {
     WeighMany<E, POOL, DP>(w, lds, place);
   } else {
-    WeighFew<E, POOL, DP, 2, FULL>(w, reinterpret_cast<int*>(lds), place - w.attend.many_grid);
+    WeighFew<E, POOL, DP, 2, FULL>(w, reinterpret_cast<int*>(lds), place - many);
   }
 }
 
@@ -611,7 +622,7 @@ hipError_t Mixed(const WeighLaunch& l, hipStream_t stream) {
   constexpr auto kernel = weigh_mixed_kernel<E, POOL, DP, FULL>;
   hipError_t e = AllowDynamicLds<kernel>(lds + 1024);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3(a.many_grid + a.few_grid), dim3(kAttendThreads), lds, stream, l);
+  hipLaunchKernelGGL(kernel, dim3(Places(a.many_grid) + a.few_grid), dim3(kAttendThreads), lds, stream, l);
   e = hipGetLastError();
   if (e != hipSuccess || a.many_grid == 1) return e;  // one worker cuts nothing
   hipLaunchKernelGGL(weigh_join_kernel, dim3(a.many_grid - 1), dim3(kAttendThreads),
@@ -670,7 +681,8 @@ int64_t PlanWeigh(WeighLaunch* l) {
   if (G <= kFewRows) {
     a.few_rows = static_cast<int>(single ? G : std::min<int64_t>(T * G, kFewRows));
     const int64_t steps = S * a.k_heads * ((capacity + kFewStep - 1) / kFewStep);
-    const int resident = (a.padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
+    const int resident = kCus * WeighFewGroups(a.padded_dim, a.few_rows <= 16 ? 1 : 2,
+                                               a.head_dim == a.padded_dim);
     a.few_grid = static_cast<int>(std::min<int64_t>(resident, (steps + kWaves - 1) / kWaves));
   }
   if (single ? G > kFewRows : T * G > kFewRows) {
