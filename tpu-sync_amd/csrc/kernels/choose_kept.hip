@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kWavesHere = kChooseThreads / 64;
 constexpr int kBins = 2048;
+constexpr int kAtOnce = 4;  // loads that a thread has on the way
 // Numbers held in LDS: what its 160 KiB leave beside the histogram.
 constexpr int kHeldMost = 36864;
 
@@ -33,6 +34,7 @@ __device__ __forceinline__ uint32_t Ordered(float x) {
   return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
 
+template <int VEC>
 __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const ChooseLaunch a,
                                                                      const int held_most) {
   extern __shared__ uint32_t held[];  // [held_most]
@@ -61,14 +63,45 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
   if (wanted == 0) return;
   const int count = length - recent - first;  // above `wanted`
   const int32_t* table = b.tables + s * b.table_stride;
-  const bool holds = count <= held_most;
-  const auto load = [&](int i) {
+  // The range in whole groups of VEC tokens, which a block holds.
+  const int base = first / VEC * VEC;
+  const int span = (first + count - base + VEC - 1) / VEC * VEC;
+  const bool holds = span <= held_most;
+  // Numbers of neighbouring tokens, VEC from place i0 of the range on and again every VEC
+  // kChooseThreads (0 behind the last): all of their blocks, then all of their weights on
+  // the way at once.
+  const auto load = [&](int i0, uint32_t (&u)[kAtOnce][VEC]) {
+    int id[kAtOnce], slot[kAtOnce];
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const int p = base + min(i0 + n * (VEC * kChooseThreads), span - VEC);
+      const int at = FastDivI(a.block_div, p);
+      id[n] = table[at];
+      slot[n] = p - at * b.block_tokens;
+    }
+    using Weights = __attribute__((ext_vector_type(VEC))) float;
+    Weights w[kAtOnce];
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const bool has = id[n] >= 0 && id[n] < b.num_blocks;
+      w[n] = *reinterpret_cast<const Weights*>(
+          a.weights + (static_cast<int64_t>(has ? id[n] : 0) * a.heads + h) * b.block_tokens +
+          slot[n]);
+      if (!has) id[n] = -1;
+    }
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) u[n][j] = id[n] >= 0 ? Ordered(w[n][j]) : 0u;
+    }
+  };
+  const auto number = [&](int i) {
+    if (holds) return held[first - base + i];
     const int p = first + i, at = FastDivI(a.block_div, p), id = table[at];
     if (id < 0 || id >= b.num_blocks) return 0u;
     return Ordered(a.weights[(static_cast<int64_t>(id) * a.heads + h) * b.block_tokens +
                              (p - at * b.block_tokens)]);
   };
-  const auto number = [&](int i) { return holds ? held[i] : load(i); };
 
   // Digits of the number that is the wanted-th largest.
   uint32_t digits = 0;
@@ -78,16 +111,27 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
     for (int i = threadIdx.x; i < kBins; i += kChooseThreads) bins[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < count; i += kChooseThreads) {
-      uint32_t u;
-      if (pass == 0) {
-        u = load(i);
-        if (holds) held[i] = u;
-      } else {
-        u = number(i);
-        if (((u ^ digits) >> (pass == 1 ? 21 : 10)) != 0) continue;
-      }
+    const auto note = [&](uint32_t u) {
+      if (pass > 0 && ((u ^ digits) >> (pass == 1 ? 21 : 10)) != 0) return;
       atomicAdd(&bins[u >> shift & mask], 1);
+    };
+    if (pass > 0 && holds) {
+      for (int i = threadIdx.x; i < count; i += kChooseThreads) note(held[first - base + i]);
+    } else {
+      for (int i0 = threadIdx.x * VEC; i0 < span; i0 += kAtOnce * VEC * kChooseThreads) {
+        uint32_t u[kAtOnce][VEC];
+        load(i0, u);
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int i = i0 + n * (VEC * kChooseThreads);
+          if (i >= span) break;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            if (holds) held[i + j] = u[n][j];
+            if (VEC == 1 || (i + j >= first - base && i + j < first - base + count)) note(u[n][j]);
+          }
+        }
+      }
     }
     __syncthreads();
     // Counts from the top: thread t has bins from the top 2t and 2t + 1.
@@ -102,7 +146,8 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
     if (lane == 63) wave_sums[wave] = sum;
     __syncthreads();
     int before = above + sum - n0 - n1;
-    for (int w = 0; w < wave; ++w) before += wave_sums[w];
+#pragma unroll
+    for (int w = 0; w < kWavesHere; ++w) before += w < wave ? wave_sums[w] : 0;
     if (before < wanted && before + n0 >= wanted) {
       found_bin = top;
       found_above = before;
@@ -130,9 +175,10 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
   }
   __syncthreads();
   more = equal = 0;
-  for (int w = 0; w < wave; ++w) {
-    more += wave_more[w];
-    equal += wave_sums[w];
+#pragma unroll
+  for (int w = 0; w < kWavesHere; ++w) {
+    more += w < wave ? wave_more[w] : 0;
+    equal += w < wave ? wave_sums[w] : 0;
   }
   const int of_equal = wanted - above;  // so many of those that equal it stay
   const uint64_t below = (uint64_t{1} << lane) - 1;
@@ -153,12 +199,17 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
 }  // namespace
 
 hipError_t LaunchChooseKept(const ChooseLaunch& l, hipStream_t stream) {
-  const int held = std::min(l.batch.capacity, kHeldMost);
+  // Four weights at a time where blocks hold whole fours.
+  const bool fours = l.batch.block_tokens % 4 == 0 && reinterpret_cast<uintptr_t>(l.weights) % 16 == 0;
+  const int held = std::min((l.batch.capacity + 3) / 4 * 4, kHeldMost);
   const size_t lds = static_cast<size_t>(held) * sizeof(uint32_t);
-  const hipError_t e = AllowDynamicLds<choose_kept_kernel>(lds + kBins * sizeof(int) + 1024);
+  constexpr auto by_four = choose_kept_kernel<4>, by_one = choose_kept_kernel<1>;
+  // (The limit counts the kernel's own arrays too.)
+  const size_t all = lds + kBins * sizeof(int) + 1024;
+  const hipError_t e = fours ? AllowDynamicLds<by_four>(all) : AllowDynamicLds<by_one>(all);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(choose_kept_kernel, dim3(l.batch.sequences * l.heads), dim3(kChooseThreads),
-                     lds, stream, l, held);
+  hipLaunchKernelGGL(fours ? by_four : by_one, dim3(l.batch.sequences * l.heads),
+                     dim3(kChooseThreads), lds, stream, l, held);
   return hipGetLastError();
 }
 

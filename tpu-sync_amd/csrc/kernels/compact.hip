@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_kernel(const CompactLaunc
 
 // -- e4m3
 
-constexpr int kScaledRows = 128;  // of a round
+constexpr int kScaledRows = 256;  // of a round
 
 __device__ __forceinline__ uint32_t Rescaled(uint32_t w, float ratio) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
@@ -175,23 +175,49 @@ __device__ __forceinline__ uint32_t Rescaled(uint32_t w, float ratio) {
   return static_cast<uint32_t>(q);
 }
 
-__global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const CompactLaunch a) {
-  // Per block of a group: the new scale's bits, and whether a row moves.
-  __shared__ uint32_t largest[kScaledRows];
-  __shared__ int moves[kScaledRows];
-  __shared__ int64_t from[kScaledRows], to[kScaledRows];
-  __shared__ float ratios[kScaledRows];
-  constexpr int kPieces = kScaledRows * (kMaxHeadDim / 8) / kThreads;  // of a thread
+// WIDE: rows are whole 16 bytes.
+template <int DP, bool WIDE>
+__global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
+    const CompactLaunch a) {
+  // Rounds in turn, four at a time. Of a row: where it is and goes, its scale, its place
+  // in `largest`. Of a block: the new scale's bits, and whether one of its rows moves.
+  constexpr int kSlots = 4;
+  using Piece = std::conditional_t<WIDE, u32x4, u32x2>;
+  using Bytes = Piece __attribute__((aligned(1)));
+  constexpr int kPiece = sizeof(Piece);
+  __shared__ int64_t from[kSlots][kScaledRows], to[kSlots][kScaledRows];
+  __shared__ float factors[2][kScaledRows];  // what a row's codes are multiplied with, 0: stays
+  __shared__ float old_scale[kSlots][kScaledRows];
+  __shared__ uint32_t largest[kSlots][kScaledRows];
+  __shared__ int moves[kSlots][kScaledRows];
+  constexpr int kPieces = kScaledRows * (DP / kPiece) / kThreads;  // of a thread
+  static_assert(kScaledRows == kThreads);
   const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
   const bool key = blockIdx.y == 0;
   uint8_t* pool = static_cast<uint8_t*>(key ? a.k_pool : a.v_pool);
   float* scales = static_cast<float*>(key ? a.k_scales : a.v_scales);
   const int32_t* table = a.batch.tables + s * a.batch.table_stride;
   const int32_t* kept = a.kept + s * a.kept_sequence + h * a.kept_head;
-  const int B = a.batch.block_tokens, pieces = a.head_dim / 8;
+  const int B = a.batch.block_tokens, pieces = a.head_dim / kPiece;
+  const int me = static_cast<int>(threadIdx.x);
+  // Threads of a row, a power of two, and where this one is in its rows.
+  const int shift = 32 - __clz(pieces - 1 > 0 ? pieces - 1 : 0);
+  const int my_row = me >> shift, my_piece = me & ((1 << shift) - 1), rows_apart = kThreads >> shift;
+  const int passes = my_piece < pieces ? 1 << shift : 0;
   const bool takes_weight = a.weights != nullptr && key;
-  // A group: the blocks that a round holds, or one that takes several rounds.
-  const int of_group = B <= kScaledRows ? kScaledRows / B : 1;
+  // A round: as many whole blocks as it has rows for, or a part of one block.
+  const int of_round = B <= kScaledRows ? kScaledRows / B : 1;
+  const int parts = B <= kScaledRows ? 1 : (B + kScaledRows - 1) / kScaledRows;
+  const int last = min(a.budget, a.batch.capacity);
+  const int rounds =
+      static_cast<int>((last + static_cast<int64_t>(of_round) * B - 1) / (of_round * B)) * parts;
+  // First place of a round's blocks and of the round, and the end of the latter.
+  const auto begin_of = [&](int r) { return r / parts * static_cast<int64_t>(of_round) * B; };
+  const auto first_of = [&](int r) { return begin_of(r) + r % parts * kScaledRows; };
+  const auto end_of = [&](int r) {
+    const int64_t all = min(begin_of(r) + static_cast<int64_t>(of_round) * B, static_cast<int64_t>(last));
+    return static_cast<int>(parts == 1 ? all : min(all, first_of(r) + kScaledRows));
+  };
   const auto block_of = [&](int p) {  // block id, or -1
     if (p < 0 || p >= a.batch.capacity) return -1;
     const int id = table[FastDivI(a.block_div, p)];
@@ -201,94 +227,141 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
     const float f = scales[static_cast<int64_t>(id) * a.heads + h];
     return f > 0.0f ? f : 0.0f;
   };
-  const int64_t last = min(a.budget, a.batch.capacity);
-  for (int64_t first = 0; first < last; first += static_cast<int64_t>(of_group) * B) {
-    const int end = static_cast<int>(min(first + static_cast<int64_t>(of_group) * B, last));
-    const int begin = static_cast<int>(first);
-    for (int i = threadIdx.x; i < of_group; i += kThreads) {
-      largest[i] = 0;
-      moves[i] = 0;
-    }
-    __syncthreads();
-    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
-      const int p = kept[i * a.kept_place];
-      const int id = block_of(p);
-      if (id >= 0) {
-        const int g = FastDivI(a.block_div, i - begin);
-        atomicMax(&largest[g], __builtin_bit_cast(uint32_t, scale_of(id)));
-        if (p != i) atomicOr(&moves[g], 1);
-      }
-    }
-    __syncthreads();
-    for (int r0 = begin; r0 < end; r0 += kScaledRows) {
-      const int i = r0 + static_cast<int>(threadIdx.x);
-      if (threadIdx.x < kScaledRows) {
-        int64_t x = -1, y = -1;
-        float ratio = 1.0f;
-        if (i < end) {
-          const int p = kept[i * a.kept_place], id = block_of(p), into = block_of(i);
-          const int g = FastDivI(a.block_div, i - begin);
-          if (id >= 0 && into >= 0 && moves[g] != 0) {
-            const auto row = [&](int of, int at) {
-              const int slot = at - FastDivI(a.block_div, at) * B;
-              return (static_cast<int64_t>(of) * B + slot) * a.heads + h;
-            };
-            const float old = scale_of(id), now = __builtin_bit_cast(float, largest[g]);
-            if (old != now) ratio = old / now;
-            if (p != i || old != now) {
-              x = row(id, p);
-              y = row(into, i);
-            }
+  const auto row = [&](int id, int p) {
+    const int slot = p - FastDivI(a.block_div, p) * B;
+    return (static_cast<int64_t>(id) * B + slot) * a.heads + h;
+  };
+  // A block of several rounds keeps its scale in the slot of its own number.
+  const auto slot_of = [&](int r) { return r / parts % kSlots; };
+  const auto note = [&](int r, int g, int i, int p, float scale) {
+    atomicMax(&largest[slot_of(r)][g], __builtin_bit_cast(uint32_t, scale));
+    if (p != i) atomicOr(&moves[slot_of(r)][g], 1);
+  };
+  int place = 0, position = -1, next_place = 0, next_position = -1;
+  // Thread t looks up row t of round r.
+  const auto look = [&](int r) {
+    int64_t x = -1, y = -1;
+    float scale = 0.0f;
+    next_position = -1;
+    if (r < rounds) {
+      const int begin = static_cast<int>(begin_of(r));
+      const int64_t i64 = first_of(r) + me;
+      if (i64 < end_of(r)) {
+        const int i = static_cast<int>(i64), p = kept[i * a.kept_place];
+        const int id = block_of(p), into = block_of(i);
+        next_place = i;
+        next_position = p;
+        if (id >= 0) {
+          scale = scale_of(id);
+          if (parts == 1) note(r, FastDivI(a.block_div, i - begin), i, p, scale);
+          // (Where a block's last row stays, all of them do.)
+          const int end = min(i + B - (i - FastDivI(a.block_div, i) * B), last) - 1;
+          if (into >= 0 && (p != i || kept[end * a.kept_place] != end)) {
+            x = row(id, p);
+            y = row(into, i);
           }
         }
-        from[threadIdx.x] = x;
-        to[threadIdx.x] = y;
-        ratios[threadIdx.x] = ratio;
       }
-      __syncthreads();
-      u32x2 held[kPieces];
-      float weight = 0.0f;
-      const int items = kScaledRows * pieces;
-      int64_t weight_to = -1;
-#pragma unroll
-      for (int n = 0; n < kPieces; ++n) {
-        const int item = static_cast<int>(threadIdx.x) + n * kThreads;
-        held[n] = u32x2{0, 0};
-        if (item < items && from[item / pieces] >= 0) {
-          held[n] = *reinterpret_cast<const Bytes8*>(pool + from[item / pieces] * a.head_dim +
-                                                     item % pieces * 8);
+      if (parts > 1 && r % parts == 0) {
+        const int end = min(begin + B, last);
+        for (int i = begin + me; i < end; i += kThreads) {
+          const int p = kept[i * a.kept_place], id = block_of(p);
+          if (id >= 0) note(r, 0, i, p, scale_of(id));
         }
       }
-      if (takes_weight && threadIdx.x < kScaledRows && from[threadIdx.x] >= 0) {
-        weight = a.weights[WeightAt<false>(a, h, from[threadIdx.x], kept[i * a.kept_place])];
-        weight_to = WeightAt<false>(a, h, to[threadIdx.x], i);
+    }
+    from[r % kSlots][me] = x;
+    to[r % kSlots][me] = y;
+    old_scale[r % kSlots][me] = scale;
+  };
+  const auto clear = [&](int slot) {
+    largest[slot][me] = 0;
+    moves[slot][me] = 0;
+  };
+  // Thread t decides on row t of round r.
+  const auto decide = [&](int r) {
+    float f = 0.0f;
+    const int64_t x = from[r % kSlots][me];
+    const int g = parts == 1 ? FastDivI(a.block_div, me) : 0;
+    if (x >= 0 && moves[slot_of(r)][g] != 0) {
+      const float now = __builtin_bit_cast(float, largest[slot_of(r)][g]), old = old_scale[r % kSlots][me];
+      if (old == now) {
+        f = x == to[r % kSlots][me] ? 0.0f : 1.0f;
+      } else {
+        f = old > 0.0f ? old / now : -1.0f;  // (-1: all codes become 0)
       }
-      // Every wave has this round's rows before one of them is written over.
+    }
+    factors[r & 1][me] = f;
+  };
+  Piece held[kPieces];
+  float weight = 0.0f;
+  int64_t weight_to = -1;
+  const auto load = [&](int r) {
 #pragma unroll
-      for (int n = 0; n < kPieces; ++n) asm volatile("" : : "v"(held[n]));
-      asm volatile("" : : "v"(weight));
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < kPieces; ++n) {
-        const int item = static_cast<int>(threadIdx.x) + n * kThreads;
-        if (item < items && to[item / pieces] >= 0) {
-          const float ratio = ratios[item / pieces];
-          if (ratio != 1.0f) held[n] = u32x2{Rescaled(held[n][0], ratio), Rescaled(held[n][1], ratio)};
-          *reinterpret_cast<Bytes8*>(pool + to[item / pieces] * a.head_dim + item % pieces * 8) =
-              held[n];
+    for (int n = 0; n < kPieces; ++n) {
+      held[n] = Piece(0);
+      if (n < passes) {
+        const int64_t x = from[r % kSlots][my_row + n * rows_apart];
+        if (x >= 0) {
+          held[n] = *reinterpret_cast<const Bytes*>(pool + x * a.head_dim + my_piece * kPiece);
         }
       }
-      if (weight_to >= 0) a.weights[weight_to] = weight;
-      __syncthreads();
     }
-    for (int g = threadIdx.x; g < of_group; g += kThreads) {
-      const int into = begin + g * static_cast<int64_t>(B) < end ? block_of(begin + g * B) : -1;
-      if (into >= 0 && moves[g] != 0) {
-        scales[static_cast<int64_t>(into) * a.heads + h] =
-            __builtin_bit_cast(float, largest[g]);
-      }
+    place = next_place;
+    position = next_position;
+    weight_to = -1;
+    if (takes_weight && position != place && from[r % kSlots][me] >= 0) {
+      weight = a.weights[WeightAt<false>(a, h, from[r % kSlots][me], position)];
+      weight_to = WeightAt<false>(a, h, to[r % kSlots][me], place);
     }
+  };
+  for (int n = 0; n < kSlots; ++n) clear(n);
+  __syncthreads();
+  look(0);
+  __syncthreads();
+  decide(0);
+  load(0);
+  look(1);
+  for (int r = 0; r < rounds; ++r) {
+    // Every wave has this round's rows before one of them is written over.
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) asm volatile("" : : "v"(held[n]));
+    asm volatile("" : : "v"(weight));
     __syncthreads();
+    Piece now[kPieces];
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) now[n] = held[n];
+    const float now_weight = weight;
+    const int64_t now_to = weight_to;
+    decide(r + 1);
+    load(r + 1);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      if (n >= passes) continue;
+      const int row_of = my_row + n * rows_apart;
+      const float f = factors[r & 1][row_of];
+      if (f == 0.0f) continue;
+      if (f != 1.0f) {
+        const float ratio = f < 0.0f ? 0.0f : f;
+#pragma unroll
+        for (int i = 0; i < kPiece / 4; ++i) now[n][i] = Rescaled(now[n][i], ratio);
+      }
+      *reinterpret_cast<Bytes*>(pool + to[r % kSlots][row_of] * a.head_dim + my_piece * kPiece) =
+          now[n];
+    }
+    if (now_to >= 0) a.weights[now_to] = now_weight;
+    // The scales of blocks that are whole now: nothing reads the old ones any more.
+    if (me < of_round && r % parts == parts - 1 && moves[slot_of(r)][me] != 0) {
+      const int64_t at = begin_of(r) + static_cast<int64_t>(me) * B;
+      const int into = at < last ? block_of(static_cast<int>(at)) : -1;
+      if (into >= 0) {
+        scales[static_cast<int64_t>(into) * a.heads + h] =
+            __builtin_bit_cast(float, largest[slot_of(r)][me]);
+      }
+    }
+    // For the round after the next two, whose rows are looked up behind the next barrier.
+    if (r % parts == 0) clear((slot_of(r) + kSlots - 1) % kSlots);
+    look(r + 2);
   }
 }
 
@@ -297,7 +370,11 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(const Compact
 hipError_t LaunchCompact(const CompactLaunch& l, hipStream_t stream) {
   const unsigned rows = static_cast<unsigned>(l.batch.sequences) * l.heads;
   if (l.pool == kPoolE4m3) {
-    hipLaunchKernelGGL(compact_e4m3_kernel, dim3(rows, 2), dim3(kThreads), 0, stream, l);
+    const bool wide = l.head_dim % 16 == 0;
+    const auto kernel = l.head_dim <= 128
+                            ? (wide ? compact_e4m3_kernel<128, true> : compact_e4m3_kernel<128, false>)
+                            : (wide ? compact_e4m3_kernel<256, true> : compact_e4m3_kernel<256, false>);
+    hipLaunchKernelGGL(kernel, dim3(rows, 2), dim3(kThreads), 0, stream, l);
     return hipGetLastError();
   }
   const bool fp4 = l.pool == kPoolFp4;
