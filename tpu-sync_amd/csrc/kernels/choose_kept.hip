@@ -9,8 +9,8 @@
 // same order (NaN, and tokens without a place, below all). The N-th largest is found by
 // its digits from the top, 11, 11 and 10 bits: a histogram in LDS of the digit among
 // those that agree in the digits before, then the digit in which the count from above
-// reaches N. With the N-th largest T known, waves count what is above and what equals it
-// in their ranges of positions, and write the positions that stay in a second pass, so
+// reaches N. With the N-th largest T known, threads count what is above and what equals
+// it in their ranges of positions, and write the positions that stay in a second pass, so
 // nothing depends on the order of atomic additions. Numbers are kept in LDS between
 // passes where they fit.
 #include "evict.h"
@@ -160,39 +160,47 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
     above = found_above;
   }
 
-  // A wave's range of positions: what is above and what equals the number.
-  const int each = (count + kWavesHere * 64 - 1) / (kWavesHere * 64) * 64;
-  const int i0 = min(wave * each, count), i1 = min(i0 + each, count);
+  // A thread's range of positions (of an odd length, so that a wave reads LDS on all
+  // banks): what is above and what equals the number.
+  const int each = (count + kChooseThreads - 1) / kChooseThreads | 1;
+  const int i0 = min(static_cast<int>(threadIdx.x) * each, count), i1 = min(i0 + each, count);
   int more = 0, equal = 0;
-  for (int i = i0 + lane; i - lane < i1; i += 64) {
-    const uint32_t u = i < i1 ? number(i) : 0u;
-    more += __popcll(__ballot(i < i1 && u > digits));
-    equal += __popcll(__ballot(i < i1 && u == digits));
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t u = number(i);
+    more += u > digits ? 1 : 0;
+    equal += u == digits ? 1 : 0;
   }
-  if (lane == 0) {
-    wave_more[wave] = more;
-    wave_sums[wave] = equal;
+  int more_to = more, equal_to = equal;  // with the lanes before
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    const int x = __shfl_up(more_to, m), y = __shfl_up(equal_to, m);
+    if (lane >= m) {
+      more_to += x;
+      equal_to += y;
+    }
+  }
+  if (lane == 63) {
+    wave_more[wave] = more_to;
+    wave_sums[wave] = equal_to;
   }
   __syncthreads();
-  more = equal = 0;
+  more = more_to - more;
+  equal = equal_to - equal;
 #pragma unroll
   for (int w = 0; w < kWavesHere; ++w) {
     more += w < wave ? wave_more[w] : 0;
     equal += w < wave ? wave_sums[w] : 0;
   }
   const int of_equal = wanted - above;  // so many of those that equal it stay
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  for (int i = i0 + lane; i - lane < i1; i += 64) {
-    const uint32_t u = i < i1 ? number(i) : 0u;
-    const uint64_t larger = __ballot(i < i1 && u > digits);
-    const uint64_t same = __ballot(i < i1 && u == digits);
-    const int mine = equal + __popcll(same & below);
-    const bool stays = (larger >> lane & 1) != 0 || ((same >> lane & 1) != 0 && mine < of_equal);
-    if (stays) {
-      kept[first + more + __popcll(larger & below) + min(mine, of_equal)] = first + i;
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t u = number(i);
+    if (u > digits) {
+      kept[first + more + min(equal, of_equal)] = first + i;
+      ++more;
+    } else if (u == digits) {
+      if (equal < of_equal) kept[first + more + equal] = first + i;
+      ++equal;
     }
-    more += __popcll(larger);
-    equal += __popcll(same);
   }
 }
 
