@@ -495,3 +495,119 @@ def test_captured_eviction_follows_lengths(kvx, cuda):
             assert torch.equal(weights, sides[0][2])
     for mgr, *_ in sides:
         mgr.close()
+
+
+def test_kept_at_any_strides(kvx, cuda):
+    caches, _ = storages(cuda, BF16, 40, 16, 2, 64, 1)
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
+    tables = torch.arange(40, dtype=torch.int32, device=cuda).view(2, 20)
+    gen = torch.Generator().manual_seed(1)
+    kept = torch.stack([torch.randperm(320, generator=gen)[:100].sort().values
+                        for _ in range(4)]).view(2, 2, 100).int().to(cuda)
+    old = [c.clone() for c in caches]
+    mgr.compact(0, 1, kept, tables)
+    want = [c.clone() for c in caches]
+    wide = torch.full((2, 2, 300), -7, dtype=torch.int32, device=cuda)
+    wide[:, :, 2::3] = kept
+    for other in (kept.transpose(0, 2).contiguous().transpose(0, 2),
+                  kept.transpose(1, 2).contiguous().transpose(1, 2), wide[:, :, 2::3]):
+        for c, o in zip(caches, old):
+            c.copy_(o)
+        mgr.compact(0, 1, other, tables)
+        assert all(torch.equal(c, w) for c, w in zip(caches, want))
+    # One list for all sequences and heads.
+    for c, o in zip(caches, old):
+        c.copy_(o)
+    mgr.compact(0, 1, kept[:1, :1].expand(2, 2, 100), tables)
+    one = [c.clone() for c in caches]
+    for c, o in zip(caches, old):
+        c.copy_(o)
+    mgr.compact(0, 1, kept[:1, :1].expand(2, 2, 100).contiguous(), tables)
+    assert all(torch.equal(c, w) for c, w in zip(caches, one))
+    mgr.close()
+
+
+def test_two_calls_at_once(kvx, cuda):
+    """Layers of one pool evicted on two streams, chunks weighed on both: as in turn."""
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    S, Hq, Hk, D, B, W = 3, 8, 2, 128, 16, 40
+    start = [torch.randn(S * W, B, Hk, D, device=cuda, generator=gen).to(BF16) for _ in range(4)]
+    tables = torch.randperm(S * W, generator=torch.Generator().manual_seed(4)).int().view(S, W)
+    tables, lengths = tables.to(cuda), ints([600, 77, 431], cuda)
+    starts = ints([0, 150, 170, 300], cuda)
+    q = [torch.randn(300, Hq, D, device=cuda, generator=gen).to(BF16) for _ in range(2)]
+    results = []
+    for at_once in (False, True):
+        caches = [c.clone() for c in start]
+        mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
+        tabs = [torch.zeros(S * W, Hk, B, device=cuda) for _ in range(2)]
+        streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+        lse = [mgr.attend(2 * i, 2 * i + 1, q[i], tables, lengths, starts=starts,
+                          return_lse=True)[1] for i in range(2)]
+        torch.cuda.synchronize()
+        cuts = []
+        for i in range(2):
+            for _ in range(3):
+                mgr.weigh(2 * i, q[i], tables, lengths, lse[i], tabs[i], starts=starts, decay=0.5,
+                          stream=streams[i])
+            cuts.append(mgr.evict(2 * i, 2 * i + 1, tabs[i], tables, lengths, 100, recent=9,
+                                  stream=streams[i]))
+            if not at_once:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append(caches + tabs + cuts)
+        mgr.close()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("cache", [BF16, FP8, "fp4"])
+def test_blocks_past_32_bits(kvx, cuda, cache):
+    """A step and an eviction in the last blocks of storages of over 4 GiB (and of over
+    2^31 weights), against the same in a small pool."""
+    S, Hq, Hk, D, B, W = 2, 16, 8, 128, 16, 12
+    each = {BF16: 32768, FP8: 16384, "fp4": 8192}[cache]
+    far = (4 << 30) // each + 1000
+    small, scales = storages(cuda, cache, S * W, B, Hk, D, 7)
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    q = torch.randn(40, Hq, D, device=cuda, generator=gen).to(BF16)
+    k, v = (torch.randn(40, Hk, D, device=cuda, generator=gen).to(BF16) for _ in range(2))
+    starts, lengths = ints([0, 39, 40], cuda), ints([180, 100], cuda)
+    results = []
+    for blocks in (S * W, far):
+        def grown(t):
+            if blocks == S * W:
+                return t.clone()
+            big = torch.zeros((blocks,) + tuple(t.shape[1:]), device=cuda,
+                              dtype=torch.uint8 if t.element_size() == 1 else t.dtype)
+            big = big.view(t.dtype)
+            big.view(torch.uint8)[-S * W:] = t.view(torch.uint8)
+            return big
+        caches, tabs = [grown(c) for c in small], [grown(t) for t in scales]
+        table_blocks = blocks if blocks == S * W else (1 << 31) // (Hk * B) + 1000
+        if table_blocks < blocks:
+            table_blocks = blocks
+        weights = torch.zeros(table_blocks, Hk, B, device=cuda)
+        mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, scale_tables=tabs)
+        tables = torch.arange(S * W, dtype=torch.int32, device=cuda).view(S, W) + (blocks - S * W)
+        mgr.append_kv(0, 1, k, v, tables, lengths, starts=starts)
+        out, lse = mgr.attend(0, 1, q, tables, lengths, starts=starts, return_lse=True)
+        one = mgr.attend(0, 1, q[:2], tables, lengths)
+        mgr.weigh(0, q, tables, lengths, lse, weights, starts=starts)
+        mgr.weigh(0, q[:2], tables, lengths, lse[:2].contiguous(), weights)
+        last = weights[blocks - S * W:blocks]
+        got = last.clone()
+        cut = mgr.evict(0, 1, weights, tables, lengths, 70, recent=4)
+        results.append([out, one, got, cut, last.clone()]
+                       + [t.view(torch.uint8)[-S * W:].clone() for t in caches + tabs])
+        mgr.close()
+        del caches, tabs, weights, last
+        torch.cuda.empty_cache()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # Weights past 2^31 entries.
+    blocks = (1 << 31) // (Hk * B) + 50
+    big = torch.zeros(blocks, Hk, B, device=cuda)
+    few = torch.rand(20, Hk, B, device=cuda)
+    big[-20:] = few
+    tables = torch.arange(20, dtype=torch.int32, device=cuda)[None]
+    kept, _ = kvx.choose_kept(few, tables, ints([320], cuda), 100)
+    assert torch.equal(kvx.choose_kept(big, tables + (blocks - 20), ints([320], cuda), 100)[0], kept)
