@@ -50,12 +50,6 @@ constexpr int WorkerAt(int place, int workers) {
   return at < each && worker < workers ? worker : -1;
 }
 
-// Workgroups of a CU of attend_few. A step of a 4-bit pool is a quarter of a 16-bit
-// one's bytes, so more of them have to be on their way. FEWNOTE
-constexpr int FewGroups(int pool, int padded_dim, int rows, int head_dim) {
-  return padded_dim > 128 ? 1 : pool == kPoolFp4 && rows <= 16 && head_dim == padded_dim ? 3 : 2;
-}
-
 struct AttendLaunch {
   BatchView batch;
   FastDivU32 block_div;  // by batch.block_tokens

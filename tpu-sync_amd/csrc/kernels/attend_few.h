@@ -306,8 +306,6 @@ __device__ __forceinline__ void AttendFew(const AttendLaunch& a, char* lds, int 
           }
         }
       }
-      // (Values are not widened earlier, where they would be waited for.)
-      if constexpr (F4) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll

@@ -7,7 +7,7 @@ namespace kvx {
 namespace {
 
 template <class E, int POOL, int DP, int RT, bool FULL>
-__global__ __launch_bounds__(kAttendThreads, FewGroups(POOL, DP, RT * 16, FULL ? DP : 0)) void attend_few_kernel(
+__global__ __launch_bounds__(kAttendThreads, DP <= 128 ? 2 : 1) void attend_few_kernel(
     const AttendLaunch a) {
   extern __shared__ __align__(16) char lds[];
   // With a join to come, the first workgroup leaves the plan for it.

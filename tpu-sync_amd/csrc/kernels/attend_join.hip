@@ -206,16 +206,13 @@ int64_t PlanAttend(AttendLaunch* l) {
   l->few_grid = l->few_rows = l->many_grid = l->join_grid = l->join_rows = 0;
   l->part_rows = 0;
   const int resident = (l->padded_dim > 128 ? 1 : 2) * kCus;  // workgroups
-  const bool many_sequences = single ? G > kFewRows : T * G > kFewRows;
   if (G <= kFewRows) {
     l->few_rows = static_cast<int>(single ? G : std::min<int64_t>(T * G, kFewRows));
     const int64_t steps = S * l->k_heads * CeilDiv(capacity, kFewStep);
     // One place is left to the plan's workgroup.
-    const int groups = many_sequences || l->groups > 0
-                           ? resident
-                           : kCus * FewGroups(l->pool, l->padded_dim, l->few_rows, l->head_dim);
-    l->few_grid = static_cast<int>(std::min<int64_t>(groups - 1, CeilDiv(steps, kWaves)));
+    l->few_grid = static_cast<int>(std::min<int64_t>(resident - 1, CeilDiv(steps, kWaves)));
   }
+  const bool many_sequences = single ? G > kFewRows : T * G > kFewRows;
   if (many_sequences || l->groups > 0) {
     const int64_t tiles = CeilDiv(T * G, kManyRows) * 2 + S + l->groups;
     const int64_t steps = tiles * l->k_heads * (CeilDiv(capacity, kManyStep) + 2);
