@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
   extern __shared__ uint32_t held[];  // [held_most]
   __shared__ int bins[kBins];
   __shared__ int wave_sums[kWavesHere], wave_more[kWavesHere];
-  __shared__ int found_bin, found_above;
+  __shared__ int found_bin, found_above, found_count;
   const BatchView& b = a.batch;
   const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -151,13 +151,22 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
     if (before < wanted && before + n0 >= wanted) {
       found_bin = top;
       found_above = before;
+      found_count = n0;
     } else if (before + n0 < wanted && before + n0 + n1 >= wanted) {
       found_bin = top - 1;
       found_above = before + n0;
+      found_count = n1;
     }
     __syncthreads();
     digits |= static_cast<uint32_t>(found_bin) << shift;
     above = found_above;
+    // All with these digits stay (mostly one, after 22 bits): what is above the number
+    // before the least of them does.
+    if (above + found_count == wanted && digits != 0) {
+      --digits;
+      above = wanted;
+      break;
+    }
   }
 
   // A thread's range of positions (of an odd length, so that a wave reads LDS on all
