@@ -13,6 +13,14 @@
 // again and again on rows that the last-level cache holds; one token of each of
 // 64 sequences 4.1 us, which is the launch and its dependent loads.
 //
+// 4-bit pool: the same kernel with another way to store a row (Fp4Row). Every 32
+// dimensions of a token's head have a power-of-two scale of their own, so a row is
+// stored by itself, whatever the block holds: four lanes find the largest of the 32
+// values as the bits of integers, the scale is integer arithmetic on its exponent, and
+// the conversion divides by it exactly and rounds once. 16384 tokens x 8 heads x 128,
+// normed, 25.8 us (67 MB read, 18 written): the rows' norm and rotation, as in 16 bits,
+// where 134 MB take 26.1. One token of each of 64 sequences: 4.3 us.
+//
 // e4m3 pool (append_e4m3_kernel): one fp32 scale per (block, head), so all
 // rows of a block and head have to be seen before the first is written. A
 // workgroup takes the new rows of one block, K or V, a wave the heads in turn:

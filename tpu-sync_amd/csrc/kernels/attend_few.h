@@ -24,6 +24,12 @@
 // GB (5.2 TB/s; 256-byte rows of one head at random 16-token blocks are read at 5.6
 // to 6.0 by a kernel that does nothing else), in e4m3 on one key head 46 us for 266
 // MB (5.7 TB/s). Three waves a SIMD instead of two: the same, e4m3 4 % slower.
+//
+// A 4-bit pool's keys and values become operands in registers, their scales on the
+// way (pool_lane.h): 64 sequences of 65 to 16384 tokens, 32 heads on 8, D = 128: 120 us
+// with the join for 560 MB (4.7 TB/s; runs of 1 KiB at random are read at 4.3 to 5.6 by
+// a kernel that does nothing else). The same step over tokens that the L2 holds takes 93
+// us, which the reads hide behind in part. Three waves a SIMD: 119 to 121 us.
 #ifndef KVX_KERNELS_ATTEND_FEW_H_
 #define KVX_KERNELS_ATTEND_FEW_H_
 

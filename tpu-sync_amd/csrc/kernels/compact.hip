@@ -7,12 +7,19 @@
 // waits for every wave, and writes them; what it writes is below every row that a later
 // round reads. Rows of the next round are on their way while this one's are written.
 // Where there are few sequences and heads, several workgroups take a part of every
-// row's bytes each. Rows that stay at their place are neither read nor written.
+// row's bytes each. Rows that stay at their place are neither read nor written. 64
+// sequences cut to 2048 tokens, 8 heads x 128, bf16: 192 us for 849 MB (4.4 TB/s, reads
+// of scattered 256-byte rows and writes; torch's copy of 1 GiB reaches 5.1); one such
+// sequence 18 us.
 //
 // e4m3 (compact_e4m3_kernel): rows that meet in a block come from blocks with scales of
 // their own, so the block gets the largest of them, and codes are stored again as
 // e4m3(code * old / new), which rounds those of smaller scales once. A block's scale is
-// replaced when all of its rows are there; later rounds read later blocks.
+// replaced when all of its rows are there; later rounds read later blocks. What a round
+// needs is looked up two rounds ahead and decided on one ahead, by a thread a row. 24
+// sequences cut to 3000 tokens, 8 heads x 128: 96 us for 301 MB; with three waits a round
+// of 128 rows and a division a piece 155 us. 384 workgroups of 4 waves leave the GPU's
+// memory idle between their rounds: a block's scale ties its rows to one workgroup.
 #include "evict.h"
 
 #include <algorithm>
