@@ -444,7 +444,8 @@ def test_a_loop_that_evicts(kvx, cuda, cache):
     mgr.close()
 
 
-def test_captured_eviction_follows_lengths(kvx, cuda):
+@pytest.mark.parametrize("each", [1, 30])
+def test_captured_eviction_follows_lengths(kvx, cuda, each):
     """weigh and evict captured once in two graphs that are replayed in turn,
     against the eager calls."""
     gen = torch.Generator(device=cuda).manual_seed(3)
@@ -453,17 +454,19 @@ def test_captured_eviction_follows_lengths(kvx, cuda):
     tables = torch.randperm(S * W, generator=torch.Generator().manual_seed(4)).int().view(S, W)
     tables = tables.to(cuda)
     table = torch.rand(S * W, Hk, B, device=cuda, generator=gen)
+    starts = ints([n * each for n in range(S + 1)], cuda)
 
     def step(mgr, q, lengths, weights):
-        _, lse = mgr.attend(0, 1, q, tables, lengths, return_lse=True)
-        mgr.weigh(0, q, tables, lengths, lse, weights)
+        kw = dict(starts=starts) if each > 1 else {}
+        _, lse = mgr.attend(0, 1, q, tables, lengths, return_lse=True, **kw)
+        mgr.weigh(0, q, tables, lengths, lse, weights, **kw)
         return mgr.evict(0, 1, weights, tables, lengths, 50, recent=8)
 
     sides = []
     for captured in (False, True, True):
         caches, weights = [c.clone() for c in start], table.clone()
         mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1)
-        q = torch.zeros(S, Hq, D, dtype=BF16, device=cuda)
+        q = torch.zeros(S * each, Hq, D, dtype=BF16, device=cuda)
         lengths = torch.zeros(S, dtype=torch.int32, device=cuda)
         graph = out = None
         if captured:
@@ -477,7 +480,7 @@ def test_captured_eviction_follows_lengths(kvx, cuda):
                 out = step(mgr, q, lengths, weights)
         sides.append((mgr, caches, weights, q, lengths, graph, out))
     for i in range(4):
-        x = torch.randn(S, Hq, D, device=cuda, generator=gen).to(BF16)
+        x = torch.randn(S * each, Hq, D, device=cuda, generator=gen).to(BF16)
         now = ints([0, 30 + 10 * i, 51 + i, 190 - 30 * i], cuda)
         cuts = []
         for mgr, _, weights, q, lengths, graph, out in sides:
@@ -611,3 +614,21 @@ def test_blocks_past_32_bits(kvx, cuda, cache):
     tables = torch.arange(20, dtype=torch.int32, device=cuda)[None]
     kept, _ = kvx.choose_kept(few, tables, ints([320], cuda), 100)
     assert torch.equal(kvx.choose_kept(big, tables + (blocks - 20), ints([320], cuda), 100)[0], kept)
+
+
+def test_many_sequences(kvx, cuda):
+    for counts, lengths in (([1] * 1500, [(7 * s) % 50 for s in range(1500)]),
+                            ([s % 12 for s in range(400)], [s % 41 + 12 for s in range(400)])):
+        step = Step(kvx, cuda, counts, lengths, 8, 2, 64, 16, BF16, BF16)
+        _, lse = step.run(return_lse=True)
+        before = torch.rand(step.caches[0].shape[0], 2, 16, device=cuda)
+        after = before.clone()
+        step.mgr.weigh(0, step.q, *step.args(), lse, after, decay=0.5, **step.kw())
+        check_weights(step, before, after, lse, None, 0.5)
+        w, (tables, held) = before.cpu(), step.args()
+        kept, cut = kvx.choose_kept(before, tables, held, 13, recent=2)
+        for s, n in enumerate(lengths):
+            x = torch.cat([w[b, 1] for b in step.tables[s]] or [w[0, 0, :0]])[:n].tolist()
+            want = plain_choice(x, 13, 2, 0)
+            assert kept[s, 1].tolist() == want + [-1] * (13 - len(want)) and int(cut[s]) == min(n, 13)
+        step.mgr.close()

@@ -10,6 +10,7 @@ sequences. A served loop weighs its steps and cuts a sequence when it has grown:
 Streams, memory, graphs and gradients are as in ``paged_attention``.
 """
 import ctypes
+import operator
 import struct
 from typing import Tuple
 
@@ -47,8 +48,12 @@ def _begins(begins, device, sequences):
 
 
 def _count(value, what):
-    if isinstance(value, bool) or not isinstance(value, int):
-        raise ValueError(f"{what} must be an int, got {value!r}")
+    try:
+        value = None if isinstance(value, bool) else operator.index(value)
+    except TypeError:
+        value = None
+    if value is None:
+        raise ValueError(f"{what} must be an int")
     if not 0 <= value <= 1 << 30:
         raise ValueError(f"{what} must be 0..2^30, got {value}")
     return value
