@@ -369,6 +369,23 @@ def test_compact_stays_inside(kvx, cuda, cache):
     mgr.close()
 
 
+def test_compact_of_scales_far_apart(kvx, cuda):
+    """Quotients of scales below fp32's least number: the rows become zeros."""
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    caches = [torch.randn(4, 16, 1, 64, device=cuda, generator=gen).to(FP8) for _ in range(2)]
+    old = [c.float() for c in caches]
+    scales = [torch.tensor([1e-30, 1e20, 0.0, 1.0], device=cuda)[:, None].contiguous() for _ in range(2)]
+    mgr = kvx.KVCacheManager(caches, host_blocks_to_allocate=1, scale_tables=scales)
+    positions = list(range(3, 9)) + [17, 20, 33]
+    mgr.compact(0, 1, ints([[positions]], cuda), ints([[0, 1, 2]], cuda))
+    for c, o, f in zip(caches, old, scales):
+        assert torch.equal(f[:, 0], torch.tensor([1e20, 1e20, 0.0, 1.0], device=cuda))
+        for i, p in enumerate(positions):
+            want = o[1, p - 16, 0] if 16 <= p < 32 else torch.zeros(64, device=cuda)
+            assert torch.equal(c.float()[0, i, 0], want), p
+    mgr.close()
+
+
 # -- together ---------------------------------------------------------------------
 
 @pytest.mark.parametrize("cache", [BF16, FP8, "fp4"])

@@ -295,7 +295,8 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
       if (old == now) {
         f = x == to[r % kSlots][me] ? 0.0f : 1.0f;
       } else {
-        f = old > 0.0f ? old / now : -1.0f;  // (-1: all codes become 0)
+        f = old / now;
+        if (f == 0.0f) f = -1.0f;  // all codes become 0
       }
     }
     factors[r & 1][me] = f;
