@@ -108,6 +108,7 @@ def test_choose_kept_refuses(kvx):
     refused("weights must be", fn, fake((9, 32), F32), tables, lengths, 5, stream=0)
     refused("tables must be", fn, w, fake((3, 4), torch.int64), lengths, 5, stream=0)
     refused("tables must be", fn, w, fake((12,), I32), lengths, 5, stream=0)
+    refused("tables must be", fn, w, [[0, 1, 2]], lengths, 5, stream=0)
     refused("lengths must be", fn, w, tables, fake((2,), I32), 5, stream=0)
     refused("begins must be", fn, w, tables, lengths, 5, begins=fake((4,), I32), stream=0)
     for bad in (-1, 1 << 31, 2.5, True, None):

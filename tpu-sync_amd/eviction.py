@@ -121,7 +121,8 @@ def choose_kept(weights, tables, lengths, budget: int, *, recent: int = 0, begin
     device = weights.device.index or 0
     weights_at, blocks = _weights(weights, device)
     _, heads, block_tokens = weights.shape
-    sequences = tables.shape[0] if len(tables.shape) == 2 else -1
+    base._tables(device, tables)
+    sequences = tables.shape[0]
     batch = base._batch(device, tables, lengths, None, sequences)
     budget, recent = _count(budget, "budget"), _count(recent, "recent")
     begins_at = _begins(begins, device, sequences)

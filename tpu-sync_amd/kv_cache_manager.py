@@ -205,7 +205,8 @@ class KVCacheManager:
       raiden_controller_address: joins the KVCacheStore whose controller
         has this address (in this process) as its transfer worker.
       scale_tables: per-layer side tables with the same major dimension (for
-        an fp8 cache, [num_blocks, kv_heads] float32 scales); they are block
+        an fp8 cache, [num_blocks, kv_heads] float32 scales; for a 4-bit one
+        [num_blocks, kv_heads, tokens, head_dim / 32] e8m0); they are block
         arrays num_kv_layers.. and move with every copy of the same block ids.
       numa: host mirror placement: "auto" (the GPU's NUMA node), "off", or a
         node number.

@@ -1,7 +1,8 @@
 """Operators that fill and read the paged KV pool (libkvx's attention kernels).
 
 ``norm_rope`` is the RMS norm of query and key heads and the position rotation
-in one pass. ``append_kv`` and ``attend`` are methods of ``KVCacheManager``;
+in one pass. ``append_kv`` and ``attend`` are methods of ``KVCacheManager``, over
+pools of the tensors' type, float8 or 4 bits with their scales;
 their argument handling is here. The three are a step's work around the cache:
 
     q, _ = norm_rope(q, None, positions, inv_freq, q_weight=wq)
