@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t Ordered(float x) {
 }
 
 template <int VEC>
-__global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const ChooseLaunch a,
+__global__ __launch_bounds__(kChooseThreads, 8) void choose_kept_kernel(const ChooseLaunch a,
                                                                      const int held_most) {
   extern __shared__ uint32_t held[];  // [held_most]
   __shared__ int bins[kBins];
@@ -179,10 +179,23 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
   const int each = (count + kChooseThreads - 1) / kChooseThreads | 1;
   const int i0 = min(static_cast<int>(threadIdx.x) * each, count), i1 = min(i0 + each, count);
   int more = 0, equal = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t u = number(i);
-    more += u > digits ? 1 : 0;
-    equal += u == digits ? 1 : 0;
+  // Bit i: place i0 + i, of ranges that have no more than 32.
+  const bool masks = holds && each <= 32;
+  uint32_t at_least = 0, same = 0;
+  if (masks) {
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t u = held[first - base + i], bit = 1u << (i - i0);
+      at_least |= u >= digits ? bit : 0u;
+      same |= u == digits ? bit : 0u;
+    }
+    equal = __popc(same);
+    more = __popc(at_least) - equal;
+  } else {
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t u = number(i);
+      more += u > digits ? 1 : 0;
+      equal += u == digits ? 1 : 0;
+    }
   }
   int more_to = more, equal_to = equal;  // with the lanes before
 #pragma unroll
@@ -206,6 +219,18 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kept_kernel(const Choos
     equal += w < wave ? wave_sums[w] : 0;
   }
   const int of_equal = wanted - above;  // so many of those that equal it stay
+  if (masks) {
+    for (; at_least != 0; at_least &= at_least - 1) {
+      const int i = __builtin_ctz(at_least);
+      const bool is_equal = (same >> i & 1) != 0;
+      if (!is_equal || equal < of_equal) {
+        kept[first + more + min(equal, of_equal)] = first + i0 + i;
+      }
+      equal += is_equal ? 1 : 0;
+      more += is_equal ? 0 : 1;
+    }
+    return;
+  }
   for (int i = i0; i < i1; ++i) {
     const uint32_t u = number(i);
     if (u > digits) {
