@@ -276,7 +276,8 @@ COMPACTS = [  # (sequences, heads, dim, block, held, budget, prefix)
     (1, 8, 128, 16, 500, 100, 4), (5, 2, 64, 16, 200, 130, 0), (3, 1, 96, 7, 90, 45, 20),
     (2, 3, 256, 64, 400, 399, 0), (9, 4, 128, 8, 64, 1, 0), (2, 2, 32, 1, 50, 25, 3),
     (40, 8, 128, 16, 300, 200, 0), (2, 1, 64, 200, 900, 500, 0), (1, 2, 160, 24, 3000, 2000, 9),
-    (1, 1, 128, 300, 1000, 700, 0)]
+    (1, 1, 128, 300, 1000, 700, 0), (1, 2, 64, 600, 1900, 1500, 5), (33, 8, 32, 300, 400, 350, 0),
+    (33, 8, 64, 16, 700, 600, 0)]
 
 
 @pytest.mark.parametrize("cache", [BF16, F16, FP8, "fp4"])

@@ -17,9 +17,10 @@
 // e4m3(code * old / new), which rounds those of smaller scales once. A block's scale is
 // replaced when all of its rows are there; later rounds read later blocks. What a round
 // needs is looked up two rounds ahead and decided on one ahead, by a thread a row. 24
-// sequences cut to 3000 tokens, 8 heads x 128: 96 us for 301 MB; with three waits a round
-// of 128 rows and a division a piece 155 us. 384 workgroups of 4 waves leave the GPU's
-// memory idle between their rounds: a block's scale ties its rows to one workgroup.
+// sequences cut to 3000 tokens, 8 heads x 128: 94 us for 301 MB; with three waits a round
+// of 128 rows and a division a piece 155 us; lookups in three steps over rounds, a load
+// each, 97 us. 384 workgroups of 8 waves leave the GPU's memory idle between their
+// rounds: a block's scale ties its rows to one workgroup.
 #include "evict.h"
 
 #include <algorithm>
@@ -172,8 +173,6 @@ __global__ __launch_bounds__(kThreads, 2) void compact_kernel(const CompactLaunc
 
 // -- e4m3
 
-constexpr int kScaledRows = 256;  // of a round
-
 __device__ __forceinline__ uint32_t Rescaled(uint32_t w, float ratio) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
   const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
@@ -182,9 +181,9 @@ __device__ __forceinline__ uint32_t Rescaled(uint32_t w, float ratio) {
   return static_cast<uint32_t>(q);
 }
 
-// WIDE: rows are whole 16 bytes.
-template <int DP, bool WIDE>
-__global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
+// WIDE: rows are whole 16 bytes. THREADS: of a workgroup, and rows of a round.
+template <int DP, bool WIDE, int THREADS>
+__global__ __launch_bounds__(THREADS, 2) void compact_e4m3_kernel(
     const CompactLaunch a) {
   // Rounds in turn, four at a time. Of a row: where it is and goes, its scale, its place
   // in `largest`. Of a block: the new scale's bits, and whether one of its rows moves.
@@ -192,13 +191,12 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
   using Piece = std::conditional_t<WIDE, u32x4, u32x2>;
   using Bytes = Piece __attribute__((aligned(1)));
   constexpr int kPiece = sizeof(Piece);
-  __shared__ int64_t from[kSlots][kScaledRows], to[kSlots][kScaledRows];
-  __shared__ float factors[2][kScaledRows];  // what a row's codes are multiplied with, 0: stays
-  __shared__ float old_scale[kSlots][kScaledRows];
-  __shared__ uint32_t largest[kSlots][kScaledRows];
-  __shared__ int moves[kSlots][kScaledRows];
-  constexpr int kPieces = kScaledRows * (DP / kPiece) / kThreads;  // of a thread
-  static_assert(kScaledRows == kThreads);
+  __shared__ int64_t from[kSlots][THREADS], to[kSlots][THREADS];
+  __shared__ float factors[2][THREADS];  // what a row's codes are multiplied with, 0: stays
+  __shared__ float old_scale[kSlots][THREADS];
+  __shared__ uint32_t largest[kSlots][THREADS];
+  __shared__ int moves[kSlots][THREADS];
+  constexpr int kPieces = DP / kPiece;  // of a thread
   const int s = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
   const bool key = blockIdx.y == 0;
   uint8_t* pool = static_cast<uint8_t*>(key ? a.k_pool : a.v_pool);
@@ -209,21 +207,21 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
   const int me = static_cast<int>(threadIdx.x);
   // Threads of a row, a power of two, and where this one is in its rows.
   const int shift = 32 - __clz(pieces - 1 > 0 ? pieces - 1 : 0);
-  const int my_row = me >> shift, my_piece = me & ((1 << shift) - 1), rows_apart = kThreads >> shift;
+  const int my_row = me >> shift, my_piece = me & ((1 << shift) - 1), rows_apart = THREADS >> shift;
   const int passes = my_piece < pieces ? 1 << shift : 0;
   const bool takes_weight = a.weights != nullptr && key;
   // A round: as many whole blocks as it has rows for, or a part of one block.
-  const int of_round = B <= kScaledRows ? kScaledRows / B : 1;
-  const int parts = B <= kScaledRows ? 1 : (B + kScaledRows - 1) / kScaledRows;
+  const int of_round = B <= THREADS ? THREADS / B : 1;
+  const int parts = B <= THREADS ? 1 : (B + THREADS - 1) / THREADS;
   const int last = min(a.budget, a.batch.capacity);
   const int rounds =
       static_cast<int>((last + static_cast<int64_t>(of_round) * B - 1) / (of_round * B)) * parts;
   // First place of a round's blocks and of the round, and the end of the latter.
   const auto begin_of = [&](int r) { return r / parts * static_cast<int64_t>(of_round) * B; };
-  const auto first_of = [&](int r) { return begin_of(r) + r % parts * kScaledRows; };
+  const auto first_of = [&](int r) { return begin_of(r) + r % parts * THREADS; };
   const auto end_of = [&](int r) {
     const int64_t all = min(begin_of(r) + static_cast<int64_t>(of_round) * B, static_cast<int64_t>(last));
-    return static_cast<int>(parts == 1 ? all : min(all, first_of(r) + kScaledRows));
+    return static_cast<int>(parts == 1 ? all : min(all, first_of(r) + THREADS));
   };
   const auto block_of = [&](int p) {  // block id, or -1
     if (p < 0 || p >= a.batch.capacity) return -1;
@@ -271,7 +269,7 @@ __global__ __launch_bounds__(kThreads, 2) void compact_e4m3_kernel(
       }
       if (parts > 1 && r % parts == 0) {
         const int end = min(begin + B, last);
-        for (int i = begin + me; i < end; i += kThreads) {
+        for (int i = begin + me; i < end; i += THREADS) {
           const int p = kept[i * a.kept_place], id = block_of(p);
           if (id >= 0) note(r, 0, i, p, scale_of(id));
         }
@@ -379,10 +377,17 @@ hipError_t LaunchCompact(const CompactLaunch& l, hipStream_t stream) {
   const unsigned rows = static_cast<unsigned>(l.batch.sequences) * l.heads;
   if (l.pool == kPoolE4m3) {
     const bool wide = l.head_dim % 16 == 0;
-    const auto kernel = l.head_dim <= 128
-                            ? (wide ? compact_e4m3_kernel<128, true> : compact_e4m3_kernel<128, false>)
-                            : (wide ? compact_e4m3_kernel<256, true> : compact_e4m3_kernel<256, false>);
-    hipLaunchKernelGGL(kernel, dim3(rows, 2), dim3(kThreads), 0, stream, l);
+    // Twice the threads, and half as many rounds, while the GPU holds all workgroups at
+    // once: one sequence of 8 heads cut to 3000 tokens 51 to 31 us, 24 of them 97 to 94,
+    // but 64 of them 199 to 208. (At D = 256 a CU would hold one of them.)
+    const bool big = l.head_dim <= 128 && rows * 2ull <= 512;
+    const unsigned threads = big ? 512 : 256;
+    const auto kernel =
+        big ? (wide ? compact_e4m3_kernel<128, true, 512> : compact_e4m3_kernel<128, false, 512>)
+        : l.head_dim <= 128
+            ? (wide ? compact_e4m3_kernel<128, true, 256> : compact_e4m3_kernel<128, false, 256>)
+            : (wide ? compact_e4m3_kernel<256, true, 256> : compact_e4m3_kernel<256, false, 256>);
+    hipLaunchKernelGGL(kernel, dim3(rows, 2), dim3(threads), 0, stream, l);
     return hipGetLastError();
   }
   const bool fp4 = l.pool == kPoolFp4;
