@@ -1,11 +1,16 @@
 """Operators that make the paged KV cache shorter: what attention each cached token
 got, which tokens stay within a budget, and their move to the front of their
-sequences. A served loop weighs its steps and cuts a sequence when it has grown:
+sequences. A served loop weighs its steps and cuts sequences when they have grown;
+every layer is cut from the same lengths, and the new ones hold for all of them after
+that:
 
-    out, lse = mgr.attend(2 * i, 2 * i + 1, q, tables, lengths, return_lse=True)
-    mgr.weigh(2 * i, q, tables, lengths, lse, weights[i])
-    ...
-    lengths = mgr.evict(2 * i, 2 * i + 1, weights[i], tables, lengths, 2048, recent=256)
+    for i in range(layers):  # a step
+        out, lse = mgr.attend(2 * i, 2 * i + 1, q, tables, lengths, return_lse=True)
+        mgr.weigh(2 * i, q, tables, lengths, lse, weights[i])
+
+    for i in range(layers):  # now and then
+        cut = mgr.evict(2 * i, 2 * i + 1, weights[i], tables, lengths, 2048, recent=256)
+    lengths = cut
 
 Streams, memory, graphs and gradients are as in ``paged_attention``.
 """

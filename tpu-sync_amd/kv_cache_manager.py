@@ -597,7 +597,11 @@ class KVCacheManager:
               recent: int = 0, begins=None, shard_idx: int = 0, stream=None):
         """Cuts every sequence to ``budget`` tokens: ``choose_kept``, then
         ``compact``. Returns the new lengths, int32 [sequences] on the device: the
-        lesser of each length and the budget. Blocks behind them are free."""
+        lesser of each length and the budget. Blocks behind them are free.
+
+        A model's layers are cut one by one, each from the lengths before the
+        cut: a layer that is given the new ones already keeps its first tokens,
+        whatever they got."""
         from . import eviction
         kept, cut = eviction.choose_kept(weights, tables, lengths, budget, recent=recent,
                                          begins=begins, stream=stream)
