@@ -36,6 +36,7 @@ for _pack, _args in ((_NORM_ROPE, _capi.NormRopeArgs), (_APPEND_KV, _capi.Append
 
 _TYPES = {}
 _torch = _forward_ad = None
+_FP4 = None  # torch's 4-bit type, where it has one
 
 
 def _current_stream(device):
@@ -43,7 +44,7 @@ def _current_stream(device):
 
 
 def _load_torch():
-    global _torch, _forward_ad, _current_stream
+    global _torch, _forward_ad, _current_stream, _FP4
     if _torch is None:
         import torch
         from torch.autograd import forward_ad
@@ -51,8 +52,10 @@ def _load_torch():
         # The handle alone, without a Stream object around it, where torch has it.
         _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
         _TYPES.update({torch.bfloat16: _capi.BF16, torch.float16: _capi.F16,
-                       torch.float32: _capi.F32, torch.float8_e4m3fn: _capi.E4M3,
-                       torch.float4_e2m1fn_x2: _capi.FP4})
+                       torch.float32: _capi.F32, torch.float8_e4m3fn: _capi.E4M3})
+        _FP4 = getattr(torch, "float4_e2m1fn_x2", None)
+        if _FP4 is not None:
+            _TYPES[_FP4] = _capi.FP4
         _torch = torch
     return _torch
 
@@ -258,17 +261,17 @@ def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
             raise ValueError("the cache's storages must be [blocks, tokens, heads, head_dim] "
                              "tensors (in 4 bits [blocks, heads, tokens, head_dim / 2]), "
                              f"got {tuple(t.shape)}")
-        if t.dtype not in types + (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+        if t.dtype not in types + (torch.float8_e4m3fn, _FP4):
             raise ValueError(f"the cache must be {allowed}, float8_e4m3fn or float4_e2m1fn_x2, "
                              f"got {t.dtype}")
         shapes.append((t.dtype,) + tuple(t.shape[1:]))
     if shapes[0] != shapes[1]:
         raise ValueError("the key and value storages must have the same type and block shape")
     kind, block_tokens, heads, head_dim = shapes[0]
-    if kind == torch.float4_e2m1fn_x2:
+    if kind == _FP4:
         heads, block_tokens, head_dim = block_tokens, heads, 2 * head_dim
     k_scales = v_scales = 0
-    if kind in (torch.float8_e4m3fn, torch.float4_e2m1fn_x2):
+    if kind in (torch.float8_e4m3fn, _FP4):
         # Scale tables follow the KV storages, one a storage.
         if len(layers) != 2 * n:
             raise ValueError(f"a {str(kind)[6:]} cache needs one scale table a KV storage "
