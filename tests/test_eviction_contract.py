@@ -3,7 +3,11 @@ import textwrap
 
 import pytest
 
-pytest.importorskip("torch")
+torch = pytest.importorskip("torch")
+
+from fake_device import FakeDeviceTensor  # noqa: E402
+from test_eviction_checks import Manager, bytes_as  # noqa: E402
+from test_paged_attention_checks import fake, refused  # noqa: E402
 
 
 def example(doc):
@@ -36,3 +40,18 @@ def test_the_documented_loop_cuts_every_layer_from_the_same_lengths(kvx):
     assert mgr.weighed == {p[0]: (5000, w) for p, w in zip(pairs, "abc")}
     assert mgr.evicted == {p: (5000, w) for p, w in zip(pairs, "abc")}
     assert names["lengths"] == 2048
+
+
+def test_side_tables_may_follow_the_scales(kvx):
+    fp8, fp4, e8m0 = torch.float8_e4m3fn, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+    weights = [fake((9, 2, 16), torch.float32)]
+    for storage, scale in ((FakeDeviceTensor(torch.zeros(9, 16, 2, 64).to(fp8)),
+                            fake((9, 2), torch.float32)),
+                           (bytes_as((9, 2, 16, 32), fp4), bytes_as((9, 2, 16, 2), e8m0))):
+        for more in ([], weights, weights * 2):
+            mgr = Manager(kvx, [storage] * 2, [scale] * 2 + more)
+            # The cache is taken, so the refusal is that of the next argument.
+            refused("kept must be", mgr.compact, 0, 1, fake((3, 4, 5), torch.int32),
+                    fake((3, 4), torch.int32), stream=0)
+        refused("one scale table", Manager(kvx, [storage] * 2, [scale]).compact, 0, 1,
+                fake((3, 2, 5), torch.int32), fake((3, 4), torch.int32), stream=0)

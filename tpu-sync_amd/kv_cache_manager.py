@@ -208,6 +208,8 @@ class KVCacheManager:
         an fp8 cache, [num_blocks, kv_heads] float32 scales; for a 4-bit one
         [num_blocks, kv_heads, tokens, head_dim / 32] e8m0); they are block
         arrays num_kv_layers.. and move with every copy of the same block ids.
+        Scales come first, one table a KV storage; tables behind them are the
+        caller's, such as those that ``weigh`` keeps.
       numa: host mirror placement: "auto" (the GPU's NUMA node), "off", or a
         node number.
       dispatch: "env" (queued when RAIDEN_ENABLE_ASYNC_DISPATCH=1), "queued"
@@ -569,7 +571,9 @@ class KVCacheManager:
         where the call's own tokens had none before (so a block's entries need no
         clearing when it is handed out). decay=0 keeps this call's alone. Tokens
         before ``begins[s]`` (int32 [sequences]; a prefix shared with others) are
-        left out; a block that holds later ones must belong to one sequence.
+        left out; a block that holds later ones must belong to one sequence. A
+        table among the manager's ``scale_tables`` goes with its blocks to the
+        host and back.
         """
         from . import eviction
         eviction.weigh(self, k_layer, q, tables, lengths, lse, weights, starts=starts,

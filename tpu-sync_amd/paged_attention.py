@@ -272,8 +272,9 @@ def _describe_cache(mgr, k_layer, v_layer, shard_idx, dtype):
         heads, block_tokens, head_dim = block_tokens, heads, 2 * head_dim
     k_scales = v_scales = 0
     if kind in (torch.float8_e4m3fn, _FP4):
-        # Scale tables follow the KV storages, one a storage.
-        if len(layers) != 2 * n:
+        # Scale tables follow the KV storages, one a storage; other side tables may
+        # follow them.
+        if len(layers) < 2 * n:
             raise ValueError(f"a {str(kind)[6:]} cache needs one scale table a KV storage "
                              f"({n}), got {len(layers) - n}")
         _check_scales(layers, (n + k_layer, n + v_layer), shard_idx, kind,
