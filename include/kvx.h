@@ -1176,10 +1176,11 @@ int kvx_manager_attend(kvx_manager* m, const kvx_attend_args* args, void* stream
  * What attention each cached token got, for the eviction of those that got little.
  * For the tokens j of a sequence from begins[s] on and every head of the cache:
  *   weights[block of j][head][slot of j] =
- *       decay * (the same, 0 for the call's own tokens) +
+ *       decay * (the same, 0 for the call's own tokens and for those from weighed[s] on) +
  *       sum over the query rows of the head that see j of exp(scale q.k_j - lse).
- * lse is what kvx_manager_attend returns for the same queries. decay 0 does not read
- * what was there. Sums are fp32 and taken in one order whatever the lengths, so the same
+ * lse is what kvx_manager_attend returns for the same queries. Entries need no clearing
+ * when a block is handed out if every step that appends tokens is weighed, or if weighed
+ * tells which tokens were. decay 0 does not read what was there. Sums are fp32 and taken in one order whatever the lengths, so the same
  * call gives the same bytes. Other entries of the table are left alone; a token that has
  * no place is skipped. A block that holds a token from begins[s] on must belong to one
  * sequence of the call (those of a shared prefix lie before begins). A sequence without
@@ -1204,6 +1205,7 @@ typedef struct kvx_weigh_args {
   int32_t reserved;
   uint64_t workspace;
   int64_t workspace_bytes;
+  uint64_t weighed; /* int32 [sequences]: tokens that hold a weight; 0: all but the call's own */
 } kvx_weigh_args;
 
 int kvx_manager_weigh_workspace(kvx_manager* m, const kvx_weigh_args* args, int64_t* bytes);

@@ -55,3 +55,13 @@ def test_side_tables_may_follow_the_scales(kvx):
                     fake((3, 4), torch.int32), stream=0)
         refused("one scale table", Manager(kvx, [storage] * 2, [scale]).compact, 0, 1,
                 fake((3, 2, 5), torch.int32), fake((3, 4), torch.int32), stream=0)
+
+
+def test_weigh_refuses_other_counts_of_weighed_tokens(kvx):
+    mgr = Manager(kvx, [fake((9, 16, 2, 64)), fake((9, 16, 2, 64))])
+    args = (0, fake((3, 8, 64)), fake((3, 4), torch.int32), fake((3,), torch.int32),
+            fake((3, 8), torch.float32), fake((9, 2, 16), torch.float32))
+    refused("weighed must be", mgr.weigh, *args, weighed=fake((2,), torch.int32), stream=0)
+    refused("weighed must be one of", mgr.weigh, *args, weighed=fake((3,), torch.int64), stream=0)
+    refused("weighed is on device 1", mgr.weigh, *args, weighed=fake((3,), torch.int32, 1), stream=0)
+    refused("HIP device", mgr.weigh, *args, weighed=torch.zeros(3, dtype=torch.int32), stream=0)

@@ -284,7 +284,8 @@ class WeighArgs(ctypes.Structure):
                    ("blocks", ctypes.c_int64), ("begins", ctypes.c_uint64),
                    ("non_causal", ctypes.c_int32), ("scale", ctypes.c_float),
                    ("decay", ctypes.c_float), ("reserved", ctypes.c_int32),
-                   ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64)])
+                   ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_int64),
+                   ("weighed", ctypes.c_uint64)])
 
 
 class ChooseKeptArgs(ctypes.Structure):

@@ -58,6 +58,9 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
     if (a.begins != 0 && a.batch.sequences > 0) {
       KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.begins, a.batch.sequences, "begins"));
     }
+    if (a.weighed != 0 && a.batch.sequences > 0) {
+      KVX_RETURN_IF_ERROR(CheckWords(&ranges, a.weighed, a.batch.sequences, "weighed"));
+    }
     KVX_RETURN_IF_ERROR(CheckTable(&ranges, a.weights, a.blocks, c.heads, c.block_tokens, &table));
     if (a.blocks < cache.num_blocks) return Bad("weights: fewer blocks than the cache's");
     if (l.pool == kPoolSame && cache.k.base % 16 != 0) {
@@ -94,6 +97,7 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
   out->lse = reinterpret_cast<const float*>(a.lse);
   out->weights = reinterpret_cast<float*>(a.weights);
   out->begins = reinterpret_cast<const int32_t*>(a.begins);
+  out->weighed = reinterpret_cast<const int32_t*>(a.weighed);
   out->decay = a.decay;
   const int64_t need = l.batch.tokens == 0 ? 0 : PlanWeigh(out);
   if (workspace_bytes != nullptr) {
@@ -118,7 +122,8 @@ Status CheckWeigh(const PoolSource& pool, const kvx_weigh_args& a, WeighLaunch* 
                    {Lengths(a.batch), "lengths"},
                    {Starts(a.batch), "starts"},
                    {Whole(a.lse, a.tokens * a.q_heads * 4), "lse"},
-                   {Whole(a.begins, a.begins != 0 ? a.batch.sequences * 4 : 0), "begins"}}));
+                   {Whole(a.begins, a.begins != 0 ? a.batch.sequences * 4 : 0), "begins"},
+                   {Whole(a.weighed, a.weighed != 0 ? a.batch.sequences * 4 : 0), "weighed"}}));
   }
   return CheckApart(workspace, {weights});
 }

@@ -13,6 +13,7 @@ struct WeighLaunch {
   const float* lse = nullptr;       // [tokens][q_heads]
   float* weights = nullptr;         // [num_blocks][k_heads][block_tokens]
   const int32_t* begins = nullptr;  // [sequences]: first token weighed, or null: 0
+  const int32_t* weighed = nullptr;  // [sequences]: tokens that hold a weight, or null: all
   float decay = 1.0f;
   // Sums of cut tiles: two slots of WeighTile floats a worker.
   float* parts = nullptr;

@@ -1,9 +1,9 @@
 // The attention that each cached token got, added to a table of what it got before:
 //   w_j = decay w_j + sum over the rows of its key head that see it of
 //         e^{scale q.k_j - lse},
-// w_j = 0 before where the token is one of the call's own. lse is what attention
-// returns for the row, so that the exponentials of a row add up to 1. Everything
-// after the product is fp32.
+// w_j = 0 before where the token is one of the call's own or has not been weighed yet.
+// lse is what attention returns for the row, so that the exponentials of a row add up to
+// 1. Everything after the product is fp32.
 //
 // Tokens take the place of the output's columns, S = Q K^T, so a lane holds one
 // token's scores against several rows: the sum over rows stays in the lane but for
@@ -47,6 +47,7 @@ constexpr int WeighFewGroups(int padded_dim, int row_tiles, bool full) {
 struct WeighKeys {
   SequenceSpan q;
   int rows, begin, end;
+  int held;  // tokens that hold a weight
 };
 
 __device__ __forceinline__ WeighKeys LoadWeighKeys(const WeighLaunch& w, int s) {
@@ -55,6 +56,8 @@ __device__ __forceinline__ WeighKeys LoadWeighKeys(const WeighLaunch& w, int s) 
   k.rows = k.q.count * (w.attend.q_heads / w.attend.k_heads);
   k.end = min(k.q.length, w.attend.batch.capacity);
   k.begin = w.begins != nullptr ? min(max(w.begins[s], 0), k.end) : 0;
+  k.held = k.q.length - k.q.count;
+  if (w.weighed != nullptr) k.held = min(k.held, w.weighed[s]);
   return k;
 }
 
@@ -114,7 +117,7 @@ __device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int gr
     const WeighKeys k = LoadWeighKeys(w, s);
     const int begin = one(k.begin), end = one(k.end), rows = one(k.rows);
     const SequenceSpan span = {one(k.q.first), one(k.q.count), one(k.q.length)};
-    const int old_end = span.length - span.count;  // tokens that had a weight before
+    const int held_end = one(k.held);
 
     // Queries: row l % 16 of each row tile; and of the rows that this lane gets
     // scores of, 4 (l / 16) + i, the log of their sums and the tokens that they see.
@@ -177,7 +180,7 @@ __device__ __forceinline__ void WeighFew(const WeighLaunch& w, int* sums, int gr
       }
       mine = quarter == 1 ? to[1] : to[0];
       writes = quarter < 2 && (quarter == 1 ? has[1] : has[0]);
-      adds = w.decay != 0.0f && begin + step * kFewStep + quarter * 16 + in16 < old_end;
+      adds = w.decay != 0.0f && begin + step * kFewStep + quarter * 16 + in16 < held_end;
       held = w.weights[mine];
     };
     Words kw[2][KS];
@@ -258,6 +261,7 @@ struct WeighUnit {
   int rows;
   int begin, end;  // tokens
   int old_end;     // tokens that are not the call's own
+  int held;        // tokens that hold a weight
   int tiles;
   // Tiles that all rows see, of `stages` each; the others have `less` stages less each
   // than the one before, the first of them `later`.
@@ -273,6 +277,7 @@ __device__ __forceinline__ WeighUnit LoadWeighUnit(const WeighLaunch& w, int s) 
   u.begin = k.begin;
   u.end = k.end;
   u.old_end = k.q.length - k.q.count;
+  u.held = k.held;
   u.tiles = k.rows > kFewRows ? (k.end - k.begin + tile - 1) / tile : 0;
   u.stages = (k.rows + kWeighRows - 1) / kWeighRows;
   u.full = u.tiles;
@@ -376,7 +381,7 @@ __device__ __forceinline__ void WeighMany(const WeighLaunch& w, char* lds, int p
     const int stages = one(WeighCost(u, tile + 1)) - tile_at;
     // The part's stages: the last of them end with the last row.
     const int stage0 = at_unit - tile_at, stage1 = min(stages, stage0 + (x_end - x));
-    const int end = one(u.end), old_end = one(u.old_end);
+    const int end = one(u.end), held_end = one(u.held);
     const int row0 = (one(u.stages) - stages + stage0) * kWeighRows;
     const int rows = min(one(u.rows), row0 + (stage1 - stage0) * kWeighRows);
     const SequenceSpan span = LoadSequence(b, s);
@@ -550,7 +555,7 @@ __device__ __forceinline__ void WeighMany(const WeighLaunch& w, char* lds, int p
         w.parts[axis.Slot(worker, x) * kTile + (wave * CT + ct) * 32 + in32] = sum;
       } else if (mine[ct] != nullptr) {
         const float was =
-            j0 + ct * 32 + in32 < old_end && w.decay != 0.0f ? *mine[ct] : 0.0f;
+            j0 + ct * 32 + in32 < held_end && w.decay != 0.0f ? *mine[ct] : 0.0f;
         *mine[ct] = fmaf(w.decay, was, sum);
       }
     }
@@ -592,7 +597,7 @@ __global__ __launch_bounds__(kAttendThreads) void weigh_join_kernel(const WeighL
   if (id < 0 || id >= b.num_blocks) return;
   float* mine = w.weights + (static_cast<int64_t>(id) * a.k_heads + h) * b.block_tokens +
                 (p - at * b.block_tokens);
-  *mine = fmaf(w.decay, p < u.old_end && w.decay != 0.0f ? *mine : 0.0f, sum);
+  *mine = fmaf(w.decay, p < u.held && w.decay != 0.0f ? *mine : 0.0f, sum);
 }
 
 template <class E, int POOL, int DP, int RT, bool FULL>

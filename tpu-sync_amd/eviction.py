@@ -22,7 +22,7 @@ from typing import Tuple
 from . import _capi, paged_attention as base
 from .kv_cache_manager import _stream_ptr
 
-_WEIGH = struct.Struct(base._CACHE + base._BATCH + "q2iQ2q2QqQi2fiQq")
+_WEIGH = struct.Struct(base._CACHE + base._BATCH + "q2iQ2q2QqQi2fiQqQ")
 _CHOOSE = struct.Struct("4iqQ" + base._BATCH + "3Q2q")
 _COMPACT = struct.Struct(base._CACHE + "Q3qQ4qQq")
 for _pack, _args in ((_WEIGH, _capi.WeighArgs), (_CHOOSE, _capi.ChooseKeptArgs),
@@ -46,10 +46,10 @@ def _weights(t, device, blocks=None, heads=None, block_tokens=None):
     return t.data_ptr(), t.shape[0]
 
 
-def _begins(begins, device, sequences):
-    if begins is None:
+def _positions(t, what, device, sequences):
+    if t is None:
         return 0
-    return base._vector(begins, "begins", device, (base._torch.int32,), sequences)
+    return base._vector(t, what, device, (base._torch.int32,), sequences)
 
 
 def _count(value, what):
@@ -64,8 +64,8 @@ def _count(value, what):
     return value
 
 
-def weigh(mgr, k_layer, q, tables, lengths, lse, weights, *, starts, begins, decay, scale, causal,
-          shard_idx, stream) -> None:
+def weigh(mgr, k_layer, q, tables, lengths, lse, weights, *, starts, begins, weighed, decay, scale,
+          causal, shard_idx, stream) -> None:
     torch = base._torch or base._load_torch()
     device = mgr._device or 0
     q_at, q_token, q_head = base._rows(q, "q", device)
@@ -84,8 +84,9 @@ def weigh(mgr, k_layer, q, tables, lengths, lse, weights, *, starts, begins, dec
     weights_at, table_blocks = _weights(weights, device, blocks, cache[7], cache[6])
     args = _capi.WeighArgs.from_buffer_copy(_WEIGH.pack(
         *cache, *batch, tokens, base._TYPES[q.dtype], q_heads, q_at, q_token, q_head,
-        lse.data_ptr(), weights_at, table_blocks, _begins(begins, device, batch[5]), not causal,
-        dim ** -0.5 if scale is None else scale, decay, 0, 0, 0))
+        lse.data_ptr(), weights_at, table_blocks, _positions(begins, "begins", device, batch[5]),
+        not causal, dim ** -0.5 if scale is None else scale, decay, 0, 0, 0,
+        _positions(weighed, "weighed", device, batch[5])))
     lib = _capi.load()
     if starts is not None or q_heads > 32 * cache[7]:  # single tokens need no workspace
         need = ctypes.c_int64()
@@ -109,7 +110,8 @@ def choose_kept(weights, tables, lengths, budget: int, *, recent: int = 0, begin
     prefix, or the ones that every query attends to), the last ``recent`` ones,
     and of the others those with the largest weights, the earlier one where two
     are equal. (NaN counts as less than any number.) Where they do not all fit,
-    the first ones go before the recent ones.
+    the first ones go before the recent ones. Tokens that have not been weighed
+    should be among the recent ones: their entries are another token's.
 
     Args:
       weights: float32 [blocks, heads, tokens], as ``KVCacheManager.weigh`` keeps.
@@ -130,7 +132,7 @@ def choose_kept(weights, tables, lengths, budget: int, *, recent: int = 0, begin
     sequences = tables.shape[0]
     batch = base._batch(device, tables, lengths, None, sequences)
     budget, recent = _count(budget, "budget"), _count(recent, "recent")
-    begins_at = _begins(begins, device, sequences)
+    begins_at = _positions(begins, "begins", device, sequences)
     kept = base._empty(stream, weights.device, (sequences, heads, budget), torch.int32)
     cut = base._empty(stream, weights.device, (sequences,), torch.int32)
     args = _capi.ChooseKeptArgs.from_buffer_copy(_CHOOSE.pack(

@@ -559,7 +559,7 @@ class KVCacheManager:
 
     # -- eviction ------------------------------------------------------------
     def weigh(self, k_layer: int, q, tables, lengths, lse, weights, *, starts=None, begins=None,
-              decay: float = 1.0, scale: Optional[float] = None, causal: bool = True,
+              weighed=None, decay: float = 1.0, scale: Optional[float] = None, causal: bool = True,
               shard_idx: int = 0, stream=None) -> None:
         """Adds what attention each cached token got from ``q`` to ``weights``.
 
@@ -568,16 +568,20 @@ class KVCacheManager:
         of a sequence, its block and slot, and each of the storage's heads,
           weights = decay * weights + sum over the head's queries of
                     exp(scale * q.k_j - lse),
-        where the call's own tokens had none before (so a block's entries need no
-        clearing when it is handed out). decay=0 keeps this call's alone. Tokens
-        before ``begins[s]`` (int32 [sequences]; a prefix shared with others) are
-        left out; a block that holds later ones must belong to one sequence. A
-        table among the manager's ``scale_tables`` goes with its blocks to the
-        host and back.
+        where the call's own tokens had none before. If every step that appends
+        is weighed, a block's entries need no clearing when it is handed out. If
+        steps are left out, or a sequence's blocks come back without its table,
+        ``weighed[s]`` (int32 [sequences]) is how many of its tokens hold a weight:
+        those from there on had none either, whatever lies in their entries. (A
+        cut by n tokens that have all been weighed takes n from it.)
+        decay=0 keeps this call's alone. Tokens before ``begins[s]`` (int32
+        [sequences]; a prefix shared with others) are left out; a block that holds
+        later ones must belong to one sequence. A table among the manager's
+        ``scale_tables`` goes with its blocks to the host and back.
         """
         from . import eviction
         eviction.weigh(self, k_layer, q, tables, lengths, lse, weights, starts=starts,
-                       begins=begins, decay=decay, scale=scale, causal=causal,
+                       begins=begins, weighed=weighed, decay=decay, scale=scale, causal=causal,
                        shard_idx=shard_idx, stream=stream)
 
     def compact(self, k_layer: int, v_layer: int, kept, tables, *, weights=None,
