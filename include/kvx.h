@@ -1180,12 +1180,15 @@ int kvx_manager_attend(kvx_manager* m, const kvx_attend_args* args, void* stream
  *       sum over the query rows of the head that see j of exp(scale q.k_j - lse).
  * lse is what kvx_manager_attend returns for the same queries. Entries need no clearing
  * when a block is handed out if every step that appends tokens is weighed, or if weighed
- * tells which tokens were. decay 0 does not read what was there. Sums are fp32 and taken in one order whatever the lengths, so the same
- * call gives the same bytes. Other entries of the table are left alone; a token that has
- * no place is skipped. A block that holds a token from begins[s] on must belong to one
- * sequence of the call (those of a shared prefix lie before begins). A sequence without
- * query rows is left alone. workspace: as for kvx_manager_attend; without starts and
- * with up to 32 query heads a key head none is needed.
+ * tells which tokens were. decay 0 does not read what was there. Sums are fp32,
+ * in an order that shapes and lengths give, so the same call gives the same bytes. What a
+ * single token gives does not depend on the other sequences; the rows of a chunk may be
+ * summed in other parts when another sequence of the call is longer or shorter. Other
+ * entries of the table are left alone; a token that has no place is skipped. A block that
+ * holds a token from begins[s] on must belong to one sequence of the call (those of a
+ * shared prefix lie before begins). A sequence without query rows is left alone.
+ * workspace: as for kvx_manager_attend; without starts and with up to 32 query heads a key
+ * head none is needed.
  */
 typedef struct kvx_weigh_args {
   kvx_paged_cache cache; /* v_layer and v_scale_layer are not used */
