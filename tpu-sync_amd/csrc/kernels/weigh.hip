@@ -322,11 +322,8 @@ __device__ __forceinline__ void WeighSums(const WeighLaunch& w, int* sums) {
   BlockSums(sums, w.attend.batch.sequences, w.attend.most_many);
 }
 
-// A worker's least part, in stages.
-constexpr int kLeastStages = 1;
 __device__ __forceinline__ Axis WeighAxis(const WeighLaunch& w, int work) {
-  const int total = work * w.attend.k_heads;
-  return Axis(total, min(w.attend.many_grid, max(total / kLeastStages, 1)));
+  return Axis(work * w.attend.k_heads, w.attend.many_grid);
 }
 
 constexpr int kAhead = 4;  // products that operands are read ahead
@@ -708,8 +705,8 @@ int64_t PlanWeigh(WeighLaunch* l) {
     const int64_t units = std::min(S, T * G / kFewRows);
     const int64_t stages = (T * G + kWeighRows - 1) / kWeighRows + units;
     const int64_t work = stages * a.k_heads * ((capacity + tile - 1) / tile);
-    a.many_grid = static_cast<int>(std::min<int64_t>(
-        WeighGroups(a.padded_dim) * kCus, std::max<int64_t>(work / kLeastStages, 1)));
+    a.many_grid =
+        static_cast<int>(std::min<int64_t>(WeighGroups(a.padded_dim) * kCus, work));
   }
   return 2ll * a.many_grid * WeighTile(a.padded_dim) * static_cast<int64_t>(sizeof(float));
 }
