@@ -14,13 +14,17 @@
 // nothing depends on the order of atomic additions. Numbers are kept in LDS between
 // passes where they fit.
 //
+// LDS is taken for as many numbers as the tables have places, so above some 18000 of them
+// a CU holds one workgroup, however short the sequences are.
+//
 // 64 sequences of 1000 to 16384 tokens, 8 heads, cut to 2048: 23.5 us (21 MB): the passes
 // of each of the 512 workgroups, two a CU, with barriers between them (one a CU, which is
-// all that scalar registers without a limit allow: 30 us); a cut of one sequence of 5000
-// to 1024 takes 9 us. Four weights a load instead of one: 41 to 39 us; ranges of
+// what tables of 131072 tokens or scalar registers without a limit allow: 30 us); a cut of
+// one sequence of 5000 to 1024 takes 9 us, one of 100000 tokens, whose numbers LDS does not
+// hold, 166 us. Four weights a load instead of one: 41 to 39 us; ranges of
 // positions for threads instead of ballots over 64 at a time: 39 to 36 us; what stays
 // kept as bits of a word between counting and writing: 25.5 to 23.5 us. Equal weights
-// make additions to one bin take turns: 79 us where all are equal. (Lanes that first
+// make additions to one bin take turns: 88 us where all are equal. (Lanes that first
 // agree on a bin halve that, and take a tenth longer for others.)
 #include "evict.h"
 

@@ -10,7 +10,8 @@
 // row's bytes each. Rows that stay at their place are neither read nor written. 64
 // sequences cut to 2048 tokens, 8 heads x 128, bf16: 192 us for 849 MB (4.4 TB/s, reads
 // of scattered 256-byte rows and writes; torch's copy of 1 GiB reaches 5.1); one such
-// sequence 18 us.
+// sequence 18 us. In 4 bits 85 us for 232 MB: rows of 64 bytes, and their scales, which a
+// thread a row moves byte by byte.
 //
 // e4m3 (compact_e4m3_kernel): rows that meet in a block come from blocks with scales of
 // their own, so the block gets the largest of them, and codes are stored again as
